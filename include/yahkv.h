@@ -215,6 +215,105 @@ int yahkv_attend_prefill_qraw(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, con
                               const int32_t* chunk_lens, const float* q_raw_dev, const float* q_weight_dev, float eps,
                               const float* gate_dev, void* out_dev, int32_t out_dtype, void* stream);
 
+/* ---- long contexts: shared prefixes, eviction, rotary positions -------------------------------------------------
+ * No counterparts in the reference, which serves one sequence. What a batch server needs around the calls above when
+ * prompts and generations get long: a prompt prefilled once and forked, decode attention that reads the forks' common
+ * prefix once, accumulated attention weights with the eviction of the keys that collected least, and the rotation of
+ * head rows at positions that are data (after an eviction a key's slot is not its position any more).
+ * The calls work on the formats that store a key's K and V as rows of their own (YAHKV_FMT_Q8_0, YAHKV_FMT_Q4_0,
+ * YAHKV_FMT_F16; the rotation on any context) and refuse the tile formats with YAHKV_ERR_INVALID. */
+
+/* A new sequence that starts as the first n_tokens tokens of `seq` in every layer (each layer must hold that many:
+ * YAHKV_ERR_ORDER). Whole pages are shared, not copied, and counted; a prefix that ends inside a page gets a copy of that
+ * page, made on `stream` behind what is queued there (a host-only context can fork at page boundaries only). Either
+ * sequence may be freed or appended to afterwards; a page stays allocated while any sequence names it. A shared page is
+ * never written: yahkv_append and the decode steps refuse, with YAHKV_ERR_INVALID, a position in a page that another
+ * sequence holds too (a sequence rolled back below its fork with yahkv_seq_set_len). yahkv_append_slots and
+ * yahkv_write_page write where they are told to. */
+int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, void* stream);
+
+/* yahkv_attend_decode with every shared prefix computed once for all the rows that share it: same arguments, same result up
+ * to rounding. Rows whose block tables start with the same pages form a group (found here, any order, several groups
+ * and rows without one in a call); its prefix is what all of its rows have in common and filled. The prefix runs on the
+ * tensor cores for the whole group: K and V enter as fp16 (quantized values rounded once, as in
+ * yahkv_attend_prefill) and the softmax weights too, so a result is about 1e-3 of the largest output's size from
+ * yahkv_attend_decode's at worst and about 4e-4 of an output's size on average. n_splits: split-K units of what lies
+ * behind the prefix, 0 = automatic. q_dev 16-byte aligned. The first call allocates a workspace (about 40 MB; 24 KB
+ * per sequence of max_seqs where that is more). */
+int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
+                               const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, void* stream);
+
+/* yahkv_attend_decode, the same bits, which also adds to weights_dev the softmax weight of every key, summed over the six
+ * query heads of its kv head: weights_dev[(seq * 4 + kv head) * weights_stride + key] += sum_g p_g(key), f32, seq the
+ * sequence id (so rows stay where they are when the batch changes), key = 0 .. len - 1 its slot. weights_dev is
+ * [max_seqs][4][weights_stride], the caller's, one per layer: zero a row before a sequence's first call; keys appended
+ * later start from what the row holds there. weights_stride at least the longest sequence's length
+ * (YAHKV_ERR_CAPACITY). A sequence may be listed once. The gate does not enter the weights. q_dev 16-byte aligned. */
+int yahkv_attend_decode_weights(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
+                                const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, float* weights_dev,
+                                int64_t weights_stride, void* stream);
+
+/* Cuts every listed sequence that is longer than n_keep down to n_keep keys, in all layers (which must be equally long:
+ * YAHKV_ERR_ORDER), each kv head of each layer by its own weights: the first n_sink and the last n_recent keys are kept
+ * and of the others the n_keep - n_sink - n_recent of largest weight; of equal weights the lowest slots, NaN counts as
+ * less than any number. Kept keys move to slots 0 .. n_keep - 1 in their old order, their weights with them (weights
+ * of slots from n_keep to the old length become 0). weights_dev as above, layer l at weights_dev + l *
+ * weights_layer_stride. kept_dev [n_layers][n_seqs][4][n_keep] i32 receives the old slots; a sequence of at most n_keep keys stays
+ * as it is and its rows hold 0 .. len - 1, then -1. A head-sharded context cuts and writes its own kv heads only.
+ * Afterwards the sequence's length is n_keep in every layer and it holds just the pages for them: reserve again before
+ * appending. A page that another sequence shares is left alone and a free page takes its place (YAHKV_ERR_NO_PAGES if
+ * there is none, and nothing changes). Attention does not depend on the order of keys, but a key's slot is no longer
+ * its position: the next yahkv_append continues at position n_keep with a K row that the caller rotated at the true
+ * position (yahkv_rope_rows); yahkv_rope_append and the raw-projection calls refuse the sequence and its forks with
+ * YAHKV_ERR_ORDER until yahkv_seq_set_len(seq, -1, 0). A sequence in a prepared yahkv_batch must not be evicted: create
+ * the batch again. */
+int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t n_keep, int64_t n_sink, int64_t n_recent,
+                float* weights_dev, int64_t weights_stride, int64_t weights_layer_stride, int32_t* kept_dev, void* stream);
+
+/* Rotary positions for head rows of 256 dims. Pair p of rotary_dim / 2 is dims (p, p + rotary_dim / 2) (HALF, as in
+ * yahkv_rope_append) or (2p, 2p + 1) (INTERLEAVED); dims from rotary_dim on pass through. Pair p at position n is turned by
+ * n f_p and scaled by the magnitude m:
+ *   NONE    f_p = theta^(-2p / rotary_dim)
+ *   LINEAR  f_p / factor (position interpolation)
+ *   NTK     theta * factor^(rotary_dim / (rotary_dim - 2)) in place of theta
+ *   YARN    by parts: with r = original_len f_p / 2 pi turns over the original length and k = (r - beta_slow) / (beta_fast -
+ *           beta_slow) clamped to [0, 1], f_p' = (1 - k) f_p / factor + k f_p; magnitude 0 stands for 0.1 ln(factor) + 1
+ * magnitude 0 = 1 otherwise. Angles are evaluated in double precision. max_positions bounds the positions. */
+#define YAHKV_ROPE_HALF 0
+#define YAHKV_ROPE_INTERLEAVED 1
+#define YAHKV_ROPE_SCALE_NONE 0
+#define YAHKV_ROPE_SCALE_LINEAR 1
+#define YAHKV_ROPE_SCALE_NTK 2
+#define YAHKV_ROPE_SCALE_YARN 3
+typedef struct yahkv_rope_config {
+  int32_t layout;        /* YAHKV_ROPE_HALF | YAHKV_ROPE_INTERLEAVED */
+  int32_t rotary_dim;    /* even, 2 .. 256 */
+  int32_t scaling;       /* YAHKV_ROPE_SCALE_* */
+  int32_t reserved;      /* 0 */
+  double theta;          /* base, above 1 */
+  double factor;         /* >= 1; not read without scaling */
+  double original_len;   /* YARN only */
+  double beta_fast;      /* YARN only */
+  double beta_slow;      /* YARN only */
+  double magnitude;      /* 0 = the scaling's own */
+  int64_t max_positions; /* positions 0 .. max_positions - 1, at most 2^31 */
+} yahkv_rope_config;
+typedef struct yahkv_rope yahkv_rope;
+/* Builds the angle tables (8 B x rotary_dim / 2 x (1024 + max_positions / 1024)). Destroy it before the context, with its
+ * work done. Failures of the calls on it are reported by the context. */
+int yahkv_rope_create(yahkv_ctx* ctx, const yahkv_rope_config* cfg, yahkv_rope** out);
+void yahkv_rope_destroy(yahkv_rope* rope);
+/* Rotates n_heads consecutive rows of 256 of each of n_tokens tokens at positions_dev[token] (device, int64): x_dev fp16
+ * or f32 (x_dtype a YAHKV_OUT_* constant), tokens x_stride elements apart, so that x may be a slice of a wider projection output;
+ * out_dev likewise, and may be x_dev itself with equal type and stride. weight_dev [256] f32 not NULL: each row is first
+ * normed (x / sqrt(mean x^2 + eps) * weight, as yahkv_rope_append does). Arithmetic in f32, rounded once. Strides are
+ * multiples of 8 elements, x, out and weight 16-byte aligned. Capturable. A position outside [0, max_positions) sets the
+ * status word: the next yahkv_sync fails with YAHKV_ERR_CUDA, that token's rows are invalid (turned by the nearest
+ * angle). */
+int yahkv_rope_rows(yahkv_rope* rope, int32_t n_tokens, int32_t n_heads, const int64_t* positions_dev, const void* x_dev,
+                    int32_t x_dtype, int64_t x_stride, const float* weight_dev, float eps, void* out_dev, int32_t out_dtype,
+                    int64_t out_stride, void* stream);
+
 /* One decode step of one layer with HOST buffers (what an engine without device-resident activations calls):
  * copies k/v/q (and gate) in, appends one token per sequence at its current length, attends, copies out back and
  * waits for it. k_host, v_host [n_seqs][4][256] fp16; q_host [n_seqs][24][256] fp16; out_host by out_dtype. */
@@ -318,7 +417,11 @@ int yahkv_debug_set_prefill_sms(yahkv_ctx* ctx, int32_t n_sm);
 #define YAHKV_KERNEL_DECODE_COMBINE 2
 #define YAHKV_KERNEL_PREFILL 3
 #define YAHKV_KERNEL_PREFILL_DEQUANT 4
-#define YAHKV_KERNEL_COUNT 5
+#define YAHKV_KERNEL_SHARED_PREFIX 5
+#define YAHKV_KERNEL_WEIGHTS 6
+#define YAHKV_KERNEL_EVICT 7       /* selection and move together */
+#define YAHKV_KERNEL_ROPE 8
+#define YAHKV_KERNEL_COUNT 9
 int yahkv_kernel_timing(yahkv_ctx* ctx, int32_t enable);
 int yahkv_kernel_timing_read(yahkv_ctx* ctx, int32_t kernel, double* total_ms, int64_t* launches);
 

@@ -1,0 +1,396 @@
+// Attention weights per cached key, and the eviction of keys by them; the page copy of a forked sequence.
+//
+// AttnWeightsKernel adds to w[key] the softmax weights that the six query heads of a kv head's group gave the key in the
+// decode call just made: w[key] += sum_g 2^(s_g - M_g - log2 L_g), s_g = q_g.k * scale in log2 units. The call's
+// partials give M_g and L_g (joined in unit order), so one pass over K is enough; it reads K again (the part kernels
+// keep no scores) and is HBM-bound: half of the cache bytes plus 8 B per key and kv head. Scores are computed in fp32
+// from the fp16 query and the exact codes (f16 MMA on exact fp16 integers, the block scale applied in fp32), so a
+// weight is as exact as fp32 sums make it; the part kernels' 16-bit query planes would cost 2e-5 of a weight.
+// One warp takes 16 keys at a time; a lane's B operand is what it loads: dims 8t .. 8t + 7 of every 32-element block of
+// key g (q4_0: elements 4t .. and 16 + 4t ..), and A takes the query's dims in the same order. No atomics: each key is
+// added to by one lane of one CTA, so the result does not depend on the order of CTAs.
+//
+// EvictSelectKernel, one CTA per (layer, sequence, kv head): the n_keep keys to keep, ascending. The first n_sink and the
+// last n_recent are kept, of the rest the largest weights; ties go to the lowest index, NaN counts as less than
+// everything. A radix select over the order-preserving bits finds the smallest kept weight and how many keys of exactly
+// that weight are kept; a last pass in index order writes the kept indices and moves the weights to the front.
+//
+// EvictMoveKernel moves the kept rows to slots 0 .. n_keep - 1, in place where the sequence has its pages to itself: kept
+// index i is at least i, so with 64-slot chunks in ascending order a chunk's sources lie at or behind its slots, and
+// only the chunk's own reads have to come before its writes. Pages that another sequence shares are replaced by fresh
+// ones (the host lists them) and stay as they were.
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "kernels.cuh"
+#include "ptx.cuh"
+
+namespace yahkv {
+namespace {
+
+// ----------------------------------------------------------------------------------------------------------------
+// attention weights
+// ----------------------------------------------------------------------------------------------------------------
+constexpr int kWeightThreads = 256;
+constexpr int kWeightWarps = kWeightThreads / 32;
+
+// Four bytes u -> fp16 pairs (0, 1), (2, 3) of u - bias (0x6400 | u is 1024 + u; bias_h = 1024 + bias).
+__device__ __forceinline__ void Bytes4(std::uint32_t u, __half2 bias_h, std::uint32_t& h01, std::uint32_t& h23) {
+  const std::uint32_t a = __byte_perm(u, 0x64646464U, 0x4140), b = __byte_perm(u, 0x64646464U, 0x4342);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias_h), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias_h);
+  h01 = *reinterpret_cast<const std::uint32_t*>(&x), h23 = *reinterpret_cast<const std::uint32_t*>(&y);
+}
+__device__ __forceinline__ float HalfOf(const uint4& v, int i) {   // fp16 number i of eight, i a constant after unrolling
+  const std::uint32_t w = i < 4 ? (i < 2 ? v.x : v.y) : (i < 6 ? v.z : v.w);
+  const __half2 h = *reinterpret_cast<const __half2*>(&w);
+  return (i & 1) ? __high2float(h) : __low2float(h);
+}
+
+template <int kFmt>
+__global__ void __launch_bounds__(kWeightThreads, 2)
+    AttnWeightsKernel(PoolView pool, int layer, const std::int32_t* __restrict__ tables, int table_stride,
+                      const DecodeUnit* __restrict__ units, const CombineItem* __restrict__ items,
+                      const __half* __restrict__ q, float scale_log2, const float* __restrict__ partial_ml,
+                      float* __restrict__ weights, long long weights_stride) {
+  __shared__ float norm_s[8];   // M + log2 L per query head
+  ChainedKernelEntry();
+  const DecodeUnit u = units[blockIdx.x];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (u.page_end <= u.page_begin) return;
+  if (warp < kGroup) {
+    const CombineItem it = items[u.batch * kKvHeads + u.kvh];
+    const float* ml = partial_ml + static_cast<std::size_t>(it.first_partial) * kPartialMlFloats + 2 * warp;
+    float m = -INFINITY, l = 0.0F;
+    for (int i = lane; i < it.n_partials; i += 32) m = fmaxf(m, ml[static_cast<std::size_t>(i) * kPartialMlFloats]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFU, m, o));
+    for (int i = lane; i < it.n_partials; i += 32) {
+      const float mi = ml[static_cast<std::size_t>(i) * kPartialMlFloats];
+      l += mi == -INFINITY ? 0.0F : exp2f(mi - m) * ml[static_cast<std::size_t>(i) * kPartialMlFloats + 1];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFU, l, o);
+    if (lane == 0) norm_s[warp] = m + log2f(l);
+  }
+  // A operand: lane (g, t) holds head g's dims of block b in the order the lane's own B words have them
+  uint4 qa[kBlocksPerRow];
+#pragma unroll
+  for (int b = 0; b < kBlocksPerRow; ++b) {
+    qa[b] = make_uint4(0, 0, 0, 0);
+    if (g < kGroup) {
+      const __half* src = q + (static_cast<std::size_t>(u.batch) * kQHeads + u.kvh * kGroup + g) * kHeadDim + 32 * b;
+      if constexpr (kFmt == kFmtQ4) {
+        const uint2 lo = __ldg(reinterpret_cast<const uint2*>(src + 4 * t)), hi = __ldg(reinterpret_cast<const uint2*>(src + 16 + 4 * t));
+        qa[b] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      } else {
+        qa[b] = __ldg(reinterpret_cast<const uint4*>(src + 8 * t));
+      }
+    }
+  }
+  __syncthreads();
+  const float norm = g < kGroup ? norm_s[g] : INFINITY;
+  const std::int32_t* row = tables + static_cast<std::size_t>(u.seq) * table_stride;
+  float* w_out = weights + (static_cast<std::size_t>(u.seq) * kKvHeads + u.kvh) * static_cast<std::size_t>(weights_stride);
+  const __half2 bias = __half2half2(__ushort_as_half(kFmt == kFmtQ8 ? 0x6480 : 0x6408));
+
+  // 16-key groups of the unit's pages, one warp each
+  const int n_groups = (u.page_end - u.page_begin) * (kPageTokens / 16);
+  for (int i = warp; i < n_groups; i += kWeightWarps) {
+    const int p = u.page_begin + (i >> 2);
+    const int key0 = p * kPageTokens + (i & 3) * 16;
+    if (key0 >= u.n_keys) break;
+    const std::int32_t page = min(max(__ldg(row + p), 0), pool.num_pages - 1);   // never trust a table entry
+    const std::size_t rec = (static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + u.kvh;
+    const std::uint8_t* codes = pool.kcodes + rec * RecordCodeBytes(kFmt) + ((i & 3) * 16 + g) * CodeBytes(kFmt);
+    float s[2][2] = {{0.0F, 0.0F}, {0.0F, 0.0F}};
+    if constexpr (kFmt == kFmtF16) {
+      float acc[2][4] = {{0.0F, 0.0F, 0.0F, 0.0F}, {0.0F, 0.0F, 0.0F, 0.0F}};
+      uint4 w[2][kBlocksPerRow];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int b = 0; b < kBlocksPerRow; ++b)
+          w[kt][b] = *reinterpret_cast<const uint4*>(codes + kt * 8 * CodeBytes(kFmt) + b * 64 + t * 16);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int b = 0; b < kBlocksPerRow; ++b) {
+          MmaF16(acc[kt], qa[b].x, 0U, qa[b].y, 0U, w[kt][b].x, w[kt][b].y);
+          MmaF16(acc[kt], qa[b].z, 0U, qa[b].w, 0U, w[kt][b].z, w[kt][b].w);
+        }
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) s[kt][0] = acc[kt][0], s[kt][1] = acc[kt][1];
+    } else {
+      const std::uint16_t* scales = pool.kscales + (rec * kPageTokens + (i & 3) * 16) * kBlocksPerRow;
+      uint4 d[2][2];   // the eight block scales of keys 8 kt + 2t + j
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) d[kt][j] = *reinterpret_cast<const uint4*>(scales + (kt * 8 + 2 * t + j) * kBlocksPerRow);
+      uint2 w[2][kBlocksPerRow];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int b = 0; b < kBlocksPerRow; ++b) {
+          const std::uint8_t* src = codes + kt * 8 * CodeBytes(kFmt);
+          if constexpr (kFmt == kFmtQ8) {
+            const uint2 raw = *reinterpret_cast<const uint2*>(src + b * 32 + t * 8);
+            w[kt][b] = make_uint2(raw.x ^ kQ8FlipWord, raw.y ^ kQ8FlipWord);
+          } else {
+            const std::uint32_t raw = *reinterpret_cast<const std::uint32_t*>(src + b * 16 + t * 4);
+            w[kt][b] = make_uint2(raw & 0x0F0F0F0FU, (raw >> 4) & 0x0F0F0F0FU);
+          }
+        }
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int b = 0; b < kBlocksPerRow; ++b) {
+          float acc[4] = {0.0F, 0.0F, 0.0F, 0.0F};
+          std::uint32_t b0, b1;
+          Bytes4(w[kt][b].x, bias, b0, b1);
+          MmaF16(acc, qa[b].x, 0U, qa[b].y, 0U, b0, b1);
+          Bytes4(w[kt][b].y, bias, b0, b1);
+          MmaF16(acc, qa[b].z, 0U, qa[b].w, 0U, b0, b1);
+          s[kt][0] = fmaf(HalfOf(d[kt][0], b), acc[0], s[kt][0]);
+          s[kt][1] = fmaf(HalfOf(d[kt][1], b), acc[1], s[kt][1]);
+        }
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float p_sum = g < kGroup ? exp2f(fmaf(s[kt][j], scale_log2, -norm)) : 0.0F;
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1) p_sum += __shfl_xor_sync(0xFFFFFFFFU, p_sum, o);
+        const int key = key0 + kt * 8 + 2 * t + j;
+        if (g == 0 && key < u.n_keys) w_out[key] += p_sum;
+      }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// selection
+// ----------------------------------------------------------------------------------------------------------------
+constexpr int kSelectThreads = 1024;
+
+// Order-preserving bits of a weight: larger weight, larger word; NaN below everything, -0 equal to +0.
+__device__ __forceinline__ std::uint32_t OrderOf(float w) {
+  if (w != w) return 0U;
+  const std::uint32_t b = __float_as_uint(w == 0.0F ? 0.0F : w);
+  return (b & 0x80000000U) != 0 ? ~b : b | 0x80000000U;
+}
+
+__global__ void __launch_bounds__(kSelectThreads)
+    EvictSelectKernel(const EvictSeq* __restrict__ seqs, int n_seqs, int kv_head_begin, int n_keep, int n_sink, int n_recent,
+                      float* __restrict__ weights, long long weights_stride, long long layer_stride,
+                      std::int32_t* __restrict__ kept) {
+  __shared__ int hist[2048];
+  __shared__ int scan_s[kSelectThreads / 32];
+  __shared__ std::uint32_t prefix_s;
+  __shared__ int want_s;
+  ChainedKernelEntry();
+  const int b = blockIdx.x, h = kv_head_begin + blockIdx.y, layer = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const EvictSeq es = seqs[b];
+  std::int32_t* out = kept + ((static_cast<std::size_t>(layer) * n_seqs + b) * kKvHeads + h) * static_cast<std::size_t>(n_keep);
+  if (es.n_keys <= n_keep) {   // nothing to evict: the sequence stays as it is
+    for (int i = tid; i < n_keep; i += kSelectThreads) out[i] = i < es.n_keys ? i : -1;
+    return;
+  }
+  float* w = weights + static_cast<std::size_t>(layer) * layer_stride +
+             (static_cast<std::size_t>(es.seq) * kKvHeads + h) * static_cast<std::size_t>(weights_stride);
+  const int lo = n_sink, hi = es.n_keys - n_recent;
+  int want = n_keep - n_sink - n_recent;   // keys to choose of [lo, hi): fewer than hi - lo
+  // the want-th largest word, eleven, eleven and ten bits at a time
+  std::uint32_t prefix = 0, mask = 0;
+  if (want > 0) {
+    const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      for (int i = tid; i < 2048; i += kSelectThreads) hist[i] = 0;
+      __syncthreads();
+      const std::uint32_t bin_mask = (1U << bits[pass]) - 1U;
+      for (int i0 = lo; i0 < hi; i0 += kSelectThreads) {
+        const int i = i0 + tid;
+        const std::uint32_t o = i < hi ? OrderOf(w[i]) : 0U;
+        const bool on = i < hi && (o & mask) == prefix;
+        // lanes with the same bin add once (weights that are equal, zeros above all, would serialise otherwise)
+        const std::uint32_t bin = on ? (o >> shifts[pass]) & bin_mask : 0xFFFFFFFFU;
+        const unsigned same = __match_any_sync(0xFFFFFFFFU, bin);
+        if (on && lane == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
+      }
+      __syncthreads();
+      // counts from the largest bin down; two bins per thread
+      const int top = 2047 - 2 * tid;
+      const int c0 = hist[top], c1 = hist[top - 1];
+      int sum = c0 + c1;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xFFFFFFFFU, sum, d);
+        if (lane >= d) sum += v;
+      }
+      if (lane == 31) scan_s[warp] = sum;
+      __syncthreads();
+      if (warp == 0) {
+        int v = scan_s[lane];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int x = __shfl_up_sync(0xFFFFFFFFU, v, d);
+          if (lane >= d) v += x;
+        }
+        scan_s[lane] = v;
+      }
+      __syncthreads();
+      const int before = (warp > 0 ? scan_s[warp - 1] : 0) + sum - c0 - c1;
+      if (before < want && before + c0 >= want) {
+        prefix_s = prefix | (static_cast<std::uint32_t>(top) << shifts[pass]);
+        want_s = want - before;
+      } else if (before + c0 < want && before + c0 + c1 >= want) {
+        prefix_s = prefix | (static_cast<std::uint32_t>(top - 1) << shifts[pass]);
+        want_s = want - before - c0;
+      }
+      __syncthreads();
+      prefix = prefix_s, want = want_s;
+      mask |= bin_mask << shifts[pass];
+      __syncthreads();
+    }
+  }
+  // prefix is the smallest kept word and `want` keys of exactly that word are kept, the lowest indices; in index order,
+  // a kept key's slot is the number of keys kept before it
+  const int n_eq = n_keep - n_sink - n_recent > 0 ? want : 0;
+  int base_gt = 0, base_eq = 0;
+  for (int i0 = 0; i0 < es.n_keys; i0 += kSelectThreads) {
+    const int i = i0 + tid;
+    const bool in = i < es.n_keys;
+    const float wi = in ? w[i] : 0.0F;
+    const bool middle = in && i >= lo && i < hi;
+    const std::uint32_t o = middle ? OrderOf(wi) : 0U;
+    const bool choose = n_keep - n_sink - n_recent > 0;
+    const bool gt = in && (!middle || (choose && o > prefix));
+    const bool eq = middle && choose && o == prefix;
+    const unsigned bg = __ballot_sync(0xFFFFFFFFU, gt), be = __ballot_sync(0xFFFFFFFFU, eq);
+    const unsigned below = (1U << lane) - 1U;
+    if (lane == 0) scan_s[warp] = __popc(bg) | (__popc(be) << 16);
+    __syncthreads();   // every weight of the tile has been read: its slots may be written
+    if (warp == 0) {
+      int v = scan_s[lane];
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xFFFFFFFFU, v, d);
+        if (lane >= d) v += x;
+      }
+      scan_s[lane] = v;
+    }
+    __syncthreads();
+    const int pre = warp > 0 ? scan_s[warp - 1] : 0, all = scan_s[31];
+    const int eq_before = base_eq + (pre >> 16) + __popc(be & below);
+    const int gt_before = base_gt + (pre & 0xFFFF) + __popc(bg & below);
+    if (gt || (eq && eq_before < n_eq)) {
+      const int slot = gt_before + min(eq_before, n_eq);
+      if (slot < n_keep) out[slot] = i, w[slot] = wi;
+    }
+    base_gt += all & 0xFFFF, base_eq += all >> 16;
+    __syncthreads();
+  }
+  for (int i = n_keep + tid; i < es.n_keys; i += kSelectThreads) w[i] = 0.0F;   // slots of keys to come
+}
+
+// ----------------------------------------------------------------------------------------------------------------
+// moving the kept rows
+// ----------------------------------------------------------------------------------------------------------------
+constexpr int kMoveThreads = 256;
+
+template <int kFmt>
+__global__ void __launch_bounds__(kMoveThreads)
+    EvictMoveKernel(PoolView pool, const std::int32_t* __restrict__ tables, int table_stride, const EvictSeq* __restrict__ seqs,
+                    int n_seqs, const std::int32_t* __restrict__ dst_pages, int n_keep, const std::int32_t* __restrict__ kept) {
+  constexpr int kRowVecs = CodeBytes(kFmt) / 16;                          // 16-byte pieces of a row
+  constexpr int kPer = kPageTokens * kRowVecs / kMoveThreads;             // of a 64-row chunk, per thread
+  ChainedKernelEntry();
+  const int b = blockIdx.x, side = blockIdx.y & 1, h = pool.kv_head_begin + (blockIdx.y >> 1), layer = blockIdx.z;
+  const EvictSeq es = seqs[b];
+  if (es.n_keys <= n_keep) return;
+  const int tid = threadIdx.x;
+  const std::int32_t* idx = kept + ((static_cast<std::size_t>(layer) * n_seqs + b) * kKvHeads + h) * static_cast<std::size_t>(n_keep);
+  const std::int32_t* table = tables + static_cast<std::size_t>(es.seq) * table_stride;
+  std::uint8_t* codes = side == 0 ? pool.kcodes : pool.vcodes;
+  std::uint8_t* scales = reinterpret_cast<std::uint8_t*>(side == 0 ? pool.kscales : pool.vscales);
+  auto row_of = [&](std::int32_t page, int tok) -> std::size_t {
+    page = min(max(page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
+    return ((static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + h) * kPageTokens + tok;
+  };
+  uint4 v[kPer], sc = make_uint4(0, 0, 0, 0);
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int piece = tid + k * kMoveThreads, slot = c0 + piece / kRowVecs;
+      if (slot < n_keep) {
+        const int i = min(max(__ldg(idx + slot), 0), es.n_keys - 1);
+        v[k] = *reinterpret_cast<const uint4*>(codes + row_of(__ldg(table + i / kPageTokens), i % kPageTokens) * CodeBytes(kFmt) +
+                                               (piece % kRowVecs) * 16);
+      }
+    }
+    if (kFmt != kFmtF16 && tid < kPageTokens && c0 + tid < n_keep) {
+      const int i = min(max(__ldg(idx + c0 + tid), 0), es.n_keys - 1);
+      sc = *reinterpret_cast<const uint4*>(scales + row_of(__ldg(table + i / kPageTokens), i % kPageTokens) * (kBlocksPerRow * 2));
+    }
+  };
+  load(0);
+  for (int c0 = 0; c0 < n_keep; c0 += kPageTokens) {
+    __syncthreads();   // every row of the chunk is in registers: its slots may be written
+    uint4 mine[kPer], my_sc = sc;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) mine[k] = v[k];
+    if (c0 + kPageTokens < n_keep) load(c0 + kPageTokens);   // sources at or behind the next chunk's first slot
+    const std::int32_t page = __ldg(dst_pages + es.first_dst + c0 / kPageTokens);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int piece = tid + k * kMoveThreads, tok = piece / kRowVecs;
+      if (c0 + tok < n_keep)
+        *reinterpret_cast<uint4*>(codes + row_of(page, tok) * CodeBytes(kFmt) + (piece % kRowVecs) * 16) = mine[k];
+    }
+    if (kFmt != kFmtF16 && tid < kPageTokens && c0 + tid < n_keep)
+      *reinterpret_cast<uint4*>(scales + row_of(page, tid) * (kBlocksPerRow * 2)) = my_sc;
+  }
+}
+
+// Page src -> page dst, every layer, all kv heads, both sides: the partly filled last page of a forked prefix.
+__global__ void __launch_bounds__(256) CopyPageKernel(PoolView pool, int src, int dst) {
+  ChainedKernelEntry();
+  const int layer = blockIdx.x, what = blockIdx.y;   // 0, 1: K, V codes; 2, 3: K, V scales
+  const std::size_t bytes = static_cast<std::size_t>(kKvHeads) * (what < 2 ? RecordCodeBytes(pool.fmt) : RecordScaleBytes(pool.fmt, what - 2));
+  std::uint8_t* base = what == 0   ? pool.kcodes
+                       : what == 1 ? pool.vcodes
+                                   : reinterpret_cast<std::uint8_t*>(what == 2 ? pool.kscales : pool.vscales);
+  const uint4* from = reinterpret_cast<const uint4*>(base + (static_cast<std::size_t>(layer) * pool.num_pages + src) * bytes);
+  uint4* to = reinterpret_cast<uint4*>(base + (static_cast<std::size_t>(layer) * pool.num_pages + dst) * bytes);
+  for (std::size_t i = static_cast<std::size_t>(blockIdx.z) * 256 + threadIdx.x; i < bytes / 16; i += 256ULL * gridDim.z) to[i] = from[i];
+}
+
+}  // namespace
+
+cudaError_t LaunchAttnWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream) {
+  if (a.n_units <= 0) return cudaSuccess;
+  const auto kernel = a.pool.fmt == kFmtF16 ? AttnWeightsKernel<kFmtF16> : a.pool.fmt == kFmtQ8 ? AttnWeightsKernel<kFmtQ8> : AttnWeightsKernel<kFmtQ4>;
+  return LaunchChained(kernel, a.n_units, kWeightThreads, 0, stream, a.pool, a.layer, a.tables_dev, a.table_stride, a.units_dev,
+                       a.items_dev, static_cast<const __half*>(a.q_dev), a.scale_log2, a.partial_ml, weights, weights_stride);
+}
+
+cudaError_t LaunchEvict(const EvictLaunch& a, cudaStream_t stream) {
+  if (a.n_seqs <= 0) return cudaSuccess;
+  const dim3 per_row(static_cast<unsigned>(a.n_seqs), static_cast<unsigned>(a.pool.kv_head_count), static_cast<unsigned>(a.pool.n_layers));
+  cudaError_t e = LaunchChained(EvictSelectKernel, per_row, kSelectThreads, 0, stream, a.seqs_dev, a.n_seqs, a.pool.kv_head_begin,
+                                a.n_keep, a.n_sink, a.n_recent, a.weights, a.weights_stride, a.layer_stride, a.kept);
+  if (e != cudaSuccess) return e;
+  const dim3 per_side(per_row.x, 2 * per_row.y, per_row.z);
+  const auto move = a.pool.fmt == kFmtF16 ? EvictMoveKernel<kFmtF16> : a.pool.fmt == kFmtQ8 ? EvictMoveKernel<kFmtQ8> : EvictMoveKernel<kFmtQ4>;
+  return LaunchChained(move, per_side, kMoveThreads, 0, stream, a.pool, a.tables_dev, a.table_stride, a.seqs_dev, a.n_seqs,
+                       a.dst_pages_dev, a.n_keep, a.kept);
+}
+
+cudaError_t LaunchCopyPage(const PoolView& pool, int src, int dst, cudaStream_t stream) {
+  return LaunchChained(CopyPageKernel, dim3(static_cast<unsigned>(pool.n_layers), 4, 4), 256, 0, stream, pool, src, dst);
+}
+
+}  // namespace yahkv

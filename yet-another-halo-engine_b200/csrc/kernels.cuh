@@ -159,6 +159,32 @@ constexpr int kPrefillMaxParts = 4;   // key ranges a tile is split into at most
 constexpr int kPrefillPartAccFloats = kPrefillTileRows * kHeadDim;
 constexpr int kPrefillPartMlFloats = kPrefillTileRows * 2;
 
+// One CTA of the shared-prefix pass of decode attention (shared_attn.cu): up to 128 of a group's (row, query head) pairs of
+// one kv head over the pages [page_begin, page_end) that the group shares. Group row r is query head r % 6 of the kv
+// head's group, of the group's batch row r / 6. Neighbouring entries 2 i and 2 i + 1 are the two CTAs of a pair.
+struct PrefixTile {
+  std::int32_t row_list;    // the group's batch rows start here in the row list
+  std::int32_t row0;        // first group row of the CTA
+  std::int32_t n_rows;      // valid rows (0: the second CTA of a pair has none)
+  std::int32_t kvh;
+  std::int32_t seq;         // a block-table row that holds the shared pages
+  std::int32_t page_begin;
+  std::int32_t page_end;
+  std::int32_t part_row0;   // first row of the prefix workspace the CTA writes
+};
+static_assert(sizeof(PrefixTile) == 32, "uploaded as an array");
+// Where the prefix partials of one (batch row, kv head) lie: part k of query head j is row first + k * stride + j.
+struct PrefixItem {
+  std::int32_t first;
+  std::int32_t n_parts;     // 0: the row shares no prefix
+  std::int32_t stride;
+  std::int32_t pad;
+};
+static_assert(sizeof(PrefixItem) == 16, "uploaded as an array");
+constexpr int kSharedMinPages = 1;         // shortest prefix read once for a group
+constexpr double kSharedPartPages = 3.0;   // what a part costs beside its pages, in pages
+constexpr int kSharedMaxParts = 1024;      // prefix parts the combine kernel joins per row
+
 // Partial workspace per unit: acc [6][256] f32 (unnormalised), then ml [6][2] f32 (max in log2 units, sum).
 constexpr int kPartialAccFloats = kGroup * kHeadDim;
 constexpr int kPartialMlFloats = kGroup * 2;
@@ -256,6 +282,64 @@ cudaError_t LaunchDecodeCombine(const DecodeLaunch& a, cudaStream_t stream);
 // Shared-memory bytes the decode kernel asks for (for the one-time attribute set-up).
 cudaError_t ConfigureDecodeKernels();
 
+// The shared-prefix pass and the combine over prefix and suffix partials (shared_attn.cu).
+struct SharedLaunch {
+  const CUtensorMap* kmap;  // fp16 pages: K pool as [rows][256] fp16 in boxes of 64 dims x 32 keys
+  const CUtensorMap* vmap;  // fp16 pages: V pool, 64 dims x 64 keys; q8_0: V codes, 128 B x 64 keys
+  const PrefixTile* tiles_dev;
+  int n_tiles;              // CTAs, a multiple of two
+  const std::int32_t* rows_dev;
+  const PrefixItem* prefix_items_dev;
+  float* part_acc;          // [rows][256] f32, unnormalised
+  float* part_ml;           // [rows][2] f32 (max in log2 units, sum)
+};
+cudaError_t LaunchSharedPrefix(const DecodeLaunch& a, const SharedLaunch& p, cudaStream_t stream);
+cudaError_t LaunchSharedCombine(const DecodeLaunch& a, const SharedLaunch& p, cudaStream_t stream);
+cudaError_t ConfigureSharedKernels(int fmt, int* max_active_pairs);
+
+// One sequence of an eviction call (evict.cu).
+struct EvictSeq {
+  std::int32_t seq;         // block-table row, and row of the weights
+  std::int32_t n_keys;      // its length; at most n_keep: nothing is evicted
+  std::int32_t first_dst;   // its pages after the call start here in the page list
+  std::int32_t pad;
+};
+static_assert(sizeof(EvictSeq) == 16, "uploaded as an array");
+struct EvictLaunch {
+  PoolView pool;
+  const std::int32_t* tables_dev;   // the tables before the call
+  int table_stride;
+  const EvictSeq* seqs_dev;
+  int n_seqs;
+  const std::int32_t* dst_pages_dev;
+  int n_keep, n_sink, n_recent;
+  float* weights;
+  long long weights_stride, layer_stride;   // floats between rows of one (sequence, kv head), and between layers
+  std::int32_t* kept;
+};
+cudaError_t LaunchEvict(const EvictLaunch& a, cudaStream_t stream);
+// After LaunchDecodePart of the same plan (its partial_ml holds the rows' statistics); fp16 query.
+cudaError_t LaunchAttnWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream);
+cudaError_t LaunchCopyPage(const PoolView& pool, int src, int dst, cudaStream_t stream);
+
+// Rotary positions on given rows (rope.cu).
+constexpr int kRopeLowBits = 10;   // positions are split as 1024 hi + lo
+struct RopeRowsLaunch {
+  const void* x;
+  void* out;
+  const std::int64_t* positions;
+  const float* weight;      // norm weights [256] or null: no norm
+  const float2* tab_hi;     // [positions / 1024][rotary_dim / 2]
+  const float2* tab_lo;     // [1024][rotary_dim / 2]
+  int* status;
+  long long max_positions, x_stride, out_stride;   // strides between tokens, in elements
+  float eps;
+  int n_tokens, n_heads, rotary_dim;
+  bool interleaved, x_f32, out_f32;
+  int heads_per_warp, head_groups;   // set by the launcher
+};
+cudaError_t LaunchRopeRows(RopeRowsLaunch a, cudaStream_t stream);
+
 struct PrefillLaunch {
   PoolView pool;
   int layer;
@@ -299,6 +383,7 @@ bool EncodeTensorMap2D(CUtensorMap* map, int elem_bytes, void* base, std::uint64
 
 // Status codes the kernels write into the sticky status word.
 constexpr int kStatusWaitTimeout = 1;
+constexpr int kStatusRopePosition = 6;   // a position outside the rotation's range
 // One CTA waits at most limit_ns on an mbarrier nobody arrives at, gives up, records kStatusWaitTimeout and returns:
 // the give-up path of every bounded wait in this library, run on purpose (yahkv_debug_wait_timeout).
 cudaError_t LaunchWaitProbe(int* status_dev, std::uint64_t limit_ns, cudaStream_t stream);

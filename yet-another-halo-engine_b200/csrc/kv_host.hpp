@@ -33,7 +33,8 @@ class KvHost {
     len_.assign(ns * static_cast<std::size_t>(cfg.n_layers), 0);
     dirty_lo_.assign(ns, 0);
     dirty_hi_.assign(ns, 0);
-    owner_.assign(static_cast<std::size_t>(cfg.num_pages), -1);
+    refs_.assign(static_cast<std::size_t>(cfg.num_pages), 0);
+    evicted_.assign(ns, 0);
     // LIFO free list: page 0 is handed out first.
     free_pages_.reserve(static_cast<std::size_t>(cfg.num_pages));
     for (int p = cfg.num_pages - 1; p >= 0; --p) free_pages_.push_back(p);
@@ -90,6 +91,7 @@ class KvHost {
     free_seqs_.pop_back();
     live_[static_cast<std::size_t>(s)] = 1;
     n_pages_[static_cast<std::size_t>(s)] = 0;
+    evicted_[static_cast<std::size_t>(s)] = 0;
     SetLenAll(s, 0);
     *seq = s;
     return {};
@@ -119,7 +121,7 @@ class KvHost {
     for (int i = have; i < need; ++i) {
       const std::int32_t p = free_pages_.back();
       free_pages_.pop_back();
-      owner_[static_cast<std::size_t>(p)] = seq;
+      refs_[static_cast<std::size_t>(p)] = 1;
       row[i] = p;
     }
     n_pages_[static_cast<std::size_t>(seq)] = static_cast<int>(need);
@@ -140,9 +142,9 @@ class KvHost {
         return {YAHKV_ERR_INVALID, "page table entry out of range: " + std::to_string(p)};
       if (i > 0 && sorted[static_cast<std::size_t>(i - 1)] == p)
         return {YAHKV_ERR_INVALID, "page table names page " + std::to_string(p) + " twice"};
-      const int own = owner_[static_cast<std::size_t>(p)];
-      if (own != -1 && own != seq)
-        return {YAHKV_ERR_INVALID, "page " + std::to_string(p) + " belongs to sequence " + std::to_string(own)};
+      // free, or held by this sequence alone
+      if (const int holder = OtherHolder(p, seq); holder >= 0)
+        return {YAHKV_ERR_INVALID, "page " + std::to_string(p) + " belongs to sequence " + std::to_string(holder)};
     }
     ReleasePages(seq);
     // Take the named pages out of the free list.
@@ -154,7 +156,7 @@ class KvHost {
     std::int32_t* row = mutable_row(seq);
     for (int i = 0; i < n; ++i) {
       row[i] = pages[i];
-      owner_[static_cast<std::size_t>(pages[i])] = seq;
+      refs_[static_cast<std::size_t>(pages[i])] = 1;
     }
     n_pages_[static_cast<std::size_t>(seq)] = n;
     MarkDirty(seq, 0, n);
@@ -170,7 +172,115 @@ class KvHost {
       SetLenAll(seq, len);
     else
       len_ref(seq, layer) = len;
+    if (layer == -1 && len == 0) evicted_[static_cast<std::size_t>(seq)] = 0;   // starts over: slots are positions again
     return {};
+  }
+
+  // A new sequence whose first n_tokens / 64 pages are seq's own (counted references, never written while shared) and
+  // whose length is n_tokens in every layer. A prefix that ends inside a page takes a page of its own for the rest:
+  // *copy_src / *copy_dst then name the page to copy (-1: nothing to copy). Nothing changes on error.
+  HostError SeqFork(int seq, std::int64_t n_tokens, std::int32_t* out, std::int32_t* copy_src, std::int32_t* copy_dst) {
+    if (!live(seq)) return {YAHKV_ERR_INVALID, "seq_fork: not a live sequence: " + std::to_string(seq)};
+    if (n_tokens < 0) return {YAHKV_ERR_INVALID, "seq_fork: negative token count"};
+    for (int l = 0; l < cfg_.n_layers; ++l)
+      if (len(seq, l) < n_tokens)
+        return {YAHKV_ERR_ORDER, "seq_fork: sequence " + std::to_string(seq) + " holds " + std::to_string(len(seq, l)) +
+                                     " tokens in layer " + std::to_string(l) + ", " + std::to_string(n_tokens) + " asked for"};
+    const int whole = static_cast<int>(n_tokens / kPageTokens);
+    const bool rest = n_tokens % kPageTokens != 0;
+    if (rest && free_pages_.empty()) return {YAHKV_ERR_NO_PAGES, "seq_fork: no free page for the prefix's last, partly filled page"};
+    std::int32_t s = -1;
+    HostError e = SeqCreate(&s);
+    if (e.code != YAHKV_OK) return e;
+    std::int32_t* row = mutable_row(s);
+    const std::int32_t* from = table_row(seq);
+    for (int i = 0; i < whole; ++i) {
+      row[i] = from[i];
+      refs_[static_cast<std::size_t>(from[i])] += 1;
+    }
+    *copy_src = *copy_dst = -1;
+    if (rest) {
+      row[whole] = free_pages_.back();
+      free_pages_.pop_back();
+      refs_[static_cast<std::size_t>(row[whole])] = 1;
+      *copy_src = from[whole], *copy_dst = row[whole];
+    }
+    n_pages_[static_cast<std::size_t>(s)] = whole + (rest ? 1 : 0);
+    evicted_[static_cast<std::size_t>(s)] = evicted_[static_cast<std::size_t>(seq)];
+    MarkDirty(s, 0, n_pages_[static_cast<std::size_t>(s)]);
+    SetLenAll(s, n_tokens);
+    *out = s;
+    return {};
+  }
+
+  // Eviction of every listed sequence longer than n_keep (all layers equally long) down to n_keep slots: the pages it
+  // will have. A page it holds alone is kept and overwritten; a page that another sequence holds too at the time of the
+  // call is replaced by a free one, also when that other sequence is evicted by the same call and lets go of it.
+  // Changes nothing; CommitEvict with the same lists then moves the tables over.
+  HostError PlanEvict(int n_seqs, const std::int32_t* seq_ids, std::int64_t n_keep, std::vector<EvictSeq>* seqs,
+                      std::vector<std::int32_t>* dst_pages, bool* any) const {
+    seqs->clear();
+    dst_pages->clear();
+    *any = false;
+    std::vector<char> seen(static_cast<std::size_t>(cfg_.max_seqs), 0);
+    const int np = static_cast<int>((n_keep + kPageTokens - 1) / kPageTokens);
+    std::size_t fresh = 0;
+    for (int b = 0; b < n_seqs; ++b) {
+      const int s = seq_ids[b];
+      if (!live(s)) return {YAHKV_ERR_INVALID, "evict: not a live sequence: " + std::to_string(s)};
+      if (seen[static_cast<std::size_t>(s)]++) return {YAHKV_ERR_INVALID, "evict: sequence " + std::to_string(s) + " is listed twice"};
+      const std::int64_t n = len(s, 0);
+      for (int l = 1; l < cfg_.n_layers; ++l)
+        if (len(s, l) != n)
+          return {YAHKV_ERR_ORDER, "evict: sequence " + std::to_string(s) + " has different lengths in its layers"};
+      EvictSeq e{};
+      e.seq = s, e.n_keys = static_cast<std::int32_t>(n), e.first_dst = static_cast<std::int32_t>(dst_pages->size());
+      seqs->push_back(e);
+      if (n <= n_keep) continue;
+      *any = true;
+      for (int i = 0; i < np; ++i) {
+        std::int32_t page = table_row(s)[i];
+        if (refs_[static_cast<std::size_t>(page)] > 1) {
+          if (fresh == free_pages_.size())
+            return {YAHKV_ERR_NO_PAGES, "evict: no free page to take the place of a shared one"};
+          page = free_pages_[free_pages_.size() - 1 - fresh++];
+        }
+        dst_pages->push_back(page);
+      }
+    }
+    return {};
+  }
+  void CommitEvict(std::int64_t n_keep, const std::vector<EvictSeq>& seqs, const std::vector<std::int32_t>& dst_pages) {
+    const int np = static_cast<int>((n_keep + kPageTokens - 1) / kPageTokens);
+    std::vector<std::int32_t> dropped;
+    for (const EvictSeq& e : seqs) {
+      if (e.n_keys <= n_keep) continue;
+      std::int32_t* row = mutable_row(e.seq);
+      for (int i = 0; i < n_pages(e.seq); ++i) {
+        const std::int32_t to = i < np ? dst_pages[static_cast<std::size_t>(e.first_dst + i)] : -1;
+        if (to == row[i]) continue;
+        dropped.push_back(row[i]);
+        if (to < 0) continue;
+        free_pages_.pop_back();   // in PlanEvict's order
+        refs_[static_cast<std::size_t>(to)] = 1;
+        row[i] = to;
+      }
+      n_pages_[static_cast<std::size_t>(e.seq)] = np;
+      SetLenAll(e.seq, n_keep);
+      SetEvicted(e.seq);
+      MarkDirty(e.seq, 0, np);
+    }
+    for (std::int32_t p : dropped) Unref(p);   // only now: a page let go of here was nobody's fresh page
+  }
+  int page_refs(std::int32_t page) const { return refs_[static_cast<std::size_t>(page)]; }
+  // Keys of the sequence have been evicted: its slots no longer count positions.
+  bool evicted(int seq) const { return evicted_[static_cast<std::size_t>(seq)] != 0; }
+  void SetEvicted(int seq) { evicted_[static_cast<std::size_t>(seq)] = 1; }
+  // The first page of [position lo, hi) that another sequence holds too; -1: none. Such a page may not be written.
+  std::int32_t SharedPageIn(int seq, std::int64_t lo, std::int64_t hi) const {
+    for (std::int64_t i = lo / kPageTokens; i < (hi + kPageTokens - 1) / kPageTokens && i < n_pages(seq); ++i)
+      if (refs_[static_cast<std::size_t>(table_row(seq)[i])] > 1) return table_row(seq)[i];
+    return -1;
   }
 
   // Checks one append call and computes its slots; on success also advances the lengths. Nothing changes on error.
@@ -194,7 +304,11 @@ class KvHost {
       if (pos >= static_cast<std::int64_t>(n_pages_[static_cast<std::size_t>(s)]) * kPageTokens)
         return {YAHKV_ERR_INVALID, "append: position " + std::to_string(pos) + " of sequence " + std::to_string(s) +
                                        " is past its reserved pages"};
-      slots_out[t] = static_cast<std::int64_t>(table_row(s)[pos / kPageTokens]) * kPageTokens + pos % kPageTokens;
+      const std::int32_t page = table_row(s)[pos / kPageTokens];
+      if (refs_[static_cast<std::size_t>(page)] > 1)   // a prefix rolled back below a fork
+        return {YAHKV_ERR_INVALID, "append: position " + std::to_string(pos) + " of sequence " + std::to_string(s) +
+                                       " lies in page " + std::to_string(page) + ", which another sequence shares"};
+      slots_out[t] = static_cast<std::int64_t>(page) * kPageTokens + pos % kPageTokens;
       bool found = false;
       for (auto& e : scratch_len_)
         if (e.first == s) e.second = pos + 1, found = true;
@@ -243,29 +357,8 @@ class KvHost {
       const int s = seq_ids[b];
       const std::int64_t n = len(s, layer);
       const int pages = static_cast<int>((n + kPageTokens - 1) / kPageTokens);
-      int per = n_splits > 0 ? (pages + n_splits - 1) / n_splits : auto_pages;
-      per = std::max(per, (pages + max_splits - 1) / max_splits);
-      // The part kernel's two page sets take alternate pages of a unit: an odd count leaves one set idle for a page,
-      // so a unit costs as much as the next even count. Rounding up never raises the number of units.
-      if (per > 1) per += per & 1;
-      int nu = (pages + per - 1) / per;
-      // Graded sizes: with eight or more units the last quarter of them is half as long (and the others a little
-      // longer, the count stays). CTAs take units longest first, so the short ones of all sequences run last and fill
-      // the gaps of the final wave: equal units on a grid that is not a multiple of the resident CTAs leave a last
-      // wave that is mostly idle (8 x 131072 tokens in 64 splits: 1952 equal units on 592 CTA slots).
-      bounds_.clear();
-      if (nu >= 8) {
-        const int n_small = nu / 4, n_big = nu - n_small;
-        int big = (2 * pages + 2 * n_big + n_small - 1) / (2 * n_big + n_small);
-        big += big & 1;
-        const int small = std::max(((big / 2) + 1) & ~1, 2);
-        int p = 0;
-        for (int k = 0; k < n_big && p < pages; ++k) bounds_.push_back(p = std::min(p + big, pages));
-        while (p < pages) bounds_.push_back(p = std::min(p + small, pages));
-      } else {
-        for (int k = 0; k < nu; ++k) bounds_.push_back(std::min(pages, (k + 1) * per));
-      }
-      nu = static_cast<int>(bounds_.size());
+      CutUnits(pages, n_splits, max_splits, auto_pages);
+      const int nu = static_cast<int>(bounds_.size());
       for (int h = hb; h < hb + hc; ++h) {   // heads outside the context's range keep n_partials = 0
         items[static_cast<std::size_t>(b) * kKvHeads + h] = {static_cast<std::int32_t>(units.size()), nu};
         for (int k = 0; k < nu; ++k) {
@@ -292,6 +385,186 @@ class KvHost {
     return {};
   }
   void InvalidateDecodePlan() { plan_key_.clear(); }
+
+  // ---- decode attention over shared prefixes -------------------------------------------------------------------
+  // Rows of the call whose tables start with the same page share a prefix: the longest run of pages common to all of
+  // them that every one of them has filled. A group of two rows or more gets prefix tiles (all its rows at once,
+  // csrc/shared_attn.cu); what a row has behind its group's prefix, or the whole of a row without one, becomes
+  // ordinary split-K units. n_pairs: CTA pairs the device runs at once; max_part_rows: rows of the prefix workspace.
+  HostError PlanDecodeShared(int layer, int n_seqs, const std::int32_t* seq_ids, int n_splits, int max_splits,
+                             int max_units, int n_pairs, std::int64_t max_part_rows, bool* changed) {
+    if (layer < 0 || layer >= cfg_.n_layers) return {YAHKV_ERR_INVALID, "attend_decode_shared: layer out of range"};
+    if (n_seqs < 0 || (n_seqs > 0 && seq_ids == nullptr)) return {YAHKV_ERR_INVALID, "attend_decode_shared: bad sequence list"};
+    if (n_seqs > cfg_.max_seqs) return {YAHKV_ERR_CAPACITY, "attend_decode_shared: more rows than max_seqs"};
+    if (n_splits < 0) return {YAHKV_ERR_INVALID, "attend_decode_shared: negative n_splits"};
+    if (n_splits > max_splits) return {YAHKV_ERR_CAPACITY, "attend_decode_shared: n_splits above max_splits"};
+    key_scratch_.clear();
+    key_scratch_.push_back(n_splits);
+    key_scratch_.push_back(table_epoch_);
+    for (int b = 0; b < n_seqs; ++b) {
+      const int s = seq_ids[b];
+      if (!live(s)) return {YAHKV_ERR_INVALID, "attend_decode_shared: not a live sequence: " + std::to_string(s)};
+      const std::int64_t n = len(s, layer);
+      if (n <= 0)
+        return {YAHKV_ERR_ORDER, "attend_decode_shared: sequence " + std::to_string(s) + " has no keys in layer " +
+                                     std::to_string(layer) + " (append first)"};
+      key_scratch_.push_back(s);
+      key_scratch_.push_back(n);
+    }
+    if (key_scratch_ == shared_.key) {
+      *changed = false;
+      return {};
+    }
+    SharedPlan plan;
+    plan.key = key_scratch_;
+    std::vector<std::int64_t> lens(static_cast<std::size_t>(n_seqs));
+    for (int b = 0; b < n_seqs; ++b) lens[static_cast<std::size_t>(b)] = len(seq_ids[b], layer);
+    PlanPrefixes(n_seqs, seq_ids, lens.data(), n_pairs, max_part_rows, &plan);
+    const int hb = kv_head_begin(), hc = kv_head_count();
+    long long suffix_pages = 0;
+    for (int b = 0; b < n_seqs; ++b)
+      suffix_pages += (lens[static_cast<std::size_t>(b)] + kPageTokens - 1) / kPageTokens - plan.first_page[static_cast<std::size_t>(b)];
+    int auto_pages = static_cast<int>((suffix_pages * hc + 1479) / 1480);   // as in PlanDecode
+    auto_pages = std::min(std::max(auto_pages, 1), 24);
+    plan.items.resize(static_cast<std::size_t>(n_seqs) * kKvHeads);
+    for (int b = 0; b < n_seqs; ++b) {
+      const int first = plan.first_page[static_cast<std::size_t>(b)];
+      const std::int64_t n = lens[static_cast<std::size_t>(b)];
+      const int pages = static_cast<int>((n + kPageTokens - 1) / kPageTokens) - first;
+      bounds_.clear();
+      if (pages > 0) CutUnits(pages, n_splits, max_splits, auto_pages);
+      const int nu = static_cast<int>(bounds_.size());
+      for (int h = hb; h < hb + hc; ++h) {
+        plan.items[static_cast<std::size_t>(b) * kKvHeads + h] = {static_cast<std::int32_t>(plan.units.size()), nu};
+        for (int k = 0; k < nu; ++k) {
+          DecodeUnit u{};
+          u.batch = b, u.seq = seq_ids[b], u.kvh = h;
+          u.page_begin = first + (k == 0 ? 0 : bounds_[static_cast<std::size_t>(k) - 1]);
+          u.page_end = first + bounds_[static_cast<std::size_t>(k)];
+          u.n_keys = static_cast<std::int32_t>(n);
+          u.partial = static_cast<std::int32_t>(plan.units.size());
+          plan.units.push_back(u);
+        }
+      }
+    }
+    if (static_cast<long long>(plan.units.size()) > max_units)
+      return {YAHKV_ERR_CAPACITY, "attend_decode_shared: split-K plan needs " + std::to_string(plan.units.size()) +
+                                      " units, workspace holds " + std::to_string(max_units)};
+    std::stable_sort(plan.units.begin(), plan.units.end(), [](const DecodeUnit& a, const DecodeUnit& b) {
+      return a.page_end - a.page_begin > b.page_end - b.page_begin;
+    });
+    shared_ = std::move(plan);
+    *changed = true;
+    return {};
+  }
+  struct SharedPlan {
+    std::vector<std::int64_t> key;
+    std::vector<int> first_page;            // per row: pages its group's prefix covers (0: no group)
+    std::vector<PrefixTile> tiles;          // neighbouring pairs: the two CTAs of a cluster
+    std::vector<std::int32_t> rows;         // batch rows of the groups, one list after the other
+    std::vector<PrefixItem> prefix_items;   // per (row, kv head): where its prefix partials lie
+    std::vector<DecodeUnit> units;
+    std::vector<CombineItem> items;
+  };
+  const SharedPlan& shared_plan() const { return shared_; }
+  void InvalidateSharedPlan() { shared_.key.clear(); }
+
+  // The prefix part of a shared plan: groups, their tiles and where every row finds its partials.
+  void PlanPrefixes(int n_seqs, const std::int32_t* seq_ids, const std::int64_t* lens, int n_pairs,
+                    std::int64_t max_part_rows, SharedPlan* plan) const {
+    const int hb = kv_head_begin(), hc = kv_head_count();
+    plan->first_page.assign(static_cast<std::size_t>(n_seqs), 0);
+    plan->prefix_items.assign(static_cast<std::size_t>(n_seqs) * kKvHeads, PrefixItem{});
+    struct Group {
+      std::vector<std::int32_t> rows;
+      int pages = 0, n_mt = 0;
+    };
+    std::vector<Group> groups;
+    std::vector<std::pair<std::int32_t, std::int32_t>> by_page;   // (first page, row), rows in order
+    for (int b = 0; b < n_seqs; ++b)
+      if (lens[b] >= kPageTokens) by_page.emplace_back(table_row(seq_ids[b])[0], b);
+    std::stable_sort(by_page.begin(), by_page.end(), [](const auto& x, const auto& y) { return x.first < y.first; });
+    for (std::size_t i = 0; i < by_page.size();) {
+      std::size_t j = i;
+      while (j < by_page.size() && by_page[j].first == by_page[i].first) ++j;
+      if (j - i >= 2) {
+        Group g;
+        const std::int32_t* base = table_row(seq_ids[by_page[i].second]);
+        std::int64_t pages = lens[by_page[i].second] / kPageTokens;
+        for (std::size_t k = i; k < j; ++k) {
+          const int b = by_page[k].second;
+          const std::int32_t* row = table_row(seq_ids[b]);
+          pages = std::min(pages, lens[b] / kPageTokens);
+          std::int64_t same = 0;
+          while (same < pages && row[same] == base[same]) ++same;
+          pages = same;
+          g.rows.push_back(b);
+        }
+        g.pages = static_cast<int>(pages);
+        g.n_mt = (static_cast<int>(g.rows.size()) * kGroup + 2 * kPrefillTileRows - 1) / (2 * kPrefillTileRows);
+        if (g.pages >= kSharedMinPages) groups.push_back(std::move(g));
+      }
+      i = j;
+    }
+    if (groups.empty()) return;
+    // Pages per part. Every (group, kv head, 256 rows) is cut along its pages into parts, one CTA pair each; all pairs
+    // of a wave take about as long as the largest part, so for one to four waves the smallest part that fits them is
+    // taken, and of those the cheapest: waves x (pages + what a part costs beside its pages).
+    auto pairs_at = [&](int per) {
+      long long n = 0;
+      for (const Group& g : groups) n += static_cast<long long>(g.n_mt) * hc * ((g.pages + per - 1) / per);
+      return n;
+    };
+    int most = 1;
+    for (const Group& g : groups) most = std::max(most, g.pages);
+    int per = most;
+    double best = -1.0;
+    for (int waves = 1; waves <= 4; ++waves) {
+      int lo = 1, hi = most;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (pairs_at(mid) <= static_cast<long long>(waves) * n_pairs) hi = mid;
+        else lo = mid + 1;
+      }
+      const double n_waves = static_cast<double>((pairs_at(lo) + n_pairs - 1) / n_pairs);
+      const double cost = n_waves * (lo + kSharedPartPages);
+      if (best < 0.0 || cost < best - 1e-9) best = cost, per = lo;
+    }
+    auto rows_at = [&](int p) {
+      long long n = 0;
+      for (const Group& g : groups) n += static_cast<long long>(g.rows.size()) * kGroup * hc * ((g.pages + p - 1) / p);
+      return n;
+    };
+    while (per < most && rows_at(per) > max_part_rows) ++per;   // one part per tile always fits (24 rows per batch row)
+    std::int64_t part_row = 0;
+    for (const Group& g : groups) {
+      const std::int32_t list = static_cast<std::int32_t>(plan->rows.size());
+      const int n_rows = static_cast<int>(g.rows.size()) * kGroup;
+      const int n_parts = (g.pages + per - 1) / per;
+      plan->rows.insert(plan->rows.end(), g.rows.begin(), g.rows.end());
+      for (std::int32_t b : g.rows) plan->first_page[static_cast<std::size_t>(b)] = g.pages;
+      for (int h = hb; h < hb + hc; ++h) {
+        for (std::size_t i = 0; i < g.rows.size(); ++i)
+          plan->prefix_items[static_cast<std::size_t>(g.rows[i]) * kKvHeads + h] = {
+              static_cast<std::int32_t>(part_row + static_cast<std::int64_t>(i) * kGroup), n_parts, n_rows, 0};
+        for (int k = 0; k < n_parts; ++k) {
+          for (int r = 0; r < g.n_mt * 2 * kPrefillTileRows; r += kPrefillTileRows) {   // two CTAs per pair, the last may be empty
+            PrefixTile t{};
+            t.row_list = list, t.row0 = r, t.n_rows = std::min(std::max(n_rows - r, 0), kPrefillTileRows);
+            t.kvh = h, t.seq = seq_ids[g.rows[0]];
+            t.page_begin = g.pages * k / n_parts, t.page_end = g.pages * (k + 1) / n_parts;
+            t.part_row0 = static_cast<std::int32_t>(part_row + r);
+            plan->tiles.push_back(t);
+          }
+          part_row += n_rows;
+        }
+      }
+    }
+    // longest parts first; the two CTAs of a pair have equal keys and stay neighbours
+    std::stable_sort(plan->tiles.begin(), plan->tiles.end(), [](const PrefixTile& a, const PrefixTile& b) {
+      return a.page_end - a.page_begin > b.page_end - b.page_begin;
+    });
+  }
 
   // ---- kv8a16: which of a (sequence, layer)'s two open-tile buffers is current, and the V tile work of an append --
   int open_cur(int seq, int layer) const {
@@ -462,6 +735,31 @@ class KvHost {
   }
 
  private:
+  // Page boundaries of one sequence's split-K units over `pages` pages, into bounds_.
+  void CutUnits(int pages, int n_splits, int max_splits, int auto_pages) {
+    int per = n_splits > 0 ? (pages + n_splits - 1) / n_splits : auto_pages;
+    per = std::max(per, (pages + max_splits - 1) / max_splits);
+    // The part kernel's two page sets take alternate pages of a unit: an odd count leaves one set idle for a page,
+    // so a unit costs as much as the next even count. Rounding up never raises the number of units.
+    if (per > 1) per += per & 1;
+    const int nu = (pages + per - 1) / per;
+    // Graded sizes: with eight or more units the last quarter of them is half as long (and the others a little
+    // longer, the count stays). CTAs take units longest first, so the short ones of all sequences run last and fill
+    // the gaps of the final wave: equal units on a grid that is not a multiple of the resident CTAs leave a last
+    // wave that is mostly idle (8 x 131072 tokens in 64 splits: 1952 equal units on 592 CTA slots).
+    bounds_.clear();
+    if (nu >= 8) {
+      const int n_small = nu / 4, n_big = nu - n_small;
+      int big = (2 * pages + 2 * n_big + n_small - 1) / (2 * n_big + n_small);
+      big += big & 1;
+      const int small = std::max(((big / 2) + 1) & ~1, 2);
+      int p = 0;
+      for (int k = 0; k < n_big && p < pages; ++k) bounds_.push_back(p = std::min(p + big, pages));
+      while (p < pages) bounds_.push_back(p = std::min(p + small, pages));
+    } else {
+      for (int k = 0; k < nu; ++k) bounds_.push_back(std::min(pages, (k + 1) * per));
+    }
+  }
   std::int32_t* mutable_row(int seq) {
     return table_.data() + static_cast<std::size_t>(seq) * static_cast<std::size_t>(cfg_.max_pages_per_seq);
   }
@@ -474,13 +772,27 @@ class KvHost {
   void ReleasePages(int seq) {
     const std::int32_t* row = table_row(seq);
     // Pushed in table order, so the most recently added page is reused first.
-    for (int i = 0; i < n_pages_[static_cast<std::size_t>(seq)]; ++i) {
-      owner_[static_cast<std::size_t>(row[i])] = -1;
-      free_pages_.push_back(row[i]);
-    }
+    for (int i = 0; i < n_pages_[static_cast<std::size_t>(seq)]; ++i) Unref(row[i]);
     n_pages_[static_cast<std::size_t>(seq)] = 0;
+    ++table_epoch_;
+  }
+  void Unref(std::int32_t page) {
+    if (--refs_[static_cast<std::size_t>(page)] == 0) free_pages_.push_back(page);
+  }
+  // A live sequence that keeps `seq` from having page p to itself; -1: the page is free or only seq's.
+  int OtherHolder(std::int32_t p, int seq) const {
+    const int refs = refs_[static_cast<std::size_t>(p)];
+    if (refs == 0 || (refs == 1 && std::find(table_row(seq), table_row(seq) + n_pages(seq), p) != table_row(seq) + n_pages(seq)))
+      return -1;
+    for (int s = 0; s < cfg_.max_seqs; ++s) {
+      if (s == seq || !live(s)) continue;
+      for (int i = 0; i < n_pages(s); ++i)
+        if (table_row(s)[i] == p) return s;
+    }
+    return -1;
   }
   void MarkDirty(int seq, int lo, int hi) {
+    ++table_epoch_;
     const std::size_t i = static_cast<std::size_t>(seq);
     if (dirty_hi_[i] == dirty_lo_[i]) {
       dirty_lo_[i] = lo, dirty_hi_[i] = hi;
@@ -496,13 +808,16 @@ class KvHost {
   std::vector<char> live_;
   std::vector<std::int64_t> len_;
   std::vector<int> dirty_lo_, dirty_hi_, dirty_list_;
-  std::vector<int> owner_;
+  std::vector<int> refs_;       // sequences whose table names the page
+  std::vector<char> evicted_;   // per sequence: keys were evicted, slots are not positions
+  std::int64_t table_epoch_ = 0;   // counts table changes: what a cached prefix grouping depends on
   std::vector<std::int32_t> free_pages_;
   std::vector<int> free_seqs_;
   std::vector<std::pair<int, std::int64_t>> scratch_len_;
   std::vector<std::int64_t> key_scratch_, plan_key_;
   std::vector<DecodeUnit> units_;
   std::vector<CombineItem> items_;
+  SharedPlan shared_;           // cached plan of attend_decode_shared
   std::vector<int> open_cur_;   // kv8a16: current open-tile buffer per (sequence, layer)
   std::vector<int> bounds_;     // PlanDecode: page boundaries of one sequence's units
 };

@@ -1,0 +1,139 @@
+// Rotary positions for head rows of 256 dims: any even rotated part, half or interleaved pairs, scaled frequencies,
+// optionally behind the head RMS norm, at positions that are device-resident data.
+//
+// Pair p < R / 2 of a row at position n is turned by n f_p:  (a, b) -> (a c - b s, a s + b c), c + i s = m e^(i n f_p), with
+// a, b at dims (p, p + R / 2) or (2p, 2p + 1) and m the scaling's magnitude. The host evaluates e^(i n f_p) in double
+// precision for n = 0 .. 1023 and for the multiples of 1024 (times m) and rounds each once to fp32; the kernel multiplies
+// the two, e^(i n f) = e^(i 1024 (n / 1024) f) e^(i (n % 1024) f): two roundings more than a full table (a relative 1e-7)
+// for a thousandth of its size, so that the angles of a million positions stay in cache. HBM-bound: every row is read and
+// written once.
+//
+// One warp per token and a few of its heads (the angles stay in registers), lane l holding dims 8 l .. 8 l + 7. With
+// R / 2 a multiple of 8 the other half of a pair is the same register of another lane (a shuffle); otherwise the row
+// goes through shared memory. Interleaved pairs never leave their lane.
+#include <cuda_fp16.h>
+
+#include "kernels.cuh"
+#include "ptx.cuh"
+
+namespace yahkv {
+namespace {
+
+constexpr int kRopeRowWarps = 8;
+
+template <bool kF32>
+__device__ __forceinline__ void LoadRow8(const void* base, std::size_t at, float (&x)[8]) {
+  if constexpr (kF32) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+    const float4 a = p[0], b = p[1];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const __half*>(base) + at);
+    const __half2* h = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+}
+template <bool kF32>
+__device__ __forceinline__ void StoreRow8(void* base, std::size_t at, const float (&x)[8]) {
+  if constexpr (kF32) {
+    float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + at);
+    p[0] = make_float4(x[0], x[1], x[2], x[3]), p[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(static_cast<__half*>(base) + at) = *reinterpret_cast<const uint4*>(h);
+  }
+}
+
+template <bool kInF32, bool kOutF32>
+__global__ void __launch_bounds__(32 * kRopeRowWarps) RopeRowsKernel(const RopeRowsLaunch a) {
+  __shared__ float row_s[kRopeRowWarps][kHeadDim];
+  ChainedKernelEntry();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long task = static_cast<long long>(blockIdx.x) * kRopeRowWarps + warp;
+  const int token = static_cast<int>(task / a.head_groups), hg = static_cast<int>(task % a.head_groups);
+  if (token >= a.n_tokens) return;
+  const int half = a.rotary_dim / 2;
+  long long pos = a.positions[token];
+  if (pos < 0 || pos >= a.max_positions) {   // reported, and turned by the nearest angle there is
+    if (lane == 0) atomicExch(a.status, kStatusRopePosition);
+    pos = pos < 0 ? 0 : a.max_positions - 1;
+  }
+  // cos and sin of this lane's dims
+  float2 cs[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int d = 8 * lane + j;
+    cs[j] = make_float2(1.0F, 0.0F);
+    if (d < a.rotary_dim) {
+      const int p = a.interleaved ? d >> 1 : (d < half ? d : d - half);
+      const float2 x = __ldg(a.tab_hi + (pos >> kRopeLowBits) * half + p);
+      const float2 y = __ldg(a.tab_lo + (pos & ((1 << kRopeLowBits) - 1)) * half + p);
+      cs[j] = make_float2(fmaf(x.x, y.x, -(x.y * y.y)), fmaf(x.x, y.y, x.y * y.x));
+    }
+  }
+  float wt[8];
+  if (a.weight != nullptr) LoadRow8<true>(a.weight, 8 * lane, wt);
+  const int h1 = min((hg + 1) * a.heads_per_warp, a.n_heads);
+  for (int h = hg * a.heads_per_warp; h < h1; ++h) {
+    float x[8];
+    LoadRow8<kInF32>(a.x, static_cast<std::size_t>(token) * a.x_stride + static_cast<std::size_t>(h) * kHeadDim + 8 * lane, x);
+    if (a.weight != nullptr) {
+      float acc = 0.0F;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc = fmaf(x[j], x[j], acc);
+#pragma unroll
+      for (int m = 16; m >= 1; m >>= 1) acc += __shfl_xor_sync(0xFFFFFFFFU, acc, m);
+      const float inv = 1.0F / sqrtf(acc * (1.0F / kHeadDim) + a.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = x[j] * inv * wt[j];
+    }
+    float other[8];   // the pair's other half
+    if (a.interleaved) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) other[j] = x[j ^ 1];
+    } else if ((half & 7) == 0) {   // the same register of the lane half / 8 away
+      const int src = 8 * lane < half ? lane + half / 8 : lane - half / 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) other[j] = __shfl_sync(0xFFFFFFFFU, x[j], src & 31);
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) row_s[warp][8 * lane + j] = x[j];
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int d = 8 * lane + j;
+        other[j] = d < a.rotary_dim ? row_s[warp][d < half ? d + half : d - half] : 0.0F;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int d = 8 * lane + j;
+      const bool first = a.interleaved ? (j & 1) == 0 : d < half;
+      if (d < a.rotary_dim) x[j] = first ? fmaf(x[j], cs[j].x, -(other[j] * cs[j].y)) : fmaf(other[j], cs[j].y, x[j] * cs[j].x);
+    }
+    StoreRow8<kOutF32>(a.out, static_cast<std::size_t>(token) * a.out_stride + static_cast<std::size_t>(h) * kHeadDim + 8 * lane, x);
+  }
+}
+
+}  // namespace
+
+cudaError_t LaunchRopeRows(RopeRowsLaunch a, cudaStream_t stream) {
+  if (a.n_tokens <= 0 || a.n_heads <= 0) return cudaSuccess;
+  // few tokens: one head per warp, so that the call fills the device; many: the angles are worth keeping
+  a.heads_per_warp = static_cast<long long>(a.n_tokens) * a.n_heads < 148 * 64 ? 1 : 4;
+  a.head_groups = (a.n_heads + a.heads_per_warp - 1) / a.heads_per_warp;
+  const long long tasks = static_cast<long long>(a.n_tokens) * a.head_groups;
+  const unsigned grid = static_cast<unsigned>((tasks + kRopeRowWarps - 1) / kRopeRowWarps);
+  const auto kernel = a.x_f32 ? (a.out_f32 ? RopeRowsKernel<true, true> : RopeRowsKernel<true, false>)
+                              : (a.out_f32 ? RopeRowsKernel<false, true> : RopeRowsKernel<false, false>);
+  return LaunchChained(kernel, grid, 32 * kRopeRowWarps, 0, stream, a);
+}
+
+}  // namespace yahkv

@@ -1,0 +1,610 @@
+// Decode attention over a prefix that the rows of a batch share: the prefix pass, computed once for all of a group's
+// rows, and the combine that joins it with what every row has behind the prefix.
+//
+// With K = [K_p; K_b] (prefix; the row's own suffix) a row's attention is the join of two softmax partials,
+//   o = (2^(m_p - M) A_p + 2^(m_b - M) A_b) / (2^(m_p - M) l_p + 2^(m_b - M) l_b),   A = sum_i 2^(s_i - m) v_i,
+// and for the prefix the rows of a group of B sequences x 6 query heads are one [6 B x 256] x [256 x P] product per kv
+// head: every cache byte of the prefix is read once per call instead of B times. The suffixes run through the decode
+// kernels of the cache formats (one split-K unit list that starts behind the prefix).
+//
+// SharedPrefixKernel: one CTA pair (a cluster of two on the two SMs of a TPC, tcgen05 cta_group::2) per kv head, 256
+// group rows (128 per CTA) and a run of 64-token pages, one page = one key tile. The layout of the prefill kernel's
+// pair: Q in tensor memory as the A operand (group row r of the CTA = lane r), S = Q K^T (M 256, N 64, K 256) double-
+// buffered in tensor memory, two softmax warpgroups of one thread per row taking alternate tiles, P as fp16 through
+// shared memory, O += P V (M 256, N 256, K 64) in 256 tensor-memory columns, S two tiles ahead of P V. No causal mask: a
+// shared page is full and visible to every row. Every part leaves its unnormalised accumulator and (max, sum) per row.
+//
+// Operands. fp16 pages are the operands as they lie in the pool: a page of one kv head is 64 rows of 512 B, and each CTA
+// of the pair loads half of it (keys 32 rank .. + 31 of K, dims 128 rank .. + 127 of V) by TMA with 128-byte swizzle,
+// no multicast. q8_0 / q4_0 pages arrive as codes and block scales in a ring of raw stages (linear bulk copies; q8_0 V
+// as a TMA box) and four more warps turn each CTA's half into the same fp16 tiles: the code is an exact fp16 integer,
+// the product with the block's fp16 scale is rounded once to fp16, the values the prefill pass works on too. Rounding
+// K and V to 11 bits (the codes have 8 and the scales 11) costs about 2e-4 of an output's size each, as much as the fp16
+// rounding of the output itself; exact products would need a second MMA per operand.
+//
+// What bounds it: HBM as long as a group has few rows (a 64-key tile is 64 KB of fp16, 34 KB of q8_0, 18 KB of q4_0
+// pages per kv head, and takes the pair's tensor pipes 1,024 clocks whatever the number of rows), the tensor pipe from
+// about 42 rows per group on (a second pair re-reads the pages from L2).
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "kernels.cuh"
+#include "ptx.cuh"
+#include "umma.cuh"
+
+namespace yahkv {
+namespace {
+
+constexpr int kTileM = kPrefillTileRows;   // 128 group rows per CTA, 256 per pair
+constexpr int kTileN = kPageTokens;        // keys per tile: one page
+constexpr int kSoftmaxThreads = 256;       // warps 0-7: two warpgroups of one thread per row
+constexpr int kWarpTma = 8, kWarpMma = 9;
+constexpr int kDequantWarps = 4;           // warps 10-13, quantized pages only
+constexpr int kKHalfBytes = (kTileN / 2) * kHeadDim * 2;   // fp16 half tiles, 16 KB each
+constexpr int kVHalfBytes = kTileN * (kHeadDim / 2) * 2;
+constexpr int kKBlockBytes = (kTileN / 2) * 128;           // one [32 keys][64 dims] box
+constexpr int kVBlockBytes = kTileN * 128;                 // one [64 keys][64 dims] box
+constexpr int kPBytes = kTileM * kTileN * 2;
+constexpr int kTmemCols = 512, kColS = 0, kColO = 128, kColQ = 384;   // S 2 x 64, O 256, Q 128 columns
+constexpr float kLazyRescale = 8.0F;
+constexpr int kStatusAbort = 5;
+constexpr int kMaxStages = 5, kMaxRaw = 4;
+
+template <int kFmt>
+struct Shape {
+  static constexpr bool kQuant = kFmt != kFmtF16;
+  static constexpr int kStages = kQuant ? 3 : 5;   // fp16 half tiles in flight (S runs two tiles ahead: at least 3)
+  static constexpr int kThreads = kSoftmaxThreads + 64 + (kQuant ? 32 * kDequantWarps : 0);
+  // One raw stage of this CTA's half of a page: V codes (q8_0: a 64 x 128 B box of the half's dims; q4_0: the whole
+  // record, whose rows are 128 B), K codes of 32 keys, block scales of 32 K rows and of 64 V rows.
+  static constexpr int kRawStages = kQuant ? kMaxRaw : 0;
+  static constexpr int kRawV = 0, kRawVBytes = kTileN * 128;
+  static constexpr int kRawK = kRawVBytes, kRawKBytes = (kTileN / 2) * CodeBytes(kFmt);
+  static constexpr int kRawKs = kRawK + kRawKBytes, kRawKsBytes = (kTileN / 2) * kBlocksPerRow * 2;
+  static constexpr int kRawVs = kRawKs + kRawKsBytes, kRawVsBytes = kTileN * kBlocksPerRow * 2;
+  static constexpr int kRawTx = kRawVBytes + kRawKBytes + kRawKsBytes + kRawVsBytes;
+  static constexpr int kRawBytes = (kRawTx + 1023) / 1024 * 1024;
+  static constexpr int kSmemK = 0;
+  static constexpr int kSmemV = kSmemK + kStages * kKHalfBytes;
+  static constexpr int kSmemP = kSmemV + kStages * kVHalfBytes;
+  static constexpr int kSmemRaw = kSmemP + 2 * kPBytes;
+  static constexpr int kSmemBars = kSmemRaw + kRawStages * kRawBytes;
+  static constexpr int kBarBytes = 512;
+  static constexpr int kBytes = kSmemBars + kBarBytes + 3 * kTileM * 4;   // barriers, then the max / sum exchange
+  static_assert(kBytes <= 232448, "shared memory of one CTA");
+};
+
+// As in the prefill kernel: "leader" barriers are used in CTA 0 of the pair only, "both" are waited on by each CTA on
+// its own copy, "local" inside one CTA.
+struct SharedBars {
+  std::uint64_t q_full;                  // leader: softmax warps of both CTAs -> MMA
+  std::uint64_t kv_full[kMaxStages];     // leader: TMA (fp16 pages) or the dequantizing warps of both CTAs -> MMA
+  std::uint64_t kv_empty[kMaxStages];    // both: MMA -> the stage's writer
+  std::uint64_t raw_full[kMaxRaw];       // local: TMA -> dequantizing warps
+  std::uint64_t raw_empty[kMaxRaw];      // local: dequantizing warps -> TMA
+  std::uint64_t s_full[2];               // both
+  std::uint64_t s_free[2];               // leader
+  std::uint64_t p_full[2];               // leader
+  std::uint64_t m_posted[2];             // local
+  std::uint64_t pv_done[2];              // both
+  std::uint64_t o_done;                  // both
+  std::uint32_t tmem_base;
+  int abort_flag;
+};
+
+// Eight values of a row as fp16: exact integer codes times the block scale, one rounding.
+__device__ __forceinline__ uint4 ScaleCodes(const std::uint32_t (&h)[4], std::uint16_t scale) {
+  const __half2 d = __half2half2(__ushort_as_half(scale));
+  uint4 o;
+  std::uint32_t* w = &o.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), d);
+    w[i] = *reinterpret_cast<const std::uint32_t*>(&v);
+  }
+  return o;
+}
+// Four bytes u = code + 128 -> fp16 pairs (0, 1), (2, 3) of the codes: 0x6400 | u is 1024 + u.
+__device__ __forceinline__ void Bytes4ToHalf2(std::uint32_t u, std::uint32_t& h01, std::uint32_t& h23) {
+  const std::uint32_t a = __byte_perm(u, 0x64646464U, 0x4140), b = __byte_perm(u, 0x64646464U, 0x4342);
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));   // 1152
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+  h01 = *reinterpret_cast<const std::uint32_t*>(&x), h23 = *reinterpret_cast<const std::uint32_t*>(&y);
+}
+// Four bytes holding 0 .. 15 -> fp16 pairs of n - 8.
+__device__ __forceinline__ void Nibs4ToHalf2(std::uint32_t n, std::uint32_t& h01, std::uint32_t& h23) {
+  const std::uint32_t a = __byte_perm(n, 0x64646464U, 0x4140), b = __byte_perm(n, 0x64646464U, 0x4342);
+  const __half2 bias = __half2half2(__ushort_as_half(0x6408));   // 1032
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+  h01 = *reinterpret_cast<const std::uint32_t*>(&x), h23 = *reinterpret_cast<const std::uint32_t*>(&y);
+}
+// 16-byte chunk c8 (dims 8 c8 .. + 7) of a token row. row: the row's codes; kFlipped: q8_0 bytes are code + 128 already.
+template <int kFmt, bool kFlipped>
+__device__ __forceinline__ uint4 DequantChunk(uint2 codes, int c8, std::uint16_t scale) {
+  std::uint32_t h[4];
+  if constexpr (kFmt == kFmtQ8) {
+    const std::uint32_t flip = kFlipped ? 0U : kQ8FlipWord;
+    Bytes4ToHalf2(codes.x ^ flip, h[0], h[1]);
+    Bytes4ToHalf2(codes.y ^ flip, h[2], h[3]);
+  } else {   // elements 0-15 of a block are the low nibbles of its 16 bytes, 16-31 the high ones
+    const int sh = (c8 & 2) != 0 ? 4 : 0;
+    Nibs4ToHalf2((codes.x >> sh) & 0x0F0F0F0FU, h[0], h[1]);
+    Nibs4ToHalf2((codes.y >> sh) & 0x0F0F0F0FU, h[2], h[3]);
+  }
+  return ScaleCodes(h, scale);
+}
+
+template <int kFmt>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThreads, 1)
+    SharedPrefixKernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PoolView pool,
+                       int layer, const std::int32_t* __restrict__ tables, int table_stride,
+                       const PrefixTile* __restrict__ tiles, const std::int32_t* __restrict__ rows,
+                       const __half* __restrict__ q, float scale_log2, float* __restrict__ part_acc,
+                       float* __restrict__ part_ml, int* status) {
+  ChainedKernelEntry();
+  using S = Shape<kFmt>;
+  extern __shared__ __align__(1024) std::uint8_t smem[];
+  SharedBars* bars = reinterpret_cast<SharedBars*>(smem + S::kSmemBars);
+  static_assert(sizeof(SharedBars) <= S::kBarBytes, "the max / sum exchange follows the barriers");
+  volatile int* abort_flag = &bars->abort_flag;
+  const PrefixTile tile = tiles[blockIdx.x];
+  const std::uint32_t rank = ClusterCtaRank();   // 0 = leader: its MMA warp issues for the pair
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_tiles = tile.page_end - tile.page_begin;   // at least one, the same in both CTAs
+  const std::int32_t* table = tables + static_cast<std::size_t>(tile.seq) * table_stride + tile.page_begin;
+
+  if ((SmemAddr(smem) & 1023U) != 0) {   // the same in both CTAs: either both leave or neither does
+    if (threadIdx.x == 0) atomicExch(status, kStatusAbort);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    MbarInit(&bars->q_full, 2 * kSoftmaxThreads / 32);
+    for (int s = 0; s < S::kStages; ++s) {
+      MbarInit(&bars->kv_full[s], S::kQuant ? 2 * kDequantWarps : 1);
+      MbarInit(&bars->kv_empty[s], 1);
+    }
+    for (int s = 0; s < S::kRawStages; ++s) {
+      MbarInit(&bars->raw_full[s], 1);
+      MbarInit(&bars->raw_empty[s], kDequantWarps);
+    }
+    for (int g = 0; g < 2; ++g) {
+      MbarInit(&bars->s_full[g], 1);
+      MbarInit(&bars->s_free[g], 2 * kSoftmaxThreads / 64);
+      MbarInit(&bars->p_full[g], 2 * kSoftmaxThreads / 64);
+      MbarInit(&bars->m_posted[g], kSoftmaxThreads / 64);
+      MbarInit(&bars->pv_done[g], 1);
+    }
+    MbarInit(&bars->o_done, 1);
+    bars->abort_flag = 0;
+    FenceBarrierInit();
+  }
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SmemAddr(&bars->tmem_base)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  TcFenceBefore();
+  ClusterSync();
+  TcFenceAfter();
+  const std::uint32_t tmem = bars->tmem_base;
+
+  if (warp == kWarpTma) {
+    // ------------------------------ producer: this CTA's half of every page ------------------------------
+    const bool elected = ElectOne();
+    if (elected) {
+      PrefetchTensorMap(&kmap);
+      PrefetchTensorMap(&vmap);
+    }
+    bool ok = true;
+    constexpr int kRing = S::kQuant ? S::kRawStages : S::kStages;
+    int s = 0, issued = 0;
+    std::uint32_t ph = 1;
+    std::int32_t next_page = __ldg(table);
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const std::int32_t page = min(max(next_page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
+      if (j + 1 < n_tiles) next_page = __ldg(table + j + 1);
+      const std::size_t rec = (static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + tile.kvh;
+      const int y = static_cast<int>(rec * kPageTokens);
+      if (j >= kRing) ok = WaitOrAbort(S::kQuant ? &bars->raw_empty[s] : &bars->kv_empty[s], ph, abort_flag);
+      if (!ok) break;
+      if (elected) {
+        if constexpr (!S::kQuant) {
+          const std::uint32_t full = MapToCta(SmemAddr(&bars->kv_full[s]), 0);
+          if (rank == 0) MbarArriveExpectTx(&bars->kv_full[s], 2 * (kKHalfBytes + kVHalfBytes));
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb)   // keys 32 rank .. + 31, 64 dims per box
+            TmaLoad2DPair(smem + S::kSmemK + s * kKHalfBytes + kb * kKBlockBytes, &kmap, kb * 64,
+                          y + static_cast<int>(rank) * (kTileN / 2), full);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)   // all 64 keys, dims 128 rank + 64 kb .. + 63
+            TmaLoad2DPair(smem + S::kSmemV + s * kVHalfBytes + kb * kVBlockBytes, &vmap, (static_cast<int>(rank) * 2 + kb) * 64,
+                          y, full);
+        } else {
+          std::uint8_t* st = smem + S::kSmemRaw + s * S::kRawBytes;
+          const int k0 = static_cast<int>(rank) * (kTileN / 2);
+          MbarArriveExpectTx(&bars->raw_full[s], S::kRawTx);
+          BulkLoad(st + S::kRawK, pool.kcodes + rec * RecordCodeBytes(kFmt) + k0 * CodeBytes(kFmt), S::kRawKBytes, &bars->raw_full[s]);
+          if constexpr (kFmt == kFmtQ8)
+            TmaLoad2D(st + S::kRawV, &vmap, static_cast<int>(rank) * 128, y, &bars->raw_full[s]);
+          else
+            BulkLoad(st + S::kRawV, pool.vcodes + rec * RecordCodeBytes(kFmt), S::kRawVBytes, &bars->raw_full[s]);
+          BulkLoad(st + S::kRawKs, pool.kscales + (rec * kPageTokens + k0) * kBlocksPerRow, S::kRawKsBytes, &bars->raw_full[s]);
+          BulkLoad(st + S::kRawVs, pool.vscales + rec * (kPageTokens * kBlocksPerRow), S::kRawVsBytes, &bars->raw_full[s]);
+        }
+      }
+      ++issued;
+      if (++s == kRing) s = 0, ph ^= 1U;
+    }
+    // After a wait that gave up, the copies still in flight get one more bounded wait each (the last fill of a stage
+    // says which phase is outstanding), so that none lands in shared memory after the CTA has left it. fp16 pages: the
+    // bytes of both CTAs are counted on the leader's barriers, and both CTAs meet at the cluster barrier below.
+    if (*abort_flag != 0 && (S::kQuant || rank == 0)) {
+      for (int x = 0; x < kRing; ++x) {
+        const int fills = issued / kRing + (x < issued % kRing ? 1 : 0);
+        if (fills > 0) MbarWait(S::kQuant ? &bars->raw_full[x] : &bars->kv_full[x], static_cast<std::uint32_t>(fills - 1) & 1U, 20000000ULL);
+      }
+    }
+  } else if (warp == kWarpMma) {
+    // ------------------------------ MMA issuer (leader CTA only): S(0), S(1), then S(j + 2), P(j) V(j) ------------------------------
+    if (rank == 0) {
+      const bool elected = ElectOne();
+      constexpr std::uint32_t idesc_s = InstrDesc(2 * kTileM, kTileN, false);
+      constexpr std::uint32_t idesc_o = InstrDesc(2 * kTileM, kHeadDim, true);
+      const std::uint32_t k_lo0 = DescLo(SmemAddr(smem + S::kSmemK), 16);
+      const std::uint32_t v_lo0 = DescLo(SmemAddr(smem + S::kSmemV), kVBlockBytes);
+      const std::uint32_t p_lo0 = DescLo(SmemAddr(smem + S::kSmemP), 16);
+      const std::uint32_t q_col = tmem + kColQ, o_col = tmem + kColO;
+      int ks = 0, pv_s = 0;
+      std::uint32_t kph = 0;
+      auto issue_s = [&](int j) -> bool {
+        if (!WaitOrAbort<true>(&bars->kv_full[ks], kph, abort_flag)) return false;
+        if (j >= 2 && !WaitOrAbort<true>(&bars->s_free[j & 1], static_cast<std::uint32_t>((j - 2) >> 1) & 1U, abort_flag))
+          return false;
+        TcFenceAfter();
+        const std::uint32_t lo = k_lo0 + ks * (kKHalfBytes >> 4);
+        const std::uint32_t s_col = tmem + kColS + (j & 1) * kTileN;
+        if (elected) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            UmmaF16Ts2(s_col, q_col + i * 8, lo + (((i >> 2) * kKBlockBytes + (i & 3) * 32) >> 4), idesc_s, i > 0);
+          UmmaCommitPair(&bars->s_full[j & 1]);
+        }
+        if (++ks == S::kStages) ks = 0, kph ^= 1U;
+        return true;
+      };
+      auto issue_pv = [&](int j) -> bool {
+        if (!WaitOrAbort<true>(&bars->p_full[j & 1], static_cast<std::uint32_t>(j >> 1) & 1U, abort_flag)) return false;
+        TcFenceAfter();
+        const std::uint32_t plo = p_lo0 + (j & 1) * (kPBytes >> 4);
+        const std::uint32_t lo = v_lo0 + pv_s * (kVHalfBytes >> 4);
+        if (elected) {
+#pragma unroll
+          for (int k16 = 0; k16 < kTileN / 16; ++k16)
+            UmmaF16Ss2(o_col, plo + k16 * (32 >> 4), lo + k16 * ((16 * 128) >> 4), idesc_o, j > 0 || k16 > 0);
+          UmmaCommitPair(&bars->kv_empty[pv_s]);
+          UmmaCommitPair(&bars->pv_done[j & 1]);
+        }
+        if (++pv_s == S::kStages) pv_s = 0;
+        return true;
+      };
+      bool ok = WaitOrAbort<true>(&bars->q_full, 0, abort_flag);
+      if (ok && n_tiles > 0) ok = issue_s(0);
+      if (ok && n_tiles > 1) ok = issue_s(1);
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        if (j + 2 < n_tiles) ok = issue_s(j + 2);
+        if (ok) ok = issue_pv(j);
+      }
+      if (ok && elected) UmmaCommitPair(&bars->o_done);
+    }
+  } else if (S::kQuant && warp >= kWarpMma + 1) {
+    // ------------------------------ dequantizing warps: raw stage -> fp16 half tiles ------------------------------
+    if constexpr (S::kQuant) {
+      const int t = threadIdx.x - 32 * (kWarpMma + 1);   // 0 .. 127
+      int rs = 0, fs = 0;
+      std::uint32_t rph = 0, fph = 1;
+      for (int j = 0; j < n_tiles; ++j) {
+        bool ok = WaitOrAbort(&bars->raw_full[rs], rph, abort_flag);
+        if (ok && j >= S::kStages) ok = WaitOrAbort<true>(&bars->kv_empty[fs], fph, abort_flag);
+        ok = __all_sync(0xFFFFFFFFU, ok);
+        if (!ok) break;
+        const std::uint8_t* st = smem + S::kSmemRaw + rs * S::kRawBytes;
+        std::uint8_t* kd = smem + S::kSmemK + fs * kKHalfBytes;
+        std::uint8_t* vd = smem + S::kSmemV + fs * kVHalfBytes;
+        const std::uint16_t* ksc = reinterpret_cast<const std::uint16_t*>(st + S::kRawKs);
+        const std::uint16_t* vsc = reinterpret_cast<const std::uint16_t*>(st + S::kRawVs);
+        // a chunk = 8 dims of a row = 16 B of fp16; lanes run along the row
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {   // K: 32 keys x 32 chunks
+          const int c = t + i * (32 * kDequantWarps), key = c >> 5, c8 = c & 31;
+          uint2 w;
+          if constexpr (kFmt == kFmtQ8)
+            w = *reinterpret_cast<const uint2*>(st + S::kRawK + key * 256 + c8 * 8);
+          else   // block c8 / 4 is 16 bytes; elements 8 (c8 & 1) .. of its low or high nibbles
+            w = *reinterpret_cast<const uint2*>(st + S::kRawK + key * 128 + (c8 >> 2) * 16 + (c8 & 1) * 8);
+          *reinterpret_cast<uint4*>(kd + (c8 >> 3) * kKBlockBytes + key * 128 + (((c8 & 7) ^ (key & 7)) << 4)) =
+              DequantChunk<kFmt, false>(w, c8, ksc[key * kBlocksPerRow + (c8 >> 2)]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {   // V: 64 keys x 16 chunks of this CTA's 128 dims
+          const int c = t + i * (32 * kDequantWarps), key = c >> 4, cl = c & 15;
+          const int c8 = static_cast<int>(rank) * 16 + cl;
+          uint2 w;
+          if constexpr (kFmt == kFmtQ8)   // the TMA box is swizzled: 16-byte piece p of row key sits at p ^ (key % 8)
+            w = *reinterpret_cast<const uint2*>(st + S::kRawV + key * 128 + (((cl >> 1) ^ (key & 7)) << 4) + (cl & 1) * 8);
+          else
+            w = *reinterpret_cast<const uint2*>(st + S::kRawV + key * 128 + (c8 >> 2) * 16 + (c8 & 1) * 8);
+          *reinterpret_cast<uint4*>(vd + (cl >> 3) * kVBlockBytes + key * 128 + (((cl & 7) ^ (key & 7)) << 4)) =
+              DequantChunk<kFmt, true>(w, c8, vsc[key * kBlocksPerRow + (c8 >> 2)]);
+        }
+        FenceProxyAsync();   // the tensor core reads the tiles through the async proxy
+        __syncwarp();
+        if (lane == 0) {
+          MbarArrive(&bars->raw_empty[rs]);
+          MbarArriveCluster(MapToCta(SmemAddr(&bars->kv_full[fs]), 0));
+        }
+        if (++rs == S::kRawStages) rs = 0, rph ^= 1U;
+        if (++fs == S::kStages) fs = 0, fph ^= 1U;
+      }
+    }
+  } else {
+    // ------------------ softmax, correction, epilogue: two warpgroups of one thread per group row ------------------
+    const int r = threadIdx.x & (kTileM - 1);
+    const int hc = threadIdx.x >> 7;
+    const std::uint32_t lane_addr = tmem + (static_cast<std::uint32_t>((warp & 3) * 32) << 16);
+    const bool valid = r < tile.n_rows;
+    {   // this thread's 128 dims of the row's query -> tensor memory; rows past the group are zero
+      const int gr = tile.row0 + (valid ? r : 0);
+      const std::int32_t b = valid ? __ldg(rows + tile.row_list + gr / kGroup) : 0;
+      const uint4* src = reinterpret_cast<const uint4*>(
+          q + (static_cast<std::size_t>(b) * kQHeads + tile.kvh * kGroup + gr % kGroup) * kHeadDim + hc * (kHeadDim / 2));
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        std::uint32_t qr[32];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint4 v = valid ? __ldg(src + part * 8 + i) : make_uint4(0, 0, 0, 0);
+          qr[4 * i] = v.x, qr[4 * i + 1] = v.y, qr[4 * i + 2] = v.z, qr[4 * i + 3] = v.w;
+        }
+        TmemSt32(lane_addr + kColQ + hc * 64 + part * 32, qr);
+      }
+      TmemWaitSt();
+      TcFenceBefore();
+      __syncwarp();
+      if (lane == 0) MbarArriveCluster(MapToCta(SmemAddr(&bars->q_full), 0));
+    }
+    // Tiles alternate between the two warpgroups; the reference maximum travels from the group of tile j to the group
+    // of tile j + 1 through shared memory, each group keeps its own partial row sum.
+    float m_mine = -INFINITY, l_mine = 0.0F;
+    float* mref = reinterpret_cast<float*>(smem + S::kSmemBars + S::kBarBytes);   // [128 rows]
+    bool ok = true;
+    for (int j = hc; j < n_tiles; j += 2) {
+      ok = WaitOrAbort(&bars->s_full[hc], static_cast<std::uint32_t>(j >> 1) & 1U, abort_flag);
+      ok = __all_sync(0xFFFFFFFFU, ok);
+      if (!ok) break;
+      TcFenceAfter();
+      std::uint32_t sraw[64];
+      TmemLd32(lane_addr + kColS + hc * kTileN, *reinterpret_cast<std::uint32_t(*)[32]>(&sraw[0]));
+      TmemLd32(lane_addr + kColS + hc * kTileN + 32, *reinterpret_cast<std::uint32_t(*)[32]>(&sraw[32]));
+      TmemWaitLd();
+      TcFenceBefore();
+      __syncwarp();
+      if (lane == 0) MbarArriveCluster(MapToCta(SmemAddr(&bars->s_free[hc]), 0));
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < kTileN; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(sraw[c]));
+      const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;   // log2 units from here on
+      float m_ref = -INFINITY;
+      if (j >= 1) {
+        ok = WaitOrAbort(&bars->m_posted[hc ^ 1], static_cast<std::uint32_t>((j - 1) >> 1) & 1U, abort_flag);
+        ok = __all_sync(0xFFFFFFFFU, ok);
+        if (!ok) break;
+        m_ref = mref[r];
+      }
+      if (m_mine != m_ref) {
+        l_mine *= Exp2Fast(m_mine - m_ref);
+        m_mine = m_ref;
+      }
+      const bool need = tmax > m_ref + kLazyRescale;
+      if (__any_sync(0xFFFFFFFFU, need)) {
+        if (j >= 1) {   // O may be rescaled only once P(j-1) V(j-1) has completed
+          ok = WaitOrAbort(&bars->pv_done[hc ^ 1], static_cast<std::uint32_t>((j - 1) >> 1) & 1U, abort_flag);
+          ok = __all_sync(0xFFFFFFFFU, ok);
+          if (!ok) break;
+          TcFenceAfter();
+        }
+        const float m_new = need ? tmax : m_ref;
+        const float alpha = m_new == -INFINITY ? 1.0F : Exp2Fast(m_ref - m_new);
+        m_mine = m_ref = m_new;
+        l_mine *= alpha;
+        if (j >= 1) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < kHeadDim; c0 += 32) {
+            std::uint32_t o[32];
+            TmemLd32(lane_addr + kColO + c0, o);
+            TmemWaitLd();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+            TmemSt32(lane_addr + kColO + c0, o);
+          }
+          TmemWaitSt();
+        }
+      }
+      mref[r] = m_ref;
+      __syncwarp();
+      if (lane == 0) MbarArrive(&bars->m_posted[hc]);
+      const float neg_m = m_ref == -INFINITY ? 0.0F : -m_ref;
+      float ls[4] = {0.0F, 0.0F, 0.0F, 0.0F};
+      std::uint32_t pk[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float p0 = Exp2Fast(fmaf(__uint_as_float(sraw[2 * i]), scale_log2, neg_m));
+        const float p1 = Exp2Fast(fmaf(__uint_as_float(sraw[2 * i + 1]), scale_log2, neg_m));
+        ls[i & 3] += p0 + p1;
+        const __half2 h = __floats2half2_rn(p0, p1);
+        pk[i] = *reinterpret_cast<const std::uint32_t*>(&h);
+      }
+      l_mine += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      if (j >= 2) {
+        ok = WaitOrAbort(&bars->pv_done[hc], static_cast<std::uint32_t>((j - 2) >> 1) & 1U, abort_flag);
+        ok = __all_sync(0xFFFFFFFFU, ok);
+        if (!ok) break;
+      }
+      {
+        std::uint8_t* prow = smem + S::kSmemP + hc * kPBytes + (r >> 3) * 1024 + (r & 7) * 128;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+      }
+      FenceProxyAsync();
+      TcFenceBefore();
+      __syncwarp();
+      if (lane == 0) MbarArriveCluster(MapToCta(SmemAddr(&bars->p_full[hc]), 0));
+    }
+    // ---- epilogue: the part's unnormalised rows and their (max, sum) ----
+    if (ok && n_tiles > 0) {
+      ok = WaitOrAbort(&bars->o_done, 0, abort_flag);
+      ok = __all_sync(0xFFFFFFFFU, ok);
+    }
+    float* xsum = mref + kTileM;   // [2 groups][128 rows]
+    NamedBarrierSync(1, kSoftmaxThreads);
+    if (n_tiles > 0) {
+      const float m_fin = mref[r];
+      if (m_mine != m_fin) l_mine *= Exp2Fast(m_mine - m_fin);
+    }
+    xsum[hc * kTileM + r] = l_mine;
+    NamedBarrierSync(1, kSoftmaxThreads);
+    if (ok && n_tiles > 0) {
+      TcFenceAfter();
+      const std::size_t row = static_cast<std::size_t>(tile.part_row0) + r;
+      if (hc == 0 && valid) *reinterpret_cast<float2*>(part_ml + 2 * row) = make_float2(mref[r], l_mine + xsum[kTileM + r]);
+#pragma unroll 1
+      for (int c0 = 0; c0 < kHeadDim / 2; c0 += 32) {
+        std::uint32_t o[32];
+        TmemLd32(lane_addr + kColO + hc * (kHeadDim / 2) + c0, o);
+        TmemWaitLd();
+        if (valid) {
+          uint4* dst = reinterpret_cast<uint4*>(part_acc + row * kHeadDim + hc * (kHeadDim / 2) + c0);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) dst[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+        }
+      }
+    }
+  }
+  // ---- teardown: every role of both CTAs arrives here, also after an abort ----
+  TcFenceBefore();
+  ClusterSync();
+  if (threadIdx.x == 0 && bars->abort_flag != 0) atomicExch(status, kStatusAbort);
+  if (warp == kWarpMma) {
+    TcFenceAfter();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Joins the prefix parts and the suffix units of one (batch row, query head), prefix first, each in order:
+// out = (sum w_i A_i) / (sum w_i l_i) * sigmoid(gate), w_i = 2^(m_i - M). One CTA per head, thread = output dim.
+__global__ void __launch_bounds__(kHeadDim)
+    SharedCombineKernel(const PrefixItem* __restrict__ prefix_items, const float* __restrict__ prefix_acc,
+                        const float* __restrict__ prefix_ml, const CombineItem* __restrict__ items,
+                        const float* __restrict__ partial_acc, const float* __restrict__ partial_ml,
+                        const float* __restrict__ gate, void* out, int out_f32) {
+  __shared__ float w_s[kSharedMaxParts + kCombineMaxUnits], l_s[kSharedMaxParts + kCombineMaxUnits];
+  __shared__ float red_s[kHeadDim / 32];
+  __shared__ float inv_l;
+  ChainedKernelEntry();
+  const int b = blockIdx.x / kQHeads, hh = blockIdx.x % kQHeads;
+  const int kvh = hh / kGroup, j = hh % kGroup;
+  const PrefixItem pi = prefix_items[b * kKvHeads + kvh];
+  const CombineItem it = items[b * kKvHeads + kvh];
+  const int np = min(pi.n_parts, kSharedMaxParts), n = np + min(it.n_partials, kCombineMaxUnits);
+  if (n <= 0) return;   // a kv head outside the context's range
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float* acc_p = prefix_acc + (static_cast<std::size_t>(pi.first) + j) * kHeadDim + tid;
+  const std::size_t stride_p = static_cast<std::size_t>(pi.stride) * kHeadDim;
+  const float* acc_u = partial_acc + static_cast<std::size_t>(it.first_partial) * kPartialAccFloats + j * kHeadDim + tid;
+  // the first rows of the weighted sum are fetched before their weights are known
+  constexpr int kEarly = 24;
+  float early[kEarly];
+#pragma unroll
+  for (int i = 0; i < kEarly; ++i)
+    early[i] = i < np ? acc_p[i * stride_p] : i < n ? acc_u[static_cast<std::size_t>(i - np) * kPartialAccFloats] : 0.0F;
+  float mx = -INFINITY;
+  for (int i = tid; i < n; i += kHeadDim) {
+    const float2 ml = i < np ? *reinterpret_cast<const float2*>(prefix_ml + 2 * (pi.first + static_cast<std::size_t>(i) * pi.stride + j))
+                             : *reinterpret_cast<const float2*>(partial_ml + (static_cast<std::size_t>(it.first_partial) + (i - np)) * kPartialMlFloats + 2 * j);
+    w_s[i] = ml.x, l_s[i] = ml.y;
+    mx = fmaxf(mx, ml.x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFU, mx, o));
+  if (lane == 0) red_s[warp] = mx;
+  __syncthreads();
+  float M = red_s[0];
+#pragma unroll
+  for (int w = 1; w < kHeadDim / 32; ++w) M = fmaxf(M, red_s[w]);
+  for (int i = tid; i < n; i += kHeadDim) w_s[i] = w_s[i] == -INFINITY ? 0.0F : Exp2Fast(w_s[i] - M);   // the thread's own entries
+  __syncthreads();
+  if (tid == 0) {
+    float sum = 0.0F;
+    for (int i = 0; i < n; ++i) sum = fmaf(w_s[i], l_s[i], sum);
+    inv_l = 1.0F / sum;
+  }
+  float A = 0.0F;
+#pragma unroll
+  for (int i = 0; i < kEarly; ++i) A = fmaf(i < n ? w_s[i] : 0.0F, early[i], A);
+#pragma unroll 8
+  for (int i = kEarly; i < n; ++i)
+    A = fmaf(w_s[i], i < np ? acc_p[i * stride_p] : acc_u[static_cast<std::size_t>(i - np) * kPartialAccFloats], A);
+  __syncthreads();
+  float o = A * inv_l;
+  const std::size_t oi = (static_cast<std::size_t>(b) * kQHeads + hh) * kHeadDim + tid;
+  if (gate != nullptr) o *= 1.0F / (1.0F + expf(-gate[oi]));
+  if (out_f32)
+    static_cast<float*>(out)[oi] = o;
+  else
+    static_cast<__half*>(out)[oi] = __float2half_rn(o);
+}
+
+template <int kFmt>
+cudaError_t Configure(int* pairs) {
+  cudaError_t e = cudaFuncSetAttribute(SharedPrefixKernel<kFmt>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<kFmt>::kBytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2, 1, 1), cfg.blockDim = dim3(Shape<kFmt>::kThreads, 1, 1), cfg.dynamicSmemBytes = Shape<kFmt>::kBytes;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  return cudaOccupancyMaxActiveClusters(pairs, SharedPrefixKernel<kFmt>, &cfg);
+}
+
+template <int kFmt>
+cudaError_t Launch(const DecodeLaunch& a, const SharedLaunch& p, cudaStream_t stream) {
+  return LaunchChained(SharedPrefixKernel<kFmt>, p.n_tiles, Shape<kFmt>::kThreads, Shape<kFmt>::kBytes, stream, *p.kmap, *p.vmap,
+                       a.pool, a.layer, a.tables_dev, a.table_stride, p.tiles_dev, p.rows_dev,
+                       static_cast<const __half*>(a.q_dev), a.scale_log2, p.part_acc, p.part_ml, a.status_dev);
+}
+
+}  // namespace
+
+cudaError_t ConfigureSharedKernels(int fmt, int* max_active_pairs) {
+  return fmt == kFmtF16  ? Configure<kFmtF16>(max_active_pairs)
+         : fmt == kFmtQ8 ? Configure<kFmtQ8>(max_active_pairs)
+                         : Configure<kFmtQ4>(max_active_pairs);
+}
+
+cudaError_t LaunchSharedPrefix(const DecodeLaunch& a, const SharedLaunch& p, cudaStream_t stream) {
+  if (p.n_tiles <= 0) return cudaSuccess;
+  if ((p.n_tiles & 1) != 0) return cudaErrorInvalidValue;   // tiles come as pairs, one cluster each
+  if (a.pool.fmt == kFmtF16) return Launch<kFmtF16>(a, p, stream);
+  return a.pool.fmt == kFmtQ8 ? Launch<kFmtQ8>(a, p, stream) : Launch<kFmtQ4>(a, p, stream);
+}
+
+cudaError_t LaunchSharedCombine(const DecodeLaunch& a, const SharedLaunch& p, cudaStream_t stream) {
+  if (a.n_seqs <= 0) return cudaSuccess;
+  return LaunchChained(SharedCombineKernel, a.n_seqs * kQHeads, kHeadDim, 0, stream, p.prefix_items_dev, p.part_acc, p.part_ml,
+                       a.items_dev, a.partial_acc, a.partial_ml, a.gate_dev, a.out_dev, a.out_f32);
+}
+
+}  // namespace yahkv

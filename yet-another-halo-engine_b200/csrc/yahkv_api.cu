@@ -151,6 +151,25 @@ struct yahkv_ctx {
   std::vector<VTileWork> vwork_scratch;
   std::vector<std::int32_t> state_row_scratch;
   std::vector<DecodeUnit> unit_scratch;
+  // shared-prefix decode attention, allocated by the first call
+  struct Shared {
+    bool ready = false;
+    int n_pairs = 0;            // CTA pairs of the prefix kernel the device runs at once
+    int max_tiles = 0;
+    std::int64_t max_part_rows = 0;
+    PrefixTile* tiles_dev = nullptr;
+    std::int32_t* rows_dev = nullptr;
+    PrefixItem* prefix_items_dev = nullptr;
+    DecodeUnit* units_dev = nullptr;
+    CombineItem* items_dev = nullptr;
+    float *part_acc = nullptr, *part_ml = nullptr;
+    CUtensorMap k16map{}, v16map{};   // fp16 pages as [rows][256] fp16
+  } shared;
+  // eviction work lists, allocated by the first call
+  EvictSeq* evict_seqs_dev = nullptr;
+  std::int32_t* evict_pages_dev = nullptr;
+  std::vector<EvictSeq> evict_scratch;
+  std::vector<std::int32_t> evict_page_scratch;
 };
 
 namespace {
@@ -295,7 +314,9 @@ void FreeDevice(yahkv_ctx* ctx) {
                   ctx->tiles_dev,   ctx->status_dev,  ctx->pseqs_dev, ctx->k16_dev, ctx->v16_dev,
                   ctx->merges_dev, ctx->part_acc_dev, ctx->part_ml_dev,
                   ctx->rope_tab_dev, ctx->rope_pos_dev, ctx->open_tiles_dev, ctx->kmean_dev, ctx->state_rows_dev,
-                  ctx->vwork_dev,   ctx->rope_kv16_dev};
+                  ctx->vwork_dev,   ctx->rope_kv16_dev, ctx->shared.tiles_dev, ctx->shared.rows_dev,
+                  ctx->shared.prefix_items_dev, ctx->shared.units_dev, ctx->shared.items_dev, ctx->shared.part_acc,
+                  ctx->shared.part_ml, ctx->evict_seqs_dev, ctx->evict_pages_dev};
   for (void* p : ptrs)
     if (p != nullptr) cudaFree(p);
   for (cudaStream_t st : {ctx->h2d_stream, ctx->d2h_stream})
@@ -418,6 +439,8 @@ int CheckStatus(yahkv_ctx* ctx) {
   YAHKV_CUDA(ctx, cudaMemcpy(&st, ctx->status_dev, sizeof(int), cudaMemcpyDeviceToHost));
   if (st != 0) {
     cudaMemset(ctx->status_dev, 0, sizeof(int));
+    if (st == kStatusRopePosition)
+      return Fail(ctx, YAHKV_ERR_CUDA, "rope_rows: a position lies outside [0, max_positions); its rows are invalid");
     return Fail(ctx, YAHKV_ERR_CUDA, "a kernel gave up a bounded wait (status " + std::to_string(st) + "); results of the call are invalid");
   }
   return YAHKV_OK;
@@ -638,6 +661,12 @@ int yahkv_append(yahkv_ctx* ctx, int32_t layer, int32_t n_tokens, const int32_t*
   return YAHKV_OK;
 }
 
+// The raw-projection calls rotate at the slot of the key, which stops being its position once keys were evicted.
+static int FailEvicted(yahkv_ctx* ctx, const char* what, int seq) {
+  return Fail(ctx, YAHKV_ERR_ORDER, std::string(what) + ": keys of sequence " + std::to_string(seq) +
+                                        " were evicted, its slots are not positions; rotate with yahkv_rope_rows");
+}
+
 // cos / sin table of the fused RoPE: angle = pos / theta^(2 p / 64), p < 32, evaluated in double precision on the
 // host and rounded to f32 once (engine/gpu/loom/yah_fused_qk_rope_f32.loom:5, :32 for the formula and theta).
 static int EnsureRopeTable(yahkv_ctx* ctx) {
@@ -669,6 +698,8 @@ int yahkv_rope_append(yahkv_ctx* ctx, int32_t layer, int32_t n_tokens, const int
                        k_weight_dev == nullptr))   // q_out_dev may be null: the query side is then left to the caller
     return Fail(ctx, YAHKV_ERR_INVALID, "rope_append: null pointer");
   if (!(eps >= 0.0F)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_append: eps must be non-negative");
+  for (int i = 0; i < n_tokens && seq_ids != nullptr; ++i)
+    if (ctx->host.live(seq_ids[i]) && ctx->host.evicted(seq_ids[i])) return FailEvicted(ctx, "rope_append", seq_ids[i]);
   if (int r = EnsureRopeTable(ctx); r != YAHKV_OK) return r;   // before the plan: a failure here changes no state
   HostError e = ctx->host.PlanAppend(layer, n_tokens, seq_ids, positions, ctx->slot_scratch.data());
   if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
@@ -717,12 +748,42 @@ int yahkv_append_slots(yahkv_ctx* ctx, int32_t layer, int32_t n_tokens, const in
 
 static int AttendDecode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev, bool q_raw,
                         const float* q_weight_dev, float eps, const float* gate_dev, void* out_dev, int32_t out_dtype,
-                        int32_t n_splits, void* stream);
+                        int32_t n_splits, float* weights_dev, int64_t weights_stride, void* stream);
 
 int yahkv_attend_decode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
                         const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, void* stream) {
   return AttendDecode(ctx, layer, n_seqs, seq_ids, q_dev, false, nullptr, 0.0F, gate_dev, out_dev, out_dtype, n_splits,
-                      stream);
+                      nullptr, 0, stream);
+}
+
+// The accumulators hold one row of `stride` floats per (sequence id, kv head).
+static int CheckWeights(yahkv_ctx* ctx, const char* what, int32_t n_seqs, const int32_t* seq_ids, const float* weights_dev,
+                        int64_t stride) {
+  if (IsTileFmt(ctx->cfg.fmt))
+    return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (a key has no row of its own)");
+  if (n_seqs < 0 || (n_seqs > 0 && seq_ids == nullptr)) return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": bad sequence list");
+  if (n_seqs > ctx->cfg.max_seqs) return Fail(ctx, YAHKV_ERR_CAPACITY, std::string(what) + ": more rows than max_seqs");
+  if (n_seqs > 0 && weights_dev == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": null weights");
+  std::vector<char> seen(static_cast<std::size_t>(ctx->cfg.max_seqs), 0);
+  for (int i = 0; i < n_seqs; ++i) {
+    if (!ctx->host.live(seq_ids[i])) return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": not a live sequence: " + std::to_string(seq_ids[i]));
+    if (seen[static_cast<std::size_t>(seq_ids[i])]++)
+      return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": sequence " + std::to_string(seq_ids[i]) + " is listed twice");
+    for (int l = 0; l < ctx->cfg.n_layers; ++l)
+      if (ctx->host.len(seq_ids[i], l) > stride)
+        return Fail(ctx, YAHKV_ERR_CAPACITY, std::string(what) + ": sequence " + std::to_string(seq_ids[i]) + " holds more keys than a row of the weights");
+  }
+  return YAHKV_OK;
+}
+
+int yahkv_attend_decode_weights(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
+                                const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, float* weights_dev,
+                                int64_t weights_stride, void* stream) {
+  if (int r = RequireDevice(ctx, "attend_decode_weights"); r != YAHKV_OK) return r;
+  if (int r = CheckWeights(ctx, "attend_decode_weights", n_seqs, seq_ids, weights_dev, weights_stride); r != YAHKV_OK) return r;
+  if ((reinterpret_cast<std::uintptr_t>(q_dev) & 15) != 0) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_weights: q must be 16-byte aligned");
+  return AttendDecode(ctx, layer, n_seqs, seq_ids, q_dev, false, nullptr, 0.0F, gate_dev, out_dev, out_dtype, n_splits,
+                      weights_dev, weights_stride, stream);
 }
 
 int yahkv_attend_decode_qraw(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const float* q_raw_dev,
@@ -733,13 +794,15 @@ int yahkv_attend_decode_qraw(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, cons
   if (!(eps >= 0.0F)) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_qraw: eps must be non-negative");
   if ((reinterpret_cast<std::uintptr_t>(q_raw_dev) & 15) != 0 || (reinterpret_cast<std::uintptr_t>(q_weight_dev) & 15) != 0)
     return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_qraw: q and the norm weights must be 16-byte aligned");
+  for (int i = 0; i < n_seqs && seq_ids != nullptr; ++i)
+    if (ctx->host.live(seq_ids[i]) && ctx->host.evicted(seq_ids[i])) return FailEvicted(ctx, "attend_decode_qraw", seq_ids[i]);
   return AttendDecode(ctx, layer, n_seqs, seq_ids, q_raw_dev, true, q_weight_dev, eps, gate_dev, out_dev, out_dtype,
-                      n_splits, stream);
+                      n_splits, nullptr, 0, stream);
 }
 
 static int AttendDecode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev, bool q_raw,
                         const float* q_weight_dev, float eps, const float* gate_dev, void* out_dev, int32_t out_dtype,
-                        int32_t n_splits, void* stream) {
+                        int32_t n_splits, float* weights_dev, int64_t weights_stride, void* stream) {
   if (int r = RequireDevice(ctx, "attend_decode"); r != YAHKV_OK) return r;
   if (q_raw)
     if (int r = EnsureRopeTable(ctx); r != YAHKV_OK) return r;   // before the plan: a failure here changes no state
@@ -808,9 +871,305 @@ static int AttendDecode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int
     le = LaunchDecodeCombine(a, st);
     tc.End();
   }
+  if (le == cudaSuccess && weights_dev != nullptr) {
+    TimedLaunch tw(ctx, YAHKV_KERNEL_WEIGHTS, st);
+    le = LaunchAttnWeights(a, weights_dev, weights_stride, st);
+    tw.End();
+  }
   if (le != cudaSuccess) return FailCuda(ctx, "decode attention launch", le);
   guard.keep = true;
+  ctx->launches += weights_dev != nullptr ? 3 : 2;
+  return YAHKV_OK;
+}
+
+// ---- shared prefixes -------------------------------------------------------------------------------------------
+int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, void* stream) {
+  if (ctx == nullptr) return YAHKV_ERR_INVALID;
+  if (out == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "seq_fork: null out pointer");
+  if (IsTileFmt(ctx->cfg.fmt))
+    return Fail(ctx, YAHKV_ERR_INVALID, "seq_fork: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (the newest tile is no page)");
+  if (n_tokens > 0 && n_tokens % kPageTokens != 0)
+    if (int r = RequireDevice(ctx, "seq_fork"); r != YAHKV_OK) return r;   // the last page is copied
+  std::int32_t src = -1, dst = -1, made = -1;
+  HostError e = ctx->host.SeqFork(seq, n_tokens, &made, &src, &dst);
+  if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
+  if (src >= 0) {
+    if (cudaError_t le = LaunchCopyPage(ctx->pool, src, dst, StreamOf(ctx, stream)); le != cudaSuccess) {
+      ctx->host.SeqFree(made);
+      return FailCuda(ctx, "seq_fork: page copy", le);
+    }
+    ctx->launches += 1;
+  }
+  *out = made;
+  return YAHKV_OK;
+}
+
+// What shared-prefix attention needs beyond the context's own buffers; built by the first call that uses it.
+static int EnsureShared(yahkv_ctx* ctx) {
+  auto& sh = ctx->shared;
+  if (sh.ready) return YAHKV_OK;
+  const yahkv_config& c = ctx->cfg;
+  if (sh.n_pairs == 0) {
+    int pairs = 0;
+    YAHKV_CUDA(ctx, ConfigureSharedKernels(c.fmt, &pairs));
+    sh.n_pairs = std::max(std::min(pairs, ctx->n_sm_device / 2), 1);
+    // up to four waves of pairs, or one pair per (group of at least two rows, kv head, 256 rows)
+    const int combos = kKvHeads * (c.max_seqs / 2 + c.max_seqs * kGroup / (2 * kPrefillTileRows) + 1);
+    sh.max_tiles = 2 * std::max(4 * sh.n_pairs, combos);
+    sh.max_part_rows = std::max<std::int64_t>(static_cast<std::int64_t>(c.max_seqs) * kQHeads, 4LL * kPrefillTileRows * sh.n_pairs);
+  }
+  auto alloc = [&](auto** p, std::size_t count) { return *p != nullptr ? cudaSuccess : DevAlloc(ctx, p, count, false); };
+  const std::size_t ns = static_cast<std::size_t>(c.max_seqs);
+  YAHKV_CUDA(ctx, alloc(&sh.tiles_dev, static_cast<std::size_t>(sh.max_tiles)));
+  YAHKV_CUDA(ctx, alloc(&sh.rows_dev, ns));
+  YAHKV_CUDA(ctx, alloc(&sh.prefix_items_dev, ns * kKvHeads));
+  YAHKV_CUDA(ctx, alloc(&sh.units_dev, static_cast<std::size_t>(ctx->max_units)));
+  YAHKV_CUDA(ctx, alloc(&sh.items_dev, ns * kKvHeads));
+  YAHKV_CUDA(ctx, alloc(&sh.part_acc, static_cast<std::size_t>(sh.max_part_rows) * kHeadDim));
+  YAHKV_CUDA(ctx, alloc(&sh.part_ml, static_cast<std::size_t>(sh.max_part_rows) * 2));
+  if (c.fmt == YAHKV_FMT_F16) {
+    const std::uint64_t rows = static_cast<std::uint64_t>(c.n_layers) * c.num_pages * kKvHeads * kPageTokens;
+    if (!EncodeTensorMap2D(&sh.k16map, 2, ctx->pool.kcodes, kHeadDim, rows, 64, 32) ||
+        !EncodeTensorMap2D(&sh.v16map, 2, ctx->pool.vcodes, kHeadDim, rows, 64, 64))
+      return Fail(ctx, YAHKV_ERR_CUDA, "tensor map encode failed for the fp16 pools");
+  }
+  sh.ready = true;
+  return YAHKV_OK;
+}
+
+static SharedLaunch SharedArgs(yahkv_ctx* ctx) {
+  SharedLaunch p{};
+  p.kmap = ctx->cfg.fmt == YAHKV_FMT_F16 ? &ctx->shared.k16map : &ctx->kmap;
+  p.vmap = ctx->cfg.fmt == YAHKV_FMT_F16 ? &ctx->shared.v16map : &ctx->vmap;
+  p.part_acc = ctx->shared.part_acc, p.part_ml = ctx->shared.part_ml;
+  return p;
+}
+
+int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
+                               const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, void* stream) {
+  if (int r = RequireDevice(ctx, "attend_decode_shared"); r != YAHKV_OK) return r;
+  if (IsTileFmt(ctx->cfg.fmt))
+    return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (their sequences share no pages)");
+  if (out_dtype != YAHKV_OUT_F16 && out_dtype != YAHKV_OUT_F32) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: bad out_dtype");
+  if (n_seqs > 0 && (q_dev == nullptr || out_dev == nullptr)) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: null q or out pointer");
+  if ((reinterpret_cast<std::uintptr_t>(q_dev) & 15) != 0) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: q must be 16-byte aligned");
+  if (int r = EnsureShared(ctx); r != YAHKV_OK) return r;   // before the plan: a failure here changes no state
+  auto& sh = ctx->shared;
+  bool changed = false;
+  HostError e = ctx->host.PlanDecodeShared(layer, n_seqs, seq_ids, n_splits, ctx->cfg.max_splits, ctx->max_units, sh.n_pairs,
+                                           sh.max_part_rows, &changed);
+  if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
+  if (n_seqs == 0) return YAHKV_OK;
+  struct PlanGuard {   // as in AttendDecode: a plan that never reached the device is dropped
+    KvHost* host;
+    bool keep = false;
+    ~PlanGuard() {
+      if (!keep) host->InvalidateSharedPlan();
+    }
+  } guard{&ctx->host};
+  const KvHost::SharedPlan& plan = ctx->host.shared_plan();
+  if (static_cast<int>(plan.tiles.size()) > sh.max_tiles) return Fail(ctx, YAHKV_ERR_CAPACITY, "attend_decode_shared: too many prefix tiles");
+  cudaStream_t st = StreamOf(ctx, stream);
+  if (int r = FlushTables(ctx, st); r != YAHKV_OK) return r;
+  if (changed) {   // one staging buffer holds all lists so that they share a completion event
+    const std::pair<void*, std::pair<const void*, std::size_t>> lists[] = {
+        {sh.tiles_dev, {plan.tiles.data(), plan.tiles.size() * sizeof(PrefixTile)}},
+        {sh.rows_dev, {plan.rows.data(), plan.rows.size() * sizeof(std::int32_t)}},
+        {sh.prefix_items_dev, {plan.prefix_items.data(), plan.prefix_items.size() * sizeof(PrefixItem)}},
+        {sh.units_dev, {plan.units.data(), plan.units.size() * sizeof(DecodeUnit)}},
+        {sh.items_dev, {plan.items.data(), plan.items.size() * sizeof(CombineItem)}}};
+    std::size_t total = 0;
+    for (const auto& l : lists) total += l.second.second;
+    char* buf = nullptr;
+    YAHKV_CUDA(ctx, ctx->staging.Acquire(total, &buf));
+    for (const auto& l : lists) {
+      if (l.second.second == 0) continue;
+      std::memcpy(buf, l.second.first, l.second.second);
+      YAHKV_CUDA(ctx, cudaMemcpyAsync(l.first, buf, l.second.second, cudaMemcpyHostToDevice, st));
+      buf += l.second.second;
+    }
+    YAHKV_CUDA(ctx, ctx->staging.Release(st));
+  }
+  DecodeLaunch a{};
+  a.kmap = &ctx->kmap, a.vmap = &ctx->vmap, a.pool = ctx->pool, a.layer = layer;
+  a.tables_dev = ctx->tables_dev, a.table_stride = ctx->cfg.max_pages_per_seq;
+  a.units_dev = sh.units_dev, a.n_units = static_cast<int>(plan.units.size());
+  a.items_dev = sh.items_dev, a.n_seqs = n_seqs;
+  a.q_dev = q_dev, a.gate_dev = gate_dev, a.out_dev = out_dev, a.out_f32 = out_dtype == YAHKV_OUT_F32;
+  a.scale_log2 = ctx->scale_log2;
+  a.partial_acc = ctx->partial_acc, a.partial_ml = ctx->partial_ml, a.status_dev = ctx->status_dev;
+  SharedLaunch p = SharedArgs(ctx);
+  p.tiles_dev = sh.tiles_dev, p.n_tiles = static_cast<int>(plan.tiles.size()), p.rows_dev = sh.rows_dev;
+  p.prefix_items_dev = sh.prefix_items_dev;
+  TimedLaunch ts(ctx, YAHKV_KERNEL_SHARED_PREFIX, st);
+  cudaError_t le = LaunchSharedPrefix(a, p, st);
+  if (p.n_tiles > 0) ts.End();
+  if (le == cudaSuccess) {
+    TimedLaunch tp(ctx, YAHKV_KERNEL_DECODE_PART, st);
+    le = ctx->cfg.fmt == YAHKV_FMT_F16 ? LaunchF16DecodePart(a, st) : LaunchDecodePart(a, st);
+    if (a.n_units > 0) tp.End();
+  }
+  if (le == cudaSuccess) {
+    TimedLaunch tc(ctx, YAHKV_KERNEL_DECODE_COMBINE, st);
+    le = LaunchSharedCombine(a, p, st);
+    tc.End();
+  }
+  if (le != cudaSuccess) return FailCuda(ctx, "shared-prefix decode attention launch", le);
+  guard.keep = true;
+  ctx->launches += 1 + (p.n_tiles > 0 ? 1 : 0) + (a.n_units > 0 ? 1 : 0);
+  return YAHKV_OK;
+}
+
+// ---- eviction --------------------------------------------------------------------------------------------------
+int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t n_keep, int64_t n_sink, int64_t n_recent,
+                float* weights_dev, int64_t weights_stride, int64_t weights_layer_stride, int32_t* kept_dev, void* stream) {
+  if (int r = RequireDevice(ctx, "evict"); r != YAHKV_OK) return r;
+  if (int r = CheckWeights(ctx, "evict", n_seqs, seq_ids, weights_dev, weights_stride); r != YAHKV_OK) return r;
+  if (n_seqs > 0 && kept_dev == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "evict: null kept list");
+  if (n_keep < 1 || n_keep > static_cast<int64_t>(ctx->cfg.max_pages_per_seq) * kPageTokens || n_sink < 0 || n_recent < 0 ||
+      n_sink > n_keep || n_recent > n_keep - n_sink)
+    return Fail(ctx, YAHKV_ERR_INVALID, "evict: n_keep must be a slot count of at least 1, n_sink + n_recent at most n_keep");
+  if (ctx->cfg.n_layers > 1 && weights_layer_stride < static_cast<int64_t>(ctx->cfg.max_seqs) * kKvHeads * weights_stride)
+    return Fail(ctx, YAHKV_ERR_INVALID, "evict: the layers of the weights overlap (weights_layer_stride below max_seqs * 4 * weights_stride)");
+  bool any = false;
+  HostError e = ctx->host.PlanEvict(n_seqs, seq_ids, n_keep, &ctx->evict_scratch, &ctx->evict_page_scratch, &any);
+  if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
+  if (n_seqs == 0) return YAHKV_OK;
+  const yahkv_config& c = ctx->cfg;
+  if (ctx->evict_seqs_dev == nullptr) YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_seqs_dev, static_cast<std::size_t>(c.max_seqs), false));
+  if (ctx->evict_pages_dev == nullptr)
+    YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_pages_dev, static_cast<std::size_t>(c.max_seqs) * c.max_pages_per_seq, false));
+  cudaStream_t st = StreamOf(ctx, stream);
+  if (int r = FlushTables(ctx, st); r != YAHKV_OK) return r;   // the kernels read the tables as they are before the call
+  const std::size_t sb = ctx->evict_scratch.size() * sizeof(EvictSeq), pb = ctx->evict_page_scratch.size() * sizeof(std::int32_t);
+  char* buf = nullptr;
+  YAHKV_CUDA(ctx, ctx->staging.Acquire(sb + pb, &buf));
+  std::memcpy(buf, ctx->evict_scratch.data(), sb);
+  if (pb > 0) std::memcpy(buf + sb, ctx->evict_page_scratch.data(), pb);
+  YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->evict_seqs_dev, buf, sb, cudaMemcpyHostToDevice, st));
+  if (pb > 0) YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->evict_pages_dev, buf + sb, pb, cudaMemcpyHostToDevice, st));
+  YAHKV_CUDA(ctx, ctx->staging.Release(st));
+  EvictLaunch a{};
+  a.pool = ctx->pool, a.tables_dev = ctx->tables_dev, a.table_stride = c.max_pages_per_seq;
+  a.seqs_dev = ctx->evict_seqs_dev, a.n_seqs = n_seqs, a.dst_pages_dev = ctx->evict_pages_dev;
+  a.n_keep = static_cast<int>(n_keep), a.n_sink = static_cast<int>(n_sink), a.n_recent = static_cast<int>(n_recent);
+  a.weights = weights_dev, a.weights_stride = weights_stride, a.layer_stride = weights_layer_stride, a.kept = kept_dev;
+  TimedLaunch tl(ctx, YAHKV_KERNEL_EVICT, st);
+  YAHKV_CUDA(ctx, LaunchEvict(a, st));
+  tl.End();
   ctx->launches += 2;
+  if (any) ctx->host.CommitEvict(n_keep, ctx->evict_scratch, ctx->evict_page_scratch);
+  return YAHKV_OK;
+}
+
+// ---- rotary positions on given rows ----------------------------------------------------------------------------
+struct yahkv_rope {
+  yahkv_ctx* ctx = nullptr;
+  yahkv_rope_config cfg{};
+  float2 *hi = nullptr, *lo = nullptr;
+};
+
+int yahkv_rope_create(yahkv_ctx* ctx, const yahkv_rope_config* cfg, yahkv_rope** out) {
+  if (int r = RequireDevice(ctx, "rope_create"); r != YAHKV_OK) return r;
+  if (out == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: null out pointer");
+  *out = nullptr;
+  if (cfg == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: null config");
+  const yahkv_rope_config& c = *cfg;
+  if (c.layout != YAHKV_ROPE_HALF && c.layout != YAHKV_ROPE_INTERLEAVED) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: bad layout");
+  if (c.rotary_dim < 2 || c.rotary_dim > kHeadDim || c.rotary_dim % 2 != 0)
+    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: rotary_dim must be even, 2 .. 256");
+  if (!(c.theta > 1.0) || !std::isfinite(c.theta)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: theta must be a number above 1");
+  if (c.scaling < YAHKV_ROPE_SCALE_NONE || c.scaling > YAHKV_ROPE_SCALE_YARN) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: bad scaling");
+  if (c.scaling != YAHKV_ROPE_SCALE_NONE && (!(c.factor >= 1.0) || !std::isfinite(c.factor)))
+    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: factor must be a number of at least 1");
+  if (c.scaling == YAHKV_ROPE_SCALE_NTK && c.rotary_dim < 4)
+    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: NTK scaling needs a rotary_dim of at least 4");
+  if (c.scaling == YAHKV_ROPE_SCALE_YARN && (!(c.original_len > 0.0) || !(c.beta_slow >= 0.0) || !(c.beta_fast > c.beta_slow) ||
+                                             !std::isfinite(c.original_len) || !std::isfinite(c.beta_fast)))
+    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: YaRN scaling needs original_len > 0 and beta_fast > beta_slow >= 0");
+  if (!(c.magnitude >= 0.0) || !std::isfinite(c.magnitude)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: magnitude must not be negative");
+  if (c.max_positions < 1 || c.max_positions > (1LL << 31)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: max_positions must be 1 .. 2^31");
+  const int half = c.rotary_dim / 2;
+  const int low = 1 << kRopeLowBits;
+  const std::int64_t n_hi = (c.max_positions + low - 1) / low;
+  std::vector<double> freq(static_cast<std::size_t>(half));
+  double magnitude = c.magnitude > 0.0 ? c.magnitude : 1.0;
+  if (c.scaling == YAHKV_ROPE_SCALE_YARN && c.magnitude == 0.0) magnitude = 0.1 * std::log(c.factor) + 1.0;
+  const double theta = c.scaling == YAHKV_ROPE_SCALE_NTK ? c.theta * std::pow(c.factor, c.rotary_dim / (c.rotary_dim - 2.0)) : c.theta;
+  for (int p = 0; p < half; ++p) {
+    double f = std::pow(theta, -2.0 * p / c.rotary_dim);
+    if (c.scaling == YAHKV_ROPE_SCALE_LINEAR) f /= c.factor;
+    if (c.scaling == YAHKV_ROPE_SCALE_YARN) {   // by the turns a pair makes over the original length
+      const double turns = c.original_len * f / (2.0 * 3.14159265358979323846);
+      const double keep = std::min(std::max((turns - c.beta_slow) / (c.beta_fast - c.beta_slow), 0.0), 1.0);
+      f = (1.0 - keep) * f / c.factor + keep * f;
+    }
+    freq[static_cast<std::size_t>(p)] = f;
+  }
+  auto* r = new (std::nothrow) yahkv_rope();
+  if (r == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: out of host memory");
+  r->ctx = ctx, r->cfg = c;
+  std::vector<float2> tab;
+  try {
+    tab.resize(static_cast<std::size_t>(n_hi + low) * half);
+  } catch (const std::bad_alloc&) {
+    delete r;
+    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: out of host memory");
+  }
+  for (std::int64_t i = 0; i < n_hi + low; ++i)
+    for (int p = 0; p < half; ++p) {
+      const double n = static_cast<double>(i < n_hi ? i * low : i - n_hi);
+      const double m = i < n_hi ? magnitude : 1.0;
+      const double a = n * freq[static_cast<std::size_t>(p)];
+      tab[static_cast<std::size_t>(i) * half + p] = make_float2(static_cast<float>(m * std::cos(a)), static_cast<float>(m * std::sin(a)));
+    }
+  cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&r->hi), tab.size() * sizeof(float2));
+  if (e == cudaSuccess) e = cudaMemcpy(r->hi, tab.data(), tab.size() * sizeof(float2), cudaMemcpyHostToDevice);
+  if (e != cudaSuccess) {
+    if (r->hi != nullptr) cudaFree(r->hi);
+    delete r;
+    return FailCuda(ctx, "rope_create", e);
+  }
+  r->lo = r->hi + static_cast<std::size_t>(n_hi) * half;
+  *out = r;
+  return YAHKV_OK;
+}
+
+void yahkv_rope_destroy(yahkv_rope* r) {
+  if (r == nullptr) return;
+  cudaSetDevice(r->ctx->cfg.device);
+  cudaFree(r->hi);
+  delete r;
+}
+
+int yahkv_rope_rows(yahkv_rope* r, int32_t n_tokens, int32_t n_heads, const int64_t* positions_dev, const void* x_dev,
+                    int32_t x_dtype, int64_t x_stride, const float* weight_dev, float eps, void* out_dev, int32_t out_dtype,
+                    int64_t out_stride, void* stream) {
+  if (r == nullptr) return YAHKV_ERR_INVALID;
+  yahkv_ctx* ctx = r->ctx;
+  if (int rc = RequireDevice(ctx, "rope_rows"); rc != YAHKV_OK) return rc;
+  if (n_tokens < 0 || n_heads < 0) return Fail(ctx, YAHKV_ERR_INVALID, "rope_rows: negative token or head count");
+  if ((x_dtype != YAHKV_OUT_F16 && x_dtype != YAHKV_OUT_F32) || (out_dtype != YAHKV_OUT_F16 && out_dtype != YAHKV_OUT_F32))
+    return Fail(ctx, YAHKV_ERR_INVALID, "rope_rows: bad dtype");
+  if (n_tokens == 0 || n_heads == 0) return YAHKV_OK;
+  if (positions_dev == nullptr || x_dev == nullptr || out_dev == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_rows: null pointer");
+  if (weight_dev != nullptr && !(eps >= 0.0F)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_rows: eps must be non-negative");
+  const int64_t width = static_cast<int64_t>(n_heads) * kHeadDim;
+  if (x_stride < width || out_stride < width || x_stride % 8 != 0 || out_stride % 8 != 0)
+    return Fail(ctx, YAHKV_ERR_INVALID, "rope_rows: a token stride must be a multiple of 8 elements and hold all heads");
+  if (((reinterpret_cast<std::uintptr_t>(x_dev) | reinterpret_cast<std::uintptr_t>(out_dev) | reinterpret_cast<std::uintptr_t>(weight_dev)) & 15) != 0 ||
+      (reinterpret_cast<std::uintptr_t>(positions_dev) & 7) != 0)
+    return Fail(ctx, YAHKV_ERR_INVALID, "rope_rows: x, out and the norm weights must be 16-byte aligned, the positions 8-byte aligned");
+  RopeRowsLaunch a{};
+  a.x = x_dev, a.out = out_dev, a.positions = positions_dev, a.weight = weight_dev, a.tab_hi = r->hi, a.tab_lo = r->lo;
+  a.status = ctx->status_dev, a.max_positions = r->cfg.max_positions, a.x_stride = x_stride, a.out_stride = out_stride;
+  a.eps = eps, a.n_tokens = n_tokens, a.n_heads = n_heads, a.rotary_dim = r->cfg.rotary_dim;
+  a.interleaved = r->cfg.layout == YAHKV_ROPE_INTERLEAVED, a.x_f32 = x_dtype == YAHKV_OUT_F32, a.out_f32 = out_dtype == YAHKV_OUT_F32;
+  cudaStream_t st = StreamOf(ctx, stream);
+  TimedLaunch tl(ctx, YAHKV_KERNEL_ROPE, st);
+  YAHKV_CUDA(ctx, LaunchRopeRows(a, st));
+  tl.End();
+  ctx->launches += 1;
   return YAHKV_OK;
 }
 
@@ -833,6 +1192,8 @@ int yahkv_attend_prefill_qraw(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, con
   if (!(eps >= 0.0F)) return Fail(ctx, YAHKV_ERR_INVALID, "attend_prefill_qraw: eps must be non-negative");
   if ((reinterpret_cast<std::uintptr_t>(q_weight_dev) & 7) != 0)
     return Fail(ctx, YAHKV_ERR_INVALID, "attend_prefill_qraw: the norm weights must be 8-byte aligned");
+  for (int i = 0; i < n_seqs && seq_ids != nullptr; ++i)
+    if (ctx->host.live(seq_ids[i]) && ctx->host.evicted(seq_ids[i])) return FailEvicted(ctx, "attend_prefill_qraw", seq_ids[i]);
   return AttendPrefill(ctx, layer, n_seqs, seq_ids, chunk_lens, q_raw_dev, true, q_weight_dev, eps, gate_dev, out_dev,
                        out_dtype, stream);
 }
@@ -1187,6 +1548,9 @@ int yahkv_batch_prepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_c
   for (int i = 0; i < n; ++i) {
     if (!ctx->host.live(b->seqs[i]) || ctx->host.len(b->seqs[i], 0) != b->lens[i])
       return Fail(ctx, YAHKV_ERR_ORDER, "batch_prepare: a sequence of the batch was freed or changed outside the batch");
+    if (const std::int32_t p = ctx->host.SharedPageIn(b->seqs[i], b->lens[i], static_cast<std::int64_t>(b->lens[i]) + horizon_steps); p >= 0)
+      return Fail(ctx, YAHKV_ERR_INVALID, "batch_prepare: sequence " + std::to_string(b->seqs[i]) + " would append to page " +
+                                              std::to_string(p) + ", which another sequence shares");
     // Tile formats: the layers of a sequence share one plan per step, so they must agree on the open-tile buffer
     // (they do whenever every layer was appended with the same calls).
     for (int l = 1; IsTileFmt(ctx->cfg.fmt) && l < ctx->cfg.n_layers; ++l)
@@ -1329,6 +1693,8 @@ int yahkv_batch_decode_layer_raw(yahkv_batch* b, int32_t layer, const float* q_d
     if (int r = EnsureRopeTable(ctx); r != YAHKV_OK) return r;
   }
   const int n = static_cast<int>(b->seqs.size());
+  for (int i = 0; i < n; ++i)
+    if (ctx->host.live(b->seqs[i]) && ctx->host.evicted(b->seqs[i])) return FailEvicted(ctx, "batch_decode_layer_raw", b->seqs[i]);
   const bool tile_fmt = IsTileFmt(ctx->cfg.fmt);
   // K and V: norm + RoPE + append at the planned slots, positions = the device-resident lengths; no q output (the part
   // kernel's prologue does the query side)
@@ -1385,7 +1751,7 @@ int yahkv_batch_commit(yahkv_batch* b, int32_t steps) {
 // ---- snapshots: sequences with their pages, in logical page order, so a load may place them anywhere ----------
 namespace {
 struct SnapshotHeader {
-  char magic[8];            // "YAHKVSN1"
+  char magic[8];            // "YAHKVSN1"; "YAHKVSN2": behind every sequence's page count, whether keys of it were evicted
   std::int32_t fmt, n_layers, n_q_heads, n_kv_heads, head_dim, page_tokens, n_seqs, reserved;
 };
 struct FileCloser {
@@ -1406,7 +1772,9 @@ int yahkv_snapshot_save(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, 
   if (!f) return Fail(ctx, YAHKV_ERR_INVALID, std::string("snapshot_save: cannot open ") + path);
   const yahkv_config& c = ctx->cfg;
   SnapshotHeader h{};
-  std::memcpy(h.magic, "YAHKVSN1", 8);
+  bool marks = false;
+  for (int i = 0; i < n_seqs; ++i) marks = marks || ctx->host.evicted(seq_ids[i]);
+  std::memcpy(h.magic, marks ? "YAHKVSN2" : "YAHKVSN1", 8);
   h.fmt = c.fmt, h.n_layers = c.n_layers, h.n_q_heads = c.n_q_heads, h.n_kv_heads = c.n_kv_heads;
   h.head_dim = c.head_dim, h.page_tokens = c.page_tokens, h.n_seqs = n_seqs;
   bool ok = std::fwrite(&h, sizeof(h), 1, f.get()) == 1;
@@ -1420,6 +1788,8 @@ int yahkv_snapshot_save(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, 
     const int s = seq_ids[i];
     const std::int32_t np = ctx->host.n_pages(s);
     ok = std::fwrite(&np, 4, 1, f.get()) == 1;
+    const std::int32_t mark = ctx->host.evicted(s) ? 1 : 0;
+    if (ok && marks) ok = std::fwrite(&mark, 4, 1, f.get()) == 1;
     for (int l = 0; l < c.n_layers && ok; ++l) {
       const std::int64_t len = ctx->host.len(s, l);
       ok = std::fwrite(&len, 8, 1, f.get()) == 1;
@@ -1458,8 +1828,10 @@ int yahkv_snapshot_load(yahkv_ctx* ctx, const char* path, int32_t* seq_ids_out, 
   if (!f) return Fail(ctx, YAHKV_ERR_INVALID, std::string("snapshot_load: cannot open ") + path);
   const yahkv_config& c = ctx->cfg;
   SnapshotHeader h{};
-  if (std::fread(&h, sizeof(h), 1, f.get()) != 1 || std::memcmp(h.magic, "YAHKVSN1", 8) != 0)
+  if (std::fread(&h, sizeof(h), 1, f.get()) != 1 ||
+      (std::memcmp(h.magic, "YAHKVSN1", 8) != 0 && std::memcmp(h.magic, "YAHKVSN2", 8) != 0))
     return Fail(ctx, YAHKV_ERR_INVALID, "snapshot_load: not a yahkv snapshot");
+  const bool marks = h.magic[7] == '2';
   // Only into an identical set, as the reference's LoadState (engine/model/loom_prefill.hpp:973-1024).
   if (h.fmt != c.fmt || h.n_layers != c.n_layers || h.n_q_heads != c.n_q_heads || h.n_kv_heads != c.n_kv_heads ||
       h.head_dim != c.head_dim || h.page_tokens != c.page_tokens)
@@ -1479,12 +1851,15 @@ int yahkv_snapshot_load(yahkv_ctx* ctx, const char* path, int32_t* seq_ids_out, 
   for (int i = 0; i < h.n_seqs; ++i) {
     std::int32_t np = 0;
     if (std::fread(&np, 4, 1, f.get()) != 1 || np < 0) return undo(YAHKV_ERR_INVALID, "snapshot_load: truncated file");
+    std::int32_t mark = 0;
+    if (marks && std::fread(&mark, 4, 1, f.get()) != 1) return undo(YAHKV_ERR_INVALID, "snapshot_load: truncated file");
     std::vector<std::int64_t> lens(static_cast<std::size_t>(c.n_layers));
     if (std::fread(lens.data(), 8, lens.size(), f.get()) != lens.size()) return undo(YAHKV_ERR_INVALID, "snapshot_load: truncated file");
     std::int32_t s = -1;
     HostError e = ctx->host.SeqCreate(&s);
     if (e.code != YAHKV_OK) return undo(e.code, e.message);
     made.push_back(s);
+    if (mark != 0) ctx->host.SetEvicted(s);
     e = ctx->host.SeqReserve(s, static_cast<std::int64_t>(np) * kPageTokens);
     if (e.code != YAHKV_OK) return undo(e.code, e.message);
     for (int l = 0; l < c.n_layers; ++l) {

@@ -21,6 +21,9 @@ FMT_Q8_0, FMT_Q4_0, FMT_KV8A16, FMT_KV4A16, FMT_F16 = 0, 1, 2, 3, 4
 SIDE_K, SIDE_V = 0, 1
 OUT_F16, OUT_F32 = 0, 1
 KERNEL_APPEND, KERNEL_DECODE_PART, KERNEL_DECODE_COMBINE, KERNEL_PREFILL, KERNEL_PREFILL_DEQUANT = 0, 1, 2, 3, 4
+KERNEL_SHARED_PREFIX, KERNEL_WEIGHTS, KERNEL_EVICT, KERNEL_ROPE = 5, 6, 7, 8
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 OK = 0
 ERR_INVALID, ERR_NO_PAGES, ERR_CUDA, ERR_NO_DEVICE, ERR_ORDER, ERR_CAPACITY = -1, -2, -3, -4, -5, -6
 
@@ -100,6 +103,22 @@ class NoAllocArgs(ctypes.Structure):
     ]
 
 
+class RopeConfig(ctypes.Structure):
+    _fields_ = [
+        ("layout", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("scaling", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("theta", ctypes.c_double),
+        ("factor", ctypes.c_double),
+        ("original_len", ctypes.c_double),
+        ("beta_fast", ctypes.c_double),
+        ("beta_slow", ctypes.c_double),
+        ("magnitude", ctypes.c_double),
+        ("max_positions", ctypes.c_int64),
+    ]
+
+
 NOALLOC_MAX_SEQS, NOALLOC_MAX_UNITS = 256, 1024
 
 
@@ -144,6 +163,13 @@ SIGNATURES = {
     "yahkv_append_slots": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP]),
     "yahkv_attend_decode": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP, _I32, _I32, _VP]),
     "yahkv_attend_decode_qraw": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, ctypes.c_float, _VP, _VP, _I32, _I32, _VP]),
+    "yahkv_seq_fork": (_I32, [_VP, _I32, _I64, _PI32, _VP]),
+    "yahkv_attend_decode_shared": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP, _I32, _I32, _VP]),
+    "yahkv_attend_decode_weights": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP, _I32, _I32, _VP, _I64, _VP]),
+    "yahkv_evict": (_I32, [_VP, _I32, _VP, _I64, _I64, _I64, _VP, _I64, _I64, _VP, _VP]),
+    "yahkv_rope_create": (_I32, [_VP, _c.POINTER(RopeConfig), _c.POINTER(_VP)]),
+    "yahkv_rope_destroy": (None, [_VP]),
+    "yahkv_rope_rows": (_I32, [_VP, _I32, _I32, _VP, _VP, _I32, _I64, _VP, ctypes.c_float, _VP, _I32, _I64, _VP]),
     "yahkv_attend_prefill": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP, _VP, _I32, _VP]),
     "yahkv_attend_prefill_qraw": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP, ctypes.c_float, _VP, _VP, _I32, _VP]),
     "yahkv_decode_step_host": (_I32, [_VP, _I32, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _I32]),
@@ -288,6 +314,51 @@ class DecodeBatch:
         self.cache._check(lib.yahkv_batch_commit(self._h, steps))
 
 
+class Rope:
+    """Rotary positions for head rows of 256 dims (yahkv_rope): layout "half" or "interleaved", any even rotary_dim,
+    scaling "none", "linear", "ntk" or "yarn". Keeps its cache alive."""
+
+    def __init__(self, cache, *, rotary_dim=64, theta=1e7, layout="half", scaling="none", factor=1.0, original_len=0.0,
+                 beta_fast=32.0, beta_slow=1.0, magnitude=0.0, max_positions=1 << 20):
+        for name, value, known in (("layout", layout, ROPE_LAYOUTS), ("scaling", scaling, ROPE_SCALINGS)):
+            if value not in known:
+                raise ValueError(f"{name} must be one of {sorted(known)}, not {value!r}")
+        self.cache = cache
+        cfg = RopeConfig(ROPE_LAYOUTS[layout], rotary_dim, ROPE_SCALINGS[scaling], 0, theta, factor, original_len, beta_fast,
+                         beta_slow, magnitude, max_positions)
+        self._h = ctypes.c_void_p()
+        cache._check(lib.yahkv_rope_create(cache._h, ctypes.byref(cfg), ctypes.byref(self._h)))
+
+    def close(self):
+        if self._h:
+            lib.yahkv_rope_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def rows(self, x, positions, out, weight=None, eps=0.0, stream=None):
+        """x, out: CUDA tensors [tokens, heads, 256], fp16 or f32, heads and dims contiguous (tokens may be strided);
+        positions: CUDA int64 [tokens]; weight: CUDA f32 [256] or None."""
+        n, heads, dim = x.shape
+        if tuple(out.shape) != (n, heads, dim) or dim != HEAD_DIM or tuple(positions.shape) != (n,):
+            raise ValueError("rows: x and out are [tokens, heads, 256], positions [tokens]")
+        for t in (x, out):
+            if str(t.dtype) not in ("torch.float16", "torch.float32") or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+                raise ValueError("rows: x and out must be fp16 or f32 with contiguous heads")
+        if str(positions.dtype) != "torch.int64" or not positions.is_contiguous():
+            raise ValueError("rows: positions must be contiguous int64")
+        if weight is not None and (str(weight.dtype) != "torch.float32" or tuple(weight.shape) != (dim,) or not weight.is_contiguous()):
+            raise ValueError("rows: weight must be contiguous f32 [256]")
+        kind = [OUT_F32 if str(t.dtype) == "torch.float32" else OUT_F16 for t in (x, out)]
+        step = [t.stride(0) if n > 1 else heads * dim for t in (x, out)]
+        self.cache._check(lib.yahkv_rope_rows(self._h, n, heads, _ptr(positions), _ptr(x), kind[0], step[0], _ptr(weight),
+                                              float(eps), _ptr(out), kind[1], step[1], _ptr(stream)))
+
+
 class KvCache:
     """One context = one GPU's pools, block tables and allocator (yahkv_ctx)."""
 
@@ -322,6 +393,12 @@ class KvCache:
     def seq_create(self):
         s = ctypes.c_int32(-1)
         self._check(lib.yahkv_seq_create(self._h, ctypes.byref(s)))
+        return s.value
+
+    def seq_fork(self, seq, n_tokens, stream=None):
+        """A new sequence that shares the first n_tokens tokens of `seq` (whole pages by reference, the rest copied)."""
+        s = ctypes.c_int32(-1)
+        self._check(lib.yahkv_seq_fork(self._h, seq, n_tokens, ctypes.byref(s), _ptr(stream)))
         return s.value
 
     def seq_free(self, seq):
@@ -383,6 +460,41 @@ class KvCache:
         seq_ids = _i32(seq_ids)
         self._check(lib.yahkv_attend_decode_qraw(self._h, layer, len(seq_ids), _ptr(seq_ids), _ptr(q_raw), _ptr(q_weight),
                                                  float(eps), _ptr(gate), _ptr(out), out_dtype, n_splits, _ptr(stream)))
+
+    def attend_decode_shared(self, layer, seq_ids, q, out, gate=None, out_dtype=OUT_F16, n_splits=0, stream=None):
+        """attend_decode with every prefix that rows share (seq_fork) computed once for all of them."""
+        seq_ids = _i32(seq_ids)
+        self._check(lib.yahkv_attend_decode_shared(self._h, layer, len(seq_ids), _ptr(seq_ids), _ptr(q), _ptr(gate),
+                                                   _ptr(out), out_dtype, n_splits, _ptr(stream)))
+
+    def _weights(self, weights, dims):
+        """Row pitch of the accumulators of attend_decode_weights / evict."""
+        layer = weights[0] if weights.dim() == 4 else weights
+        if str(weights.dtype) != "torch.float32" or weights.dim() != dims or not layer.is_contiguous() or \
+                tuple(layer.shape[:2]) != (self.cfg.max_seqs, KV_HEADS) or \
+                (dims == 4 and weights.shape[0] != self.cfg.n_layers):
+            raise ValueError("weights must be f32 [%smax_seqs, 4, keys], every layer contiguous" % ("n_layers, " if dims == 4 else ""))
+        return layer.shape[2]
+
+    def attend_decode_weights(self, layer, seq_ids, q, out, weights, gate=None, out_dtype=OUT_F16, n_splits=0, stream=None):
+        """attend_decode that also adds every key's attention weight to weights (CUDA f32 [max_seqs, 4, keys], rows by
+        sequence id)."""
+        seq_ids = _i32(seq_ids)
+        self._check(lib.yahkv_attend_decode_weights(self._h, layer, len(seq_ids), _ptr(seq_ids), _ptr(q), _ptr(gate),
+                                                    _ptr(out), out_dtype, n_splits, _ptr(weights), self._weights(weights, 3),
+                                                    _ptr(stream)))
+
+    def evict(self, seq_ids, n_keep, weights, kept, n_sink=0, n_recent=0, stream=None):
+        """Cuts every sequence to n_keep keys by weights (CUDA f32 [n_layers, max_seqs, 4, keys]); kept: CUDA int32
+        [n_layers, n_seqs, 4, n_keep] receives the old slots."""
+        seq_ids = _i32(seq_ids)
+        if str(kept.dtype) != "torch.int32" or tuple(kept.shape) != (self.cfg.n_layers, len(seq_ids), KV_HEADS, n_keep) or \
+                not kept.is_contiguous():
+            raise ValueError("kept must be contiguous int32 [n_layers, n_seqs, 4, n_keep]")
+        stride = self._weights(weights, 4)
+        self._check(lib.yahkv_evict(self._h, len(seq_ids), _ptr(seq_ids), n_keep, n_sink, n_recent, _ptr(weights), stride,
+                                    weights.stride(0) if weights.shape[0] > 1 else self.cfg.max_seqs * KV_HEADS * stride,
+                                    _ptr(kept), _ptr(stream)))
 
     def attend_prefill(self, layer, seq_ids, chunk_lens, q, out, gate=None, out_dtype=OUT_F16, stream=None):
         seq_ids, chunk_lens = _i32(seq_ids), _i32(chunk_lens)
