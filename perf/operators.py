@@ -285,14 +285,33 @@ def _library():
     return yahkv
 
 
-def _fill(cache, layer, seqs, starts, lens, k16, v16):
-    """Appends rows [i, :lens[i]] of k16, v16 to sequence seqs[i] behind its first starts[i] tokens."""
+def _fill(cache, layer, seqs, starts, lens, k16, v16, k, v):
+    """Appends rows [i, :lens[i]] of k16, v16 to sequence seqs[i] behind its first starts[i] tokens. q8_0: the cache is
+    then given the very codes that k, v hold of them; a value that lies between two codes may be rounded to either side
+    by two quantizers whose block maxima are divided in different ways."""
     chunk = 8192
     for i, seq in enumerate(seqs):
         cache.seq_reserve(seq, starts[i] + lens[i])
         for a in range(0, lens[i], chunk):
             n = min(chunk, lens[i] - a)
             cache.append(layer, [seq] * n, list(range(starts[i] + a, starts[i] + a + n)), k16[i, a:a + n], v16[i, a:a + n])
+    if cache.fmt != _library().FMT_Q8_0:
+        return
+    for i, seq in enumerate(seqs):
+        first, shift = starts[i] // PAGE, starts[i] % PAGE
+        pages = cache.seq_table(seq)[first:(starts[i] + lens[i] + PAGE - 1) // PAGE]
+        for side, held in enumerate((k, v)):
+            as_pages = []
+            for t in held:
+                x = torch.zeros(len(pages) * PAGE, KVH, t.shape[-1], dtype=t.dtype, device="cuda")
+                x[shift:shift + lens[i]] = t[i, :lens[i]]
+                as_pages.append(x.unflatten(0, (-1, PAGE)).transpose(1, 2).contiguous().cpu().numpy())
+            codes, scales = as_pages[0].view("uint8"), as_pages[1].view("uint16")
+            for n, page in enumerate(pages):
+                if n == 0 and shift:
+                    old = cache.read_page(layer, side, int(page))
+                    codes[0, :, :shift], scales[0, :, :shift] = old[0][:, :shift], old[1][:, :shift]
+                cache.write_page(layer, side, int(page), codes[n], scales[n])
 
 
 def _handle(case, s):
@@ -315,9 +334,10 @@ def _handle(case, s):
         cache = yahkv.KvCache(num_pages=pages(case["prefix"]) + rows * (pages(max(lens)) + 2), fmt=fmt, max_seqs=rows + 1,
                               max_pages_per_seq=pages(longest) + 1)
         root = cache.seq_create()
-        _fill(cache, 0, [root], [0], [case["prefix"]], s["kp16"][None], s["vp16"][None])
+        _fill(cache, 0, [root], [0], [case["prefix"]], s["kp16"][None], s["vp16"][None],
+              [t[None] for t in s["kp"]], [t[None] for t in s["vp"]])
         s["seqs"] = [cache.seq_fork(root, case["prefix"]) for _ in range(rows)]
-        _fill(cache, 0, s["seqs"], [case["prefix"]] * rows, lens, s["ks16"], s["vs16"])
+        _fill(cache, 0, s["seqs"], [case["prefix"]] * rows, lens, s["ks16"], s["vs16"], s["ks"], s["vs"])
         s["out"] = torch.empty(rows, QH, DIM, device="cuda", dtype=torch.float16)
     else:
         layers = case.get("layers", 1)
@@ -326,7 +346,8 @@ def _handle(case, s):
                               num_pages=sum(pages(n) for n in lens) + (rows * (pages(case["keep"]) + 1) if extra else 0))
         s["seqs"] = [cache.seq_create() for _ in range(rows)]
         for layer in range(layers):
-            _fill(cache, layer, s["seqs"], [0] * rows, lens, s["k16"][layer], s["v16"][layer])
+            _fill(cache, layer, s["seqs"], [0] * rows, lens, s["k16"][layer], s["v16"][layer],
+                  [t[layer] for t in s["k"]], [t[layer] for t in s["v"]])
         s["out"] = torch.empty(layers, rows, QH, DIM, device="cuda", dtype=torch.float16)
         if extra:
             s["branch_w"] = torch.zeros(layers, 2 * rows, KVH, max(lens), device="cuda")
