@@ -40,7 +40,9 @@ constexpr int kTileM = kPrefillTileRows;   // 128 group rows per CTA, 256 per pa
 constexpr int kTileN = kPageTokens;        // keys per tile: one page
 constexpr int kSoftmaxThreads = 256;       // warps 0-7: two warpgroups of one thread per row
 constexpr int kWarpTma = 8, kWarpMma = 9;
-constexpr int kDequantWarps = 4;           // warps 10-13, quantized pages only
+constexpr int kDequantWarps = 4;           // per group; warps 10-17 are two groups, quantized pages only
+constexpr int kDequantGroups = 2;          // tiles alternate between them
+constexpr int kWarpDequant = 10;
 constexpr int kKHalfBytes = (kTileN / 2) * kHeadDim * 2;   // fp16 half tiles, 16 KB each
 constexpr int kVHalfBytes = kTileN * (kHeadDim / 2) * 2;
 constexpr int kKBlockBytes = (kTileN / 2) * 128;           // one [32 keys][64 dims] box
@@ -54,8 +56,12 @@ constexpr int kMaxStages = 5, kMaxRaw = 4;
 template <int kFmt>
 struct Shape {
   static constexpr bool kQuant = kFmt != kFmtF16;
-  static constexpr int kStages = kQuant ? 3 : 5;   // fp16 half tiles in flight (S runs two tiles ahead: at least 3)
-  static constexpr int kThreads = kSoftmaxThreads + 64 + (kQuant ? 32 * kDequantWarps : 0);
+  // fp16 half tiles of K and of V in flight, each with barriers of its own: S runs two tiles ahead of P V, so K is done
+  // with long before V is, and the stage of K(j + 3) must not wait for P(j) V(j) (one ring for both: the conversion of a
+  // tile and its products took turns, 3,500 clocks per q4_0 tile against 1,700 with two)
+  static constexpr int kKStages = kQuant ? 3 : 5;
+  static constexpr int kVStages = kQuant ? 4 : 5;
+  static constexpr int kThreads = kQuant ? 32 * (kWarpDequant + kDequantWarps * kDequantGroups) : kSoftmaxThreads + 64;
   // One raw stage of this CTA's half of a page: V codes (q8_0: a 64 x 128 B box of the half's dims; q4_0: the whole
   // record, whose rows are 128 B), K codes of 32 keys, block scales of 32 K rows and of 64 V rows.
   static constexpr int kRawStages = kQuant ? kMaxRaw : 0;
@@ -66,8 +72,8 @@ struct Shape {
   static constexpr int kRawTx = kRawVBytes + kRawKBytes + kRawKsBytes + kRawVsBytes;
   static constexpr int kRawBytes = (kRawTx + 1023) / 1024 * 1024;
   static constexpr int kSmemK = 0;
-  static constexpr int kSmemV = kSmemK + kStages * kKHalfBytes;
-  static constexpr int kSmemP = kSmemV + kStages * kVHalfBytes;
+  static constexpr int kSmemV = kSmemK + kKStages * kKHalfBytes;
+  static constexpr int kSmemP = kSmemV + kVStages * kVHalfBytes;
   static constexpr int kSmemRaw = kSmemP + 2 * kPBytes;
   static constexpr int kSmemBars = kSmemRaw + kRawStages * kRawBytes;
   static constexpr int kBarBytes = 512;
@@ -79,8 +85,10 @@ struct Shape {
 // its own copy, "local" inside one CTA.
 struct SharedBars {
   std::uint64_t q_full;                  // leader: softmax warps of both CTAs -> MMA
-  std::uint64_t kv_full[kMaxStages];     // leader: TMA (fp16 pages) or the dequantizing warps of both CTAs -> MMA
-  std::uint64_t kv_empty[kMaxStages];    // both: MMA -> the stage's writer
+  std::uint64_t k_full[kMaxStages];      // leader: TMA (fp16 pages) or the dequantizing warps of both CTAs -> MMA
+  std::uint64_t v_full[kMaxStages];
+  std::uint64_t k_empty[kMaxStages];     // both: MMA -> the stage's writer: S(j) is complete
+  std::uint64_t v_empty[kMaxStages];     // both: P(j) V(j) is complete
   std::uint64_t raw_full[kMaxRaw];       // local: TMA -> dequantizing warps
   std::uint64_t raw_empty[kMaxRaw];      // local: dequantizing warps -> TMA
   std::uint64_t s_full[2];               // both
@@ -160,9 +168,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
   }
   if (threadIdx.x == 0) {
     MbarInit(&bars->q_full, 2 * kSoftmaxThreads / 32);
-    for (int s = 0; s < S::kStages; ++s) {
-      MbarInit(&bars->kv_full[s], S::kQuant ? 2 * kDequantWarps : 1);
-      MbarInit(&bars->kv_empty[s], 1);
+    for (int s = 0; s < S::kKStages; ++s) {
+      MbarInit(&bars->k_full[s], S::kQuant ? 2 * kDequantWarps : 1);
+      MbarInit(&bars->k_empty[s], 1);
+    }
+    for (int s = 0; s < S::kVStages; ++s) {
+      MbarInit(&bars->v_full[s], S::kQuant ? 2 * kDequantWarps : 1);
+      MbarInit(&bars->v_empty[s], 1);
     }
     for (int s = 0; s < S::kRawStages; ++s) {
       MbarInit(&bars->raw_full[s], 1);
@@ -198,8 +210,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
       PrefetchTensorMap(&vmap);
     }
     bool ok = true;
-    constexpr int kRing = S::kQuant ? S::kRawStages : S::kStages;
-    int s = 0, issued = 0;
+    constexpr int kRing = S::kQuant ? S::kRawStages : S::kKStages;
+    static_assert(S::kQuant || S::kKStages == S::kVStages, "one stage index for both");
+    int s = 0, issued = 0, issued_k = 0;
     std::uint32_t ph = 1;
     std::int32_t next_page = __ldg(table);
     for (int j = 0; j < n_tiles && ok; ++j) {
@@ -207,21 +220,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
       if (j + 1 < n_tiles) next_page = __ldg(table + j + 1);
       const std::size_t rec = (static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + tile.kvh;
       const int y = static_cast<int>(rec * kPageTokens);
-      if (j >= kRing) ok = WaitOrAbort(S::kQuant ? &bars->raw_empty[s] : &bars->kv_empty[s], ph, abort_flag);
+      if (j >= kRing) ok = WaitOrAbort(S::kQuant ? &bars->raw_empty[s] : &bars->k_empty[s], ph, abort_flag);
       if (!ok) break;
-      if (elected) {
-        if constexpr (!S::kQuant) {
-          const std::uint32_t full = MapToCta(SmemAddr(&bars->kv_full[s]), 0);
-          if (rank == 0) MbarArriveExpectTx(&bars->kv_full[s], 2 * (kKHalfBytes + kVHalfBytes));
+      if constexpr (!S::kQuant) {
+        if (elected) {
+          const std::uint32_t full = MapToCta(SmemAddr(&bars->k_full[s]), 0);
+          if (rank == 0) MbarArriveExpectTx(&bars->k_full[s], 2 * kKHalfBytes);
 #pragma unroll
           for (int kb = 0; kb < 4; ++kb)   // keys 32 rank .. + 31, 64 dims per box
             TmaLoad2DPair(smem + S::kSmemK + s * kKHalfBytes + kb * kKBlockBytes, &kmap, kb * 64,
                           y + static_cast<int>(rank) * (kTileN / 2), full);
+        }
+        issued_k = j + 1;
+        if (j >= kRing) ok = WaitOrAbort(&bars->v_empty[s], ph, abort_flag);
+        if (!ok) break;
+        if (elected) {
+          const std::uint32_t full = MapToCta(SmemAddr(&bars->v_full[s]), 0);
+          if (rank == 0) MbarArriveExpectTx(&bars->v_full[s], 2 * kVHalfBytes);
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)   // all 64 keys, dims 128 rank + 64 kb .. + 63
             TmaLoad2DPair(smem + S::kSmemV + s * kVHalfBytes + kb * kVBlockBytes, &vmap, (static_cast<int>(rank) * 2 + kb) * 64,
                           y, full);
-        } else {
+        }
+      } else {
+        if (elected) {
           std::uint8_t* st = smem + S::kSmemRaw + s * S::kRawBytes;
           const int k0 = static_cast<int>(rank) * (kTileN / 2);
           MbarArriveExpectTx(&bars->raw_full[s], S::kRawTx);
@@ -243,7 +265,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
     if (*abort_flag != 0 && (S::kQuant || rank == 0)) {
       for (int x = 0; x < kRing; ++x) {
         const int fills = issued / kRing + (x < issued % kRing ? 1 : 0);
-        if (fills > 0) MbarWait(S::kQuant ? &bars->raw_full[x] : &bars->kv_full[x], static_cast<std::uint32_t>(fills - 1) & 1U, 20000000ULL);
+        if (fills > 0) MbarWait(S::kQuant ? &bars->raw_full[x] : &bars->v_full[x], static_cast<std::uint32_t>(fills - 1) & 1U, 20000000ULL);
+        const int k_fills = issued_k / kRing + (x < issued_k % kRing ? 1 : 0);
+        if (!S::kQuant && k_fills > 0) MbarWait(&bars->k_full[x], static_cast<std::uint32_t>(k_fills - 1) & 1U, 20000000ULL);
       }
     }
   } else if (warp == kWarpMma) {
@@ -256,10 +280,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
       const std::uint32_t v_lo0 = DescLo(SmemAddr(smem + S::kSmemV), kVBlockBytes);
       const std::uint32_t p_lo0 = DescLo(SmemAddr(smem + S::kSmemP), 16);
       const std::uint32_t q_col = tmem + kColQ, o_col = tmem + kColO;
-      int ks = 0, pv_s = 0;
-      std::uint32_t kph = 0;
+      int ks = 0, vs = 0;
+      std::uint32_t kph = 0, vph = 0;
       auto issue_s = [&](int j) -> bool {
-        if (!WaitOrAbort<true>(&bars->kv_full[ks], kph, abort_flag)) return false;
+        if (!WaitOrAbort<true>(&bars->k_full[ks], kph, abort_flag)) return false;
         if (j >= 2 && !WaitOrAbort<true>(&bars->s_free[j & 1], static_cast<std::uint32_t>((j - 2) >> 1) & 1U, abort_flag))
           return false;
         TcFenceAfter();
@@ -270,23 +294,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
           for (int i = 0; i < 16; ++i)
             UmmaF16Ts2(s_col, q_col + i * 8, lo + (((i >> 2) * kKBlockBytes + (i & 3) * 32) >> 4), idesc_s, i > 0);
           UmmaCommitPair(&bars->s_full[j & 1]);
+          UmmaCommitPair(&bars->k_empty[ks]);
         }
-        if (++ks == S::kStages) ks = 0, kph ^= 1U;
+        if (++ks == S::kKStages) ks = 0, kph ^= 1U;
         return true;
       };
       auto issue_pv = [&](int j) -> bool {
+        if (!WaitOrAbort<true>(&bars->v_full[vs], vph, abort_flag)) return false;
         if (!WaitOrAbort<true>(&bars->p_full[j & 1], static_cast<std::uint32_t>(j >> 1) & 1U, abort_flag)) return false;
         TcFenceAfter();
         const std::uint32_t plo = p_lo0 + (j & 1) * (kPBytes >> 4);
-        const std::uint32_t lo = v_lo0 + pv_s * (kVHalfBytes >> 4);
+        const std::uint32_t lo = v_lo0 + vs * (kVHalfBytes >> 4);
         if (elected) {
 #pragma unroll
           for (int k16 = 0; k16 < kTileN / 16; ++k16)
             UmmaF16Ss2(o_col, plo + k16 * (32 >> 4), lo + k16 * ((16 * 128) >> 4), idesc_o, j > 0 || k16 > 0);
-          UmmaCommitPair(&bars->kv_empty[pv_s]);
+          UmmaCommitPair(&bars->v_empty[vs]);
           UmmaCommitPair(&bars->pv_done[j & 1]);
         }
-        if (++pv_s == S::kStages) pv_s = 0;
+        if (++vs == S::kVStages) vs = 0, vph ^= 1U;
         return true;
       };
       bool ok = WaitOrAbort<true>(&bars->q_full, 0, abort_flag);
@@ -298,57 +324,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
       }
       if (ok && elected) UmmaCommitPair(&bars->o_done);
     }
-  } else if (S::kQuant && warp >= kWarpMma + 1) {
+  } else if (S::kQuant && warp >= kWarpDequant) {
     // ------------------------------ dequantizing warps: raw stage -> fp16 half tiles ------------------------------
     if constexpr (S::kQuant) {
-      const int t = threadIdx.x - 32 * (kWarpMma + 1);   // 0 .. 127
-      int rs = 0, fs = 0;
-      std::uint32_t rph = 0, fph = 1;
-      for (int j = 0; j < n_tiles; ++j) {
-        bool ok = WaitOrAbort(&bars->raw_full[rs], rph, abort_flag);
-        if (ok && j >= S::kStages) ok = WaitOrAbort<true>(&bars->kv_empty[fs], fph, abort_flag);
+      const int group = (warp - kWarpDequant) / kDequantWarps;
+      const int t = threadIdx.x - 32 * (kWarpDequant + group * kDequantWarps);   // 0 .. 127
+      for (int j = group; j < n_tiles; j += kDequantGroups) {
+        const int rs = j % S::kRawStages, ks = j % S::kKStages, vs = j % S::kVStages;
+        bool ok = WaitOrAbort(&bars->raw_full[rs], static_cast<std::uint32_t>(j / S::kRawStages) & 1U, abort_flag);
+        if (ok && j >= S::kKStages)
+          ok = WaitOrAbort<true>(&bars->k_empty[ks], static_cast<std::uint32_t>(j / S::kKStages - 1) & 1U, abort_flag);
         ok = __all_sync(0xFFFFFFFFU, ok);
         if (!ok) break;
         const std::uint8_t* st = smem + S::kSmemRaw + rs * S::kRawBytes;
-        std::uint8_t* kd = smem + S::kSmemK + fs * kKHalfBytes;
-        std::uint8_t* vd = smem + S::kSmemV + fs * kVHalfBytes;
+        std::uint8_t* kd = smem + S::kSmemK + ks * kKHalfBytes;
+        std::uint8_t* vd = smem + S::kSmemV + vs * kVHalfBytes;
         const std::uint16_t* ksc = reinterpret_cast<const std::uint16_t*>(st + S::kRawKs);
         const std::uint16_t* vsc = reinterpret_cast<const std::uint16_t*>(st + S::kRawVs);
-        // a chunk = 8 dims of a row = 16 B of fp16; lanes run along the row
+        // A chunk = 8 dims of a row = 16 B of fp16; lanes run along the row. All loads of a side come before its stores:
+        // the compiler cannot tell that the raw stage and the tiles do not overlap, and took turns (2,500 clocks a tile).
+        uint2 w[8];
+        std::uint16_t sc[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {   // K: 32 keys x 32 chunks
           const int c = t + i * (32 * kDequantWarps), key = c >> 5, c8 = c & 31;
-          uint2 w;
           if constexpr (kFmt == kFmtQ8)
-            w = *reinterpret_cast<const uint2*>(st + S::kRawK + key * 256 + c8 * 8);
+            w[i] = *reinterpret_cast<const uint2*>(st + S::kRawK + key * 256 + c8 * 8);
           else   // block c8 / 4 is 16 bytes; elements 8 (c8 & 1) .. of its low or high nibbles
-            w = *reinterpret_cast<const uint2*>(st + S::kRawK + key * 128 + (c8 >> 2) * 16 + (c8 & 1) * 8);
-          *reinterpret_cast<uint4*>(kd + (c8 >> 3) * kKBlockBytes + key * 128 + (((c8 & 7) ^ (key & 7)) << 4)) =
-              DequantChunk<kFmt, false>(w, c8, ksc[key * kBlocksPerRow + (c8 >> 2)]);
+            w[i] = *reinterpret_cast<const uint2*>(st + S::kRawK + key * 128 + (c8 >> 2) * 16 + (c8 & 1) * 8);
+          sc[i] = ksc[key * kBlocksPerRow + (c8 >> 2)];
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {   // V: 64 keys x 16 chunks of this CTA's 128 dims
-          const int c = t + i * (32 * kDequantWarps), key = c >> 4, cl = c & 15;
-          const int c8 = static_cast<int>(rank) * 16 + cl;
-          uint2 w;
+        for (int i = 0; i < 8; ++i) {
+          const int c = t + i * (32 * kDequantWarps), key = c >> 5, c8 = c & 31;
+          *reinterpret_cast<uint4*>(kd + (c8 >> 3) * kKBlockBytes + key * 128 + (((c8 & 7) ^ (key & 7)) << 4)) =
+              DequantChunk<kFmt, false>(w[i], c8, sc[i]);
+        }
+        const int cl = t & 15, vc8 = static_cast<int>(rank) * 16 + cl;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {   // V: 64 keys x 16 chunks of this CTA's 128 dims; loaded before K's fence
+          const int c = t + i * (32 * kDequantWarps), key = c >> 4;
           if constexpr (kFmt == kFmtQ8)   // the TMA box is swizzled: 16-byte piece p of row key sits at p ^ (key % 8)
-            w = *reinterpret_cast<const uint2*>(st + S::kRawV + key * 128 + (((cl >> 1) ^ (key & 7)) << 4) + (cl & 1) * 8);
+            w[i] = *reinterpret_cast<const uint2*>(st + S::kRawV + key * 128 + (((cl >> 1) ^ (key & 7)) << 4) + (cl & 1) * 8);
           else
-            w = *reinterpret_cast<const uint2*>(st + S::kRawV + key * 128 + (c8 >> 2) * 16 + (c8 & 1) * 8);
-          *reinterpret_cast<uint4*>(vd + (cl >> 3) * kVBlockBytes + key * 128 + (((cl & 7) ^ (key & 7)) << 4)) =
-              DequantChunk<kFmt, true>(w, c8, vsc[key * kBlocksPerRow + (c8 >> 2)]);
+            w[i] = *reinterpret_cast<const uint2*>(st + S::kRawV + key * 128 + (vc8 >> 2) * 16 + (vc8 & 1) * 8);
+          sc[i] = vsc[key * kBlocksPerRow + (vc8 >> 2)];
         }
         FenceProxyAsync();   // the tensor core reads the tiles through the async proxy
         __syncwarp();
+        if (lane == 0) MbarArriveCluster(MapToCta(SmemAddr(&bars->k_full[ks]), 0));
+        if (j >= S::kVStages) ok = WaitOrAbort<true>(&bars->v_empty[vs], static_cast<std::uint32_t>(j / S::kVStages - 1) & 1U, abort_flag);
+        ok = __all_sync(0xFFFFFFFFU, ok);
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = t + i * (32 * kDequantWarps), key = c >> 4;
+          *reinterpret_cast<uint4*>(vd + (cl >> 3) * kVBlockBytes + key * 128 + (((cl & 7) ^ (key & 7)) << 4)) =
+              DequantChunk<kFmt, true>(w[i], vc8, sc[i]);
+        }
+        FenceProxyAsync();
+        __syncwarp();
         if (lane == 0) {
           MbarArrive(&bars->raw_empty[rs]);
-          MbarArriveCluster(MapToCta(SmemAddr(&bars->kv_full[fs]), 0));
+          MbarArriveCluster(MapToCta(SmemAddr(&bars->v_full[vs]), 0));
         }
-        if (++rs == S::kRawStages) rs = 0, rph ^= 1U;
-        if (++fs == S::kStages) fs = 0, fph ^= 1U;
       }
     }
-  } else {
+  } else if (warp < kWarpTma) {
     // ------------------ softmax, correction, epilogue: two warpgroups of one thread per group row ------------------
     const int r = threadIdx.x & (kTileM - 1);
     const int hc = threadIdx.x >> 7;
@@ -420,13 +462,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
         l_mine *= alpha;
         if (j >= 1) {
 #pragma unroll 1
-          for (int c0 = 0; c0 < kHeadDim; c0 += 32) {
-            std::uint32_t o[32];
-            TmemLd32(lane_addr + kColO + c0, o);
+          for (int c0 = 0; c0 < kHeadDim; c0 += 16) {   // 16 columns at a time: the 64 scores stay in registers
+            std::uint32_t o[16];
+            TmemLd16(lane_addr + kColO + c0, o);
             TmemWaitLd();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-            TmemSt32(lane_addr + kColO + c0, o);
+            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+            TmemSt16(lane_addr + kColO + c0, o);
           }
           TmemWaitSt();
         }
