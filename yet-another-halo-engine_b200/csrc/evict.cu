@@ -6,9 +6,9 @@
 // keep no scores) and is HBM-bound: half of the cache bytes plus 8 B per key and kv head. Scores are computed in fp32
 // from the fp16 query and the exact codes (f16 MMA on exact fp16 integers, the block scale applied in fp32), so a
 // weight is as exact as fp32 sums make it; the part kernels' 16-bit query planes would cost 2e-5 of a weight.
-// One warp takes 16 keys at a time; a lane's B operand is what it loads: dims 8t .. 8t + 7 of every 32-element block of
-// key g (q4_0: elements 4t .. and 16 + 4t ..), and A takes the query's dims in the same order. No atomics: each key is
-// added to by one lane of one CTA, so the result does not depend on the order of CTAs.
+// The shape of the decode kernels without their V side: one CTA per split-K unit, a ring of K pages filled by TMA
+// (no multicast), eight warps on two pages at a time, 16 keys of a page per warp, the last of a page's warps refills its
+// stage. No order-dependent sums: each key is added to once per call.
 //
 // EvictSelectKernel, one CTA per (layer, sequence, kv head): the n_keep keys to keep, ascending. The first n_sink and the
 // last n_recent are kept, of the rest the largest weights; ties go to the lowest index, NaN counts as less than
@@ -23,6 +23,7 @@
 
 #include <cmath>
 
+#include "decode_ring.cuh"
 #include "kernels.cuh"
 #include "ptx.cuh"
 
@@ -32,8 +33,30 @@ namespace {
 // ----------------------------------------------------------------------------------------------------------------
 // attention weights
 // ----------------------------------------------------------------------------------------------------------------
-constexpr int kWeightThreads = 256;
-constexpr int kWeightWarps = kWeightThreads / 32;
+constexpr int kKeyGroups = 4;                      // 16 keys of a page each
+constexpr int kPageSets = 2;                       // pages in work at a time: warp w takes those of parity w / 4
+constexpr int kWeightWarps = kKeyGroups * kPageSets;
+constexpr int kWeightThreads = kWeightWarps * 32;
+constexpr int kBoxBytes = kPageTokens * 128;       // one swizzled TMA box: 64 token rows x 128 B
+
+// Shared memory: ring of K boxes | ring of block scales | barriers, counters, abort flag. Two CTAs per SM in every format
+// (q8_0 6 x 17 KB, q4_0 8 x 9 KB, fp16 3 x 32 KB).
+template <int kFmt>
+struct WeightSmem {
+  static constexpr int kBoxes = CodeBytes(kFmt) / 128;
+  static constexpr int kStages = kFmt == kFmtF16 ? 3 : kFmt == kFmtQ8 ? 6 : 8;
+  static constexpr int kScaleBytes = RecordScaleBytes(kFmt, 0);
+  static constexpr int kTx = kBoxes * kBoxBytes + kScaleBytes;
+  static constexpr int kScaleOff = kStages * kBoxes * kBoxBytes;
+  static constexpr int kBarOff = kScaleOff + kStages * kScaleBytes;
+  static constexpr int kDoneOff = kBarOff + 8 * kStages;
+  static constexpr int kFillOff = kDoneOff + 4 * kStages;
+  static constexpr int kAbortOff = kFillOff + 4 * kStages;
+  static constexpr int kBytes = (kAbortOff + 4 + 127) / 128 * 128;
+  static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two CTAs per SM");
+  static_assert(kPageSets <= kStages, "a set never waits for a stage it holds itself");
+};
+constexpr int kStatusSmemMisaligned = 2;
 
 // Four bytes u -> fp16 pairs (0, 1), (2, 3) of u - bias (0x6400 | u is 1024 + u; bias_h = 1024 + bias).
 __device__ __forceinline__ void Bytes4(std::uint32_t u, __half2 bias_h, std::uint32_t& h01, std::uint32_t& h23) {
@@ -49,15 +72,61 @@ __device__ __forceinline__ float HalfOf(const uint4& v, int i) {   // fp16 numbe
 
 template <int kFmt>
 __global__ void __launch_bounds__(kWeightThreads, 2)
-    AttnWeightsKernel(PoolView pool, int layer, const std::int32_t* __restrict__ tables, int table_stride,
-                      const DecodeUnit* __restrict__ units, const CombineItem* __restrict__ items,
-                      const __half* __restrict__ q, float scale_log2, const float* __restrict__ partial_ml,
-                      float* __restrict__ weights, long long weights_stride) {
+    AttnWeightsKernel(const __grid_constant__ CUtensorMap kmap, PoolView pool, int layer,
+                      const std::int32_t* __restrict__ tables, int table_stride, const DecodeUnit* __restrict__ units,
+                      const CombineItem* __restrict__ items, const __half* __restrict__ q, float scale_log2,
+                      const float* __restrict__ partial_ml, float* __restrict__ weights, long long weights_stride, int* status) {
+  using L = WeightSmem<kFmt>;
+  extern __shared__ __align__(1024) std::uint8_t smem[];
   __shared__ float norm_s[8];   // M + log2 L per query head
   ChainedKernelEntry();
+  std::uint64_t* full_bar = reinterpret_cast<std::uint64_t*>(smem + L::kBarOff);
+  int* done_cnt = reinterpret_cast<int*>(smem + L::kDoneOff);
+  int* fill_cnt = reinterpret_cast<int*>(smem + L::kFillOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOff);
+  if ((SmemAddr(smem) & 1023U) != 0) {   // never seen; a misaligned swizzle would corrupt results
+    if (threadIdx.x == 0) atomicExch(status, kStatusSmemMisaligned);
+    return;
+  }
   const DecodeUnit u = units[blockIdx.x];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if (u.page_end <= u.page_begin) return;
+  const int kw = warp & (kKeyGroups - 1), par = warp / kKeyGroups;
+  const int n_pages = u.page_end - u.page_begin;
+  if (n_pages <= 0) return;
+  const std::int32_t* row = tables + static_cast<std::size_t>(u.seq) * table_stride + u.page_begin;
+
+  // Gather of one page's K into a ring stage; a whole converged warp calls it, one elected lane issues. Once a wait has
+  // given up nothing more is fetched.
+  auto issue = [&](int s, std::int32_t page) {
+    if (*abort_flag != 0) return;
+    page = min(max(page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
+    const std::size_t rec = (static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + u.kvh;
+    if (ElectOne()) {
+      fill_cnt[s] += 1;
+      MbarArriveExpectTx(&full_bar[s], L::kTx);
+#pragma unroll
+      for (int b = 0; b < L::kBoxes; ++b)
+        TmaLoad2D(smem + (s * L::kBoxes + b) * kBoxBytes, &kmap, b * 128, static_cast<int>(rec * kPageTokens), &full_bar[s]);
+      if constexpr (L::kScaleBytes > 0)
+        BulkLoad(smem + L::kScaleOff + s * L::kScaleBytes, pool.kscales + rec * (kPageTokens * kBlocksPerRow), L::kScaleBytes, &full_bar[s]);
+    }
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      PrefetchTensorMap(&kmap);
+      for (int s = 0; s < L::kStages; ++s) {
+        MbarInit(&full_bar[s], 1);
+        done_cnt[s] = 0;
+        fill_cnt[s] = 0;
+      }
+      *abort_flag = 0;
+      FenceBarrierInit();
+    }
+    __syncwarp();
+    for (int i = 0; i < L::kStages && i < n_pages; ++i) issue(i, __ldg(row + i));
+  }
+
+  // M + log2 L of the six heads from the partials of the decode call, warp h < 6 for head h
   if (warp < kGroup) {
     const CombineItem it = items[u.batch * kKvHeads + u.kvh];
     const float* ml = partial_ml + static_cast<std::size_t>(it.first_partial) * kPartialMlFloats + 2 * warp;
@@ -73,100 +142,101 @@ __global__ void __launch_bounds__(kWeightThreads, 2)
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFU, l, o);
     if (lane == 0) norm_s[warp] = m + log2f(l);
   }
-  // A operand: lane (g, t) holds head g's dims of block b in the order the lane's own B words have them
-  uint4 qa[kBlocksPerRow];
+  // A operand: head g's dims in the order in which ldmatrix hands over K. fp16: dims 16 s + 2t, + 1 and 16 s + 8 + 2t, + 1
+  // of step s. Codes: a 16-byte piece is 16 codes (q8_0) or a block's 32 nibbles (q4_0), lane t has its bytes 4t .. 4t + 3:
+  // elements 4t .. of a 32-element block and 16 + 4t ..
+  std::uint32_t qa[32];
+  {
+    const __half* src = q + (static_cast<std::size_t>(u.batch) * kQHeads + u.kvh * kGroup + min(g, kGroup - 1)) * kHeadDim;
 #pragma unroll
-  for (int b = 0; b < kBlocksPerRow; ++b) {
-    qa[b] = make_uint4(0, 0, 0, 0);
-    if (g < kGroup) {
-      const __half* src = q + (static_cast<std::size_t>(u.batch) * kQHeads + u.kvh * kGroup + g) * kHeadDim + 32 * b;
-      if constexpr (kFmt == kFmtQ4) {
-        const uint2 lo = __ldg(reinterpret_cast<const uint2*>(src + 4 * t)), hi = __ldg(reinterpret_cast<const uint2*>(src + 16 + 4 * t));
-        qa[b] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      } else {
-        qa[b] = __ldg(reinterpret_cast<const uint4*>(src + 8 * t));
-      }
+    for (int i = 0; i < 32; ++i) {
+      const int at = kFmt == kFmtF16 ? 8 * i + 2 * t : 32 * (i >> 2) + 16 * ((i >> 1) & 1) + 4 * t + 2 * (i & 1);
+      qa[i] = g < kGroup ? __ldg(reinterpret_cast<const std::uint32_t*>(src + at)) : 0U;
     }
   }
-  __syncthreads();
-  const float norm = g < kGroup ? norm_s[g] : INFINITY;
-  const std::int32_t* row = tables + static_cast<std::size_t>(u.seq) * table_stride;
+  __syncthreads();   // barriers initialised, norms visible
+  const float norm = g < kGroup ? norm_s[g] : INFINITY;   // the padding rows of the MMA weigh nothing
   float* w_out = weights + (static_cast<std::size_t>(u.seq) * kKvHeads + u.kvh) * static_cast<std::size_t>(weights_stride);
   const __half2 bias = __half2half2(__ushort_as_half(kFmt == kFmtQ8 ? 0x6480 : 0x6408));
+  // ldmatrix rows: matrices = (keys 0-7 | 8-15 of the group) x (16-byte pieces 2x | 2x + 1); piece p of row r sits at p ^ (r % 8)
+  const int lm_key = kw * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+  const std::uint32_t lm0 = lm_key * 128 + (((lane >> 4) ^ (lm_key & 7)) << 4);
 
-  // 16-key groups of the unit's pages, one warp each
-  const int n_groups = (u.page_end - u.page_begin) * (kPageTokens / 16);
-  for (int i = warp; i < n_groups; i += kWeightWarps) {
-    const int p = u.page_begin + (i >> 2);
-    const int key0 = p * kPageTokens + (i & 3) * 16;
-    if (key0 >= u.n_keys) break;
-    const std::int32_t page = min(max(__ldg(row + p), 0), pool.num_pages - 1);   // never trust a table entry
-    const std::size_t rec = (static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + u.kvh;
-    const std::uint8_t* codes = pool.kcodes + rec * RecordCodeBytes(kFmt) + ((i & 3) * 16 + g) * CodeBytes(kFmt);
-    float s[2][2] = {{0.0F, 0.0F}, {0.0F, 0.0F}};
+  bool alive = true;
+  for (int i = par; i < n_pages; i += kPageSets) {
+    const int s = i % L::kStages, gen = i / L::kStages;
+    std::int32_t refill_page = 0;
+    if (lane == 0 && i + L::kStages < n_pages) refill_page = __ldg(row + i + L::kStages);
+    alive = RingWait(alive, fill_cnt + s, &full_bar[s], gen, abort_flag);
+    const std::uint32_t k_base = SmemAddr(smem + s * L::kBoxes * kBoxBytes);
+    float sc[2][2] = {{0.0F, 0.0F}, {0.0F, 0.0F}};   // keys 8 kt + 2t + j of the group, head g
     if constexpr (kFmt == kFmtF16) {
       float acc[2][4] = {{0.0F, 0.0F, 0.0F, 0.0F}, {0.0F, 0.0F, 0.0F, 0.0F}};
-      uint4 w[2][kBlocksPerRow];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int x = 0; x < 16; ++x) {
+        std::uint32_t w[4];
+        LdMatrixX4(k_base + (x >> 2) * kBoxBytes + (lm0 ^ (static_cast<std::uint32_t>(x & 3) << 5)), w);
+        MmaF16(acc[0], qa[2 * x], 0U, qa[2 * x + 1], 0U, w[0], w[2]);
+        MmaF16(acc[1], qa[2 * x], 0U, qa[2 * x + 1], 0U, w[1], w[3]);
+      }
 #pragma unroll
-        for (int b = 0; b < kBlocksPerRow; ++b)
-          w[kt][b] = *reinterpret_cast<const uint4*>(codes + kt * 8 * CodeBytes(kFmt) + b * 64 + t * 16);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int b = 0; b < kBlocksPerRow; ++b) {
-          MmaF16(acc[kt], qa[b].x, 0U, qa[b].y, 0U, w[kt][b].x, w[kt][b].y);
-          MmaF16(acc[kt], qa[b].z, 0U, qa[b].w, 0U, w[kt][b].z, w[kt][b].w);
-        }
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) s[kt][0] = acc[kt][0], s[kt][1] = acc[kt][1];
+      for (int kt = 0; kt < 2; ++kt) sc[kt][0] = acc[kt][0], sc[kt][1] = acc[kt][1];
     } else {
-      const std::uint16_t* scales = pool.kscales + (rec * kPageTokens + (i & 3) * 16) * kBlocksPerRow;
-      uint4 d[2][2];   // the eight block scales of keys 8 kt + 2t + j
+      uint4 d[2][2];   // the eight block scales of this thread's keys
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) d[kt][j] = *reinterpret_cast<const uint4*>(scales + (kt * 8 + 2 * t + j) * kBlocksPerRow);
-      uint2 w[2][kBlocksPerRow];
+        for (int j = 0; j < 2; ++j)
+          d[kt][j] = *reinterpret_cast<const uint4*>(smem + L::kScaleOff + s * L::kScaleBytes + (kw * 16 + kt * 8 + 2 * t + j) * (kBlocksPerRow * 2));
+      // one block of 32 elements for eight keys: two k-steps into a fresh accumulator, then the keys' scales
+      auto block = [&](int b, int kt, std::uint32_t lo, std::uint32_t hi) {
+        float acc[4] = {0.0F, 0.0F, 0.0F, 0.0F};
+        std::uint32_t b0, b1;
+        Bytes4(lo, bias, b0, b1);
+        MmaF16(acc, qa[4 * b], 0U, qa[4 * b + 1], 0U, b0, b1);
+        Bytes4(hi, bias, b0, b1);
+        MmaF16(acc, qa[4 * b + 2], 0U, qa[4 * b + 3], 0U, b0, b1);
+        sc[kt][0] = fmaf(HalfOf(d[kt][0], b), acc[0], sc[kt][0]);
+        sc[kt][1] = fmaf(HalfOf(d[kt][1], b), acc[1], sc[kt][1]);
+      };
+      if constexpr (kFmt == kFmtQ8) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int b = 0; b < kBlocksPerRow; ++b) {
-          const std::uint8_t* src = codes + kt * 8 * CodeBytes(kFmt);
-          if constexpr (kFmt == kFmtQ8) {
-            const uint2 raw = *reinterpret_cast<const uint2*>(src + b * 32 + t * 8);
-            w[kt][b] = make_uint2(raw.x ^ kQ8FlipWord, raw.y ^ kQ8FlipWord);
-          } else {
-            const std::uint32_t raw = *reinterpret_cast<const std::uint32_t*>(src + b * 16 + t * 4);
-            w[kt][b] = make_uint2(raw & 0x0F0F0F0FU, (raw >> 4) & 0x0F0F0F0FU);
-          }
+        for (int b = 0; b < kBlocksPerRow; ++b) {   // pieces 2b, 2b + 1: one block
+          std::uint32_t w[4];
+          LdMatrixX4(k_base + (b >> 2) * kBoxBytes + (lm0 ^ (static_cast<std::uint32_t>(b & 3) << 5)), w);
+          block(b, 0, w[0] ^ kQ8FlipWord, w[2] ^ kQ8FlipWord);
+          block(b, 1, w[1] ^ kQ8FlipWord, w[3] ^ kQ8FlipWord);
         }
+      } else {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+        for (int x = 0; x < kBlocksPerRow / 2; ++x) {   // a piece is a block
+          std::uint32_t w[4];
+          LdMatrixX4(k_base + (lm0 ^ (static_cast<std::uint32_t>(x) << 5)), w);
 #pragma unroll
-        for (int b = 0; b < kBlocksPerRow; ++b) {
-          float acc[4] = {0.0F, 0.0F, 0.0F, 0.0F};
-          std::uint32_t b0, b1;
-          Bytes4(w[kt][b].x, bias, b0, b1);
-          MmaF16(acc, qa[b].x, 0U, qa[b].y, 0U, b0, b1);
-          Bytes4(w[kt][b].y, bias, b0, b1);
-          MmaF16(acc, qa[b].z, 0U, qa[b].w, 0U, b0, b1);
-          s[kt][0] = fmaf(HalfOf(d[kt][0], b), acc[0], s[kt][0]);
-          s[kt][1] = fmaf(HalfOf(d[kt][1], b), acc[1], s[kt][1]);
+          for (int k = 0; k < 4; ++k) block(2 * x + (k >> 1), k & 1, w[k] & 0x0F0F0F0FU, (w[k] >> 4) & 0x0F0F0F0FU);
         }
+      }
     }
+    // the stage is in registers: the last of the page's four warps refills it
+    const bool last = RingRelease(&done_cnt[s], lane, kKeyGroups);
+    if (last && i + L::kStages < n_pages) issue(s, __shfl_sync(0xFFFFFFFFU, refill_page, 0));
+    float mine = 0.0F;   // lane (g, t), g < 4, adds key 8 (g / 2) + 2t + g % 2
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float p_sum = g < kGroup ? exp2f(fmaf(s[kt][j], scale_log2, -norm)) : 0.0F;
+        float p_sum = exp2f(fmaf(sc[kt][j], scale_log2, -norm));
 #pragma unroll
         for (int o = 4; o <= 16; o <<= 1) p_sum += __shfl_xor_sync(0xFFFFFFFFU, p_sum, o);
-        const int key = key0 + kt * 8 + 2 * t + j;
-        if (g == 0 && key < u.n_keys) w_out[key] += p_sum;
+        if (g == 2 * kt + j) mine = p_sum;
       }
+    const int key = (u.page_begin + i) * kPageTokens + kw * 16 + 8 * (g >> 1) + 2 * t + (g & 1);
+    // one addition per key and call, so the order of CTAs does not matter; nothing waits for it
+    if (g < 4 && key < u.n_keys) atomicAdd(w_out + key, mine);
   }
+  if (!alive && lane == 0) atomicExch(status, kStatusWaitTimeout);
+  __syncthreads();
+  RingDrainAfterAbort(abort_flag, fill_cnt, full_bar, L::kStages);
 }
 
 // ----------------------------------------------------------------------------------------------------------------
@@ -368,13 +438,27 @@ __global__ void __launch_bounds__(256) CopyPageKernel(PoolView pool, int src, in
   for (std::size_t i = static_cast<std::size_t>(blockIdx.z) * 256 + threadIdx.x; i < bytes / 16; i += 256ULL * gridDim.z) to[i] = from[i];
 }
 
+template <int kFmt>
+cudaError_t LaunchWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream) {
+  return LaunchChained(AttnWeightsKernel<kFmt>, a.n_units, kWeightThreads, WeightSmem<kFmt>::kBytes, stream, *a.kmap, a.pool, a.layer,
+                       a.tables_dev, a.table_stride, a.units_dev, a.items_dev, static_cast<const __half*>(a.q_dev), a.scale_log2,
+                       a.partial_ml, weights, weights_stride, a.status_dev);
+}
+
 }  // namespace
+
+cudaError_t ConfigureWeightKernels() {
+  cudaError_t e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtF16>::kBytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtQ8>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtQ8>::kBytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtQ4>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtQ4>::kBytes);
+  return e;
+}
 
 cudaError_t LaunchAttnWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream) {
   if (a.n_units <= 0) return cudaSuccess;
-  const auto kernel = a.pool.fmt == kFmtF16 ? AttnWeightsKernel<kFmtF16> : a.pool.fmt == kFmtQ8 ? AttnWeightsKernel<kFmtQ8> : AttnWeightsKernel<kFmtQ4>;
-  return LaunchChained(kernel, a.n_units, kWeightThreads, 0, stream, a.pool, a.layer, a.tables_dev, a.table_stride, a.units_dev,
-                       a.items_dev, static_cast<const __half*>(a.q_dev), a.scale_log2, a.partial_ml, weights, weights_stride);
+  if (a.pool.fmt == kFmtF16) return LaunchWeights<kFmtF16>(a, weights, weights_stride, stream);
+  return a.pool.fmt == kFmtQ8 ? LaunchWeights<kFmtQ8>(a, weights, weights_stride, stream)
+                              : LaunchWeights<kFmtQ4>(a, weights, weights_stride, stream);
 }
 
 cudaError_t LaunchEvict(const EvictLaunch& a, cudaStream_t stream) {

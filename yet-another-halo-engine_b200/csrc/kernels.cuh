@@ -320,6 +320,7 @@ struct EvictLaunch {
 cudaError_t LaunchEvict(const EvictLaunch& a, cudaStream_t stream);
 // After LaunchDecodePart of the same plan (its partial_ml holds the rows' statistics); fp16 query.
 cudaError_t LaunchAttnWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream);
+cudaError_t ConfigureWeightKernels();
 cudaError_t LaunchCopyPage(const PoolView& pool, int src, int dst, cudaStream_t stream);
 
 // Rotary positions on given rows (rope.cu).
@@ -336,9 +337,8 @@ struct RopeRowsLaunch {
   float eps;
   int n_tokens, n_heads, rotary_dim;
   bool interleaved, x_f32, out_f32;
-  int heads_per_warp, head_groups;   // set by the launcher
 };
-cudaError_t LaunchRopeRows(RopeRowsLaunch a, cudaStream_t stream);
+cudaError_t LaunchRopeRows(const RopeRowsLaunch& a, cudaStream_t stream);
 
 struct PrefillLaunch {
   PoolView pool;

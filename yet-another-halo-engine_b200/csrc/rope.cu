@@ -50,61 +50,109 @@ __device__ __forceinline__ void StoreRow8(void* base, std::size_t at, const floa
   }
 }
 
-template <bool kInF32, bool kOutF32>
-__global__ void __launch_bounds__(32 * kRopeRowWarps) RopeRowsKernel(const RopeRowsLaunch a) {
-  __shared__ float row_s[kRopeRowWarps][kHeadDim];
-  ChainedKernelEntry();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long task = static_cast<long long>(blockIdx.x) * kRopeRowWarps + warp;
-  const int token = static_cast<int>(task / a.head_groups), hg = static_cast<int>(task % a.head_groups);
-  if (token >= a.n_tokens) return;
+// The angles of this lane's eight dims: cs[j] belongs to dim 8 lane + j. Neighbouring dims are neighbouring pairs (half) or
+// share them (interleaved), so a lane's entries are one run of the tables, read 16 bytes at a time where it is aligned.
+__device__ __forceinline__ float2 TurnOf(float2 x, float2 y) {
+  return make_float2(fmaf(x.x, y.x, -(x.y * y.y)), fmaf(x.x, y.y, x.y * y.x));
+}
+__device__ __forceinline__ void LaneAngles(const RopeRowsLaunch& a, long long pos, int lane, float2 (&cs)[8]) {
   const int half = a.rotary_dim / 2;
-  long long pos = a.positions[token];
-  if (pos < 0 || pos >= a.max_positions) {   // reported, and turned by the nearest angle there is
-    if (lane == 0) atomicExch(a.status, kStatusRopePosition);
-    pos = pos < 0 ? 0 : a.max_positions - 1;
+  const float2* hi = a.tab_hi + (pos >> kRopeLowBits) * half;
+  const float2* lo = a.tab_lo + (pos & ((1 << kRopeLowBits) - 1)) * half;
+  if (a.interleaved) {
+    if ((half & 3) == 0 && 8 * lane < a.rotary_dim) {
+      const float4* h4 = reinterpret_cast<const float4*>(hi + 4 * lane);
+      const float4* l4 = reinterpret_cast<const float4*>(lo + 4 * lane);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 x = __ldg(h4 + i), y = __ldg(l4 + i);
+        cs[4 * i] = cs[4 * i + 1] = TurnOf(make_float2(x.x, x.y), make_float2(y.x, y.y));
+        cs[4 * i + 2] = cs[4 * i + 3] = TurnOf(make_float2(x.z, x.w), make_float2(y.z, y.w));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      cs[2 * i] = make_float2(1.0F, 0.0F);
+      if (8 * lane + 2 * i < a.rotary_dim) cs[2 * i] = TurnOf(__ldg(hi + 4 * lane + i), __ldg(lo + 4 * lane + i));
+      cs[2 * i + 1] = cs[2 * i];
+    }
+    return;
   }
-  // cos and sin of this lane's dims
-  float2 cs[8];
+  if ((half & 7) == 0 && 8 * lane < a.rotary_dim) {   // the lane's dims lie in one half
+    const int p0 = 8 * lane < half ? 8 * lane : 8 * lane - half;
+    const float4* h4 = reinterpret_cast<const float4*>(hi + p0);
+    const float4* l4 = reinterpret_cast<const float4*>(lo + p0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 x = __ldg(h4 + i), y = __ldg(l4 + i);
+      cs[2 * i] = TurnOf(make_float2(x.x, x.y), make_float2(y.x, y.y));
+      cs[2 * i + 1] = TurnOf(make_float2(x.z, x.w), make_float2(y.z, y.w));
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int d = 8 * lane + j;
     cs[j] = make_float2(1.0F, 0.0F);
     if (d < a.rotary_dim) {
-      const int p = a.interleaved ? d >> 1 : (d < half ? d : d - half);
-      const float2 x = __ldg(a.tab_hi + (pos >> kRopeLowBits) * half + p);
-      const float2 y = __ldg(a.tab_lo + (pos & ((1 << kRopeLowBits) - 1)) * half + p);
-      cs[j] = make_float2(fmaf(x.x, y.x, -(x.y * y.y)), fmaf(x.x, y.y, x.y * y.x));
+      const int p = d < half ? d : d - half;
+      cs[j] = TurnOf(__ldg(hi + p), __ldg(lo + p));
     }
   }
+}
+
+// kHeads rows of one token per warp, all loaded before anything else is waited for.
+template <bool kInF32, bool kOutF32, int kHeads>
+__global__ void __launch_bounds__(32 * kRopeRowWarps) RopeRowsKernel(const RopeRowsLaunch a) {
+  __shared__ float row_s[kRopeRowWarps][kHeadDim];
+  ChainedKernelEntry();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long task = static_cast<long long>(blockIdx.x) * kRopeRowWarps + warp;
+  const int head_groups = (a.n_heads + kHeads - 1) / kHeads;
+  const int token = static_cast<int>(task / head_groups), h0 = static_cast<int>(task % head_groups) * kHeads;
+  if (token >= a.n_tokens) return;
+  long long pos = __ldg(a.positions + token);
+  const std::size_t x_at = static_cast<std::size_t>(token) * a.x_stride + static_cast<std::size_t>(h0) * kHeadDim + 8 * lane;
+  const std::size_t out_at = static_cast<std::size_t>(token) * a.out_stride + static_cast<std::size_t>(h0) * kHeadDim + 8 * lane;
+  float x[kHeads][8];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h)
+    if (h0 + h < a.n_heads) LoadRow8<kInF32>(a.x, x_at + h * kHeadDim, x[h]);
+  const int half = a.rotary_dim / 2;
+  if (pos < 0 || pos >= a.max_positions) {   // reported, and turned by the nearest angle there is
+    if (lane == 0) atomicExch(a.status, kStatusRopePosition);
+    pos = pos < 0 ? 0 : a.max_positions - 1;
+  }
+  float2 cs[8];
+  LaneAngles(a, pos, lane, cs);
   float wt[8];
   if (a.weight != nullptr) LoadRow8<true>(a.weight, 8 * lane, wt);
-  const int h1 = min((hg + 1) * a.heads_per_warp, a.n_heads);
-  for (int h = hg * a.heads_per_warp; h < h1; ++h) {
-    float x[8];
-    LoadRow8<kInF32>(a.x, static_cast<std::size_t>(token) * a.x_stride + static_cast<std::size_t>(h) * kHeadDim + 8 * lane, x);
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    if (h0 + h >= a.n_heads) break;   // the whole warp at once
     if (a.weight != nullptr) {
       float acc = 0.0F;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc = fmaf(x[j], x[j], acc);
+      for (int j = 0; j < 8; ++j) acc = fmaf(x[h][j], x[h][j], acc);
 #pragma unroll
       for (int m = 16; m >= 1; m >>= 1) acc += __shfl_xor_sync(0xFFFFFFFFU, acc, m);
       const float inv = 1.0F / sqrtf(acc * (1.0F / kHeadDim) + a.eps);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = x[j] * inv * wt[j];
+      for (int j = 0; j < 8; ++j) x[h][j] = x[h][j] * inv * wt[j];
     }
     float other[8];   // the pair's other half
     if (a.interleaved) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) other[j] = x[j ^ 1];
+      for (int j = 0; j < 8; ++j) other[j] = x[h][j ^ 1];
     } else if ((half & 7) == 0) {   // the same register of the lane half / 8 away
       const int src = 8 * lane < half ? lane + half / 8 : lane - half / 8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) other[j] = __shfl_sync(0xFFFFFFFFU, x[j], src & 31);
+      for (int j = 0; j < 8; ++j) other[j] = __shfl_sync(0xFFFFFFFFU, x[h][j], src & 31);
     } else {
       __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) row_s[warp][8 * lane + j] = x[j];
+      for (int j = 0; j < 8; ++j) row_s[warp][8 * lane + j] = x[h][j];
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -116,24 +164,29 @@ __global__ void __launch_bounds__(32 * kRopeRowWarps) RopeRowsKernel(const RopeR
     for (int j = 0; j < 8; ++j) {
       const int d = 8 * lane + j;
       const bool first = a.interleaved ? (j & 1) == 0 : d < half;
-      if (d < a.rotary_dim) x[j] = first ? fmaf(x[j], cs[j].x, -(other[j] * cs[j].y)) : fmaf(other[j], cs[j].y, x[j] * cs[j].x);
+      if (d < a.rotary_dim) x[h][j] = first ? fmaf(x[h][j], cs[j].x, -(other[j] * cs[j].y)) : fmaf(other[j], cs[j].y, x[h][j] * cs[j].x);
     }
-    StoreRow8<kOutF32>(a.out, static_cast<std::size_t>(token) * a.out_stride + static_cast<std::size_t>(h) * kHeadDim + 8 * lane, x);
+    StoreRow8<kOutF32>(a.out, out_at + h * kHeadDim, x[h]);
   }
+}
+
+template <bool kInF32, bool kOutF32>
+cudaError_t Launch(const RopeRowsLaunch& a, cudaStream_t stream) {
+  // Few rows: one per warp, so that the call fills the device. Many: four rows of a token share the angles.
+  const int heads = static_cast<long long>(a.n_tokens) * a.n_heads < 148 * 64 ? 1 : 4;
+  const long long tasks = static_cast<long long>(a.n_tokens) * ((a.n_heads + heads - 1) / heads);
+  const long long grid = (tasks + kRopeRowWarps - 1) / kRopeRowWarps;
+  if (grid > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
+  return LaunchChained(heads == 1 ? RopeRowsKernel<kInF32, kOutF32, 1> : RopeRowsKernel<kInF32, kOutF32, 4>,
+                       static_cast<unsigned>(grid), 32 * kRopeRowWarps, 0, stream, a);
 }
 
 }  // namespace
 
-cudaError_t LaunchRopeRows(RopeRowsLaunch a, cudaStream_t stream) {
+cudaError_t LaunchRopeRows(const RopeRowsLaunch& a, cudaStream_t stream) {
   if (a.n_tokens <= 0 || a.n_heads <= 0) return cudaSuccess;
-  // few tokens: one head per warp, so that the call fills the device; many: the angles are worth keeping
-  a.heads_per_warp = static_cast<long long>(a.n_tokens) * a.n_heads < 148 * 64 ? 1 : 4;
-  a.head_groups = (a.n_heads + a.heads_per_warp - 1) / a.heads_per_warp;
-  const long long tasks = static_cast<long long>(a.n_tokens) * a.head_groups;
-  const unsigned grid = static_cast<unsigned>((tasks + kRopeRowWarps - 1) / kRopeRowWarps);
-  const auto kernel = a.x_f32 ? (a.out_f32 ? RopeRowsKernel<true, true> : RopeRowsKernel<true, false>)
-                              : (a.out_f32 ? RopeRowsKernel<false, true> : RopeRowsKernel<false, false>);
-  return LaunchChained(kernel, grid, 32 * kRopeRowWarps, 0, stream, a);
+  if (a.x_f32) return a.out_f32 ? Launch<true, true>(a, stream) : Launch<true, false>(a, stream);
+  return a.out_f32 ? Launch<false, true>(a, stream) : Launch<false, false>(a, stream);
 }
 
 }  // namespace yahkv

@@ -295,6 +295,7 @@ int InitDevice(yahkv_ctx* ctx) {
     if (int r = ResizePrefillScratch(ctx, static_cast<std::int64_t>(c.max_prefill_keys) * kKvHeads); r != YAHKV_OK) return r;
   YAHKV_CUDA(ctx, ConfigureDecodeKernels());
   if (c.fmt == YAHKV_FMT_F16) YAHKV_CUDA(ctx, ConfigureF16Kernels());
+  if (!IsTileFmt(c.fmt)) YAHKV_CUDA(ctx, ConfigureWeightKernels());
   {
     int pairs = 0;   // CTA pairs of the prefill kernel that run at the same time: the planner's wave
     YAHKV_CUDA(ctx, ConfigurePrefillKernels(&pairs));
