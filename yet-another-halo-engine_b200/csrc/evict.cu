@@ -39,21 +39,26 @@ constexpr int kWeightWarps = kKeyGroups * kPageSets;
 constexpr int kWeightThreads = kWeightWarps * 32;
 constexpr int kBoxBytes = kPageTokens * 128;       // one swizzled TMA box: 64 token rows x 128 B
 
-// Shared memory: ring of K boxes | ring of block scales | barriers, counters, abort flag. Two CTAs per SM in every format
-// (q8_0 6 x 17 KB, q4_0 8 x 9 KB, fp16 3 x 32 KB).
+// Shared memory: ring of K boxes | ring of block scales | query operands (quantized formats) | barriers, counters, abort
+// flag. fp16: three stages of 32 KB and two CTAs per SM, the query operands in registers. Quantized formats issue more
+// instructions per byte: three CTAs, q8_0 with 4 x 17 KB, q4_0 with 6 x 9 KB, the query operands in shared memory, so that
+// 80 registers do (with two CTAs and the operands in registers the kernel spilled: 120 us against TODO us).
 template <int kFmt>
 struct WeightSmem {
   static constexpr int kBoxes = CodeBytes(kFmt) / 128;
-  static constexpr int kStages = kFmt == kFmtF16 ? 3 : kFmt == kFmtQ8 ? 6 : 8;
+  static constexpr int kStages = kFmt == kFmtF16 ? 3 : kFmt == kFmtQ8 ? 4 : 6;
+  static constexpr int kCtas = kFmt == kFmtF16 ? 2 : 3;
   static constexpr int kScaleBytes = RecordScaleBytes(kFmt, 0);
   static constexpr int kTx = kBoxes * kBoxBytes + kScaleBytes;
   static constexpr int kScaleOff = kStages * kBoxes * kBoxBytes;
-  static constexpr int kBarOff = kScaleOff + kStages * kScaleBytes;
+  static constexpr int kQOff = kScaleOff + kStages * kScaleBytes;   // [8 blocks][32 lanes] 16 bytes
+  static constexpr int kBarOff = kQOff + (kFmt == kFmtF16 ? 0 : kBlocksPerRow * 32 * 16);
   static constexpr int kDoneOff = kBarOff + 8 * kStages;
   static constexpr int kFillOff = kDoneOff + 4 * kStages;
   static constexpr int kAbortOff = kFillOff + 4 * kStages;
-  static constexpr int kBytes = (kAbortOff + 4 + 127) / 128 * 128;
-  static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two CTAs per SM");
+  static constexpr int kNormOff = kAbortOff + 4;
+  static constexpr int kBytes = (kNormOff + 4 * 8 + 127) / 128 * 128;
+  static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "resident CTAs per SM");
   static_assert(kPageSets <= kStages, "a set never waits for a stage it holds itself");
 };
 constexpr int kStatusSmemMisaligned = 2;
@@ -64,22 +69,30 @@ __device__ __forceinline__ void Bytes4(std::uint32_t u, __half2 bias_h, std::uin
   const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias_h), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias_h);
   h01 = *reinterpret_cast<const std::uint32_t*>(&x), h23 = *reinterpret_cast<const std::uint32_t*>(&y);
 }
-__device__ __forceinline__ float HalfOf(const uint4& v, int i) {   // fp16 number i of eight, i a constant after unrolling
-  const std::uint32_t w = i < 4 ? (i < 2 ? v.x : v.y) : (i < 6 ? v.z : v.w);
+__device__ __forceinline__ float HalfOf(const uint2& v, int i) {   // fp16 number i of four, i a constant after unrolling
+  const std::uint32_t w = i < 2 ? v.x : v.y;
   const __half2 h = *reinterpret_cast<const __half2*>(&w);
   return (i & 1) ? __high2float(h) : __low2float(h);
 }
+// D(16 x 8, f32) = A(16 x 16, f16) . B(16 x 8, f16), no accumulator input
+__device__ __forceinline__ void MmaF16Zero(float (&d)[4], std::uint32_t a0, std::uint32_t a1, std::uint32_t a2, std::uint32_t a3,
+                                           std::uint32_t b0, std::uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0F));
+}
 
 template <int kFmt>
-__global__ void __launch_bounds__(kWeightThreads, 2)
+__global__ void __launch_bounds__(kWeightThreads, WeightSmem<kFmt>::kCtas)
     AttnWeightsKernel(const __grid_constant__ CUtensorMap kmap, PoolView pool, int layer,
                       const std::int32_t* __restrict__ tables, int table_stride, const DecodeUnit* __restrict__ units,
                       const CombineItem* __restrict__ items, const __half* __restrict__ q, float scale_log2,
                       const float* __restrict__ partial_ml, float* __restrict__ weights, long long weights_stride, int* status) {
   using L = WeightSmem<kFmt>;
   extern __shared__ __align__(1024) std::uint8_t smem[];
-  __shared__ float norm_s[8];   // M + log2 L per query head
   ChainedKernelEntry();
+  float* norm_s = reinterpret_cast<float*>(smem + L::kNormOff);   // M + log2 L per query head
   std::uint64_t* full_bar = reinterpret_cast<std::uint64_t*>(smem + L::kBarOff);
   int* done_cnt = reinterpret_cast<int*>(smem + L::kDoneOff);
   int* fill_cnt = reinterpret_cast<int*>(smem + L::kFillOff);
@@ -142,20 +155,24 @@ __global__ void __launch_bounds__(kWeightThreads, 2)
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFU, l, o);
     if (lane == 0) norm_s[warp] = m + log2f(l);
   }
-  // A operand: head g's dims in the order in which ldmatrix hands over K. fp16: dims 16 s + 2t, + 1 and 16 s + 8 + 2t, + 1
-  // of step s. Codes: a 16-byte piece is 16 codes (q8_0) or a block's 32 nibbles (q4_0), lane t has its bytes 4t .. 4t + 3:
-  // elements 4t .. of a 32-element block and 16 + 4t ..
-  std::uint32_t qa[32];
-  {
+  // S[key][head] = K[key][dim] . Q^T[dim][head]: A = 16 keys as ldmatrix hands them over, B = the query, column g = head g.
+  // fp16: dims 16 s + 2t, + 1 and 16 s + 8 + 2t, + 1 of step s. Codes: a 16-byte piece is 16 codes (q8_0) or a block's 32
+  // nibbles (q4_0), lane t has its bytes 4t .. 4t + 3: elements 4t .. of a 32-element block and 16 + 4t ..
+  std::uint32_t qa[kFmt == kFmtF16 ? 32 : 1];
+  if constexpr (kFmt == kFmtF16) {
     const __half* src = q + (static_cast<std::size_t>(u.batch) * kQHeads + u.kvh * kGroup + min(g, kGroup - 1)) * kHeadDim;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int at = kFmt == kFmtF16 ? 8 * i + 2 * t : 32 * (i >> 2) + 16 * ((i >> 1) & 1) + 4 * t + 2 * (i & 1);
-      qa[i] = g < kGroup ? __ldg(reinterpret_cast<const std::uint32_t*>(src + at)) : 0U;
-    }
+    for (int i = 0; i < 32; ++i) qa[i] = g < kGroup ? __ldg(reinterpret_cast<const std::uint32_t*>(src + 8 * i + 2 * t)) : 0U;
+  } else {   // warp b lays out block b: lane (g, t) dims 32 b + 4t .. + 3 and 32 b + 16 + 4t .. + 3 of head g
+    const __half* src = q + (static_cast<std::size_t>(u.batch) * kQHeads + u.kvh * kGroup + min(g, kGroup - 1)) * kHeadDim + 32 * warp;
+    uint2 lo = __ldg(reinterpret_cast<const uint2*>(src + 4 * t)), hi = __ldg(reinterpret_cast<const uint2*>(src + 16 + 4 * t));
+    if (g >= kGroup) lo = hi = make_uint2(0, 0);
+    *reinterpret_cast<uint4*>(smem + L::kQOff + (warp * 32 + lane) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    static_assert(kWeightWarps == kBlocksPerRow, "a warp per block");
   }
   __syncthreads();   // barriers initialised, norms visible
-  const float norm = g < kGroup ? norm_s[g] : INFINITY;   // the padding rows of the MMA weigh nothing
+  // this thread's results are heads 2t, 2t + 1 of keys g and g + 8; the padding heads weigh nothing
+  const float norm0 = t < 3 ? norm_s[2 * t] : INFINITY, norm1 = t < 3 ? norm_s[2 * t + 1] : INFINITY;
   float* w_out = weights + (static_cast<std::size_t>(u.seq) * kKvHeads + u.kvh) * static_cast<std::size_t>(weights_stride);
   const __half2 bias = __half2half2(__ushort_as_half(kFmt == kFmtQ8 ? 0x6480 : 0x6408));
   // ldmatrix rows: matrices = (keys 0-7 | 8-15 of the group) x (16-byte pieces 2x | 2x + 1); piece p of row r sits at p ^ (r % 8)
@@ -169,70 +186,67 @@ __global__ void __launch_bounds__(kWeightThreads, 2)
     if (lane == 0 && i + L::kStages < n_pages) refill_page = __ldg(row + i + L::kStages);
     alive = RingWait(alive, fill_cnt + s, &full_bar[s], gen, abort_flag);
     const std::uint32_t k_base = SmemAddr(smem + s * L::kBoxes * kBoxBytes);
-    float sc[2][2] = {{0.0F, 0.0F}, {0.0F, 0.0F}};   // keys 8 kt + 2t + j of the group, head g
+    float sc[4] = {0.0F, 0.0F, 0.0F, 0.0F};   // (key g, head 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1)
     if constexpr (kFmt == kFmtF16) {
-      float acc[2][4] = {{0.0F, 0.0F, 0.0F, 0.0F}, {0.0F, 0.0F, 0.0F, 0.0F}};
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         std::uint32_t w[4];
         LdMatrixX4(k_base + (x >> 2) * kBoxBytes + (lm0 ^ (static_cast<std::uint32_t>(x & 3) << 5)), w);
-        MmaF16(acc[0], qa[2 * x], 0U, qa[2 * x + 1], 0U, w[0], w[2]);
-        MmaF16(acc[1], qa[2 * x], 0U, qa[2 * x + 1], 0U, w[1], w[3]);
+        MmaF16(sc, w[0], w[1], w[2], w[3], qa[2 * x], qa[2 * x + 1]);
       }
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) sc[kt][0] = acc[kt][0], sc[kt][1] = acc[kt][1];
     } else {
-      uint4 d[2][2];   // the eight block scales of this thread's keys
+      const std::uint8_t* scales = smem + L::kScaleOff + s * L::kScaleBytes + (kw * 16 + g) * (kBlocksPerRow * 2);
+      const std::uint32_t q_base = SmemAddr(smem + L::kQOff) + lane * 16;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int dh = 0; dh < 2; ++dh) {   // blocks 4 dh .. + 3; scales fetched per half to keep registers low
+        const uint2 d0 = *reinterpret_cast<const uint2*>(scales + dh * 8);
+        const uint2 d1 = *reinterpret_cast<const uint2*>(scales + 8 * (kBlocksPerRow * 2) + dh * 8);
+        // one block of 32 elements: two k-steps into a fresh accumulator, then the keys' scales
+        auto block = [&](int b, std::uint32_t lo0, std::uint32_t lo1, std::uint32_t hi0, std::uint32_t hi1) {
+          std::uint32_t qb[4], a0, a1, a2, a3;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(qb[0]), "=r"(qb[1]), "=r"(qb[2]), "=r"(qb[3])
+                       : "r"(q_base + (4 * dh + b) * 512));
+          float acc[4];
+          Bytes4(lo0, bias, a0, a2);
+          Bytes4(lo1, bias, a1, a3);
+          MmaF16Zero(acc, a0, a1, a2, a3, qb[0], qb[1]);
+          Bytes4(hi0, bias, a0, a2);
+          Bytes4(hi1, bias, a1, a3);
+          MmaF16(acc, a0, a1, a2, a3, qb[2], qb[3]);
+          const float s0 = HalfOf(d0, b), s1 = HalfOf(d1, b);
+          sc[0] = fmaf(s0, acc[0], sc[0]), sc[1] = fmaf(s0, acc[1], sc[1]);
+          sc[2] = fmaf(s1, acc[2], sc[2]), sc[3] = fmaf(s1, acc[3], sc[3]);
+        };
+        if constexpr (kFmt == kFmtQ8) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          d[kt][j] = *reinterpret_cast<const uint4*>(smem + L::kScaleOff + s * L::kScaleBytes + (kw * 16 + kt * 8 + 2 * t + j) * (kBlocksPerRow * 2));
-      // one block of 32 elements for eight keys: two k-steps into a fresh accumulator, then the keys' scales
-      auto block = [&](int b, int kt, std::uint32_t lo, std::uint32_t hi) {
-        float acc[4] = {0.0F, 0.0F, 0.0F, 0.0F};
-        std::uint32_t b0, b1;
-        Bytes4(lo, bias, b0, b1);
-        MmaF16(acc, qa[4 * b], 0U, qa[4 * b + 1], 0U, b0, b1);
-        Bytes4(hi, bias, b0, b1);
-        MmaF16(acc, qa[4 * b + 2], 0U, qa[4 * b + 3], 0U, b0, b1);
-        sc[kt][0] = fmaf(HalfOf(d[kt][0], b), acc[0], sc[kt][0]);
-        sc[kt][1] = fmaf(HalfOf(d[kt][1], b), acc[1], sc[kt][1]);
-      };
-      if constexpr (kFmt == kFmtQ8) {
+          for (int b = 0; b < 4; ++b) {   // pieces 2b, 2b + 1 of box dh: one block
+            std::uint32_t w[4];
+            LdMatrixX4(k_base + dh * kBoxBytes + (lm0 ^ (static_cast<std::uint32_t>(b) << 5)), w);
+            block(b, w[0] ^ kQ8FlipWord, w[1] ^ kQ8FlipWord, w[2] ^ kQ8FlipWord, w[3] ^ kQ8FlipWord);
+          }
+        } else {
 #pragma unroll
-        for (int b = 0; b < kBlocksPerRow; ++b) {   // pieces 2b, 2b + 1: one block
-          std::uint32_t w[4];
-          LdMatrixX4(k_base + (b >> 2) * kBoxBytes + (lm0 ^ (static_cast<std::uint32_t>(b & 3) << 5)), w);
-          block(b, 0, w[0] ^ kQ8FlipWord, w[2] ^ kQ8FlipWord);
-          block(b, 1, w[1] ^ kQ8FlipWord, w[3] ^ kQ8FlipWord);
-        }
-      } else {
+          for (int x = 0; x < 2; ++x) {   // a piece is a block
+            std::uint32_t w[4];
+            LdMatrixX4(k_base + (lm0 ^ (static_cast<std::uint32_t>(2 * dh + x) << 5)), w);
 #pragma unroll
-        for (int x = 0; x < kBlocksPerRow / 2; ++x) {   // a piece is a block
-          std::uint32_t w[4];
-          LdMatrixX4(k_base + (lm0 ^ (static_cast<std::uint32_t>(x) << 5)), w);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) block(2 * x + (k >> 1), k & 1, w[k] & 0x0F0F0F0FU, (w[k] >> 4) & 0x0F0F0F0FU);
+            for (int k = 0; k < 2; ++k)
+              block(2 * x + k, w[2 * k] & 0x0F0F0F0FU, w[2 * k + 1] & 0x0F0F0F0FU, (w[2 * k] >> 4) & 0x0F0F0F0FU,
+                    (w[2 * k + 1] >> 4) & 0x0F0F0F0FU);
+          }
         }
       }
     }
     // the stage is in registers: the last of the page's four warps refills it
     const bool last = RingRelease(&done_cnt[s], lane, kKeyGroups);
     if (last && i + L::kStages < n_pages) issue(s, __shfl_sync(0xFFFFFFFFU, refill_page, 0));
-    float mine = 0.0F;   // lane (g, t), g < 4, adds key 8 (g / 2) + 2t + g % 2
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float p_sum = exp2f(fmaf(sc[kt][j], scale_log2, -norm));
-#pragma unroll
-        for (int o = 4; o <= 16; o <<= 1) p_sum += __shfl_xor_sync(0xFFFFFFFFU, p_sum, o);
-        if (g == 2 * kt + j) mine = p_sum;
-      }
-    const int key = (u.page_begin + i) * kPageTokens + kw * 16 + 8 * (g >> 1) + 2 * t + (g & 1);
-    // one addition per key and call, so the order of CTAs does not matter; nothing waits for it
-    if (g < 4 && key < u.n_keys) atomicAdd(w_out + key, mine);
+    float p0 = exp2f(fmaf(sc[0], scale_log2, -norm0)) + exp2f(fmaf(sc[1], scale_log2, -norm1));
+    float p1 = exp2f(fmaf(sc[2], scale_log2, -norm0)) + exp2f(fmaf(sc[3], scale_log2, -norm1));
+    p0 += __shfl_xor_sync(0xFFFFFFFFU, p0, 1), p1 += __shfl_xor_sync(0xFFFFFFFFU, p1, 1);
+    p0 += __shfl_xor_sync(0xFFFFFFFFU, p0, 2), p1 += __shfl_xor_sync(0xFFFFFFFFU, p1, 2);
+    // lanes t = 0 and 1 add keys g and g + 8: one addition per key and call, so the order of CTAs does not matter
+    const int key = (u.page_begin + i) * kPageTokens + kw * 16 + 8 * t + g;
+    if (t < 2 && key < u.n_keys) atomicAdd(w_out + key, t == 0 ? p0 : p1);
   }
   if (!alive && lane == 0) atomicExch(status, kStatusWaitTimeout);
   __syncthreads();
