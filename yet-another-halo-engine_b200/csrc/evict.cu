@@ -16,11 +16,12 @@
 // that weight are kept; a last pass in index order writes the kept indices and moves the weights to the front.
 //
 // EvictMoveKernel moves the kept rows to slots 0 .. n_keep - 1, in place where the sequence has its pages to itself: kept
-// index i is at least i, so with 64-slot chunks in ascending order a chunk's sources lie at or behind its slots, and
+// index i is at least i, so with chunks of slots in ascending order a chunk's sources lie at or behind its slots, and
 // only the chunk's own reads have to come before its writes. Pages that another sequence shares are replaced by fresh
 // ones (the host lists them) and stay as they were.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "decode_ring.cuh"
@@ -257,6 +258,9 @@ __global__ void __launch_bounds__(kWeightThreads, WeightSmem<kFmt>::kCtas)
 // selection
 // ----------------------------------------------------------------------------------------------------------------
 constexpr int kSelectThreads = 1024;
+constexpr int kSelectPer = 4;                                  // keys per thread and turn of the last pass
+constexpr int kSelectTile = kSelectThreads * kSelectPer;
+constexpr int kSelectCache = 48 * 1024;                        // keys whose words are kept in shared memory (192 KB)
 
 // Order-preserving bits of a weight: larger weight, larger word; NaN below everything, -0 equal to +0.
 __device__ __forceinline__ std::uint32_t OrderOf(float w) {
@@ -264,11 +268,35 @@ __device__ __forceinline__ std::uint32_t OrderOf(float w) {
   const std::uint32_t b = __float_as_uint(w == 0.0F ? 0.0F : w);
   return (b & 0x80000000U) != 0 ? ~b : b | 0x80000000U;
 }
+// Exclusive prefix sum over the CTA's threads; *total receives the sum. scan_s: one int per warp. Two barriers inside.
+__device__ __forceinline__ int CtaScan(int v, int* scan_s, int lane, int warp, int* total) {
+  int sum = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int x = __shfl_up_sync(0xFFFFFFFFU, sum, d);
+    if (lane >= d) sum += x;
+  }
+  if (lane == 31) scan_s[warp] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    int x = scan_s[lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xFFFFFFFFU, x, d);
+      if (lane >= d) x += y;
+    }
+    scan_s[lane] = x;
+  }
+  __syncthreads();
+  *total = scan_s[31];
+  return (warp > 0 ? scan_s[warp - 1] : 0) + sum - v;
+}
 
 __global__ void __launch_bounds__(kSelectThreads)
     EvictSelectKernel(const EvictSeq* __restrict__ seqs, int n_seqs, int kv_head_begin, int n_keep, int n_sink, int n_recent,
-                      float* __restrict__ weights, long long weights_stride, long long layer_stride,
+                      float* __restrict__ weights, long long weights_stride, long long layer_stride, int n_cache,
                       std::int32_t* __restrict__ kept) {
+  extern __shared__ std::uint32_t word_s[];   // [n_cache] words of the first keys of [lo, hi)
   __shared__ int hist[2048];
   __shared__ int scan_s[kSelectThreads / 32];
   __shared__ std::uint32_t prefix_s;
@@ -284,9 +312,11 @@ __global__ void __launch_bounds__(kSelectThreads)
   }
   float* w = weights + static_cast<std::size_t>(layer) * layer_stride +
              (static_cast<std::size_t>(es.seq) * kKvHeads + h) * static_cast<std::size_t>(weights_stride);
-  const int lo = n_sink, hi = es.n_keys - n_recent;
-  int want = n_keep - n_sink - n_recent;   // keys to choose of [lo, hi): fewer than hi - lo
-  // the want-th largest word, eleven, eleven and ten bits at a time
+  const int lo = n_sink, n_mid = es.n_keys - n_recent - n_sink;   // the keys to choose from are lo .. lo + n_mid - 1
+  const int n_choose = n_keep - n_sink - n_recent;                // fewer than n_mid
+  const int n_held = min(n_mid, n_cache);
+  int want = n_choose;
+  // the want-th largest word, eleven, eleven and ten bits at a time; the first pass fills the cache
   std::uint32_t prefix = 0, mask = 0;
   if (want > 0) {
     const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
@@ -295,38 +325,32 @@ __global__ void __launch_bounds__(kSelectThreads)
       for (int i = tid; i < 2048; i += kSelectThreads) hist[i] = 0;
       __syncthreads();
       const std::uint32_t bin_mask = (1U << bits[pass]) - 1U;
-      for (int i0 = lo; i0 < hi; i0 += kSelectThreads) {
-        const int i = i0 + tid;
-        const std::uint32_t o = i < hi ? OrderOf(w[i]) : 0U;
-        const bool on = i < hi && (o & mask) == prefix;
-        // lanes with the same bin add once (weights that are equal, zeros above all, would serialise otherwise)
-        const std::uint32_t bin = on ? (o >> shifts[pass]) & bin_mask : 0xFFFFFFFFU;
-        const unsigned same = __match_any_sync(0xFFFFFFFFU, bin);
-        if (on && lane == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
+      for (int i0 = 0; i0 < n_mid; i0 += kSelectTile) {
+        std::uint32_t o[kSelectPer];
+        bool on[kSelectPer];
+#pragma unroll
+        for (int k = 0; k < kSelectPer; ++k) {
+          const int i = i0 + k * kSelectThreads + tid;
+          on[k] = i < n_mid;
+          o[k] = !on[k] ? 0U : pass > 0 && i < n_held ? word_s[i] : OrderOf(w[lo + i]);
+        }
+#pragma unroll
+        for (int k = 0; k < kSelectPer; ++k) {
+          const int i = i0 + k * kSelectThreads + tid;
+          if (pass == 0 && i < n_held) word_s[i] = o[k];
+          // lanes with the same bin add once (weights that are equal, zeros above all, would serialise otherwise)
+          const bool hit = on[k] && (o[k] & mask) == prefix;
+          const std::uint32_t bin = hit ? (o[k] >> shifts[pass]) & bin_mask : 0xFFFFFFFFU;
+          const unsigned same = __match_any_sync(0xFFFFFFFFU, bin);
+          if (hit && lane == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
+        }
       }
       __syncthreads();
       // counts from the largest bin down; two bins per thread
       const int top = 2047 - 2 * tid;
       const int c0 = hist[top], c1 = hist[top - 1];
-      int sum = c0 + c1;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xFFFFFFFFU, sum, d);
-        if (lane >= d) sum += v;
-      }
-      if (lane == 31) scan_s[warp] = sum;
-      __syncthreads();
-      if (warp == 0) {
-        int v = scan_s[lane];
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int x = __shfl_up_sync(0xFFFFFFFFU, v, d);
-          if (lane >= d) v += x;
-        }
-        scan_s[lane] = v;
-      }
-      __syncthreads();
-      const int before = (warp > 0 ? scan_s[warp - 1] : 0) + sum - c0 - c1;
+      int total;
+      const int before = CtaScan(c0 + c1, scan_s, lane, warp, &total);
       if (before < want && before + c0 >= want) {
         prefix_s = prefix | (static_cast<std::uint32_t>(top) << shifts[pass]);
         want_s = want - before;
@@ -340,41 +364,36 @@ __global__ void __launch_bounds__(kSelectThreads)
       __syncthreads();
     }
   }
-  // prefix is the smallest kept word and `want` keys of exactly that word are kept, the lowest indices; in index order,
-  // a kept key's slot is the number of keys kept before it
-  const int n_eq = n_keep - n_sink - n_recent > 0 ? want : 0;
+  // prefix is the smallest kept word and `want` keys of exactly that word are kept, the lowest indices. In index order, a
+  // kept key's slot is the number of keys kept before it; a thread takes four neighbouring keys.
   int base_gt = 0, base_eq = 0;
-  for (int i0 = 0; i0 < es.n_keys; i0 += kSelectThreads) {
-    const int i = i0 + tid;
-    const bool in = i < es.n_keys;
-    const float wi = in ? w[i] : 0.0F;
-    const bool middle = in && i >= lo && i < hi;
-    const std::uint32_t o = middle ? OrderOf(wi) : 0U;
-    const bool choose = n_keep - n_sink - n_recent > 0;
-    const bool gt = in && (!middle || (choose && o > prefix));
-    const bool eq = middle && choose && o == prefix;
-    const unsigned bg = __ballot_sync(0xFFFFFFFFU, gt), be = __ballot_sync(0xFFFFFFFFU, eq);
-    const unsigned below = (1U << lane) - 1U;
-    if (lane == 0) scan_s[warp] = __popc(bg) | (__popc(be) << 16);
-    __syncthreads();   // every weight of the tile has been read: its slots may be written
-    if (warp == 0) {
-      int v = scan_s[lane];
+  for (int i0 = 0; i0 < es.n_keys; i0 += kSelectTile) {
+    const int at = i0 + kSelectPer * tid;
+    float wi[kSelectPer];
+    bool gt[kSelectPer], eq[kSelectPer];
+    int count = 0;   // keys above the border in the low half, keys on it in the high half: at most 4096 of each
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int x = __shfl_up_sync(0xFFFFFFFFU, v, d);
-        if (lane >= d) v += x;
+    for (int k = 0; k < kSelectPer; ++k) {
+      const int i = at + k, m = i - lo;
+      const bool in = i < es.n_keys, middle = in && m >= 0 && m < n_mid;
+      wi[k] = in ? w[i] : 0.0F;
+      const std::uint32_t o = middle ? OrderOf(wi[k]) : 0U;
+      gt[k] = in && (!middle || (n_choose > 0 && o > prefix));
+      eq[k] = middle && n_choose > 0 && o == prefix;
+      count += (gt[k] ? 1 : 0) + (eq[k] ? 1 << 16 : 0);
+    }
+    int total;
+    const int before = CtaScan(count, scan_s, lane, warp, &total);   // behind its barriers every weight of the tile has been read
+    int gt_before = base_gt + (before & 0xFFFF), eq_before = base_eq + (before >> 16);
+#pragma unroll
+    for (int k = 0; k < kSelectPer; ++k) {
+      if (gt[k] || (eq[k] && eq_before < want)) {
+        const int slot = gt_before + min(eq_before, want);
+        if (slot < n_keep) out[slot] = at + k, w[slot] = wi[k];
       }
-      scan_s[lane] = v;
+      gt_before += gt[k] ? 1 : 0, eq_before += eq[k] ? 1 : 0;
     }
-    __syncthreads();
-    const int pre = warp > 0 ? scan_s[warp - 1] : 0, all = scan_s[31];
-    const int eq_before = base_eq + (pre >> 16) + __popc(be & below);
-    const int gt_before = base_gt + (pre & 0xFFFF) + __popc(bg & below);
-    if (gt || (eq && eq_before < n_eq)) {
-      const int slot = gt_before + min(eq_before, n_eq);
-      if (slot < n_keep) out[slot] = i, w[slot] = wi;
-    }
-    base_gt += all & 0xFFFF, base_eq += all >> 16;
+    base_gt += total & 0xFFFF, base_eq += total >> 16;
     __syncthreads();
   }
   for (int i = n_keep + tid; i < es.n_keys; i += kSelectThreads) w[i] = 0.0F;   // slots of keys to come
@@ -384,58 +403,65 @@ __global__ void __launch_bounds__(kSelectThreads)
 // moving the kept rows
 // ----------------------------------------------------------------------------------------------------------------
 constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 256;                       // rows per chunk
+constexpr int kMoveSlice = 64;                       // bytes of a row one CTA moves (its block scales: 16)
+constexpr int kMovePer = kMoveRows * (kMoveSlice / 16) / kMoveThreads;   // 16-byte pieces per thread and chunk
 
-template <int kFmt>
+// One CTA per 64-byte column of the rows of one (layer, sequence, kv head, side), and one for their block scales: columns
+// never meet, so only the order of chunks inside a CTA matters in place. The next chunk's loads are in flight while a
+// chunk is written.
 __global__ void __launch_bounds__(kMoveThreads)
     EvictMoveKernel(PoolView pool, const std::int32_t* __restrict__ tables, int table_stride, const EvictSeq* __restrict__ seqs,
-                    int n_seqs, const std::int32_t* __restrict__ dst_pages, int n_keep, const std::int32_t* __restrict__ kept) {
-  constexpr int kRowVecs = CodeBytes(kFmt) / 16;                          // 16-byte pieces of a row
-  constexpr int kPer = kPageTokens * kRowVecs / kMoveThreads;             // of a 64-row chunk, per thread
+                    int n_seqs, const std::int32_t* __restrict__ dst_pages, int n_keep, int n_slices,
+                    const std::int32_t* __restrict__ kept) {
   ChainedKernelEntry();
-  const int b = blockIdx.x, side = blockIdx.y & 1, h = pool.kv_head_begin + (blockIdx.y >> 1), layer = blockIdx.z;
+  const int b = blockIdx.x / n_slices, slice = blockIdx.x % n_slices;
+  const int side = blockIdx.y & 1, h = pool.kv_head_begin + (blockIdx.y >> 1), layer = blockIdx.z;
   const EvictSeq es = seqs[b];
   if (es.n_keys <= n_keep) return;
   const int tid = threadIdx.x;
+  const int row_bytes_codes = CodeBytes(pool.fmt);
+  const bool is_scale = slice * kMoveSlice >= row_bytes_codes;
+  const int row_bytes = is_scale ? kBlocksPerRow * 2 : row_bytes_codes;
+  const int per_row = is_scale ? 1 : kMoveSlice / 16;            // 16-byte pieces of a row this CTA moves
+  const int column = is_scale ? 0 : slice * kMoveSlice;
+  std::uint8_t* base = is_scale ? reinterpret_cast<std::uint8_t*>(side == 0 ? pool.kscales : pool.vscales)
+                                : (side == 0 ? pool.kcodes : pool.vcodes);
   const std::int32_t* idx = kept + ((static_cast<std::size_t>(layer) * n_seqs + b) * kKvHeads + h) * static_cast<std::size_t>(n_keep);
   const std::int32_t* table = tables + static_cast<std::size_t>(es.seq) * table_stride;
-  std::uint8_t* codes = side == 0 ? pool.kcodes : pool.vcodes;
-  std::uint8_t* scales = reinterpret_cast<std::uint8_t*>(side == 0 ? pool.kscales : pool.vscales);
-  auto row_of = [&](std::int32_t page, int tok) -> std::size_t {
+  auto row_at = [&](std::int32_t page, int tok) -> std::uint8_t* {
     page = min(max(page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
-    return ((static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + h) * kPageTokens + tok;
+    return base + (((static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + h) * kPageTokens + tok) * row_bytes + column;
   };
-  uint4 v[kPer], sc = make_uint4(0, 0, 0, 0);
+  uint4 v[kMovePer];
   auto load = [&](int c0) {
+    int i[kMovePer];
+    std::int32_t page[kMovePer];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int piece = tid + k * kMoveThreads, slot = c0 + piece / kRowVecs;
-      if (slot < n_keep) {
-        const int i = min(max(__ldg(idx + slot), 0), es.n_keys - 1);
-        v[k] = *reinterpret_cast<const uint4*>(codes + row_of(__ldg(table + i / kPageTokens), i % kPageTokens) * CodeBytes(kFmt) +
-                                               (piece % kRowVecs) * 16);
-      }
+    for (int k = 0; k < kMovePer; ++k) {
+      const int piece = tid + k * kMoveThreads, slot = c0 + piece / per_row;
+      i[k] = piece < kMoveRows * per_row && slot < n_keep ? min(max(__ldg(idx + slot), 0), es.n_keys - 1) : -1;
     }
-    if (kFmt != kFmtF16 && tid < kPageTokens && c0 + tid < n_keep) {
-      const int i = min(max(__ldg(idx + c0 + tid), 0), es.n_keys - 1);
-      sc = *reinterpret_cast<const uint4*>(scales + row_of(__ldg(table + i / kPageTokens), i % kPageTokens) * (kBlocksPerRow * 2));
-    }
+#pragma unroll
+    for (int k = 0; k < kMovePer; ++k) page[k] = i[k] >= 0 ? __ldg(table + i[k] / kPageTokens) : 0;
+#pragma unroll
+    for (int k = 0; k < kMovePer; ++k)
+      if (i[k] >= 0)
+        v[k] = *reinterpret_cast<const uint4*>(row_at(page[k], i[k] % kPageTokens) + ((tid + k * kMoveThreads) % per_row) * 16);
   };
   load(0);
-  for (int c0 = 0; c0 < n_keep; c0 += kPageTokens) {
+  for (int c0 = 0; c0 < n_keep; c0 += kMoveRows) {
+    uint4 mine[kMovePer];
+#pragma unroll
+    for (int k = 0; k < kMovePer; ++k) mine[k] = v[k];
     __syncthreads();   // every row of the chunk is in registers: its slots may be written
-    uint4 mine[kPer], my_sc = sc;
+    if (c0 + kMoveRows < n_keep) load(c0 + kMoveRows);   // sources at or behind the next chunk's first slot
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) mine[k] = v[k];
-    if (c0 + kPageTokens < n_keep) load(c0 + kPageTokens);   // sources at or behind the next chunk's first slot
-    const std::int32_t page = __ldg(dst_pages + es.first_dst + c0 / kPageTokens);
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const int piece = tid + k * kMoveThreads, tok = piece / kRowVecs;
-      if (c0 + tok < n_keep)
-        *reinterpret_cast<uint4*>(codes + row_of(page, tok) * CodeBytes(kFmt) + (piece % kRowVecs) * 16) = mine[k];
+    for (int k = 0; k < kMovePer; ++k) {
+      const int piece = tid + k * kMoveThreads, slot = c0 + piece / per_row;
+      if (piece < kMoveRows * per_row && slot < n_keep)
+        *reinterpret_cast<uint4*>(row_at(__ldg(dst_pages + es.first_dst + slot / kPageTokens), slot % kPageTokens) + (piece % per_row) * 16) = mine[k];
     }
-    if (kFmt != kFmtF16 && tid < kPageTokens && c0 + tid < n_keep)
-      *reinterpret_cast<uint4*>(scales + row_of(page, tid) * (kBlocksPerRow * 2)) = my_sc;
   }
 }
 
@@ -461,10 +487,11 @@ cudaError_t LaunchWeights(const DecodeLaunch& a, float* weights, long long weigh
 
 }  // namespace
 
-cudaError_t ConfigureWeightKernels() {
+cudaError_t ConfigureEvictKernels() {
   cudaError_t e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtF16>::kBytes);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtQ8>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtQ8>::kBytes);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtQ4>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtQ4>::kBytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(EvictSelectKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectCache * 4);
   return e;
 }
 
@@ -478,13 +505,16 @@ cudaError_t LaunchAttnWeights(const DecodeLaunch& a, float* weights, long long w
 cudaError_t LaunchEvict(const EvictLaunch& a, cudaStream_t stream) {
   if (a.n_seqs <= 0) return cudaSuccess;
   const dim3 per_row(static_cast<unsigned>(a.n_seqs), static_cast<unsigned>(a.pool.kv_head_count), static_cast<unsigned>(a.pool.n_layers));
-  cudaError_t e = LaunchChained(EvictSelectKernel, per_row, kSelectThreads, 0, stream, a.seqs_dev, a.n_seqs, a.pool.kv_head_begin,
-                                a.n_keep, a.n_sink, a.n_recent, a.weights, a.weights_stride, a.layer_stride, a.kept);
+  // words of the keys in shared memory, as many as the longest sequence has (what does not fit is read again per pass)
+  const int n_cache = std::min(a.max_keys, kSelectCache);
+  cudaError_t e = LaunchChained(EvictSelectKernel, per_row, kSelectThreads, static_cast<std::size_t>(n_cache) * 4, stream, a.seqs_dev,
+                                a.n_seqs, a.pool.kv_head_begin, a.n_keep, a.n_sink, a.n_recent, a.weights, a.weights_stride,
+                                a.layer_stride, n_cache, a.kept);
   if (e != cudaSuccess) return e;
-  const dim3 per_side(per_row.x, 2 * per_row.y, per_row.z);
-  const auto move = a.pool.fmt == kFmtF16 ? EvictMoveKernel<kFmtF16> : a.pool.fmt == kFmtQ8 ? EvictMoveKernel<kFmtQ8> : EvictMoveKernel<kFmtQ4>;
-  return LaunchChained(move, per_side, kMoveThreads, 0, stream, a.pool, a.tables_dev, a.table_stride, a.seqs_dev, a.n_seqs,
-                       a.dst_pages_dev, a.n_keep, a.kept);
+  const int n_slices = CodeBytes(a.pool.fmt) / kMoveSlice + (a.pool.fmt == kFmtF16 ? 0 : 1);
+  const dim3 grid(per_row.x * n_slices, 2 * per_row.y, per_row.z);
+  return LaunchChained(EvictMoveKernel, grid, kMoveThreads, 0, stream, a.pool, a.tables_dev, a.table_stride, a.seqs_dev, a.n_seqs,
+                       a.dst_pages_dev, a.n_keep, n_slices, a.kept);
 }
 
 cudaError_t LaunchCopyPage(const PoolView& pool, int src, int dst, cudaStream_t stream) {

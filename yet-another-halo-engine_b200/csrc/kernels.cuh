@@ -313,6 +313,7 @@ struct EvictLaunch {
   int n_seqs;
   const std::int32_t* dst_pages_dev;
   int n_keep, n_sink, n_recent;
+  int max_keys;             // longest of the sequences
   float* weights;
   long long weights_stride, layer_stride;   // floats between rows of one (sequence, kv head), and between layers
   std::int32_t* kept;
@@ -320,7 +321,7 @@ struct EvictLaunch {
 cudaError_t LaunchEvict(const EvictLaunch& a, cudaStream_t stream);
 // After LaunchDecodePart of the same plan (its partial_ml holds the rows' statistics); fp16 query.
 cudaError_t LaunchAttnWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream);
-cudaError_t ConfigureWeightKernels();
+cudaError_t ConfigureEvictKernels();   // weights and selection
 cudaError_t LaunchCopyPage(const PoolView& pool, int src, int dst, cudaStream_t stream);
 
 // Rotary positions on given rows (rope.cu).

@@ -295,7 +295,7 @@ int InitDevice(yahkv_ctx* ctx) {
     if (int r = ResizePrefillScratch(ctx, static_cast<std::int64_t>(c.max_prefill_keys) * kKvHeads); r != YAHKV_OK) return r;
   YAHKV_CUDA(ctx, ConfigureDecodeKernels());
   if (c.fmt == YAHKV_FMT_F16) YAHKV_CUDA(ctx, ConfigureF16Kernels());
-  if (!IsTileFmt(c.fmt)) YAHKV_CUDA(ctx, ConfigureWeightKernels());
+  if (!IsTileFmt(c.fmt)) YAHKV_CUDA(ctx, ConfigureEvictKernels());
   {
     int pairs = 0;   // CTA pairs of the prefill kernel that run at the same time: the planner's wave
     YAHKV_CUDA(ctx, ConfigurePrefillKernels(&pairs));
@@ -1055,6 +1055,7 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
   a.seqs_dev = ctx->evict_seqs_dev, a.n_seqs = n_seqs, a.dst_pages_dev = ctx->evict_pages_dev;
   a.n_keep = static_cast<int>(n_keep), a.n_sink = static_cast<int>(n_sink), a.n_recent = static_cast<int>(n_recent);
   a.weights = weights_dev, a.weights_stride = weights_stride, a.layer_stride = weights_layer_stride, a.kept = kept_dev;
+  for (const EvictSeq& s : ctx->evict_scratch) a.max_keys = std::max(a.max_keys, s.n_keys);
   TimedLaunch tl(ctx, YAHKV_KERNEL_EVICT, st);
   YAHKV_CUDA(ctx, LaunchEvict(a, st));
   tl.End();
