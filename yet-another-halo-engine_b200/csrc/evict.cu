@@ -260,7 +260,11 @@ __global__ void __launch_bounds__(kWeightThreads, WeightSmem<kFmt>::kCtas)
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectPer = 4;                                  // keys per thread and turn of the last pass
 constexpr int kSelectTile = kSelectThreads * kSelectPer;
-constexpr int kSelectCache = 48 * 1024;                        // keys whose words are kept in shared memory (192 KB)
+constexpr int kSelectCache = 36 * 1024;                        // keys whose words are kept in shared memory (144 KB)
+// Histograms: a lane counts into copy lane % 8, copies an odd number of words apart, so that equal weights (zeros above
+// all) meet four at a time and not 32 at a time. (One histogram with the lanes of equal bins joined by match.any first:
+// 33 us for 128 rows of 14,000 keys against TODO us.)
+constexpr int kHistCopies = 8, kHistBins = 2048, kHistStride = kHistBins + 1;
 
 // Order-preserving bits of a weight: larger weight, larger word; NaN below everything, -0 equal to +0.
 __device__ __forceinline__ std::uint32_t OrderOf(float w) {
@@ -296,8 +300,9 @@ __global__ void __launch_bounds__(kSelectThreads)
     EvictSelectKernel(const EvictSeq* __restrict__ seqs, int n_seqs, int kv_head_begin, int n_keep, int n_sink, int n_recent,
                       float* __restrict__ weights, long long weights_stride, long long layer_stride, int n_cache,
                       std::int32_t* __restrict__ kept) {
-  extern __shared__ std::uint32_t word_s[];   // [n_cache] words of the first keys of [lo, hi)
-  __shared__ int hist[2048];
+  extern __shared__ std::uint32_t select_smem[];
+  int* hist = reinterpret_cast<int*>(select_smem);
+  std::uint32_t* word_s = select_smem + kHistCopies * kHistStride;   // [n_cache] words of the first keys to choose from
   __shared__ int scan_s[kSelectThreads / 32];
   __shared__ std::uint32_t prefix_s;
   __shared__ int want_s;
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(kSelectThreads)
     const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
-      for (int i = tid; i < 2048; i += kSelectThreads) hist[i] = 0;
+      for (int i = tid; i < kHistCopies * kHistStride; i += kSelectThreads) hist[i] = 0;
       __syncthreads();
       const std::uint32_t bin_mask = (1U << bits[pass]) - 1U;
       for (int i0 = 0; i0 < n_mid; i0 += kSelectTile) {
@@ -338,17 +343,15 @@ __global__ void __launch_bounds__(kSelectThreads)
         for (int k = 0; k < kSelectPer; ++k) {
           const int i = i0 + k * kSelectThreads + tid;
           if (pass == 0 && i < n_held) word_s[i] = o[k];
-          // lanes with the same bin add once (weights that are equal, zeros above all, would serialise otherwise)
-          const bool hit = on[k] && (o[k] & mask) == prefix;
-          const std::uint32_t bin = hit ? (o[k] >> shifts[pass]) & bin_mask : 0xFFFFFFFFU;
-          const unsigned same = __match_any_sync(0xFFFFFFFFU, bin);
-          if (hit && lane == __ffs(same) - 1) atomicAdd(&hist[bin], __popc(same));
+          if (on[k] && (o[k] & mask) == prefix) atomicAdd(&hist[(lane % kHistCopies) * kHistStride + ((o[k] >> shifts[pass]) & bin_mask)], 1);
         }
       }
       __syncthreads();
       // counts from the largest bin down; two bins per thread
-      const int top = 2047 - 2 * tid;
-      const int c0 = hist[top], c1 = hist[top - 1];
+      const int top = kHistBins - 1 - 2 * tid;
+      int c0 = 0, c1 = 0;
+#pragma unroll
+      for (int c = 0; c < kHistCopies; ++c) c0 += hist[c * kHistStride + top], c1 += hist[c * kHistStride + top - 1];
       int total;
       const int before = CtaScan(c0 + c1, scan_s, lane, warp, &total);
       if (before < want && before + c0 >= want) {
@@ -402,66 +405,63 @@ __global__ void __launch_bounds__(kSelectThreads)
 // ----------------------------------------------------------------------------------------------------------------
 // moving the kept rows
 // ----------------------------------------------------------------------------------------------------------------
-constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = 256;                       // rows per chunk
-constexpr int kMoveSlice = 64;                       // bytes of a row one CTA moves (its block scales: 16)
-constexpr int kMovePer = kMoveRows * (kMoveSlice / 16) / kMoveThreads;   // 16-byte pieces per thread and chunk
+constexpr int kMoveThreads = 512;
+constexpr int kMovePer = 4;   // 16-byte pieces of codes per thread and chunk
 
-// One CTA per 64-byte column of the rows of one (layer, sequence, kv head, side), and one for their block scales: columns
-// never meet, so only the order of chunks inside a CTA matters in place. The next chunk's loads are in flight while a
-// chunk is written.
+// One CTA per (layer, sequence, kv head, side): chunks of whole rows (128 of q8_0), so that a row's bytes are asked for
+// together, 32 KB at a time, and the next chunk's loads are in flight while a chunk is written.
+template <int kFmt>
 __global__ void __launch_bounds__(kMoveThreads)
     EvictMoveKernel(PoolView pool, const std::int32_t* __restrict__ tables, int table_stride, const EvictSeq* __restrict__ seqs,
-                    int n_seqs, const std::int32_t* __restrict__ dst_pages, int n_keep, int n_slices,
-                    const std::int32_t* __restrict__ kept) {
+                    int n_seqs, const std::int32_t* __restrict__ dst_pages, int n_keep, const std::int32_t* __restrict__ kept) {
+  constexpr int kPieces = CodeBytes(kFmt) / 16;                     // of a row
+  constexpr int kRows = kMoveThreads * kMovePer / kPieces;          // of a chunk
+  constexpr bool kScales = kFmt != kFmtF16;
+  static_assert(!kScales || kRows <= kMoveThreads, "one thread per row's scales");
   ChainedKernelEntry();
-  const int b = blockIdx.x / n_slices, slice = blockIdx.x % n_slices;
-  const int side = blockIdx.y & 1, h = pool.kv_head_begin + (blockIdx.y >> 1), layer = blockIdx.z;
+  const int b = blockIdx.x, side = blockIdx.y & 1, h = pool.kv_head_begin + (blockIdx.y >> 1), layer = blockIdx.z;
   const EvictSeq es = seqs[b];
   if (es.n_keys <= n_keep) return;
   const int tid = threadIdx.x;
-  const int row_bytes_codes = CodeBytes(pool.fmt);
-  const bool is_scale = slice * kMoveSlice >= row_bytes_codes;
-  const int row_bytes = is_scale ? kBlocksPerRow * 2 : row_bytes_codes;
-  const int per_row = is_scale ? 1 : kMoveSlice / 16;            // 16-byte pieces of a row this CTA moves
-  const int column = is_scale ? 0 : slice * kMoveSlice;
-  std::uint8_t* base = is_scale ? reinterpret_cast<std::uint8_t*>(side == 0 ? pool.kscales : pool.vscales)
-                                : (side == 0 ? pool.kcodes : pool.vcodes);
   const std::int32_t* idx = kept + ((static_cast<std::size_t>(layer) * n_seqs + b) * kKvHeads + h) * static_cast<std::size_t>(n_keep);
   const std::int32_t* table = tables + static_cast<std::size_t>(es.seq) * table_stride;
-  auto row_at = [&](std::int32_t page, int tok) -> std::uint8_t* {
+  const std::int32_t* dst = dst_pages + es.first_dst;
+  uint4* codes = reinterpret_cast<uint4*>(side == 0 ? pool.kcodes : pool.vcodes);
+  uint4* scales = reinterpret_cast<uint4*>(side == 0 ? pool.kscales : pool.vscales);
+  // row of the pools, in rows of one kv head
+  auto row_of = [&](std::int32_t page, int tok) -> std::size_t {
     page = min(max(page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
-    return base + (((static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + h) * kPageTokens + tok) * row_bytes + column;
+    return ((static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + h) * kPageTokens + tok;
   };
-  uint4 v[kMovePer];
+  auto source = [&](int slot) -> std::size_t {
+    const int i = min(max(__ldg(idx + slot), 0), es.n_keys - 1);
+    return row_of(__ldg(table + i / kPageTokens), i % kPageTokens);
+  };
+  auto target = [&](int slot) -> std::size_t { return row_of(__ldg(dst + slot / kPageTokens), slot % kPageTokens); };
+  uint4 v[kMovePer], sc = make_uint4(0, 0, 0, 0);
   auto load = [&](int c0) {
-    int i[kMovePer];
-    std::int32_t page[kMovePer];
+    std::size_t at[kMovePer];
 #pragma unroll
-    for (int k = 0; k < kMovePer; ++k) {
-      const int piece = tid + k * kMoveThreads, slot = c0 + piece / per_row;
-      i[k] = piece < kMoveRows * per_row && slot < n_keep ? min(max(__ldg(idx + slot), 0), es.n_keys - 1) : -1;
-    }
+    for (int k = 0; k < kMovePer; ++k) at[k] = source(min(c0 + (tid + k * kMoveThreads) / kPieces, n_keep - 1));
 #pragma unroll
-    for (int k = 0; k < kMovePer; ++k) page[k] = i[k] >= 0 ? __ldg(table + i[k] / kPageTokens) : 0;
-#pragma unroll
-    for (int k = 0; k < kMovePer; ++k)
-      if (i[k] >= 0)
-        v[k] = *reinterpret_cast<const uint4*>(row_at(page[k], i[k] % kPageTokens) + ((tid + k * kMoveThreads) % per_row) * 16);
+    for (int k = 0; k < kMovePer; ++k) v[k] = codes[at[k] * kPieces + tid % kPieces];
+    if (kScales && tid < kRows) sc = scales[source(min(c0 + tid, n_keep - 1))];
   };
+  static_assert(kMoveThreads % kPieces == 0, "a thread keeps its piece of a row");
   load(0);
-  for (int c0 = 0; c0 < n_keep; c0 += kMoveRows) {
+  for (int c0 = 0; c0 < n_keep; c0 += kRows) {
     uint4 mine[kMovePer];
+    const uint4 my_sc = sc;
 #pragma unroll
     for (int k = 0; k < kMovePer; ++k) mine[k] = v[k];
     __syncthreads();   // every row of the chunk is in registers: its slots may be written
-    if (c0 + kMoveRows < n_keep) load(c0 + kMoveRows);   // sources at or behind the next chunk's first slot
+    if (c0 + kRows < n_keep) load(c0 + kRows);   // sources at or behind the next chunk's first slot
 #pragma unroll
     for (int k = 0; k < kMovePer; ++k) {
-      const int piece = tid + k * kMoveThreads, slot = c0 + piece / per_row;
-      if (piece < kMoveRows * per_row && slot < n_keep)
-        *reinterpret_cast<uint4*>(row_at(__ldg(dst_pages + es.first_dst + slot / kPageTokens), slot % kPageTokens) + (piece % per_row) * 16) = mine[k];
+      const int slot = c0 + (tid + k * kMoveThreads) / kPieces;
+      if (slot < n_keep) codes[target(slot) * kPieces + tid % kPieces] = mine[k];
     }
+    if (kScales && tid < kRows && c0 + tid < n_keep) scales[target(c0 + tid)] = my_sc;
   }
 }
 
@@ -478,6 +478,8 @@ __global__ void __launch_bounds__(256) CopyPageKernel(PoolView pool, int src, in
   for (std::size_t i = static_cast<std::size_t>(blockIdx.z) * 256 + threadIdx.x; i < bytes / 16; i += 256ULL * gridDim.z) to[i] = from[i];
 }
 
+int SelectSmem(int n_cache) { return 4 * (kHistCopies * kHistStride + n_cache); }
+
 template <int kFmt>
 cudaError_t LaunchWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream) {
   return LaunchChained(AttnWeightsKernel<kFmt>, a.n_units, kWeightThreads, WeightSmem<kFmt>::kBytes, stream, *a.kmap, a.pool, a.layer,
@@ -491,7 +493,7 @@ cudaError_t ConfigureEvictKernels() {
   cudaError_t e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtF16>::kBytes);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtQ8>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtQ8>::kBytes);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtQ4>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtQ4>::kBytes);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(EvictSelectKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectCache * 4);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(EvictSelectKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SelectSmem(kSelectCache));
   return e;
 }
 
@@ -507,14 +509,14 @@ cudaError_t LaunchEvict(const EvictLaunch& a, cudaStream_t stream) {
   const dim3 per_row(static_cast<unsigned>(a.n_seqs), static_cast<unsigned>(a.pool.kv_head_count), static_cast<unsigned>(a.pool.n_layers));
   // words of the keys in shared memory, as many as the longest sequence has (what does not fit is read again per pass)
   const int n_cache = std::min(a.max_keys, kSelectCache);
-  cudaError_t e = LaunchChained(EvictSelectKernel, per_row, kSelectThreads, static_cast<std::size_t>(n_cache) * 4, stream, a.seqs_dev,
+  cudaError_t e = LaunchChained(EvictSelectKernel, per_row, kSelectThreads, SelectSmem(n_cache), stream, a.seqs_dev,
                                 a.n_seqs, a.pool.kv_head_begin, a.n_keep, a.n_sink, a.n_recent, a.weights, a.weights_stride,
                                 a.layer_stride, n_cache, a.kept);
   if (e != cudaSuccess) return e;
-  const int n_slices = CodeBytes(a.pool.fmt) / kMoveSlice + (a.pool.fmt == kFmtF16 ? 0 : 1);
-  const dim3 grid(per_row.x * n_slices, 2 * per_row.y, per_row.z);
-  return LaunchChained(EvictMoveKernel, grid, kMoveThreads, 0, stream, a.pool, a.tables_dev, a.table_stride, a.seqs_dev, a.n_seqs,
-                       a.dst_pages_dev, a.n_keep, n_slices, a.kept);
+  const dim3 grid(per_row.x, 2 * per_row.y, per_row.z);
+  const auto move = a.pool.fmt == kFmtF16 ? EvictMoveKernel<kFmtF16> : a.pool.fmt == kFmtQ8 ? EvictMoveKernel<kFmtQ8> : EvictMoveKernel<kFmtQ4>;
+  return LaunchChained(move, grid, kMoveThreads, 0, stream, a.pool, a.tables_dev, a.table_stride, a.seqs_dev, a.n_seqs,
+                       a.dst_pages_dev, a.n_keep, a.kept);
 }
 
 cudaError_t LaunchCopyPage(const PoolView& pool, int src, int dst, cudaStream_t stream) {

@@ -157,17 +157,13 @@ struct yahkv_ctx {
     int n_pairs = 0;            // CTA pairs of the prefix kernel the device runs at once
     int max_tiles = 0;
     std::int64_t max_part_rows = 0;
-    PrefixTile* tiles_dev = nullptr;
-    std::int32_t* rows_dev = nullptr;
-    PrefixItem* prefix_items_dev = nullptr;
-    DecodeUnit* units_dev = nullptr;
-    CombineItem* items_dev = nullptr;
+    char* plan_dev = nullptr;   // the lists of a plan one after the other
+    std::size_t plan_bytes = 0;
     float *part_acc = nullptr, *part_ml = nullptr;
     CUtensorMap k16map{}, v16map{};   // fp16 pages as [rows][256] fp16
   } shared;
   // eviction work lists, allocated by the first call
-  EvictSeq* evict_seqs_dev = nullptr;
-  std::int32_t* evict_pages_dev = nullptr;
+  char* evict_dev = nullptr;
   std::vector<EvictSeq> evict_scratch;
   std::vector<std::int32_t> evict_page_scratch;
 };
@@ -315,9 +311,8 @@ void FreeDevice(yahkv_ctx* ctx) {
                   ctx->tiles_dev,   ctx->status_dev,  ctx->pseqs_dev, ctx->k16_dev, ctx->v16_dev,
                   ctx->merges_dev, ctx->part_acc_dev, ctx->part_ml_dev,
                   ctx->rope_tab_dev, ctx->rope_pos_dev, ctx->open_tiles_dev, ctx->kmean_dev, ctx->state_rows_dev,
-                  ctx->vwork_dev,   ctx->rope_kv16_dev, ctx->shared.tiles_dev, ctx->shared.rows_dev,
-                  ctx->shared.prefix_items_dev, ctx->shared.units_dev, ctx->shared.items_dev, ctx->shared.part_acc,
-                  ctx->shared.part_ml, ctx->evict_seqs_dev, ctx->evict_pages_dev};
+                  ctx->vwork_dev,   ctx->rope_kv16_dev, ctx->shared.plan_dev, ctx->shared.part_acc,
+                  ctx->shared.part_ml, ctx->evict_dev};
   for (void* p : ptrs)
     if (p != nullptr) cudaFree(p);
   for (cudaStream_t st : {ctx->h2d_stream, ctx->d2h_stream})
@@ -905,6 +900,13 @@ int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, 
   return YAHKV_OK;
 }
 
+// The lists of a shared plan in one buffer (one upload): tiles, units, prefix items, items, rows; the sizes of all but the
+// last are multiples of 16 bytes or, of the last two, of their own element.
+static std::size_t SharedPlanBytes(std::size_t tiles, std::size_t units, std::size_t rows) {
+  return tiles * sizeof(PrefixTile) + units * sizeof(DecodeUnit) + rows * kKvHeads * (sizeof(PrefixItem) + sizeof(CombineItem)) +
+         rows * sizeof(std::int32_t);
+}
+
 // What shared-prefix attention needs beyond the context's own buffers; built by the first call that uses it.
 static int EnsureShared(yahkv_ctx* ctx) {
   auto& sh = ctx->shared;
@@ -920,12 +922,8 @@ static int EnsureShared(yahkv_ctx* ctx) {
     sh.max_part_rows = std::max<std::int64_t>(static_cast<std::int64_t>(c.max_seqs) * kQHeads, 4LL * kPrefillTileRows * sh.n_pairs);
   }
   auto alloc = [&](auto** p, std::size_t count) { return *p != nullptr ? cudaSuccess : DevAlloc(ctx, p, count, false); };
-  const std::size_t ns = static_cast<std::size_t>(c.max_seqs);
-  YAHKV_CUDA(ctx, alloc(&sh.tiles_dev, static_cast<std::size_t>(sh.max_tiles)));
-  YAHKV_CUDA(ctx, alloc(&sh.rows_dev, ns));
-  YAHKV_CUDA(ctx, alloc(&sh.prefix_items_dev, ns * kKvHeads));
-  YAHKV_CUDA(ctx, alloc(&sh.units_dev, static_cast<std::size_t>(ctx->max_units)));
-  YAHKV_CUDA(ctx, alloc(&sh.items_dev, ns * kKvHeads));
+  sh.plan_bytes = SharedPlanBytes(static_cast<std::size_t>(sh.max_tiles), static_cast<std::size_t>(ctx->max_units), static_cast<std::size_t>(c.max_seqs));
+  YAHKV_CUDA(ctx, alloc(&sh.plan_dev, sh.plan_bytes));
   YAHKV_CUDA(ctx, alloc(&sh.part_acc, static_cast<std::size_t>(sh.max_part_rows) * kHeadDim));
   YAHKV_CUDA(ctx, alloc(&sh.part_ml, static_cast<std::size_t>(sh.max_part_rows) * 2));
   if (c.fmt == YAHKV_FMT_F16) {
@@ -972,36 +970,34 @@ int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, co
   if (static_cast<int>(plan.tiles.size()) > sh.max_tiles) return Fail(ctx, YAHKV_ERR_CAPACITY, "attend_decode_shared: too many prefix tiles");
   cudaStream_t st = StreamOf(ctx, stream);
   if (int r = FlushTables(ctx, st); r != YAHKV_OK) return r;
-  if (changed) {   // one staging buffer holds all lists so that they share a completion event
-    const std::pair<void*, std::pair<const void*, std::size_t>> lists[] = {
-        {sh.tiles_dev, {plan.tiles.data(), plan.tiles.size() * sizeof(PrefixTile)}},
-        {sh.rows_dev, {plan.rows.data(), plan.rows.size() * sizeof(std::int32_t)}},
-        {sh.prefix_items_dev, {plan.prefix_items.data(), plan.prefix_items.size() * sizeof(PrefixItem)}},
-        {sh.units_dev, {plan.units.data(), plan.units.size() * sizeof(DecodeUnit)}},
-        {sh.items_dev, {plan.items.data(), plan.items.size() * sizeof(CombineItem)}}};
-    std::size_t total = 0;
-    for (const auto& l : lists) total += l.second.second;
+  const std::pair<const void*, std::size_t> lists[] = {{plan.tiles.data(), plan.tiles.size() * sizeof(PrefixTile)},
+                                                       {plan.units.data(), plan.units.size() * sizeof(DecodeUnit)},
+                                                       {plan.prefix_items.data(), plan.prefix_items.size() * sizeof(PrefixItem)},
+                                                       {plan.items.data(), plan.items.size() * sizeof(CombineItem)},
+                                                       {plan.rows.data(), plan.rows.size() * sizeof(std::int32_t)}};
+  std::size_t at[6] = {0};
+  for (int i = 0; i < 5; ++i) at[i + 1] = at[i] + lists[i].second;
+  if (at[5] > sh.plan_bytes) return Fail(ctx, YAHKV_ERR_CAPACITY, "attend_decode_shared: plan larger than its buffer");
+  if (changed) {
     char* buf = nullptr;
-    YAHKV_CUDA(ctx, ctx->staging.Acquire(total, &buf));
-    for (const auto& l : lists) {
-      if (l.second.second == 0) continue;
-      std::memcpy(buf, l.second.first, l.second.second);
-      YAHKV_CUDA(ctx, cudaMemcpyAsync(l.first, buf, l.second.second, cudaMemcpyHostToDevice, st));
-      buf += l.second.second;
-    }
+    YAHKV_CUDA(ctx, ctx->staging.Acquire(at[5], &buf));
+    for (int i = 0; i < 5; ++i)
+      if (lists[i].second > 0) std::memcpy(buf + at[i], lists[i].first, lists[i].second);
+    YAHKV_CUDA(ctx, cudaMemcpyAsync(sh.plan_dev, buf, at[5], cudaMemcpyHostToDevice, st));
     YAHKV_CUDA(ctx, ctx->staging.Release(st));
   }
   DecodeLaunch a{};
   a.kmap = &ctx->kmap, a.vmap = &ctx->vmap, a.pool = ctx->pool, a.layer = layer;
   a.tables_dev = ctx->tables_dev, a.table_stride = ctx->cfg.max_pages_per_seq;
-  a.units_dev = sh.units_dev, a.n_units = static_cast<int>(plan.units.size());
-  a.items_dev = sh.items_dev, a.n_seqs = n_seqs;
+  a.units_dev = reinterpret_cast<const DecodeUnit*>(sh.plan_dev + at[1]), a.n_units = static_cast<int>(plan.units.size());
+  a.items_dev = reinterpret_cast<const CombineItem*>(sh.plan_dev + at[3]), a.n_seqs = n_seqs;
   a.q_dev = q_dev, a.gate_dev = gate_dev, a.out_dev = out_dev, a.out_f32 = out_dtype == YAHKV_OUT_F32;
   a.scale_log2 = ctx->scale_log2;
   a.partial_acc = ctx->partial_acc, a.partial_ml = ctx->partial_ml, a.status_dev = ctx->status_dev;
   SharedLaunch p = SharedArgs(ctx);
-  p.tiles_dev = sh.tiles_dev, p.n_tiles = static_cast<int>(plan.tiles.size()), p.rows_dev = sh.rows_dev;
-  p.prefix_items_dev = sh.prefix_items_dev;
+  p.tiles_dev = reinterpret_cast<const PrefixTile*>(sh.plan_dev), p.n_tiles = static_cast<int>(plan.tiles.size());
+  p.prefix_items_dev = reinterpret_cast<const PrefixItem*>(sh.plan_dev + at[2]);
+  p.rows_dev = reinterpret_cast<const std::int32_t*>(sh.plan_dev + at[4]);
   TimedLaunch ts(ctx, YAHKV_KERNEL_SHARED_PREFIX, st);
   cudaError_t le = LaunchSharedPrefix(a, p, st);
   if (p.n_tiles > 0) ts.End();
@@ -1037,9 +1033,8 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
   if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
   if (n_seqs == 0) return YAHKV_OK;
   const yahkv_config& c = ctx->cfg;
-  if (ctx->evict_seqs_dev == nullptr) YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_seqs_dev, static_cast<std::size_t>(c.max_seqs), false));
-  if (ctx->evict_pages_dev == nullptr)
-    YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_pages_dev, static_cast<std::size_t>(c.max_seqs) * c.max_pages_per_seq, false));
+  if (ctx->evict_dev == nullptr)   // the sequences, then their pages
+    YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_dev, static_cast<std::size_t>(c.max_seqs) * (sizeof(EvictSeq) + 4 * static_cast<std::size_t>(c.max_pages_per_seq)), false));
   cudaStream_t st = StreamOf(ctx, stream);
   if (int r = FlushTables(ctx, st); r != YAHKV_OK) return r;   // the kernels read the tables as they are before the call
   const std::size_t sb = ctx->evict_scratch.size() * sizeof(EvictSeq), pb = ctx->evict_page_scratch.size() * sizeof(std::int32_t);
@@ -1047,12 +1042,12 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
   YAHKV_CUDA(ctx, ctx->staging.Acquire(sb + pb, &buf));
   std::memcpy(buf, ctx->evict_scratch.data(), sb);
   if (pb > 0) std::memcpy(buf + sb, ctx->evict_page_scratch.data(), pb);
-  YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->evict_seqs_dev, buf, sb, cudaMemcpyHostToDevice, st));
-  if (pb > 0) YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->evict_pages_dev, buf + sb, pb, cudaMemcpyHostToDevice, st));
+  YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->evict_dev, buf, sb + pb, cudaMemcpyHostToDevice, st));
   YAHKV_CUDA(ctx, ctx->staging.Release(st));
   EvictLaunch a{};
   a.pool = ctx->pool, a.tables_dev = ctx->tables_dev, a.table_stride = c.max_pages_per_seq;
-  a.seqs_dev = ctx->evict_seqs_dev, a.n_seqs = n_seqs, a.dst_pages_dev = ctx->evict_pages_dev;
+  a.seqs_dev = reinterpret_cast<const EvictSeq*>(ctx->evict_dev), a.n_seqs = n_seqs;
+  a.dst_pages_dev = reinterpret_cast<const std::int32_t*>(ctx->evict_dev + sb);
   a.n_keep = static_cast<int>(n_keep), a.n_sink = static_cast<int>(n_sink), a.n_recent = static_cast<int>(n_recent);
   a.weights = weights_dev, a.weights_stride = weights_stride, a.layer_stride = weights_layer_stride, a.kept = kept_dev;
   for (const EvictSeq& s : ctx->evict_scratch) a.max_keys = std::max(a.max_keys, s.n_keys);
