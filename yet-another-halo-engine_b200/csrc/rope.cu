@@ -102,10 +102,39 @@ __device__ __forceinline__ void LaneAngles(const RopeRowsLaunch& a, long long po
   }
 }
 
-// kHeads rows of one token per warp, all loaded before anything else is waited for.
-template <bool kInF32, bool kOutF32, int kHeads>
+enum PairMode { kInterleavedPairs, kHalfPairs, kAnyPairs };
+// The other half of the pairs of this lane's dims.
+//   kInterleavedPairs  rotary_dim a multiple of 8: neighbours in the lane
+//   kHalfPairs         rotary_dim / 2 a multiple of 8: the same register of the lane rotary_dim / 16 away
+//   kAnyPairs          any even rotary_dim, either layout: through shared memory
+template <int kMode>
+__device__ __forceinline__ void PairOf(const float (&x)[8], float (&other)[8], float* row_s, int half, bool interleaved, int lane) {
+  if constexpr (kMode == kInterleavedPairs) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) other[j] = x[j ^ 1];
+  } else if constexpr (kMode == kHalfPairs) {
+    const int src = 8 * lane < half ? lane + half / 8 : lane - half / 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) other[j] = __shfl_sync(0xFFFFFFFFU, x[j], src & 31);
+  } else {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) row_s[8 * lane + j] = x[j];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int d = 8 * lane + j;
+      other[j] = d >= 2 * half ? 0.0F : interleaved ? row_s[d ^ 1] : row_s[d < half ? d + half : d - half];
+    }
+  }
+}
+
+// kHeads rows of one token per warp, all loaded before anything else is waited for. With w the norm weights (or 1) and
+// o(d) the other dim of d's pair, out_d = inv (x_d (w_d cos) + x_o (w_o (-/+ sin))): the two products in parentheses are
+// made once per token, so a row costs two multiplications and an fma per dim, and the sum of its squares.
+template <bool kInF32, bool kOutF32, int kHeads, int kMode>
 __global__ void __launch_bounds__(32 * kRopeRowWarps) RopeRowsKernel(const RopeRowsLaunch a) {
-  __shared__ float row_s[kRopeRowWarps][kHeadDim];
+  __shared__ float row_s[kRopeRowWarps][kMode == kAnyPairs ? kHeadDim : 1];
   ChainedKernelEntry();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long task = static_cast<long long>(blockIdx.x) * kRopeRowWarps + warp;
@@ -126,67 +155,65 @@ __global__ void __launch_bounds__(32 * kRopeRowWarps) RopeRowsKernel(const RopeR
   }
   float2 cs[8];
   LaneAngles(a, pos, lane, cs);
-  float wt[8];
-  if (a.weight != nullptr) LoadRow8<true>(a.weight, 8 * lane, wt);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)   // the first dim of a pair takes -sin
+    if (a.interleaved ? (j & 1) == 0 : 8 * lane + j < half) cs[j].y = -cs[j].y;
+  if (a.weight != nullptr) {
+    float w[8], wo[8];
+    LoadRow8<true>(a.weight, 8 * lane, w);
+    PairOf<kMode>(w, wo, row_s[warp], half, a.interleaved, lane);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) cs[j].x *= w[j], cs[j].y *= wo[j];
+  }
+  // a dim that is not rotated must not see its neighbour, not even times zero
+  const bool turns = 8 * lane < a.rotary_dim;
 #pragma unroll
   for (int h = 0; h < kHeads; ++h) {
     if (h0 + h >= a.n_heads) break;   // the whole warp at once
+    float inv = 1.0F;
     if (a.weight != nullptr) {
       float acc = 0.0F;
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc = fmaf(x[h][j], x[h][j], acc);
 #pragma unroll
       for (int m = 16; m >= 1; m >>= 1) acc += __shfl_xor_sync(0xFFFFFFFFU, acc, m);
-      const float inv = 1.0F / sqrtf(acc * (1.0F / kHeadDim) + a.eps);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[h][j] = x[h][j] * inv * wt[j];
+      inv = rsqrtf(fmaf(acc, 1.0F / kHeadDim, a.eps));
     }
-    float other[8];   // the pair's other half
-    if (a.interleaved) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) other[j] = x[h][j ^ 1];
-    } else if ((half & 7) == 0) {   // the same register of the lane half / 8 away
-      const int src = 8 * lane < half ? lane + half / 8 : lane - half / 8;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) other[j] = __shfl_sync(0xFFFFFFFFU, x[h][j], src & 31);
-    } else {
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) row_s[warp][8 * lane + j] = x[h][j];
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int d = 8 * lane + j;
-        other[j] = d < a.rotary_dim ? row_s[warp][d < half ? d + half : d - half] : 0.0F;
-      }
-    }
+    float other[8];
+    PairOf<kMode>(x[h], other, row_s[warp], half, a.interleaved, lane);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int d = 8 * lane + j;
-      const bool first = a.interleaved ? (j & 1) == 0 : d < half;
-      if (d < a.rotary_dim) x[h][j] = first ? fmaf(x[h][j], cs[j].x, -(other[j] * cs[j].y)) : fmaf(other[j], cs[j].y, x[h][j] * cs[j].x);
+      x[h][j] *= cs[j].x;
+      if (kMode == kAnyPairs ? 8 * lane + j < a.rotary_dim : turns) x[h][j] = fmaf(other[j], cs[j].y, x[h][j]);
+      if (a.weight != nullptr) x[h][j] *= inv;
     }
     StoreRow8<kOutF32>(a.out, out_at + h * kHeadDim, x[h]);
   }
 }
 
-template <bool kInF32, bool kOutF32>
+template <bool kInF32, bool kOutF32, int kHeads>
 cudaError_t Launch(const RopeRowsLaunch& a, cudaStream_t stream) {
-  // Few rows: one per warp, so that the call fills the device. Many: four rows of a token share the angles.
-  const int heads = static_cast<long long>(a.n_tokens) * a.n_heads < 148 * 64 ? 1 : 4;
-  const long long tasks = static_cast<long long>(a.n_tokens) * ((a.n_heads + heads - 1) / heads);
+  const long long tasks = static_cast<long long>(a.n_tokens) * ((a.n_heads + kHeads - 1) / kHeads);
   const long long grid = (tasks + kRopeRowWarps - 1) / kRopeRowWarps;
   if (grid > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
-  return LaunchChained(heads == 1 ? RopeRowsKernel<kInF32, kOutF32, 1> : RopeRowsKernel<kInF32, kOutF32, 4>,
-                       static_cast<unsigned>(grid), 32 * kRopeRowWarps, 0, stream, a);
+  const auto kernel = a.interleaved && a.rotary_dim % 8 == 0      ? RopeRowsKernel<kInF32, kOutF32, kHeads, kInterleavedPairs>
+                      : !a.interleaved && a.rotary_dim % 16 == 0 ? RopeRowsKernel<kInF32, kOutF32, kHeads, kHalfPairs>
+                                                                 : RopeRowsKernel<kInF32, kOutF32, kHeads, kAnyPairs>;
+  return LaunchChained(kernel, static_cast<unsigned>(grid), 32 * kRopeRowWarps, 0, stream, a);
+}
+template <bool kInF32, bool kOutF32>
+cudaError_t LaunchHeads(const RopeRowsLaunch& a, cudaStream_t stream) {
+  // Few rows: one per warp, so that the call fills the device. Many: four rows of a token share the angles.
+  return static_cast<long long>(a.n_tokens) * a.n_heads < 148 * 64 ? Launch<kInF32, kOutF32, 1>(a, stream)
+                                                                   : Launch<kInF32, kOutF32, 4>(a, stream);
 }
 
 }  // namespace
 
 cudaError_t LaunchRopeRows(const RopeRowsLaunch& a, cudaStream_t stream) {
   if (a.n_tokens <= 0 || a.n_heads <= 0) return cudaSuccess;
-  if (a.x_f32) return a.out_f32 ? Launch<true, true>(a, stream) : Launch<true, false>(a, stream);
-  return a.out_f32 ? Launch<false, true>(a, stream) : Launch<false, false>(a, stream);
+  if (a.x_f32) return a.out_f32 ? LaunchHeads<true, true>(a, stream) : LaunchHeads<true, false>(a, stream);
+  return a.out_f32 ? LaunchHeads<false, true>(a, stream) : LaunchHeads<false, false>(a, stream);
 }
 
 }  // namespace yahkv
