@@ -141,6 +141,17 @@ __device__ __forceinline__ void BulkLoad(void* smem_dst, const void* gsrc, std::
                "l"(reinterpret_cast<std::uint64_t>(gsrc)), "r"(bytes), "r"(SmemAddr(bar))
                : "memory");
 }
+// 1-D bulk copy shared -> global, same alignment rules; the calling thread's earlier shared-memory writes must have been
+// fenced with FenceProxyAsync. BulkStoreWait waits until this thread's copies are complete.
+__device__ __forceinline__ void BulkStore(void* gdst, const void* smem_src, std::uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<std::uint64_t>(gdst)),
+               "r"(SmemAddr(smem_src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void BulkStoreWait() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
 __device__ __forceinline__ void PrefetchTensorMap(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<std::uint64_t>(map)) : "memory");
 }

@@ -51,6 +51,7 @@ constexpr int kPBytes = kTileM * kTileN * 2;
 constexpr int kTmemCols = 512, kColS = 0, kColO = 128, kColQ = 384;   // S 2 x 64, O 256, Q 128 columns
 constexpr float kLazyRescale = 8.0F;
 constexpr int kStatusAbort = 5;
+constexpr int kOutPitch = kHeadDim * 4 + 16;   // an output row in shared memory: four banks further per row
 constexpr int kMaxStages = 5, kMaxRaw = 4;
 
 template <int kFmt>
@@ -76,6 +77,7 @@ struct Shape {
   static constexpr int kSmemP = kSmemV + kVStages * kVHalfBytes;
   static constexpr int kSmemRaw = kSmemP + 2 * kPBytes;
   static constexpr int kSmemBars = kSmemRaw + kRawStages * kRawBytes;
+  static_assert(kTileM * kOutPitch <= kSmemRaw, "the output rows take the place of the tiles");
   static constexpr int kBarBytes = 512;
   static constexpr int kBytes = kSmemBars + kBarBytes + 3 * kTileM * 4;   // barriers, then the max / sum exchange
   static_assert(kBytes <= 232448, "shared memory of one CTA");
@@ -150,22 +152,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
                        const PrefixTile* __restrict__ tiles, const std::int32_t* __restrict__ rows,
                        const __half* __restrict__ q, float scale_log2, float* __restrict__ part_acc,
                        float* __restrict__ part_ml, int* status) {
-  ChainedKernelEntry();
   using S = Shape<kFmt>;
   extern __shared__ __align__(1024) std::uint8_t smem[];
   SharedBars* bars = reinterpret_cast<SharedBars*>(smem + S::kSmemBars);
   static_assert(sizeof(SharedBars) <= S::kBarBytes, "the max / sum exchange follows the barriers");
   volatile int* abort_flag = &bars->abort_flag;
-  const PrefixTile tile = tiles[blockIdx.x];
   const std::uint32_t rank = ClusterCtaRank();   // 0 = leader: its MMA warp issues for the pair
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_tiles = tile.page_end - tile.page_begin;   // at least one, the same in both CTAs
-  const std::int32_t* table = tables + static_cast<std::size_t>(tile.seq) * table_stride + tile.page_begin;
 
   if ((SmemAddr(smem) & 1023U) != 0) {   // the same in both CTAs: either both leave or neither does
+    ChainedKernelEntry();
     if (threadIdx.x == 0) atomicExch(status, kStatusAbort);
     return;
   }
+  // Barriers and tensor memory are set up while the kernels before this one in the stream still run (programmatic
+  // dependent launch); nothing of theirs is read before ChainedKernelEntry.
   if (threadIdx.x == 0) {
     MbarInit(&bars->q_full, 2 * kSoftmaxThreads / 32);
     for (int s = 0; s < S::kKStages; ++s) {
@@ -201,6 +202,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
   ClusterSync();
   TcFenceAfter();
   const std::uint32_t tmem = bars->tmem_base;
+  ChainedKernelEntry();
+  const PrefixTile tile = tiles[blockIdx.x];
+  const int n_tiles = tile.page_end - tile.page_begin;   // at least one, the same in both CTAs
+  const std::int32_t* table = tables + static_cast<std::size_t>(tile.seq) * table_stride + tile.page_begin;
 
   if (warp == kWarpTma) {
     // ------------------------------ producer: this CTA's half of every page ------------------------------
@@ -519,18 +524,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
     NamedBarrierSync(1, kSoftmaxThreads);
     if (ok && n_tiles > 0) {
       TcFenceAfter();
+      // The rows go through shared memory (the tiles have been read) and out as bulk copies, a thread its own 512 B: a
+      // thread's 16-byte stores would hit 32 lines per instruction.
       const std::size_t row = static_cast<std::size_t>(tile.part_row0) + r;
       if (hc == 0 && valid) *reinterpret_cast<float2*>(part_ml + 2 * row) = make_float2(mref[r], l_mine + xsum[kTileM + r]);
+      std::uint8_t* mine = smem + r * kOutPitch + hc * (kHeadDim / 2) * 4;
 #pragma unroll 1
       for (int c0 = 0; c0 < kHeadDim / 2; c0 += 32) {
         std::uint32_t o[32];
         TmemLd32(lane_addr + kColO + hc * (kHeadDim / 2) + c0, o);
         TmemWaitLd();
-        if (valid) {
-          uint4* dst = reinterpret_cast<uint4*>(part_acc + row * kHeadDim + hc * (kHeadDim / 2) + c0);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) dst[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-        }
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(mine + (c0 + 4 * c) * 4) = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+      }
+      FenceProxyAsync();
+      if (valid) {
+        BulkStore(part_acc + row * kHeadDim + hc * (kHeadDim / 2), mine, (kHeadDim / 2) * 4);
+        BulkStoreWait();
       }
     }
   }
