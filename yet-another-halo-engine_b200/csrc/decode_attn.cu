@@ -155,13 +155,17 @@ constexpr float kLazyRescale = 4.0F;
 
 // kQRaw: the query is the raw f32 projection (qraw) and the prologue norms and rotates the unit's six head rows itself,
 // at the position of the sequence's newest key (qrope.cuh).
-template <int kFmt, bool kQRaw>
+// kBeside: the units lie behind prefixes that the kernel launched just before computes; see ChainedKernelEntryBeside.
+template <int kFmt, bool kQRaw, bool kBeside>
 __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
     DecodePartKernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      PoolView pool, int layer, const std::int32_t* __restrict__ tables, int table_stride,
                      const DecodeUnit* __restrict__ units, const __half* __restrict__ q, const QueryRaw qraw,
                      float scale_log2, float* __restrict__ partial_acc, float* __restrict__ partial_ml, int* status) {
-  ChainedKernelEntry();
+  if constexpr (kBeside)
+    ChainedKernelEntryBeside();
+  else
+    ChainedKernelEntry();
   using L = StageLayout<kFmt>;
   using S = SmemLayout<kFmt>;
   constexpr int kPageSets = Shape<kFmt>::kPageSets, kWarps = Shape<kFmt>::kWarps;
@@ -175,6 +179,7 @@ __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + S::kAbortOff);   // a wait gave up
   if ((SmemAddr(smem_raw) & 1023U) != 0) {   // never seen; checked because a misaligned swizzle would corrupt results
     if (threadIdx.x == 0) atomicExch(status, kStatusSmemMisaligned);
+    if constexpr (kBeside) ChainedKernelExitBeside();
     return;
   }
 
@@ -183,7 +188,10 @@ __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
   const int kw = warp & (kKeyGroups - 1);   // key group: keys 16 kw .. 16 kw + 15 of a page
   const int par = warp / kKeyGroups;        // this warp's pages: index par, par + 2, ... of the unit
   const int n_pages = u.page_end - u.page_begin;
-  if (n_pages <= 0) return;   // a unit reserved for growth that holds no page yet: the merge does not count it
+  if (n_pages <= 0) {   // a unit reserved for growth that holds no page yet: the merge does not count it
+    if constexpr (kBeside) ChainedKernelExitBeside();
+    return;
+  }
   const std::int32_t* row = tables + static_cast<std::size_t>(u.seq) * table_stride + u.page_begin;
 
   // Gather of one page into a ring stage: 2 TMA boxes per side (q8_0; 1 for q4_0) + the two scale records, all
@@ -489,6 +497,7 @@ __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
   MergeUnitAndStore<kWarps, true>(reinterpret_cast<float*>(ring), o_acc, m_run, l_run, warp, lane,
                                   partial_acc + static_cast<std::size_t>(u.partial) * kPartialAccFloats,
                                   partial_ml + static_cast<std::size_t>(u.partial) * kPartialMlFloats);
+  if constexpr (kBeside) ChainedKernelExitBeside();
 }
 
 // Merge the units of one (batch row, query head): out = (sum w_i acc_i) / (sum w_i l_i) * sigmoid(gate) with
@@ -554,31 +563,37 @@ __global__ void __launch_bounds__(kHeadDim)
 
 }  // namespace
 
-cudaError_t ConfigureDecodeKernels() {
-  cudaError_t e = cudaFuncSetAttribute(DecodePartKernel<kFmtQ8, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       DecodeSmemBytes<kFmtQ8>());
+template <int kFmt>
+static cudaError_t ConfigurePart() {
+  cudaError_t e = cudaFuncSetAttribute(DecodePartKernel<kFmt, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmt>());
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(DecodePartKernel<kFmtQ8, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmtQ8>());
+    e = cudaFuncSetAttribute(DecodePartKernel<kFmt, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmt>());
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(DecodePartKernel<kFmtQ4, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmtQ4>());
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(DecodePartKernel<kFmtQ4, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmtQ4>());
+    e = cudaFuncSetAttribute(DecodePartKernel<kFmt, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmt>());
   return e;
 }
+cudaError_t ConfigureDecodeKernels() {
+  const cudaError_t e = ConfigurePart<kFmtQ8>();
+  return e != cudaSuccess ? e : ConfigurePart<kFmtQ4>();
+}
 
-template <int kFmt, bool kQRaw>
+template <int kFmt, bool kQRaw, bool kBeside>
 static cudaError_t LaunchPart(const DecodeLaunch& a, cudaStream_t stream) {
   const QueryRaw qr{kQRaw ? static_cast<const float*>(a.q_dev) : nullptr, a.q_weight_dev, a.rope_tab_dev, a.q_eps, a.rope_rows};
-  return LaunchChained(DecodePartKernel<kFmt, kQRaw>, a.n_units, Shape<kFmt>::kThreads, DecodeSmemBytes<kFmt>(), stream,
+  return LaunchChained(DecodePartKernel<kFmt, kQRaw, kBeside>, a.n_units, Shape<kFmt>::kThreads, DecodeSmemBytes<kFmt>(), stream,
                        *a.kmap, *a.vmap, a.pool, a.layer, a.tables_dev, a.table_stride, a.units_dev,
                        kQRaw ? nullptr : static_cast<const __half*>(a.q_dev), qr, a.scale_log2, a.partial_acc,
                        a.partial_ml, a.status_dev);
 }
+template <int kFmt>
+static cudaError_t LaunchPartOf(const DecodeLaunch& a, cudaStream_t stream) {
+  if (a.beside) return a.q_raw ? cudaErrorInvalidValue : LaunchPart<kFmt, false, true>(a, stream);
+  return a.q_raw ? LaunchPart<kFmt, true, false>(a, stream) : LaunchPart<kFmt, false, false>(a, stream);
+}
 
 cudaError_t LaunchDecodePart(const DecodeLaunch& a, cudaStream_t stream) {
   if (a.n_units <= 0 || a.n_seqs <= 0) return cudaSuccess;
-  if (a.pool.fmt == kFmtQ8) return a.q_raw ? LaunchPart<kFmtQ8, true>(a, stream) : LaunchPart<kFmtQ8, false>(a, stream);
-  return a.q_raw ? LaunchPart<kFmtQ4, true>(a, stream) : LaunchPart<kFmtQ4, false>(a, stream);
+  return a.pool.fmt == kFmtQ8 ? LaunchPartOf<kFmtQ8>(a, stream) : LaunchPartOf<kFmtQ4>(a, stream);
 }
 
 cudaError_t LaunchDecodeCombine(const DecodeLaunch& a, cudaStream_t stream) {

@@ -47,14 +47,19 @@ static_assert(kWarps * kDecodeMergeWarpFloats * 4 <= kRingBytes, "the merge scra
 constexpr float kLazyRescale = 4.0F;
 constexpr int kStatusSmemMisaligned = 2;
 
-template <bool kQRaw>   // kQRaw: the raw f32 query, normed and rotated in the prologue (qrope.cuh)
+// kQRaw: the raw f32 query, normed and rotated in the prologue (qrope.cuh). kBeside: the units lie behind prefixes that the
+// kernel launched just before computes; see ChainedKernelEntryBeside.
+template <bool kQRaw, bool kBeside>
 __global__ void __launch_bounds__(kThreads, 1)
     F16DecodePartKernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         PoolView pool, int layer, const std::int32_t* __restrict__ tables, int table_stride,
                         const DecodeUnit* __restrict__ units, const __half* __restrict__ q, const QueryRaw qraw,
                         float scale_log2,
                         float* __restrict__ partial_acc, float* __restrict__ partial_ml, int* status) {
-  ChainedKernelEntry();
+  if constexpr (kBeside)
+    ChainedKernelEntryBeside();
+  else
+    ChainedKernelEntry();
   extern __shared__ __align__(1024) std::uint8_t smem[];
   std::uint32_t* qfrag = reinterpret_cast<std::uint32_t*>(smem + kQfragOff);
   std::uint64_t* full_bar = reinterpret_cast<std::uint64_t*>(smem + kBarOff);
@@ -63,6 +68,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kAbortOff);
   if ((SmemAddr(smem) & 1023U) != 0) {   // never seen; a misaligned swizzle would corrupt results
     if (threadIdx.x == 0) atomicExch(status, kStatusSmemMisaligned);
+    if constexpr (kBeside) ChainedKernelExitBeside();
     return;
   }
 
@@ -72,7 +78,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int par = warp / kKeyGroups;        // this warp's pages: index par, par + 2, ... of the unit
   const int t = lane & 3;
   const int n_pages = u.page_end - u.page_begin;
-  if (n_pages <= 0) return;
+  if (n_pages <= 0) {
+    if constexpr (kBeside) ChainedKernelExitBeside();
+    return;
+  }
   const std::int32_t* row = tables + static_cast<std::size_t>(u.seq) * table_stride + u.page_begin;
 
   // Gather of one page into a ring stage; a whole converged warp calls it, one elected lane issues. Once a wait has
@@ -226,27 +235,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   MergeUnitAndStore<kWarps, false>(reinterpret_cast<float*>(smem), o_acc, m_run, l_run, warp, lane,
                                      partial_acc + static_cast<std::size_t>(u.partial) * kPartialAccFloats,
                                      partial_ml + static_cast<std::size_t>(u.partial) * kPartialMlFloats);
+  if constexpr (kBeside) ChainedKernelExitBeside();
 }
 
 }  // namespace
 
 cudaError_t ConfigureF16Kernels() {
-  cudaError_t e = cudaFuncSetAttribute(F16DecodePartKernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (e != cudaSuccess) return e;
-  return cudaFuncSetAttribute(F16DecodePartKernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  cudaError_t e = cudaFuncSetAttribute(F16DecodePartKernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(F16DecodePartKernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(F16DecodePartKernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  return e;
 }
 
 cudaError_t LaunchF16DecodePart(const DecodeLaunch& a, cudaStream_t stream) {
   if (a.n_units <= 0 || a.n_seqs <= 0) return cudaSuccess;
   if (a.q_raw) {
+    if (a.beside) return cudaErrorInvalidValue;
     const QueryRaw qr{static_cast<const float*>(a.q_dev), a.q_weight_dev, a.rope_tab_dev, a.q_eps, a.rope_rows};
-    return LaunchChained(F16DecodePartKernel<true>, a.n_units, kThreads, kSmemBytes, stream, *a.kmap, *a.vmap, a.pool,
+    return LaunchChained(F16DecodePartKernel<true, false>, a.n_units, kThreads, kSmemBytes, stream, *a.kmap, *a.vmap, a.pool,
                          a.layer, a.tables_dev, a.table_stride, a.units_dev, static_cast<const __half*>(nullptr), qr,
                          a.scale_log2, a.partial_acc, a.partial_ml, a.status_dev);
   }
-  return LaunchChained(F16DecodePartKernel<false>, a.n_units, kThreads, kSmemBytes, stream, *a.kmap, *a.vmap, a.pool,
-                       a.layer, a.tables_dev, a.table_stride, a.units_dev, static_cast<const __half*>(a.q_dev), QueryRaw{},
-                       a.scale_log2, a.partial_acc, a.partial_ml, a.status_dev);
+  return LaunchChained(a.beside ? F16DecodePartKernel<false, true> : F16DecodePartKernel<false, false>, a.n_units, kThreads, kSmemBytes,
+                       stream, *a.kmap, *a.vmap, a.pool, a.layer, a.tables_dev, a.table_stride, a.units_dev,
+                       static_cast<const __half*>(a.q_dev), QueryRaw{}, a.scale_log2, a.partial_acc, a.partial_ml, a.status_dev);
 }
 
 }  // namespace yahkv

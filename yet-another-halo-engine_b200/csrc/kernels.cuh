@@ -237,6 +237,7 @@ struct DecodeLaunch {
   float* partial_acc;
   float* partial_ml;
   int* status_dev;          // sticky error word, 0 = ok
+  bool beside;              // the part kernel may run beside the kernel launched just before it (fp16 query only)
 };
 cudaError_t LaunchDecodePart(const DecodeLaunch& a, cudaStream_t stream);
 // fp16 pages (decode_f16.cu)

@@ -521,6 +521,25 @@ class KvHost {
     // Pages per part. Every (group, kv head, 256 rows) is cut along its pages into parts, one CTA pair each; all pairs
     // of a wave take about as long as the largest part, so for one to four waves the smallest part that fits them is
     // taken, and of those the cheapest: waves x (pages + what a part costs beside its pages).
+    // The suffixes run beside the prefix pass on the SMs it leaves (and on all of them once it is done), so the wave is
+    // the share of the pairs that its work is of all work, in microseconds as measured per page and CTA.
+    {
+      const bool f16 = cfg_.fmt == YAHKV_FMT_F16;
+      const double pair_page = f16 ? 0.75 : 0.95, pair_fixed = 6.0;
+      const double sm_page = f16 ? 0.9 : cfg_.fmt == YAHKV_FMT_Q8_0 ? 0.45 : 0.3, sm_unit = f16 ? 2.5 : cfg_.fmt == YAHKV_FMT_Q8_0 ? 1.25 : 0.6;
+      double prefix = 0.0, suffix = 0.0;
+      std::vector<int> first(static_cast<std::size_t>(n_seqs), 0);
+      for (const Group& g : groups) {
+        prefix += pair_page * hc * g.n_mt * g.pages;
+        for (std::int32_t b : g.rows) first[static_cast<std::size_t>(b)] = g.pages;
+      }
+      prefix += pair_fixed * n_pairs;
+      for (int b = 0; b < n_seqs; ++b) {
+        const std::int64_t pages = (lens[b] + kPageTokens - 1) / kPageTokens - first[static_cast<std::size_t>(b)];
+        if (pages > 0) suffix += hc * (sm_unit + sm_page * static_cast<double>(pages));
+      }
+      n_pairs = std::max(static_cast<int>(n_pairs * prefix / (prefix + 0.5 * suffix) + 0.5), 1);
+    }
     auto pairs_at = [&](int per) {
       long long n = 0;
       for (const Group& g : groups) n += static_cast<long long>(g.n_mt) * hc * ((g.pages + per - 1) / per);

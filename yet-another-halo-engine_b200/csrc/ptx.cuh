@@ -71,6 +71,23 @@ __device__ __forceinline__ void ChainedKernelEntry() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// A kernel B that does not depend on the kernel A launched just before it, only on what came before A, may run beside A:
+//   A begins with ChainedKernelEntryBefore: it waits first and lets B be scheduled then, so B starts when every CTA of A is
+//   resident and what came before A has completed;
+//   B begins with ChainedKernelEntryBeside, which does not wait, and its last CTA leaves through ChainedKernelExitBeside,
+//   which waits for A: B is complete only when A is, so whatever follows B may read what A wrote.
+__device__ __forceinline__ void ChainedKernelEntryBefore() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void ChainedKernelEntryBeside() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __threadfence();   // what came before A has completed: nothing older than that is read from this SM's caches
+}
+__device__ __forceinline__ void ChainedKernelExitBeside() {
+  if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // True in exactly one lane of a fully converged warp (all 32 lanes must execute it).
 __device__ __forceinline__ bool ElectOne() {
   std::uint32_t e;

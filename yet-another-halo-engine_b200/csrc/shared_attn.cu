@@ -161,12 +161,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if ((SmemAddr(smem) & 1023U) != 0) {   // the same in both CTAs: either both leave or neither does
-    ChainedKernelEntry();
+    ChainedKernelEntryBefore();
     if (threadIdx.x == 0) atomicExch(status, kStatusAbort);
     return;
   }
   // Barriers and tensor memory are set up while the kernels before this one in the stream still run (programmatic
-  // dependent launch); nothing of theirs is read before ChainedKernelEntry.
+  // dependent launch); nothing of theirs is read before ChainedKernelEntryBefore. The suffix kernel runs beside this one.
   if (threadIdx.x == 0) {
     MbarInit(&bars->q_full, 2 * kSoftmaxThreads / 32);
     for (int s = 0; s < S::kKStages; ++s) {
@@ -202,7 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
   ClusterSync();
   TcFenceAfter();
   const std::uint32_t tmem = bars->tmem_base;
-  ChainedKernelEntry();
+  ChainedKernelEntryBefore();
   const PrefixTile tile = tiles[blockIdx.x];
   const int n_tiles = tile.page_end - tile.page_begin;   // at least one, the same in both CTAs
   const std::int32_t* table = tables + static_cast<std::size_t>(tile.seq) * table_stride + tile.page_begin;

@@ -998,6 +998,7 @@ int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, co
   p.tiles_dev = reinterpret_cast<const PrefixTile*>(sh.plan_dev), p.n_tiles = static_cast<int>(plan.tiles.size());
   p.prefix_items_dev = reinterpret_cast<const PrefixItem*>(sh.plan_dev + at[2]);
   p.rows_dev = reinterpret_cast<const std::int32_t*>(sh.plan_dev + at[4]);
+  a.beside = p.n_tiles > 0;   // the suffixes run beside the prefix pass
   TimedLaunch ts(ctx, YAHKV_KERNEL_SHARED_PREFIX, st);
   cudaError_t le = LaunchSharedPrefix(a, p, st);
   if (p.n_tiles > 0) ts.End();
