@@ -182,8 +182,6 @@ struct PrefixItem {
 };
 static_assert(sizeof(PrefixItem) == 16, "uploaded as an array");
 constexpr int kSharedMinPages = 1;         // shortest prefix read once for a group
-constexpr double kSharedPartPages = 3.0;   // what a part costs beside its pages, in pages
-constexpr int kSharedMaxParts = 1024;      // prefix parts the combine kernel joins per row
 
 // Partial workspace per unit: acc [6][256] f32 (unnormalised), then ml [6][2] f32 (max in log2 units, sum).
 constexpr int kPartialAccFloats = kGroup * kHeadDim;

@@ -419,24 +419,17 @@ class KvHost {
     plan.key = key_scratch_;
     std::vector<std::int64_t> lens(static_cast<std::size_t>(n_seqs));
     for (int b = 0; b < n_seqs; ++b) lens[static_cast<std::size_t>(b)] = len(seq_ids[b], layer);
-    PlanPrefixes(n_seqs, seq_ids, lens.data(), n_pairs, max_part_rows, &plan);
-    const int hb = kv_head_begin(), hc = kv_head_count();
-    // Pages per suffix unit. Suffixes are short, so what a unit costs beside its pages (prologue, merge, partial: about
-    // two pages' time) decides: the size of least (pages + 2 per unit) / resident CTAs + one last unit, at most 24 pages.
-    // PlanDecode's rule, made for whole contexts, cuts 32 suffixes of 350 tokens into single pages: 14 us against 9.
+    const std::vector<PrefixGroup> groups = FindPrefixes(n_seqs, seq_ids, lens.data());
+    plan.first_page.assign(static_cast<std::size_t>(n_seqs), 0);
+    for (const PrefixGroup& g : groups)
+      for (std::int32_t b : g.rows) plan.first_page[static_cast<std::size_t>(b)] = g.pages;
     std::vector<int> suffix(static_cast<std::size_t>(n_seqs));
     for (int b = 0; b < n_seqs; ++b)
       suffix[static_cast<std::size_t>(b)] = static_cast<int>((lens[static_cast<std::size_t>(b)] + kPageTokens - 1) / kPageTokens) -
                                             plan.first_page[static_cast<std::size_t>(b)];
-    const double slots = 2.0 * n_pairs * (cfg_.fmt == YAHKV_FMT_F16 ? 1 : cfg_.fmt == YAHKV_FMT_Q8_0 ? 2 : 4);
-    int auto_pages = 1;
-    double least = -1.0;
-    for (int p : {1, 2, 4, 6, 8, 12, 16, 24}) {
-      double work = 0.0;
-      for (int n : suffix) work += hc * (n + 2.0 * ((n + p - 1) / p));
-      const double cost = work / slots + p;
-      if (least < 0.0 || cost < least) least = cost, auto_pages = p;
-    }
+    const SharedShape shape = ChooseSharedShape(groups, suffix, n_pairs, n_splits, max_part_rows);
+    BuildPrefixTiles(n_seqs, seq_ids, groups, shape.part_pages, &plan);
+    const int hb = kv_head_begin(), hc = kv_head_count(), auto_pages = shape.unit_pages;
     plan.items.resize(static_cast<std::size_t>(n_seqs) * kKvHeads);
     for (int b = 0; b < n_seqs; ++b) {
       const int first = plan.first_page[static_cast<std::size_t>(b)];
@@ -480,17 +473,14 @@ class KvHost {
   const SharedPlan& shared_plan() const { return shared_; }
   void InvalidateSharedPlan() { shared_.key.clear(); }
 
-  // The prefix part of a shared plan: groups, their tiles and where every row finds its partials.
-  void PlanPrefixes(int n_seqs, const std::int32_t* seq_ids, const std::int64_t* lens, int n_pairs,
-                    std::int64_t max_part_rows, SharedPlan* plan) const {
-    const int hb = kv_head_begin(), hc = kv_head_count();
-    plan->first_page.assign(static_cast<std::size_t>(n_seqs), 0);
-    plan->prefix_items.assign(static_cast<std::size_t>(n_seqs) * kKvHeads, PrefixItem{});
-    struct Group {
-      std::vector<std::int32_t> rows;
-      int pages = 0, n_mt = 0;
-    };
-    std::vector<Group> groups;
+  struct PrefixGroup {
+    std::vector<std::int32_t> rows;   // rows of the call
+    int pages = 0;                    // the prefix they share
+    int n_mt = 0;                     // CTA pairs of 256 (row, query head) pairs
+  };
+  // Rows whose tables start with the same page, and the longest run of pages common to all of them that each has filled.
+  std::vector<PrefixGroup> FindPrefixes(int n_seqs, const std::int32_t* seq_ids, const std::int64_t* lens) const {
+    std::vector<PrefixGroup> groups;
     std::vector<std::pair<std::int32_t, std::int32_t>> by_page;   // (first page, row), rows in order
     for (int b = 0; b < n_seqs; ++b)
       if (lens[b] >= kPageTokens) by_page.emplace_back(table_row(seq_ids[b])[0], b);
@@ -499,7 +489,7 @@ class KvHost {
       std::size_t j = i;
       while (j < by_page.size() && by_page[j].first == by_page[i].first) ++j;
       if (j - i >= 2) {
-        Group g;
+        PrefixGroup g;
         const std::int32_t* base = table_row(seq_ids[by_page[i].second]);
         std::int64_t pages = lens[by_page[i].second] / kPageTokens;
         for (std::size_t k = i; k < j; ++k) {
@@ -517,62 +507,108 @@ class KvHost {
       }
       i = j;
     }
-    if (groups.empty()) return;
-    // Pages per part. Every (group, kv head, 256 rows) is cut along its pages into parts, one CTA pair each; all pairs
-    // of a wave take about as long as the largest part, so for one to four waves the smallest part that fits them is
-    // taken, and of those the cheapest: waves x (pages + what a part costs beside its pages).
-    // The suffixes run beside the prefix pass on the SMs it leaves (and on all of them once it is done), so the wave is
-    // the share of the pairs that its work is of all work, in microseconds as measured per page and CTA.
-    {
-      const bool f16 = cfg_.fmt == YAHKV_FMT_F16;
-      const double pair_page = f16 ? 0.75 : 0.95, pair_fixed = 6.0;
-      const double sm_page = f16 ? 0.9 : cfg_.fmt == YAHKV_FMT_Q8_0 ? 0.45 : 0.3, sm_unit = f16 ? 2.5 : cfg_.fmt == YAHKV_FMT_Q8_0 ? 1.25 : 0.6;
-      double prefix = 0.0, suffix = 0.0;
-      std::vector<int> first(static_cast<std::size_t>(n_seqs), 0);
-      for (const Group& g : groups) {
-        prefix += pair_page * hc * g.n_mt * g.pages;
-        for (std::int32_t b : g.rows) first[static_cast<std::size_t>(b)] = g.pages;
-      }
-      prefix += pair_fixed * n_pairs;
-      for (int b = 0; b < n_seqs; ++b) {
-        const std::int64_t pages = (lens[b] + kPageTokens - 1) / kPageTokens - first[static_cast<std::size_t>(b)];
-        if (pages > 0) suffix += hc * (sm_unit + sm_page * static_cast<double>(pages));
-      }
-      n_pairs = std::max(static_cast<int>(n_pairs * prefix / (prefix + 0.5 * suffix) + 0.5), 1);
-    }
+    return groups;
+  }
+
+  // How a shared plan is cut: pages per prefix part and pages per suffix unit.
+  //
+  // Every (group, kv head, 256 rows) is cut along its pages into parts, one CTA pair each; the pairs of a wave take as
+  // long as the largest part. The suffix units run beside the prefix pass on the SMs it leaves free, and on all of them
+  // once it is done, so the wave need not be the whole device: for every wave size the suffixes' end is estimated from
+  // the measured times of a pair (6 us and 0.75 us per fp16 page, 0.95 us where pages are dequantized) and of a unit
+  // (f16 one CTA per SM, 5 us and 0.9 us per page; q8_0 two, 4 and 0.9; q4_0 four, 4 and 1.6), and the cheapest pair of
+  // sizes is taken. 96 rows x 16421 fp16: 83 us with the whole device and units of two pages, 66 us as chosen here.
+  struct SharedShape {
+    int part_pages = 1, unit_pages = 1;
+  };
+  SharedShape ChooseSharedShape(const std::vector<PrefixGroup>& groups, const std::vector<int>& suffix, int n_pairs, int n_splits,
+                                std::int64_t max_part_rows) const {
+    const int hc = kv_head_count();
+    const bool f16 = cfg_.fmt == YAHKV_FMT_F16, q8 = cfg_.fmt == YAHKV_FMT_Q8_0;
+    const double pair_fixed = 6.0, pair_page = f16 ? 0.75 : 0.95;
+    const double unit_fixed = f16 ? 5.0 : 4.0, unit_page = f16 || q8 ? 0.9 : 1.6;
+    const int ctas = f16 ? 1 : q8 ? 2 : 4;
     auto pairs_at = [&](int per) {
       long long n = 0;
-      for (const Group& g : groups) n += static_cast<long long>(g.n_mt) * hc * ((g.pages + per - 1) / per);
+      for (const PrefixGroup& g : groups) n += static_cast<long long>(g.n_mt) * hc * ((g.pages + per - 1) / per);
       return n;
     };
-    int most = 1;
-    for (const Group& g : groups) most = std::max(most, g.pages);
-    int per = most;
-    double best = -1.0;
-    for (int waves = 1; waves <= 4; ++waves) {
-      int lo = 1, hi = most;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (pairs_at(mid) <= static_cast<long long>(waves) * n_pairs) hi = mid;
-        else lo = mid + 1;
-      }
-      const double n_waves = static_cast<double>((pairs_at(lo) + n_pairs - 1) / n_pairs);
-      const double cost = n_waves * (lo + kSharedPartPages);
-      if (best < 0.0 || cost < best - 1e-9) best = cost, per = lo;
-    }
-    auto rows_at = [&](int p) {
+    auto rows_at = [&](int per) {
       long long n = 0;
-      for (const Group& g : groups) n += static_cast<long long>(g.rows.size()) * kGroup * hc * ((g.pages + p - 1) / p);
+      for (const PrefixGroup& g : groups) n += static_cast<long long>(g.rows.size()) * kGroup * hc * ((g.pages + per - 1) / per);
       return n;
     };
-    while (per < most && rows_at(per) > max_part_rows) ++per;   // one part per tile always fits (24 rows per batch row)
+    int most = 1, longest = 0;
+    for (const PrefixGroup& g : groups) most = std::max(most, g.pages);
+    for (int n : suffix) longest = std::max(longest, n);
+    // units of p pages (or the asked-for number of them per row): how many, their mean time and the longest one's
+    struct Units {
+      int pages;
+      long long count;
+      double mean, longest;
+    };
+    std::vector<Units> cuts;
+    for (int p : {1, 2, 4, 6, 8, 12, 16, 24}) {
+      Units u{p, 0, unit_fixed, unit_fixed};
+      int largest = 0;
+      long long pages = 0;
+      for (int n : suffix) {
+        const int per = n_splits > 0 ? std::max((n + n_splits - 1) / n_splits, 1) : p;
+        u.count += static_cast<long long>(hc) * ((n + per - 1) / per);
+        largest = std::max(largest, std::min(n, per));
+        pages += static_cast<long long>(hc) * n;
+      }
+      u.longest += unit_page * largest;
+      if (u.count > 0) u.mean += unit_page * static_cast<double>(pages) / static_cast<double>(u.count);
+      cuts.push_back(u);
+      if (n_splits > 0 || p >= longest) break;
+    }
+    SharedShape best;
+    double least = -1.0;
+    const int waves_max = groups.empty() ? 1 : 4;
+    for (int step = 0; step <= 10; ++step) {   // the wave: all pairs down to half of them
+      const int wave = groups.empty() ? 0 : std::max(n_pairs - n_pairs * step / 20, 1);
+      for (int waves = 1; waves <= waves_max; ++waves) {
+        int per = 1;
+        double prefix = 0.0;
+        if (!groups.empty()) {   // the smallest part that fits the waves
+          int lo = 1, hi = most;
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (pairs_at(mid) <= static_cast<long long>(waves) * wave) hi = mid;
+            else lo = mid + 1;
+          }
+          per = lo;
+          while (per < most && rows_at(per) > max_part_rows) ++per;   // one part per tile always fits (24 rows per batch row)
+          prefix = static_cast<double>((pairs_at(per) + wave - 1) / wave) * (pair_fixed + pair_page * per);
+        }
+        const int busy = static_cast<int>(std::min<long long>(groups.empty() ? 0 : pairs_at(per), n_pairs));
+        const long long beside = 2LL * (n_pairs - busy) * ctas, all = 2LL * n_pairs * ctas;
+        for (const Units& u : cuts) {
+          const double left = static_cast<double>(u.count) - static_cast<double>(beside) * prefix / u.mean;
+          double end = prefix;
+          if (u.count > 0)
+            end = std::max(end, left > 0.0 ? prefix + left / static_cast<double>(all) * u.mean + 0.5 * u.longest
+                                           : static_cast<double>(u.count) / static_cast<double>(beside) * u.mean + 0.5 * u.longest);
+          end += 0.005 * static_cast<double>(u.count + pairs_at(per));   // the partials: written, read, joined
+          if (least < 0.0 || end < least - 1e-9) least = end, best.part_pages = per, best.unit_pages = u.pages;
+        }
+      }
+      if (groups.empty()) break;
+    }
+    return best;
+  }
+
+  // The tiles of the prefix pass and where every row finds its partials.
+  void BuildPrefixTiles(int n_seqs, const std::int32_t* seq_ids, const std::vector<PrefixGroup>& groups, int per, SharedPlan* plan) const {
+    const int hb = kv_head_begin(), hc = kv_head_count();
+    plan->prefix_items.assign(static_cast<std::size_t>(n_seqs) * kKvHeads, PrefixItem{});
     std::int64_t part_row = 0;
-    for (const Group& g : groups) {
+    for (const PrefixGroup& g : groups) {
       const std::int32_t list = static_cast<std::int32_t>(plan->rows.size());
       const int n_rows = static_cast<int>(g.rows.size()) * kGroup;
       const int n_parts = (g.pages + per - 1) / per;
       plan->rows.insert(plan->rows.end(), g.rows.begin(), g.rows.end());
-      for (std::int32_t b : g.rows) plan->first_page[static_cast<std::size_t>(b)] = g.pages;
       for (int h = hb; h < hb + hc; ++h) {
         for (std::size_t i = 0; i < g.rows.size(); ++i)
           plan->prefix_items[static_cast<std::size_t>(g.rows[i]) * kKvHeads + h] = {

@@ -556,67 +556,75 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
 }
 
 // Joins the prefix parts and the suffix units of one (batch row, query head), prefix first, each in order:
-// out = (sum w_i A_i) / (sum w_i l_i) * sigmoid(gate), w_i = 2^(m_i - M). One CTA per head, thread = output dim.
-__global__ void __launch_bounds__(kHeadDim)
+// out = (sum w_i A_i) / (sum w_i l_i) * sigmoid(gate), w_i = 2^(m_i - M). Two warps per head, half of the output dims
+// each: lane i weighs partials i, i + 32, ... and holds four dims, so nothing is exchanged but by shuffles. The merge is
+// latency-bound, so the first rows are fetched before their weights are known. (A CTA per head with its barriers: 12 us
+// on 96 rows of nine partials against 5.)
+constexpr int kCombineWarps = 8;
+constexpr int kCombineEarly = 12;
+__global__ void __launch_bounds__(32 * kCombineWarps)
     SharedCombineKernel(const PrefixItem* __restrict__ prefix_items, const float* __restrict__ prefix_acc,
                         const float* __restrict__ prefix_ml, const CombineItem* __restrict__ items,
                         const float* __restrict__ partial_acc, const float* __restrict__ partial_ml,
-                        const float* __restrict__ gate, void* out, int out_f32) {
-  __shared__ float w_s[kSharedMaxParts + kCombineMaxUnits], l_s[kSharedMaxParts + kCombineMaxUnits];
-  __shared__ float red_s[kHeadDim / 32];
-  __shared__ float inv_l;
+                        const float* __restrict__ gate, void* out, int out_f32, int n_heads) {
   ChainedKernelEntry();
-  const int b = blockIdx.x / kQHeads, hh = blockIdx.x % kQHeads;
-  const int kvh = hh / kGroup, j = hh % kGroup;
+  const int task = blockIdx.x * kCombineWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int head = task >> 1, dim0 = (task & 1) * (kHeadDim / 2) + 4 * lane;
+  if (head >= n_heads) return;
+  const int b = head / kQHeads, hh = head % kQHeads, kvh = hh / kGroup, j = hh % kGroup;
   const PrefixItem pi = prefix_items[b * kKvHeads + kvh];
   const CombineItem it = items[b * kKvHeads + kvh];
-  const int np = min(pi.n_parts, kSharedMaxParts), n = np + min(it.n_partials, kCombineMaxUnits);
+  const int np = pi.n_parts, n = np + it.n_partials;
   if (n <= 0) return;   // a kv head outside the context's range
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const float* acc_p = prefix_acc + (static_cast<std::size_t>(pi.first) + j) * kHeadDim + tid;
-  const std::size_t stride_p = static_cast<std::size_t>(pi.stride) * kHeadDim;
-  const float* acc_u = partial_acc + static_cast<std::size_t>(it.first_partial) * kPartialAccFloats + j * kHeadDim + tid;
-  // the first rows of the weighted sum are fetched before their weights are known
-  constexpr int kEarly = 24;
-  float early[kEarly];
+  auto ml_of = [&](int i) {
+    return i < np ? *reinterpret_cast<const float2*>(prefix_ml + 2 * (pi.first + static_cast<std::size_t>(i) * pi.stride + j))
+                  : *reinterpret_cast<const float2*>(partial_ml + (static_cast<std::size_t>(it.first_partial) + (i - np)) * kPartialMlFloats + 2 * j);
+  };
+  auto row_of = [&](int i) {
+    return *reinterpret_cast<const float4*>(
+        (i < np ? prefix_acc + (pi.first + static_cast<std::size_t>(i) * pi.stride + j) * kHeadDim
+                : partial_acc + (static_cast<std::size_t>(it.first_partial) + (i - np)) * kPartialAccFloats + j * kHeadDim) + dim0);
+  };
+  const float2 first = lane < n ? ml_of(lane) : make_float2(-INFINITY, 0.0F);
+  float4 early[kCombineEarly];
 #pragma unroll
-  for (int i = 0; i < kEarly; ++i)
-    early[i] = i < np ? acc_p[i * stride_p] : i < n ? acc_u[static_cast<std::size_t>(i - np) * kPartialAccFloats] : 0.0F;
-  float mx = -INFINITY;
-  for (int i = tid; i < n; i += kHeadDim) {
-    const float2 ml = i < np ? *reinterpret_cast<const float2*>(prefix_ml + 2 * (pi.first + static_cast<std::size_t>(i) * pi.stride + j))
-                             : *reinterpret_cast<const float2*>(partial_ml + (static_cast<std::size_t>(it.first_partial) + (i - np)) * kPartialMlFloats + 2 * j);
-    w_s[i] = ml.x, l_s[i] = ml.y;
-    mx = fmaxf(mx, ml.x);
-  }
+  for (int i = 0; i < kCombineEarly; ++i)
+    if (i < n) early[i] = row_of(i);
+  float M = first.x;
+  for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, ml_of(i).x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFU, mx, o));
-  if (lane == 0) red_s[warp] = mx;
-  __syncthreads();
-  float M = red_s[0];
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFU, M, o));
+  float A[4] = {0.0F, 0.0F, 0.0F, 0.0F}, L = 0.0F;
+  auto add = [&](float w, float wl, int i, const float4& x) {
+    const float wi = __shfl_sync(0xFFFFFFFFU, w, i);
+    L += __shfl_sync(0xFFFFFFFFU, wl, i);
+    A[0] = fmaf(wi, x.x, A[0]), A[1] = fmaf(wi, x.y, A[1]), A[2] = fmaf(wi, x.z, A[2]), A[3] = fmaf(wi, x.w, A[3]);
+  };
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const float2 ml = i0 == 0 ? first : i0 + lane < n ? ml_of(i0 + lane) : make_float2(-INFINITY, 0.0F);
+    const float w = ml.x == -INFINITY ? 0.0F : Exp2Fast(ml.x - M);
+    const float wl = w * ml.y;
+    const int m = min(n - i0, 32);
+    int i = 0;
+    if (i0 == 0) {
 #pragma unroll
-  for (int w = 1; w < kHeadDim / 32; ++w) M = fmaxf(M, red_s[w]);
-  for (int i = tid; i < n; i += kHeadDim) w_s[i] = w_s[i] == -INFINITY ? 0.0F : Exp2Fast(w_s[i] - M);   // the thread's own entries
-  __syncthreads();
-  if (tid == 0) {
-    float sum = 0.0F;
-    for (int i = 0; i < n; ++i) sum = fmaf(w_s[i], l_s[i], sum);
-    inv_l = 1.0F / sum;
-  }
-  float A = 0.0F;
-#pragma unroll
-  for (int i = 0; i < kEarly; ++i) A = fmaf(i < n ? w_s[i] : 0.0F, early[i], A);
+      for (; i < kCombineEarly; ++i)
+        if (i < m) add(w, wl, i, early[i]);
+    }
 #pragma unroll 8
-  for (int i = kEarly; i < n; ++i)
-    A = fmaf(w_s[i], i < np ? acc_p[i * stride_p] : acc_u[static_cast<std::size_t>(i - np) * kPartialAccFloats], A);
-  __syncthreads();
-  float o = A * inv_l;
-  const std::size_t oi = (static_cast<std::size_t>(b) * kQHeads + hh) * kHeadDim + tid;
-  if (gate != nullptr) o *= 1.0F / (1.0F + expf(-gate[oi]));
-  if (out_f32)
-    static_cast<float*>(out)[oi] = o;
-  else
-    static_cast<__half*>(out)[oi] = __float2half_rn(o);
+    for (; i < m; ++i) add(w, wl, i, row_of(i0 + i));
+  }
+  const float inv = 1.0F / L;
+  const std::size_t at = (static_cast<std::size_t>(b) * kQHeads + hh) * kHeadDim + dim0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    float o = A[c] * inv;
+    if (gate != nullptr) o *= 1.0F / (1.0F + expf(-gate[at + c]));
+    if (out_f32)
+      static_cast<float*>(out)[at + c] = o;
+    else
+      static_cast<__half*>(out)[at + c] = __float2half_rn(o);
+  }
 }
 
 template <int kFmt>
@@ -656,8 +664,10 @@ cudaError_t LaunchSharedPrefix(const DecodeLaunch& a, const SharedLaunch& p, cud
 
 cudaError_t LaunchSharedCombine(const DecodeLaunch& a, const SharedLaunch& p, cudaStream_t stream) {
   if (a.n_seqs <= 0) return cudaSuccess;
-  return LaunchChained(SharedCombineKernel, a.n_seqs * kQHeads, kHeadDim, 0, stream, p.prefix_items_dev, p.part_acc, p.part_ml,
-                       a.items_dev, a.partial_acc, a.partial_ml, a.gate_dev, a.out_dev, a.out_f32);
+  const int heads = a.n_seqs * kQHeads;
+  return LaunchChained(SharedCombineKernel, (2 * heads + kCombineWarps - 1) / kCombineWarps, 32 * kCombineWarps, 0, stream,
+                       p.prefix_items_dev, p.part_acc, p.part_ml, a.items_dev, a.partial_acc, a.partial_ml, a.gate_dev, a.out_dev,
+                       a.out_f32, heads);
 }
 
 }  // namespace yahkv
