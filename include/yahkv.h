@@ -366,6 +366,11 @@ void yahkv_batch_destroy(yahkv_batch* batch);
 /* Split-K units per (sequence, kv head) for the batch's longest sequence, as n_splits of yahkv_attend_decode (0 =
  * automatic, the default); shorter sequences get units of the same page count. Takes effect at the next batch_prepare. */
 int yahkv_batch_set_splits(yahkv_batch* batch, int32_t n_splits);
+/* on != 0: from the next batch_prepare on, the steps compute every prefix that rows of the batch share (yahkv_seq_fork) once
+ * for all of them, as yahkv_attend_decode_shared does; the groups are found at batch_prepare and hold for its horizon.
+ * Allocates on first use, so call it before a capture. Refused for the tile formats. The number of prefix tiles is part
+ * of the layout that *layout_changed reports. */
+int yahkv_batch_set_shared(yahkv_batch* batch, int32_t on);
 int yahkv_batch_prepare(yahkv_batch* batch, int32_t horizon_steps, int32_t* layout_changed, void* stream);
 int yahkv_batch_plan(yahkv_batch* batch, void* stream);
 int yahkv_batch_decode_layer(yahkv_batch* batch, int32_t layer, const void* k_dev, const void* v_dev, const void* q_dev,

@@ -107,3 +107,13 @@ def test_shared_prefix_planner_on_the_host(tmp_path):
     assert r.returncode == 0, r.stderr[-3000:]
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "shared_planner_test: ok" in r.stdout, r.stdout + r.stderr
+
+
+def test_cpp_adapter_calls_on_a_host_only_context(tmp_path):
+    exe = tmp_path / "longctx_test"
+    cmd = ["g++", "-std=c++20", "-O1", "-Wall", "-Wextra", "-I", os.path.join(ROOT, "include"), "-I", PKG,
+           os.path.join(ROOT, "tests", "cpp", "longctx_test.cc"), yahkv.LIB_PATH, "-Wl,-rpath," + PKG, "-o", str(exe)]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-3000:]
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "longctx_test: ok" in r.stdout, r.stdout + r.stderr

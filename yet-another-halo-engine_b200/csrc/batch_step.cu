@@ -25,17 +25,18 @@ __global__ void BatchPlanKernel(const std::int32_t* __restrict__ lens, const Bat
   const BatchSeq bs = seqs[b];
   const int pos = max(lens[b], 0);
   const int n = pos + 1;
-  const int pages = min((n + kPageTokens - 1) / kPageTokens, table_stride);
+  // units cover the pages behind the row's shared prefix
+  const int pages = max(min((n + kPageTokens - 1) / kPageTokens, table_stride) - bs.first_page, 0);
   const int used = min((pages + unit_pages - 1) / unit_pages, bs.n_units);
   const int first = bs.first_unit + h * bs.n_units;
   items[idx] = {first, used};
   for (int k = 0; k < bs.n_units; ++k) {
     DecodeUnit u;
     u.batch = b, u.seq = bs.seq_row, u.kvh = h;
-    u.page_begin = min(k * unit_pages, pages);
+    u.page_begin = bs.first_page + min(k * unit_pages, pages);
     // the last reserved unit takes whatever is left, so an under-reserved batch degrades to longer units, never to
     // missing keys
-    u.page_end = k == bs.n_units - 1 ? pages : min((k + 1) * unit_pages, pages);
+    u.page_end = bs.first_page + (k == bs.n_units - 1 ? pages : min((k + 1) * unit_pages, pages));
     u.n_keys = n;
     u.partial = first + k;
     u.pad = bs.open_cur;

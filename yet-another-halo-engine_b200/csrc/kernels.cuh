@@ -103,6 +103,7 @@ struct BatchSeq {
   std::int32_t first_unit;
   std::int32_t n_units;
   std::int32_t open_cur;    // tile formats: the sequence's current open-tile buffer (the same in every layer)
+  std::int32_t first_page;  // pages before it belong to a prefix that the batch computes once for its rows (0: none)
 };
 struct VTileWork;
 // vwork_dev / state_rows_dev: tile formats only (else null): per batch row the V tile work item of this step's token and

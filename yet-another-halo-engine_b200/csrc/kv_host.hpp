@@ -179,13 +179,17 @@ class KvHost {
   // A new sequence whose first n_tokens / 64 pages are seq's own (counted references, never written while shared) and
   // whose length is n_tokens in every layer. A prefix that ends inside a page takes a page of its own for the rest:
   // *copy_src / *copy_dst then name the page to copy (-1: nothing to copy). Nothing changes on error.
-  HostError SeqFork(int seq, std::int64_t n_tokens, std::int32_t* out, std::int32_t* copy_src, std::int32_t* copy_dst) {
+  HostError CheckFork(int seq, std::int64_t n_tokens) const {
     if (!live(seq)) return {YAHKV_ERR_INVALID, "seq_fork: not a live sequence: " + std::to_string(seq)};
     if (n_tokens < 0) return {YAHKV_ERR_INVALID, "seq_fork: negative token count"};
     for (int l = 0; l < cfg_.n_layers; ++l)
       if (len(seq, l) < n_tokens)
         return {YAHKV_ERR_ORDER, "seq_fork: sequence " + std::to_string(seq) + " holds " + std::to_string(len(seq, l)) +
                                      " tokens in layer " + std::to_string(l) + ", " + std::to_string(n_tokens) + " asked for"};
+    return {};
+  }
+  HostError SeqFork(int seq, std::int64_t n_tokens, std::int32_t* out, std::int32_t* copy_src, std::int32_t* copy_dst) {
+    if (HostError bad = CheckFork(seq, n_tokens); bad.code != YAHKV_OK) return bad;
     const int whole = static_cast<int>(n_tokens / kPageTokens);
     const bool rest = n_tokens % kPageTokens != 0;
     if (rest && free_pages_.empty()) return {YAHKV_ERR_NO_PAGES, "seq_fork: no free page for the prefix's last, partly filled page"};

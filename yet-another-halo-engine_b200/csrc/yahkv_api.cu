@@ -884,7 +884,8 @@ int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, 
   if (out == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "seq_fork: null out pointer");
   if (IsTileFmt(ctx->cfg.fmt))
     return Fail(ctx, YAHKV_ERR_INVALID, "seq_fork: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (the newest tile is no page)");
-  if (n_tokens > 0 && n_tokens % kPageTokens != 0)
+  if (HostError bad = ctx->host.CheckFork(seq, n_tokens); bad.code != YAHKV_OK) return FailHost(ctx, std::move(bad));
+  if (n_tokens % kPageTokens != 0)
     if (int r = RequireDevice(ctx, "seq_fork"); r != YAHKV_OK) return r;   // the last page is copied
   std::int32_t src = -1, dst = -1, made = -1;
   HostError e = ctx->host.SeqFork(seq, n_tokens, &made, &src, &dst);
@@ -1466,13 +1467,20 @@ struct yahkv_batch {
   int units_cap = 0;
   int n_splits = 0;      // units per (sequence, kv head) asked for with yahkv_batch_set_splits; 0 = automatic
   int unit_pages = 0;    // pages per unit of the prepared horizon (a parameter of the plan kernel)
+  // shared prefixes (yahkv_batch_set_shared): the prepared horizon's prefix tiles, row list and prefix items, one buffer
+  bool shared = false;
+  char* prefix_dev = nullptr;
+  std::size_t prefix_cap = 0;
+  int n_tiles = 0;
+  std::size_t rows_at = 0, prefix_items_at = 0;
+  void* q16_dev = nullptr;   // batch_decode_layer_raw: the normed, rotated query
 };
 namespace {
 constexpr int kBatchUnitPages = 24;   // the automatic planner's unit size on large batches (kv_host.hpp)
 void BatchFree(yahkv_batch* b) {
   for (void* p : {static_cast<void*>(b->lens_dev), static_cast<void*>(b->rows_dev), static_cast<void*>(b->units_dev),
                   static_cast<void*>(b->items_dev), static_cast<void*>(b->slots_dev), static_cast<void*>(b->vwork_dev),
-                  static_cast<void*>(b->state_rows_dev)})
+                  static_cast<void*>(b->state_rows_dev), static_cast<void*>(b->prefix_dev), b->q16_dev})
     if (p != nullptr) cudaFree(p);
   delete b;
 }
@@ -1534,6 +1542,23 @@ int yahkv_batch_set_splits(yahkv_batch* b, int32_t n_splits) {
   return YAHKV_OK;
 }
 
+int yahkv_batch_set_shared(yahkv_batch* b, int32_t on) {
+  if (b == nullptr) return YAHKV_ERR_INVALID;
+  yahkv_ctx* ctx = b->ctx;
+  if (int r = RequireDevice(ctx, "batch_set_shared"); r != YAHKV_OK) return r;
+  if (on != 0 && IsTileFmt(ctx->cfg.fmt))
+    return Fail(ctx, YAHKV_ERR_INVALID, "batch_set_shared: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (their sequences share no pages)");
+  if (on != 0) {   // everything a step needs exists before a capture
+    if (int r = EnsureShared(ctx); r != YAHKV_OK) return r;
+    const std::size_t n = b->seqs.size();
+    b->prefix_cap = SharedPlanBytes(static_cast<std::size_t>(ctx->shared.max_tiles), 0, n);
+    if (b->prefix_dev == nullptr) YAHKV_CUDA(ctx, cudaMalloc(reinterpret_cast<void**>(&b->prefix_dev), b->prefix_cap));
+    if (b->q16_dev == nullptr) YAHKV_CUDA(ctx, cudaMalloc(&b->q16_dev, n * kQHeads * kHeadDim * 2));
+  }
+  b->shared = on != 0;   // takes effect at the next batch_prepare
+  return YAHKV_OK;
+}
+
 int yahkv_batch_prepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_changed, void* stream) {
   if (b == nullptr) return YAHKV_ERR_INVALID;
   yahkv_ctx* ctx = b->ctx;
@@ -1571,8 +1596,24 @@ int yahkv_batch_prepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_c
   // sequence would need more than max_splits units (its last unit would otherwise take all the rest). Even, because
   // the part kernels' two page sets take alternate pages.
   int unit_pages = b->n_splits > 0 ? 1 : kBatchUnitPages;
+  // Shared prefixes: what rows have in common and filled now stays so while they grow, so the prefix tiles of the whole
+  // horizon are laid out here; the units then start behind the prefixes.
+  KvHost::SharedPlan prefix;
+  std::vector<int> first_page(static_cast<std::size_t>(n), 0);
+  if (b->shared) {
+    const std::vector<std::int64_t> lens(b->lens.begin(), b->lens.end());
+    const auto groups = ctx->host.FindPrefixes(n, b->seqs.data(), lens.data());
+    for (const auto& g : groups)
+      for (std::int32_t row : g.rows) first_page[static_cast<std::size_t>(row)] = g.pages;
+    std::vector<int> suffix(static_cast<std::size_t>(n));
+    for (int i = 0; i < n; ++i) suffix[i] = (b->lens[i] + horizon_steps + kPageTokens - 1) / kPageTokens - first_page[i];
+    const auto shape = ctx->host.ChooseSharedShape(groups, suffix, ctx->shared.n_pairs, b->n_splits, ctx->shared.max_part_rows);
+    ctx->host.BuildPrefixTiles(n, b->seqs.data(), groups, shape.part_pages, &prefix);
+    if (static_cast<int>(prefix.tiles.size()) > ctx->shared.max_tiles) return Fail(ctx, YAHKV_ERR_CAPACITY, "batch_prepare: too many prefix tiles");
+    if (!groups.empty() && b->n_splits == 0) unit_pages = shape.unit_pages;
+  }
   for (int i = 0; i < n; ++i) {
-    const int pages = (b->lens[i] + horizon_steps + kPageTokens - 1) / kPageTokens;
+    const int pages = (b->lens[i] + horizon_steps + kPageTokens - 1) / kPageTokens - first_page[i];
     const int cap = b->n_splits > 0 ? b->n_splits : ctx->cfg.max_splits;
     unit_pages = std::max(unit_pages, (pages + cap - 1) / cap);
   }
@@ -1584,8 +1625,9 @@ int yahkv_batch_prepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_c
   std::vector<BatchSeq> rows(static_cast<std::size_t>(n));
   int total = 0;
   for (int i : order) {
-    const int pages = (b->lens[i] + horizon_steps + kPageTokens - 1) / kPageTokens;
+    const int pages = (b->lens[i] + horizon_steps + kPageTokens - 1) / kPageTokens - first_page[i];
     BatchSeq r{};
+    r.first_page = first_page[i];
     r.seq_row = b->seqs[i];
     r.open_cur = IsTileFmt(ctx->cfg.fmt) ? ctx->host.open_cur(b->seqs[i], 0) : 0;
     r.n_units = std::min(std::max((pages + unit_pages - 1) / unit_pages, 1), ctx->cfg.max_splits);
@@ -1594,7 +1636,8 @@ int yahkv_batch_prepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_c
     rows[static_cast<std::size_t>(i)] = r;
   }
   if (total > b->units_cap) return Fail(ctx, YAHKV_ERR_CAPACITY, "batch_prepare: more split-K units than the workspace holds");
-  bool changed = rows.size() != b->rows.size() || total != b->total_units || unit_pages != b->unit_pages;
+  const int n_tiles = static_cast<int>(prefix.tiles.size());
+  bool changed = rows.size() != b->rows.size() || total != b->total_units || unit_pages != b->unit_pages || n_tiles != b->n_tiles;
   for (std::size_t i = 0; !changed && i < rows.size(); ++i)
     changed = rows[i].n_units != b->rows[i].n_units || rows[i].first_unit != b->rows[i].first_unit;
   if (layout_changed != nullptr) *layout_changed = changed ? 1 : 0;
@@ -1610,6 +1653,23 @@ int yahkv_batch_prepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_c
     YAHKV_CUDA(ctx, cudaMemcpyAsync(b->rows_dev, buf + lb, rb, cudaMemcpyHostToDevice, st));
     YAHKV_CUDA(ctx, ctx->staging.Release(st));
   }
+  if (n_tiles > 0) {
+    // tiles, then items and rows at offsets that do not depend on the number of tiles: a captured graph holds them
+    const std::size_t tb = prefix.tiles.size() * sizeof(PrefixTile), ib = prefix.prefix_items.size() * sizeof(PrefixItem);
+    const std::size_t rb = prefix.rows.size() * sizeof(std::int32_t);
+    b->prefix_items_at = static_cast<std::size_t>(ctx->shared.max_tiles) * sizeof(PrefixTile);
+    b->rows_at = b->prefix_items_at + ib;
+    if (b->rows_at + rb > b->prefix_cap) return Fail(ctx, YAHKV_ERR_CAPACITY, "batch_prepare: prefix lists larger than their buffer");
+    char* buf = nullptr;
+    YAHKV_CUDA(ctx, ctx->staging.Acquire(tb + ib + rb, &buf));
+    std::memcpy(buf, prefix.tiles.data(), tb);
+    std::memcpy(buf + tb, prefix.prefix_items.data(), ib);
+    std::memcpy(buf + tb + ib, prefix.rows.data(), rb);
+    YAHKV_CUDA(ctx, cudaMemcpyAsync(b->prefix_dev, buf, tb, cudaMemcpyHostToDevice, st));
+    YAHKV_CUDA(ctx, cudaMemcpyAsync(b->prefix_dev + b->prefix_items_at, buf + tb, ib + rb, cudaMemcpyHostToDevice, st));
+    YAHKV_CUDA(ctx, ctx->staging.Release(st));
+  }
+  b->n_tiles = n_tiles;
   b->rows = std::move(rows);
   b->total_units = total;
   b->unit_pages = unit_pages;
@@ -1630,6 +1690,21 @@ int yahkv_batch_plan(yahkv_batch* b, void* stream) {
   return YAHKV_OK;
 }
 
+// The attention of one layer's step with shared prefixes: prefix pass, the units behind the prefixes beside it, combine.
+static int BatchAttendShared(yahkv_batch* b, DecodeLaunch& a, int launches_before, cudaStream_t st) {
+  yahkv_ctx* ctx = b->ctx;
+  SharedLaunch p = SharedArgs(ctx);
+  p.tiles_dev = reinterpret_cast<const PrefixTile*>(b->prefix_dev), p.n_tiles = b->n_tiles;
+  p.prefix_items_dev = reinterpret_cast<const PrefixItem*>(b->prefix_dev + b->prefix_items_at);
+  p.rows_dev = reinterpret_cast<const std::int32_t*>(b->prefix_dev + b->rows_at);
+  a.beside = true;
+  YAHKV_CUDA(ctx, LaunchSharedPrefix(a, p, st));
+  YAHKV_CUDA(ctx, ctx->cfg.fmt == YAHKV_FMT_F16 ? LaunchF16DecodePart(a, st) : LaunchDecodePart(a, st));
+  YAHKV_CUDA(ctx, LaunchSharedCombine(a, p, st));
+  ctx->launches += launches_before + 3;
+  return YAHKV_OK;
+}
+
 int yahkv_batch_decode_layer(yahkv_batch* b, int32_t layer, const void* k_dev, const void* v_dev, const void* q_dev,
                              const float* gate_dev, void* out_dev, int32_t out_dtype, void* stream) {
   if (b == nullptr) return YAHKV_ERR_INVALID;
@@ -1639,6 +1714,8 @@ int yahkv_batch_decode_layer(yahkv_batch* b, int32_t layer, const void* k_dev, c
   if (out_dtype != YAHKV_OUT_F16 && out_dtype != YAHKV_OUT_F32) return Fail(ctx, YAHKV_ERR_INVALID, "batch_decode_layer: bad out_dtype");
   if (k_dev == nullptr || v_dev == nullptr || q_dev == nullptr || out_dev == nullptr)
     return Fail(ctx, YAHKV_ERR_INVALID, "batch_decode_layer: null device pointer");
+  if (b->n_tiles > 0 && (reinterpret_cast<std::uintptr_t>(q_dev) & 15) != 0)
+    return Fail(ctx, YAHKV_ERR_INVALID, "batch_decode_layer: q must be 16-byte aligned with shared prefixes");
   if (b->total_units == 0) return Fail(ctx, YAHKV_ERR_ORDER, "batch_decode_layer: call batch_prepare first");
   cudaStream_t st = StreamOf(ctx, stream);
   const int n = static_cast<int>(b->seqs.size());
@@ -1658,6 +1735,7 @@ int yahkv_batch_decode_layer(yahkv_batch* b, int32_t layer, const void* k_dev, c
   a.q_dev = q_dev, a.gate_dev = gate_dev, a.out_dev = out_dev, a.out_f32 = out_dtype == YAHKV_OUT_F32;
   a.scale_log2 = ctx->scale_log2;
   a.partial_acc = ctx->partial_acc, a.partial_ml = ctx->partial_ml, a.status_dev = ctx->status_dev;
+  if (b->n_tiles > 0) return BatchAttendShared(b, a, 1, st);
   YAHKV_CUDA(ctx, ctx->cfg.fmt == YAHKV_FMT_KV4A16   ? LaunchKv4DecodePart(a, ctx->open_tiles_dev, ctx->cfg.n_layers, st)
                   : ctx->cfg.fmt == YAHKV_FMT_KV8A16 ? LaunchKv8DecodePart(a, ctx->open_tiles_dev, ctx->cfg.n_layers, st)
                   : ctx->cfg.fmt == YAHKV_FMT_F16    ? LaunchF16DecodePart(a, st)
@@ -1694,10 +1772,12 @@ int yahkv_batch_decode_layer_raw(yahkv_batch* b, int32_t layer, const float* q_d
   for (int i = 0; i < n; ++i)
     if (ctx->host.live(b->seqs[i]) && ctx->host.evicted(b->seqs[i])) return FailEvicted(ctx, "batch_decode_layer_raw", b->seqs[i]);
   const bool tile_fmt = IsTileFmt(ctx->cfg.fmt);
+  // With shared prefixes the query is read by two kernels: it is normed and rotated once, with K.
+  void* q16 = b->n_tiles > 0 ? b->q16_dev : nullptr;
   // K and V: norm + RoPE + append at the planned slots, positions = the device-resident lengths; no q output (the part
   // kernel's prologue does the query side)
   YAHKV_CUDA(ctx, LaunchRopeAppend(ctx->pool, layer, n, b->slots_dev, b->lens_dev, q_dev, k_dev, v_dev, q_weight_dev,
-                                   k_weight_dev, eps, ctx->rope_tab_dev, ctx->rope_rows, nullptr, ctx->rope_kv16_dev, st));
+                                   k_weight_dev, eps, ctx->rope_tab_dev, ctx->rope_rows, q16, ctx->rope_kv16_dev, st));
   if (tile_fmt) {   // the kernel left fp16 rows: the format's own appends take them
     const std::uint16_t* k16 = ctx->rope_kv16_dev;
     const std::uint16_t* v16 = k16 + static_cast<std::size_t>(n) * kKvHeads * kHeadDim;
@@ -1712,8 +1792,10 @@ int yahkv_batch_decode_layer_raw(yahkv_batch* b, int32_t layer, const float* q_d
   a.items_dev = b->items_dev, a.n_seqs = n;
   a.q_dev = q_dev, a.gate_dev = gate_dev, a.out_dev = out_dev, a.out_f32 = out_dtype == YAHKV_OUT_F32;
   a.q_raw = true, a.q_weight_dev = q_weight_dev, a.q_eps = eps, a.rope_tab_dev = ctx->rope_tab_dev, a.rope_rows = ctx->rope_rows;
+  if (q16 != nullptr) a.q_raw = false, a.q_dev = q16;
   a.scale_log2 = ctx->scale_log2;
   a.partial_acc = ctx->partial_acc, a.partial_ml = ctx->partial_ml, a.status_dev = ctx->status_dev;
+  if (b->n_tiles > 0) return BatchAttendShared(b, a, 1, st);
   YAHKV_CUDA(ctx, ctx->cfg.fmt == YAHKV_FMT_KV4A16   ? LaunchKv4DecodePart(a, ctx->open_tiles_dev, ctx->cfg.n_layers, st)
                   : ctx->cfg.fmt == YAHKV_FMT_KV8A16 ? LaunchKv8DecodePart(a, ctx->open_tiles_dev, ctx->cfg.n_layers, st)
                   : ctx->cfg.fmt == YAHKV_FMT_F16    ? LaunchF16DecodePart(a, st)

@@ -9,6 +9,7 @@
 //   dattn_kappend_q + dattn_vappend_q | dattn_kvappend      Append(layer, seqs, positions, k, v, stream)
 //   dattn_part(_q) + dattn_reduce                           AttendDecode(layer, seqs, q, gate, out, ...)
 //   yah_kq8 | yah_vq8 ... + yah_attn_wmma                   Append(...) then AttendPrefill(...)
+//   (one sequence only)                                     Fork, AttendDecodeShared, AttendDecodeWeights, Evict, Rope
 // Header-only; link with libyahkv.so. Not reentrant, like the engine (engine/model/generator.hpp:56).
 #ifndef YAH_MODEL_KV_CACHE_HPP_
 #define YAH_MODEL_KV_CACHE_HPP_
@@ -73,6 +74,12 @@ class KvCache {
     return s;
   }
   void FreeSequence(std::int32_t seq) { Check(yahkv_seq_free(ctx_, seq)); }
+  // A new sequence that starts as the first n_tokens tokens of `seq`: whole pages by reference, the rest copied.
+  [[nodiscard]] std::int32_t Fork(std::int32_t seq, std::int64_t n_tokens, void* stream = nullptr) {
+    std::int32_t s = -1;
+    Check(yahkv_seq_fork(ctx_, seq, n_tokens, &s, stream));
+    return s;
+  }
   void Reserve(std::int32_t seq, std::int64_t n_tokens) { Check(yahkv_seq_reserve(ctx_, seq, n_tokens)); }
   void SetTable(std::int32_t seq, const std::vector<std::int32_t>& pages) {
     Check(yahkv_seq_set_table(ctx_, seq, pages.data(), static_cast<std::int32_t>(pages.size())));
@@ -118,6 +125,27 @@ class KvCache {
                     void* stream = nullptr) {
     Check(yahkv_attend_decode(ctx_, layer, static_cast<std::int32_t>(seqs.size()), seqs.data(), q_dev, gate_dev, out_dev,
                               out_dtype, n_splits, stream));
+  }
+  // AttendDecode with every prefix that the rows share (Fork) computed once for all of them.
+  void AttendDecodeShared(std::int32_t layer, const std::vector<std::int32_t>& seqs, const void* q_dev, const float* gate_dev,
+                          void* out_dev, std::int32_t out_dtype = YAHKV_OUT_F16, std::int32_t n_splits = 0,
+                          void* stream = nullptr) {
+    Check(yahkv_attend_decode_shared(ctx_, layer, static_cast<std::int32_t>(seqs.size()), seqs.data(), q_dev, gate_dev,
+                                     out_dev, out_dtype, n_splits, stream));
+  }
+  // AttendDecode that also adds every key's attention weight to weights_dev [max_seqs][4][weights_stride].
+  void AttendDecodeWeights(std::int32_t layer, const std::vector<std::int32_t>& seqs, const void* q_dev, const float* gate_dev,
+                           void* out_dev, float* weights_dev, std::int64_t weights_stride,
+                           std::int32_t out_dtype = YAHKV_OUT_F16, std::int32_t n_splits = 0, void* stream = nullptr) {
+    Check(yahkv_attend_decode_weights(ctx_, layer, static_cast<std::int32_t>(seqs.size()), seqs.data(), q_dev, gate_dev,
+                                      out_dev, out_dtype, n_splits, weights_dev, weights_stride, stream));
+  }
+  // Cuts every sequence to n_keep keys by those weights (all layers; kept_dev [n_layers][n_seqs][4][n_keep] i32).
+  void Evict(const std::vector<std::int32_t>& seqs, std::int64_t n_keep, std::int64_t n_sink, std::int64_t n_recent,
+             float* weights_dev, std::int64_t weights_stride, std::int64_t weights_layer_stride, std::int32_t* kept_dev,
+             void* stream = nullptr) {
+    Check(yahkv_evict(ctx_, static_cast<std::int32_t>(seqs.size()), seqs.data(), n_keep, n_sink, n_recent, weights_dev,
+                      weights_stride, weights_layer_stride, kept_dev, stream));
   }
   void AttendPrefill(std::int32_t layer, const std::vector<std::int32_t>& seqs, const std::vector<std::int32_t>& chunks,
                      const void* q_dev, const float* gate_dev, void* out_dev, std::int32_t out_dtype = YAHKV_OUT_F16,
@@ -177,6 +205,8 @@ class KvCache {
     DecodeBatch(const DecodeBatch&) = delete;
     DecodeBatch& operator=(const DecodeBatch&) = delete;
     ~DecodeBatch() { yahkv_batch_destroy(b_); }
+    // Prefixes that rows share are computed once for all of them from the next Prepare on.
+    void SetShared(bool on) { cache_->Check(yahkv_batch_set_shared(b_, on ? 1 : 0)); }
     // Reserves pages for `horizon_steps` more positions; true when the unit layout changed (capture again).
     bool Prepare(std::int32_t horizon_steps, void* stream = nullptr) {
       std::int32_t changed = 0;
@@ -202,6 +232,25 @@ class KvCache {
    private:
     KvCache* cache_;
     yahkv_batch* b_ = nullptr;
+  };
+
+  // ---- rotary positions for head rows at positions that are device data; the cache outlives it ----
+  class Rope {
+   public:
+    Rope(KvCache& cache, const yahkv_rope_config& cfg) : cache_(&cache) { cache.Check(yahkv_rope_create(cache.ctx_, &cfg, &r_)); }
+    Rope(const Rope&) = delete;
+    Rope& operator=(const Rope&) = delete;
+    ~Rope() { yahkv_rope_destroy(r_); }
+    void Rows(std::int32_t n_tokens, std::int32_t n_heads, const std::int64_t* positions_dev, const void* x_dev,
+              std::int32_t x_dtype, std::int64_t x_stride, const float* weight_dev, float eps, void* out_dev,
+              std::int32_t out_dtype, std::int64_t out_stride, void* stream = nullptr) {
+      cache_->Check(yahkv_rope_rows(r_, n_tokens, n_heads, positions_dev, x_dev, x_dtype, x_stride, weight_dev, eps, out_dev,
+                                    out_dtype, out_stride, stream));
+    }
+
+   private:
+    KvCache* cache_;
+    yahkv_rope* r_ = nullptr;
   };
 
  private:
