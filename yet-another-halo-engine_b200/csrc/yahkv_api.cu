@@ -95,7 +95,6 @@ struct yahkv_ctx {
   CUtensorMap kmap{}, vmap{};
   std::int32_t* tables_dev = nullptr;
   DecodeUnit* units_dev = nullptr;
-  CombineItem* items_dev = nullptr;
   PrefillTile* tiles_dev = nullptr;
   int max_tiles = 0;
   std::int64_t* slots_dev = nullptr;
@@ -247,8 +246,10 @@ int InitDevice(yahkv_ctx* ctx) {
   YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->tables_dev, static_cast<std::size_t>(c.max_seqs) * c.max_pages_per_seq, true));
   YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->slots_dev, static_cast<std::size_t>(c.max_batch_tokens), false));
   ctx->max_units = c.max_seqs * kKvHeads * c.max_splits;
-  YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->units_dev, static_cast<std::size_t>(ctx->max_units), false));
-  YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->items_dev, static_cast<std::size_t>(c.max_seqs) * kKvHeads, false));
+  // the units of a decode plan with its combine items behind them (one upload)
+  static_assert(sizeof(DecodeUnit) % sizeof(CombineItem) == 0, "items follow units");
+  YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->units_dev, static_cast<std::size_t>(ctx->max_units) +
+                                                     (static_cast<std::size_t>(c.max_seqs) * kKvHeads * sizeof(CombineItem) + sizeof(DecodeUnit) - 1) / sizeof(DecodeUnit), false));
   YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->partial_acc, static_cast<std::size_t>(ctx->max_units) * kPartialAccFloats, false));
   YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->partial_ml, static_cast<std::size_t>(ctx->max_units) * kPartialMlFloats, false));
   YAHKV_CUDA(ctx, cudaDeviceGetAttribute(&ctx->n_sm, cudaDevAttrMultiProcessorCount, c.device));
@@ -307,7 +308,7 @@ void FreeDevice(yahkv_ctx* ctx) {
   cudaSetDevice(ctx->cfg.device);
   if (ctx->stream != nullptr) cudaStreamSynchronize(ctx->stream);
   void* ptrs[] = {ctx->pool.kcodes, ctx->pool.vcodes, ctx->pool.kscales, ctx->pool.vscales, ctx->tables_dev,
-                  ctx->slots_dev,   ctx->units_dev,   ctx->items_dev,    ctx->partial_acc,  ctx->partial_ml,
+                  ctx->slots_dev,   ctx->units_dev,   ctx->partial_acc,  ctx->partial_ml,
                   ctx->tiles_dev,   ctx->status_dev,  ctx->pseqs_dev, ctx->k16_dev, ctx->v16_dev,
                   ctx->merges_dev, ctx->part_acc_dev, ctx->part_ml_dev,
                   ctx->rope_tab_dev, ctx->rope_pos_dev, ctx->open_tiles_dev, ctx->kmean_dev, ctx->state_rows_dev,
@@ -841,15 +842,14 @@ static int AttendDecode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int
     YAHKV_CUDA(ctx, ctx->staging.Acquire(ub + ib, &buf));
     std::memcpy(buf, units.data(), ub);
     std::memcpy(buf + ub, items.data(), ib);
-    YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->units_dev, buf, ub, cudaMemcpyHostToDevice, st));
-    YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->items_dev, buf + ub, ib, cudaMemcpyHostToDevice, st));
+    YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->units_dev, buf, ub + ib, cudaMemcpyHostToDevice, st));
     YAHKV_CUDA(ctx, ctx->staging.Release(st));
   }
   DecodeLaunch a{};
   a.kmap = &ctx->kmap, a.vmap = &ctx->vmap, a.pool = ctx->pool, a.layer = layer;
   a.tables_dev = ctx->tables_dev, a.table_stride = ctx->cfg.max_pages_per_seq;
   a.units_dev = ctx->units_dev, a.n_units = static_cast<int>(units.size());
-  a.items_dev = ctx->items_dev, a.n_seqs = n_seqs;
+  a.items_dev = reinterpret_cast<const CombineItem*>(ctx->units_dev + units.size()), a.n_seqs = n_seqs;
   a.q_dev = q_dev, a.gate_dev = gate_dev, a.out_dev = out_dev, a.out_f32 = out_dtype == YAHKV_OUT_F32;
   a.q_raw = q_raw, a.q_weight_dev = q_weight_dev, a.q_eps = eps, a.rope_tab_dev = ctx->rope_tab_dev, a.rope_rows = ctx->rope_rows;
   a.scale_log2 = ctx->scale_log2;

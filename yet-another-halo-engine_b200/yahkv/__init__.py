@@ -7,6 +7,7 @@ context without a GPU return YAHKV_ERR_NO_DEVICE.
 `KvCache` mirrors the calls the reference engine makes on this path (engine/model/loom_decoder.hpp:254-268: append,
 then attend over keys 0..pos, then the merge with the sigmoid gate), batched over sequences.
 """
+import array
 import ctypes
 import os
 import subprocess
@@ -236,6 +237,19 @@ def _i32(a):
     return np.ascontiguousarray(a, dtype=np.int32)
 
 
+def _ids(seq_ids):
+    """(int32 array to keep alive during the call, its address, its length): what a call costs on the host counts where
+    the kernels take ten microseconds, and a numpy array's address alone costs four."""
+    a = array.array("i", seq_ids.tolist() if hasattr(seq_ids, "tolist") else seq_ids)
+    address, n = a.buffer_info()
+    return a, address if n else None, n
+
+
+def _adr(x):
+    """The address of a torch tensor or None as an argument of a call."""
+    return None if x is None else x.data_ptr() if hasattr(x, "data_ptr") else _ptr(x)
+
+
 def device_codes(fmt, codes, side):
     """GGUF code bytes (as read_page returns them) -> the form the device pools hold: q8_0 V bytes with the sign bit
     flipped (u = code + 128); q8_0 K bytes and q4_0 unchanged. The same call converts back. For callers that build
@@ -349,19 +363,23 @@ class Rope:
         """x, out: CUDA tensors [tokens, heads, 256], fp16 or f32, heads and dims contiguous (tokens may be strided);
         positions: CUDA int64 [tokens]; weight: CUDA f32 [256] or None."""
         n, heads, dim = x.shape
-        if tuple(out.shape) != (n, heads, dim) or dim != HEAD_DIM or tuple(positions.shape) != (n,):
+        if out.shape != x.shape or dim != HEAD_DIM or positions.shape != (n,):
             raise ValueError("rows: x and out are [tokens, heads, 256], positions [tokens]")
+        kinds, steps = [], []
         for t in (x, out):
-            if str(t.dtype) not in ("torch.float16", "torch.float32") or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+            kind, step = t.dtype, t.stride()
+            if not kind.is_floating_point or kind.itemsize not in (2, 4) or str(kind) == "torch.bfloat16" or \
+                    step[2] != 1 or (heads > 1 and step[1] != dim):
                 raise ValueError("rows: x and out must be fp16 or f32 with contiguous heads")
-        if str(positions.dtype) != "torch.int64" or not positions.is_contiguous():
+            kinds.append(OUT_F32 if kind.itemsize == 4 else OUT_F16)
+            steps.append(step[0] if n > 1 else heads * dim)
+        if positions.dtype.itemsize != 8 or positions.dtype.is_floating_point or not positions.is_contiguous():
             raise ValueError("rows: positions must be contiguous int64")
-        if weight is not None and (str(weight.dtype) != "torch.float32" or tuple(weight.shape) != (dim,) or not weight.is_contiguous()):
+        if weight is not None and (weight.dtype.itemsize != 4 or not weight.dtype.is_floating_point or weight.shape != (dim,) or
+                                   not weight.is_contiguous()):
             raise ValueError("rows: weight must be contiguous f32 [256]")
-        kind = [OUT_F32 if str(t.dtype) == "torch.float32" else OUT_F16 for t in (x, out)]
-        step = [t.stride(0) if n > 1 else heads * dim for t in (x, out)]
-        self.cache._check(lib.yahkv_rope_rows(self._h, n, heads, _ptr(positions), _ptr(x), kind[0], step[0], _ptr(weight),
-                                              float(eps), _ptr(out), kind[1], step[1], _ptr(stream)))
+        self.cache._check(lib.yahkv_rope_rows(self._h, n, heads, _adr(positions), _adr(x), kinds[0], steps[0], _adr(weight), eps,
+                                              _adr(out), kinds[1], steps[1], _ptr(stream)))
 
 
 class KvCache:
@@ -455,9 +473,9 @@ class KvCache:
                                            _ptr(stream)))
 
     def attend_decode(self, layer, seq_ids, q, out, gate=None, out_dtype=OUT_F16, n_splits=0, stream=None):
-        seq_ids = _i32(seq_ids)
-        self._check(lib.yahkv_attend_decode(self._h, layer, len(seq_ids), _ptr(seq_ids), _ptr(q), _ptr(gate),
-                                            _ptr(out), out_dtype, n_splits, _ptr(stream)))
+        keep, ids, n = _ids(seq_ids)
+        self._check(lib.yahkv_attend_decode(self._h, layer, n, ids, _adr(q), _adr(gate), _adr(out), out_dtype, n_splits,
+                                            _ptr(stream)))
 
     def attend_decode_qraw(self, layer, seq_ids, q_raw, q_weight, eps, out, gate=None, out_dtype=OUT_F16, n_splits=0,
                            stream=None):
@@ -468,38 +486,37 @@ class KvCache:
 
     def attend_decode_shared(self, layer, seq_ids, q, out, gate=None, out_dtype=OUT_F16, n_splits=0, stream=None):
         """attend_decode with every prefix that rows share (seq_fork) computed once for all of them."""
-        seq_ids = _i32(seq_ids)
-        self._check(lib.yahkv_attend_decode_shared(self._h, layer, len(seq_ids), _ptr(seq_ids), _ptr(q), _ptr(gate),
-                                                   _ptr(out), out_dtype, n_splits, _ptr(stream)))
+        keep, ids, n = _ids(seq_ids)
+        self._check(lib.yahkv_attend_decode_shared(self._h, layer, n, ids, _adr(q), _adr(gate), _adr(out), out_dtype, n_splits,
+                                                   _ptr(stream)))
 
     def _weights(self, weights, dims):
         """Row pitch of the accumulators of attend_decode_weights / evict."""
-        layer = weights[0] if weights.dim() == 4 else weights
-        if str(weights.dtype) != "torch.float32" or weights.dim() != dims or not layer.is_contiguous() or \
-                tuple(layer.shape[:2]) != (self.cfg.max_seqs, KV_HEADS) or \
-                (dims == 4 and weights.shape[0] != self.cfg.n_layers):
+        shape, stride = weights.shape, weights.stride()
+        if len(shape) != dims or weights.dtype.itemsize != 4 or not weights.dtype.is_floating_point or \
+                shape[-3] != self.cfg.max_seqs or shape[-2] != KV_HEADS or \
+                stride[-1] != 1 or stride[-2] != shape[-1] or (shape[-3] > 1 and stride[-3] != KV_HEADS * shape[-1]) or \
+                (dims == 4 and shape[0] != self.cfg.n_layers):
             raise ValueError("weights must be f32 [%smax_seqs, 4, keys], every layer contiguous" % ("n_layers, " if dims == 4 else ""))
-        return layer.shape[2]
+        return shape[-1]
 
     def attend_decode_weights(self, layer, seq_ids, q, out, weights, gate=None, out_dtype=OUT_F16, n_splits=0, stream=None):
         """attend_decode that also adds every key's attention weight to weights (CUDA f32 [max_seqs, 4, keys], rows by
         sequence id)."""
-        seq_ids = _i32(seq_ids)
-        self._check(lib.yahkv_attend_decode_weights(self._h, layer, len(seq_ids), _ptr(seq_ids), _ptr(q), _ptr(gate),
-                                                    _ptr(out), out_dtype, n_splits, _ptr(weights), self._weights(weights, 3),
-                                                    _ptr(stream)))
+        keep, ids, n = _ids(seq_ids)
+        self._check(lib.yahkv_attend_decode_weights(self._h, layer, n, ids, _adr(q), _adr(gate), _adr(out), out_dtype, n_splits,
+                                                    _adr(weights), self._weights(weights, 3), _ptr(stream)))
 
     def evict(self, seq_ids, n_keep, weights, kept, n_sink=0, n_recent=0, stream=None):
         """Cuts every sequence to n_keep keys by weights (CUDA f32 [n_layers, max_seqs, 4, keys]); kept: CUDA int32
         [n_layers, n_seqs, 4, n_keep] receives the old slots."""
-        seq_ids = _i32(seq_ids)
-        if str(kept.dtype) != "torch.int32" or tuple(kept.shape) != (self.cfg.n_layers, len(seq_ids), KV_HEADS, n_keep) or \
-                not kept.is_contiguous():
+        keep, ids, n = _ids(seq_ids)
+        if kept.dtype.itemsize != 4 or kept.dtype.is_floating_point or not kept.is_contiguous() or \
+                kept.shape != (self.cfg.n_layers, n, KV_HEADS, n_keep):
             raise ValueError("kept must be contiguous int32 [n_layers, n_seqs, 4, n_keep]")
         stride = self._weights(weights, 4)
-        self._check(lib.yahkv_evict(self._h, len(seq_ids), _ptr(seq_ids), n_keep, n_sink, n_recent, _ptr(weights), stride,
-                                    weights.stride(0) if weights.shape[0] > 1 else self.cfg.max_seqs * KV_HEADS * stride,
-                                    _ptr(kept), _ptr(stream)))
+        self._check(lib.yahkv_evict(self._h, n, ids, n_keep, n_sink, n_recent, _adr(weights), stride, weights.stride(0), _adr(kept),
+                                    _ptr(stream)))
 
     def attend_prefill(self, layer, seq_ids, chunk_lens, q, out, gate=None, out_dtype=OUT_F16, stream=None):
         seq_ids, chunk_lens = _i32(seq_ids), _i32(chunk_lens)
