@@ -243,12 +243,16 @@ int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, 
 int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
                                const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, void* stream);
 
-/* yahkv_attend_decode, the same bits, which also adds to weights_dev the softmax weight of every key, summed over the six
+/* yahkv_attend_decode which also adds to weights_dev the softmax weight of every key, summed over the six
  * query heads of its kv head: weights_dev[(seq * 4 + kv head) * weights_stride + key] += sum_g p_g(key), f32, seq the
  * sequence id (so rows stay where they are when the batch changes), key = 0 .. len - 1 its slot. weights_dev is
  * [max_seqs][4][weights_stride], the caller's, one per layer: zero a row before a sequence's first call; keys appended
  * later start from what the row holds there. weights_stride at least the longest sequence's length
- * (YAHKV_ERR_CAPACITY). A sequence may be listed once. The gate does not enter the weights. q_dev 16-byte aligned. */
+ * (YAHKV_ERR_CAPACITY). A sequence may be listed once. The gate does not enter the weights. For fp16 pages the attention is
+ * yahkv_attend_decode's to the bit; for the quantized formats the query enters in 20-bit steps of its largest element
+ * where yahkv_attend_decode takes 16, so the two agree within that rounding (1e-4 of the largest output). q_dev 16-byte aligned. The scores
+ * pass through a workspace (96 B per cached key of the call) that grows to the largest call seen: growing waits for
+ * the device. */
 int yahkv_attend_decode_weights(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
                                 const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, float* weights_dev,
                                 int64_t weights_stride, void* stream);

@@ -1,10 +1,9 @@
 """Accumulated attention weights and eviction by them, against the definitions in float64 over the bytes the cache holds.
 
-Tolerances. A weight is exp of a score that the weights pass sums in fp32 from exact products (256 of them, magnitude
-sum|q k| / 16 < 16 for this data: below 256 x 2^-24 x 16 = 2.5e-4 in the worst case, some 1e-6 in earnest), over a row sum that
-comes from the decode kernel, whose quantized formats hold the query in 16-bit steps of amax / 32000 (a score error of at
-most amax / 64000 sum|k| / 16 < 6.5e-4, some 3e-5 in earnest); six of them are added to the accumulator. The bar is
-a relative 1e-3 of the largest weight. What eviction moves and selects is compared exactly."""
+Tolerances. A weight is exp of a score over a row sum. A score is the sum of exact products in fp32 (eight partial sums of 32
+products each: 8 x 2^-24 of sum|q k| / 16 < 16) of the query, which the quantized formats hold in steps of amax / 524287: half
+a step of amax < 5 on each of 256 elements against |k| < 5 is below 5e-6 x 256 x 5 / 16 x 0.5 = 2e-4 if all went one way and
+sqrt(256) instead of 256 of it, 1.3e-5, as they do. Once more for the row sum: the bar is 3e-5 of the largest weight. What eviction moves and selects is compared exactly."""
 import numpy as np
 import pytest
 import torch
@@ -45,14 +44,17 @@ def test_weights_add_up(fmt):
         cache.attend_decode_weights(0, rows, dev(q), out, w, gate=dev(gate), out_dtype=yahkv.OUT_F32, n_splits=n_splits)
         cache.attend_decode(0, rows, dev(q), ref, gate=dev(gate), out_dtype=yahkv.OUT_F32, n_splits=n_splits)
         cache.sync()
-        assert torch.equal(out, ref)                       # the attention itself is attend_decode's, bit for bit
+        if fmt == yahkv.FMT_F16:                           # the attention itself is attend_decode's
+            assert torch.equal(out, ref)
+        else:                                              # whose query is off by up to amax / 64000 per element
+            assert (out - ref).abs().max() <= 1e-4 * ref.abs().max()
         top = 0.0
         for b, s in enumerate(rows):
             n = lens[seqs.index(s)]
             p = attend64(q[b], *rows64(cache, 0, s, n))[1].reshape(4, 6, n).sum(1)
             want[s, :, :n] += p
             got = w[s, :, :n].double().cpu().numpy()
-            assert np.abs(got - want[s, :, :n]).max() <= 1e-3 * p.max() + 2.0 ** -22 * want[s].max(), (n, n_splits)
+            assert np.abs(got - want[s, :, :n]).max() <= 3e-5 * p.max() + 2.0 ** -22 * want[s].max(), (n, n_splits)
             want[s, :, :n] = got                           # the next step is judged by itself
     got = w.cpu().numpy()
     assert np.array_equal(got[unused], w0[unused])

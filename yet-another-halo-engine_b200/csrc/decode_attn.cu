@@ -122,6 +122,27 @@ __device__ __forceinline__ void MmaQK(int (&d)[4], const std::uint32_t (&a)[4], 
 // (|sum| <= 32 x 128 x 32768), as a float.
 __device__ __forceinline__ float JoinPlanes(int hi, int lo) { return static_cast<float>(hi * 256 + lo); }
 
+// The same with a third plane: 20 bits as q = 2^14 hi + 2^7 mid + lo, hi in [-32, 31], mid and lo in [0, 127]; hi and mid ride
+// in one MMA as the two planes above, lo in a second one. |q| <= 524287 keeps a block's sum, joined in 32-bit integers,
+// exact: 32 x 524287 x 128 < 2^31. One MMA and two shifted additions more per block and eight keys than with two planes.
+// (Exact scores from the fp16 query on the f16 MMA took 16 instructions per block instead of 10: 156 us against 140 us on
+// the q8_0 batch of 291,000 keys.)
+constexpr float kScoreSteps = 524287.0F;
+__device__ __forceinline__ void LoadQ3(std::uint32_t (&a)[2], std::uint32_t q_addr) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(a[0]), "=r"(a[1]) : "r"(q_addr));
+}
+__device__ __forceinline__ void MmaQK3(float (&sum)[2], const std::uint32_t (&a)[4], const std::uint32_t (&a3)[2], std::uint32_t b0,
+                                       std::uint32_t b1) {
+  int d[4], e[4];
+  const std::uint32_t lo[4] = {a3[0], 0U, a3[1], 0U};
+  MmaQK(d, a, b0, b1);
+  MmaQK(e, lo, b0, b1);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)   // wraps on the way, fits at the end
+    sum[j] = static_cast<float>(static_cast<int>((((static_cast<std::uint32_t>(d[j]) << 7) + static_cast<std::uint32_t>(d[2 + j])) << 7) +
+                                                 static_cast<std::uint32_t>(e[j])));
+}
+
 // Query quantization: 16 bits against the head's largest magnitude. 32000 keeps the hi plane inside [-125, 125].
 constexpr float kQSteps = 32000.0F;
 
@@ -131,21 +152,22 @@ constexpr float kQSteps = 32000.0F;
 // (duplicates of heads 4, 5 whose results are never stored), so the Q array is 24 lanes wide.
 constexpr int kQLanes = 24;
 constexpr int kQfragBytes = kBlocksPerRow * kQLanes * 16;   // per 32-element block the A operand's four registers
-template <int kFmt>
+constexpr int kQfrag3Bytes = kBlocksPerRow * kQLanes * 8;   // kScores: the third plane's two
+template <int kFmt, bool kScores = false>
 struct SmemLayout {
   static constexpr int kRing = StageLayout<kFmt>::kStages * StageLayout<kFmt>::kBytes;
   static_assert(kRing >= Shape<kFmt>::kWarps * kDecodeMergeWarpFloats * 4, "the merge scratch of a unit's end aliases the ring");
   static constexpr int kQfragOff = kRing;
-  static constexpr int kBarOff = kQfragOff + kQfragBytes;
+  static constexpr int kBarOff = kQfragOff + kQfragBytes + (kScores ? kQfrag3Bytes : 0);
   static constexpr int kCntOff = kBarOff + 8 * StageLayout<kFmt>::kStages;
   static constexpr int kFillOff = kCntOff + 4 * StageLayout<kFmt>::kStages;     // fills issued per stage
   static constexpr int kQScaleOff = kFillOff + 4 * StageLayout<kFmt>::kStages;  // [8] f32, one per head (6 used)
   static constexpr int kAbortOff = kQScaleOff + 4 * 8;
   static constexpr int kBytes = kAbortOff + 4;
 };
-template <int kFmt>
+template <int kFmt, bool kScores = false>
 constexpr int DecodeSmemBytes() {
-  return (SmemLayout<kFmt>::kBytes + 127) / 128 * 128;
+  return (SmemLayout<kFmt, kScores>::kBytes + 127) / 128 * 128;
 }
 constexpr int kStatusSmemMisaligned = 2;
 
@@ -156,18 +178,22 @@ constexpr float kLazyRescale = 4.0F;
 // kQRaw: the query is the raw f32 projection (qraw) and the prologue norms and rotates the unit's six head rows itself,
 // at the position of the sequence's newest key (qrope.cuh).
 // kBeside: the units lie behind prefixes that the kernel launched just before computes; see ChainedKernelEntryBeside.
-template <int kFmt, bool kQRaw, bool kBeside>
+// kScores: the scores (log2 units, -inf behind the last key) are kept for the pass that accumulates attention weights
+// (evict.cu), [page slot][6 heads][64 keys], and the query has 20 bits in three planes (see kScorePlanes) where the other
+// variants have 16 in two: an accumulated weight is held in fp32, and 16 bits would leave it 2e-5 off.
+template <int kFmt, bool kQRaw, bool kBeside, bool kScores>
 __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
     DecodePartKernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      PoolView pool, int layer, const std::int32_t* __restrict__ tables, int table_stride,
                      const DecodeUnit* __restrict__ units, const __half* __restrict__ q, const QueryRaw qraw,
-                     float scale_log2, float* __restrict__ partial_acc, float* __restrict__ partial_ml, int* status) {
+                     float scale_log2, float* __restrict__ partial_acc, float* __restrict__ partial_ml,
+                     float* __restrict__ scores, int* status) {
   if constexpr (kBeside)
     ChainedKernelEntryBeside();
   else
     ChainedKernelEntry();
   using L = StageLayout<kFmt>;
-  using S = SmemLayout<kFmt>;
+  using S = SmemLayout<kFmt, kScores>;
   constexpr int kPageSets = Shape<kFmt>::kPageSets, kWarps = Shape<kFmt>::kWarps;
   extern __shared__ __align__(1024) std::uint8_t smem_raw[];
   std::uint8_t* ring = smem_raw;
@@ -254,13 +280,14 @@ __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFU, amax, o));
-    const float inv = amax > 0.0F ? kQSteps / amax : 0.0F;
-    std::uint32_t hi_w[2] = {0, 0}, lo_w[2] = {0, 0};
+    const float inv = amax > 0.0F ? (kScores ? kScoreSteps : kQSteps) / amax : 0.0F;
+    std::uint32_t hi_w[2] = {0, 0}, lo_w[2] = {0, 0}, third_w[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int q16 = __float2int_rn(x[i] * inv);
-      const int hi = (q16 + 128) >> 8;
-      const int lo = q16 - hi * 256;
+      const int q16 = __float2int_rn(x[i] * inv);   // kScores: 20 bits
+      const int hi = kScores ? q16 >> 14 : (q16 + 128) >> 8;
+      const int lo = kScores ? (q16 >> 7) & 127 : q16 - hi * 256;
+      if constexpr (kScores) third_w[i >> 2] |= (static_cast<std::uint32_t>(q16) & 127U) << (8 * (i & 3));
       hi_w[i >> 2] |= (static_cast<std::uint32_t>(hi) & 0xFFU) << (8 * (i & 3));
       lo_w[i >> 2] |= (static_cast<std::uint32_t>(lo) & 0xFFU) << (8 * (i & 3));
     }
@@ -271,13 +298,15 @@ __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
       std::uint32_t* dst = qfrag + ((blk * kQLanes + hq * 4 + t0 + j) << 2) + reg;
       dst[0] = hi_w[j];
       dst[1] = lo_w[j];
+      if constexpr (kScores) qfrag[kBlocksPerRow * kQLanes * 4 + ((blk * kQLanes + hq * 4 + t0 + j) << 1) + (reg >> 1)] = third_w[j];
     }
     // q = step (256 hi + lo); q4_0 codes enter the MMA as 16 (n - 8), which the step absorbs
-    if (lane == 0) q_scale[hq] = (amax / kQSteps) * (kFmt == kFmtQ8 ? 1.0F : 0.0625F);
+    if (lane == 0) q_scale[hq] = (amax / (kScores ? kScoreSteps : kQSteps)) * (kFmt == kFmtQ8 ? 1.0F : 0.0625F);
   }
   __syncthreads();   // barriers initialised, query planes visible
   const int qlane = lane < kQLanes ? lane : lane - 8;
   const std::uint32_t qa_addr = SmemAddr(qfrag + (qlane << 2));   // block b: + b * kQLanes * 16 bytes
+  const std::uint32_t q3_addr = SmemAddr(qfrag + kBlocksPerRow * kQLanes * 4 + (qlane << 1));   // kScores: block b: + b * kQLanes * 8 bytes
   const float score_scale = scale_log2 * q_scale[qlane >> 2];     // softmax scale x log2(e) x the head's query step
 
   float o_acc[16][4];   // tile c = dims 16 c .. 16 c + 15 (in the MMA's permuted order)
@@ -341,6 +370,18 @@ __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
           std::uint32_t w[4], qa[4];
           LdMatrixX4(k_base + dh * kBoxBytes + lm_off(b), w);
           LoadQ(qa, qa_addr + (4 * dh + b) * (kQLanes * 16));
+          if constexpr (kScores) {
+            std::uint32_t q3[2];
+            float s0[2], s1[2];
+            LoadQ3(q3, q3_addr + (4 * dh + b) * (kQLanes * 8));
+            MmaQK3(s0, qa, q3, w[0], w[2]);
+            MmaQK3(s1, qa, q3, w[1], w[3]);
+            sc[0][0] = fmaf(ScaleOf(ks_raw[0][0], b), s0[0], sc[0][0]);
+            sc[0][1] = fmaf(ScaleOf(ks_raw[0][1], b), s0[1], sc[0][1]);
+            sc[1][0] = fmaf(ScaleOf(ks_raw[1][0], b), s1[0], sc[1][0]);
+            sc[1][1] = fmaf(ScaleOf(ks_raw[1][1], b), s1[1], sc[1][1]);
+            continue;
+          }
           int a0[4], a1[4];
           MmaQK(a0, qa, w[0], w[2]);
           MmaQK(a1, qa, w[1], w[3]);
@@ -361,6 +402,20 @@ __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
             const int b = 2 * bp + hb;   // block 4 dh + b
             std::uint32_t qa[4];
             LoadQ(qa, qa_addr + (4 * dh + b) * (kQLanes * 16));
+            if constexpr (kScores) {
+              std::uint32_t q3[2], lo3, hi3;
+              float s0[2], s1[2];
+              LoadQ3(q3, q3_addr + (4 * dh + b) * (kQLanes * 8));
+              Nib8ToS8(nib.top_mask, nib.sign_flip, w[2 * hb], lo3, hi3);
+              MmaQK3(s0, qa, q3, lo3, hi3);
+              Nib8ToS8(nib.top_mask, nib.sign_flip, w[2 * hb + 1], lo3, hi3);
+              MmaQK3(s1, qa, q3, lo3, hi3);
+              sc[0][0] = fmaf(ScaleOf(ks_raw[0][0], b), s0[0], sc[0][0]);
+              sc[0][1] = fmaf(ScaleOf(ks_raw[0][1], b), s0[1], sc[0][1]);
+              sc[1][0] = fmaf(ScaleOf(ks_raw[1][0], b), s1[0], sc[1][0]);
+              sc[1][1] = fmaf(ScaleOf(ks_raw[1][1], b), s1[1], sc[1][1]);
+              continue;
+            }
             int a0[4], a1[4];
             std::uint32_t lo, hi;
             Nib8ToS8(nib.top_mask, nib.sign_flip, w[2 * hb], lo, hi);
@@ -389,6 +444,13 @@ __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           if (key_pos0 + kt * 8 + j >= u.n_keys) sc[kt][j] = -INFINITY;
+    }
+    if constexpr (kScores) {
+      if (lane < kQLanes) {
+        float* dst = scores + ((static_cast<std::size_t>(u.pad) + i) * kGroup + (lane >> 2)) * kPageTokens + my_key0;
+        *reinterpret_cast<float2*>(dst) = make_float2(sc[0][0], sc[0][1]);
+        *reinterpret_cast<float2*>(dst + 8) = make_float2(sc[1][0], sc[1][1]);
+      }
     }
     tmax = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
     tmax = fmaxf(tmax, __shfl_xor_sync(0xFFFFFFFFU, tmax, 1));
@@ -565,30 +627,31 @@ __global__ void __launch_bounds__(kHeadDim)
 
 template <int kFmt>
 static cudaError_t ConfigurePart() {
-  cudaError_t e = cudaFuncSetAttribute(DecodePartKernel<kFmt, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmt>());
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(DecodePartKernel<kFmt, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmt>());
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(DecodePartKernel<kFmt, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmt>());
-  return e;
+  for (auto kernel : {DecodePartKernel<kFmt, false, false, false>, DecodePartKernel<kFmt, true, false, false>,
+                      DecodePartKernel<kFmt, false, true, false>})
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmemBytes<kFmt>()); e != cudaSuccess)
+      return e;
+  return cudaFuncSetAttribute(DecodePartKernel<kFmt, false, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              DecodeSmemBytes<kFmt, true>());
 }
 cudaError_t ConfigureDecodeKernels() {
   const cudaError_t e = ConfigurePart<kFmtQ8>();
   return e != cudaSuccess ? e : ConfigurePart<kFmtQ4>();
 }
 
-template <int kFmt, bool kQRaw, bool kBeside>
+template <int kFmt, bool kQRaw, bool kBeside, bool kScores>
 static cudaError_t LaunchPart(const DecodeLaunch& a, cudaStream_t stream) {
   const QueryRaw qr{kQRaw ? static_cast<const float*>(a.q_dev) : nullptr, a.q_weight_dev, a.rope_tab_dev, a.q_eps, a.rope_rows};
-  return LaunchChained(DecodePartKernel<kFmt, kQRaw, kBeside>, a.n_units, Shape<kFmt>::kThreads, DecodeSmemBytes<kFmt>(), stream,
+  return LaunchChained(DecodePartKernel<kFmt, kQRaw, kBeside, kScores>, a.n_units, Shape<kFmt>::kThreads, DecodeSmemBytes<kFmt, kScores>(), stream,
                        *a.kmap, *a.vmap, a.pool, a.layer, a.tables_dev, a.table_stride, a.units_dev,
                        kQRaw ? nullptr : static_cast<const __half*>(a.q_dev), qr, a.scale_log2, a.partial_acc,
-                       a.partial_ml, a.status_dev);
+                       a.partial_ml, a.scores_dev, a.status_dev);
 }
 template <int kFmt>
 static cudaError_t LaunchPartOf(const DecodeLaunch& a, cudaStream_t stream) {
-  if (a.beside) return a.q_raw ? cudaErrorInvalidValue : LaunchPart<kFmt, false, true>(a, stream);
-  return a.q_raw ? LaunchPart<kFmt, true, false>(a, stream) : LaunchPart<kFmt, false, false>(a, stream);
+  if (a.q_raw) return a.beside || a.scores_dev != nullptr ? cudaErrorInvalidValue : LaunchPart<kFmt, true, false, false>(a, stream);
+  if (a.scores_dev != nullptr) return a.beside ? cudaErrorInvalidValue : LaunchPart<kFmt, false, false, true>(a, stream);
+  return a.beside ? LaunchPart<kFmt, false, true, false>(a, stream) : LaunchPart<kFmt, false, false, false>(a, stream);
 }
 
 cudaError_t LaunchDecodePart(const DecodeLaunch& a, cudaStream_t stream) {

@@ -49,13 +49,14 @@ constexpr int kStatusSmemMisaligned = 2;
 
 // kQRaw: the raw f32 query, normed and rotated in the prologue (qrope.cuh). kBeside: the units lie behind prefixes that the
 // kernel launched just before computes; see ChainedKernelEntryBeside.
-template <bool kQRaw, bool kBeside>
+// kScores: the scores are kept for the pass that accumulates attention weights (evict.cu).
+template <bool kQRaw, bool kBeside, bool kScores>
 __global__ void __launch_bounds__(kThreads, 1)
     F16DecodePartKernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         PoolView pool, int layer, const std::int32_t* __restrict__ tables, int table_stride,
                         const DecodeUnit* __restrict__ units, const __half* __restrict__ q, const QueryRaw qraw,
                         float scale_log2,
-                        float* __restrict__ partial_acc, float* __restrict__ partial_ml, int* status) {
+                        float* __restrict__ partial_acc, float* __restrict__ partial_ml, float* __restrict__ scores, int* status) {
   if constexpr (kBeside)
     ChainedKernelEntryBeside();
   else
@@ -181,6 +182,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (key_pos0 + kt * 8 + j >= u.n_keys) sc[kt][j] = -INFINITY;
     }
 
+    if constexpr (kScores) {
+      if (lane < kQLanes) {
+        float* dst = scores + ((static_cast<std::size_t>(u.pad) + i) * kGroup + (lane >> 2)) * kPageTokens + my_key0;
+        *reinterpret_cast<float2*>(dst) = make_float2(sc[0][0], sc[0][1]);
+        *reinterpret_cast<float2*>(dst + 8) = make_float2(sc[1][0], sc[1][1]);
+      }
+    }
+
     // ---- softmax statistics (per head g, the 16 keys spread over the four lanes of a quad) ----
     float tmax = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1]));
     tmax = fmaxf(tmax, __shfl_xor_sync(0xFFFFFFFFU, tmax, 1));
@@ -241,24 +250,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 }  // namespace
 
 cudaError_t ConfigureF16Kernels() {
-  cudaError_t e = cudaFuncSetAttribute(F16DecodePartKernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(F16DecodePartKernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(F16DecodePartKernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  return e;
+  for (auto kernel : {F16DecodePartKernel<false, false, false>, F16DecodePartKernel<true, false, false>,
+                      F16DecodePartKernel<false, true, false>, F16DecodePartKernel<false, false, true>})
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes); e != cudaSuccess) return e;
+  return cudaSuccess;
 }
 
 cudaError_t LaunchF16DecodePart(const DecodeLaunch& a, cudaStream_t stream) {
   if (a.n_units <= 0 || a.n_seqs <= 0) return cudaSuccess;
   if (a.q_raw) {
-    if (a.beside) return cudaErrorInvalidValue;
+    if (a.beside || a.scores_dev != nullptr) return cudaErrorInvalidValue;
     const QueryRaw qr{static_cast<const float*>(a.q_dev), a.q_weight_dev, a.rope_tab_dev, a.q_eps, a.rope_rows};
-    return LaunchChained(F16DecodePartKernel<true, false>, a.n_units, kThreads, kSmemBytes, stream, *a.kmap, *a.vmap, a.pool,
+    return LaunchChained(F16DecodePartKernel<true, false, false>, a.n_units, kThreads, kSmemBytes, stream, *a.kmap, *a.vmap, a.pool,
                          a.layer, a.tables_dev, a.table_stride, a.units_dev, static_cast<const __half*>(nullptr), qr,
-                         a.scale_log2, a.partial_acc, a.partial_ml, a.status_dev);
+                         a.scale_log2, a.partial_acc, a.partial_ml, a.scores_dev, a.status_dev);
   }
-  return LaunchChained(a.beside ? F16DecodePartKernel<false, true> : F16DecodePartKernel<false, false>, a.n_units, kThreads, kSmemBytes,
-                       stream, *a.kmap, *a.vmap, a.pool, a.layer, a.tables_dev, a.table_stride, a.units_dev,
-                       static_cast<const __half*>(a.q_dev), QueryRaw{}, a.scale_log2, a.partial_acc, a.partial_ml, a.status_dev);
+  if (a.beside && a.scores_dev != nullptr) return cudaErrorInvalidValue;
+  const auto kernel = a.beside                  ? F16DecodePartKernel<false, true, false>
+                      : a.scores_dev != nullptr ? F16DecodePartKernel<false, false, true>
+                                                : F16DecodePartKernel<false, false, false>;
+  return LaunchChained(kernel, a.n_units, kThreads, kSmemBytes, stream, *a.kmap, *a.vmap, a.pool, a.layer, a.tables_dev, a.table_stride,
+                       a.units_dev, static_cast<const __half*>(a.q_dev), QueryRaw{}, a.scale_log2, a.partial_acc, a.partial_ml, a.scores_dev, a.status_dev);
 }
 
 }  // namespace yahkv

@@ -1,14 +1,10 @@
 // Attention weights per cached key, and the eviction of keys by them; the page copy of a forked sequence.
 //
 // AttnWeightsKernel adds to w[key] the softmax weights that the six query heads of a kv head's group gave the key in the
-// decode call just made: w[key] += sum_g 2^(s_g - M_g - log2 L_g), s_g = q_g.k * scale in log2 units. The call's
-// partials give M_g and L_g (joined in unit order), so one pass over K is enough; it reads K again (the part kernels
-// keep no scores) and is HBM-bound: half of the cache bytes plus 8 B per key and kv head. Scores are computed in fp32
-// from the fp16 query and the exact codes (f16 MMA on exact fp16 integers, the block scale applied in fp32), so a
-// weight is as exact as fp32 sums make it; the part kernels' 16-bit query planes would cost 2e-5 of a weight.
-// The shape of the decode kernels without their V side: one CTA per split-K unit, a ring of K pages filled by TMA
-// (no multicast), eight warps on two pages at a time, 16 keys of a page per warp, the last of a page's warps refills its
-// stage. No order-dependent sums: each key is added to once per call.
+// decode call just made: w[key] += sum_g 2^(s_g - M_g - log2 L_g). The part kernel has kept the scores s_g (log2 units: the
+// kScores variants in decode_attn.cu and decode_f16.cu), its partials give M_g and L_g, so the pass
+// reads 96 B per key and adds to 16 B. (Reading K again and making the scores anew cost 56 us on a q8_0 batch of 291,000
+// keys beside a part kernel of 113; this pass takes 5 and keeping the scores 20, with fp16 pages 3.) No sum depends on the order of CTAs: each key is added to once per call.
 //
 // EvictSelectKernel, one CTA per (layer, sequence, kv head): the n_keep keys to keep, ascending. The first n_sink and the
 // last n_recent are kept, of the rest the largest weights; ties go to the lowest index, NaN counts as less than
@@ -24,7 +20,6 @@
 #include <algorithm>
 #include <cmath>
 
-#include "decode_ring.cuh"
 #include "kernels.cuh"
 #include "ptx.cuh"
 
@@ -34,224 +29,56 @@ namespace {
 // ----------------------------------------------------------------------------------------------------------------
 // attention weights
 // ----------------------------------------------------------------------------------------------------------------
-constexpr int kKeyGroups = 4;                      // 16 keys of a page each
-constexpr int kPageSets = 2;                       // pages in work at a time: warp w takes those of parity w / 4
-constexpr int kWeightWarps = kKeyGroups * kPageSets;
-constexpr int kWeightThreads = kWeightWarps * 32;
-constexpr int kBoxBytes = kPageTokens * 128;       // one swizzled TMA box: 64 token rows x 128 B
+constexpr int kWeightThreads = 256;
+constexpr int kWeightPages = kWeightThreads / kPageTokens;   // pages per turn, a thread per key
 
-// Shared memory: ring of K boxes | ring of block scales | query operands (quantized formats) | barriers, counters, abort
-// flag. fp16: three stages of 32 KB and two CTAs per SM, the query operands in registers. Quantized formats issue more
-// instructions per byte: three CTAs, q8_0 with 4 x 17 KB, q4_0 with 6 x 9 KB, the query operands in shared memory, so that
-// 80 registers do (with two CTAs and the operands in registers the kernel spilled: 120 us against TODO us).
-template <int kFmt>
-struct WeightSmem {
-  static constexpr int kBoxes = CodeBytes(kFmt) / 128;
-  static constexpr int kStages = kFmt == kFmtF16 ? 3 : kFmt == kFmtQ8 ? 4 : 6;
-  static constexpr int kCtas = kFmt == kFmtF16 ? 2 : 3;
-  static constexpr int kScaleBytes = RecordScaleBytes(kFmt, 0);
-  static constexpr int kTx = kBoxes * kBoxBytes + kScaleBytes;
-  static constexpr int kScaleOff = kStages * kBoxes * kBoxBytes;
-  static constexpr int kQOff = kScaleOff + kStages * kScaleBytes;   // [8 blocks][32 lanes] 16 bytes
-  static constexpr int kBarOff = kQOff + (kFmt == kFmtF16 ? 0 : kBlocksPerRow * 32 * 16);
-  static constexpr int kDoneOff = kBarOff + 8 * kStages;
-  static constexpr int kFillOff = kDoneOff + 4 * kStages;
-  static constexpr int kAbortOff = kFillOff + 4 * kStages;
-  static constexpr int kNormOff = kAbortOff + 4;
-  static constexpr int kBytes = (kNormOff + 4 * 8 + 127) / 128 * 128;
-  static_assert(kCtas * (kBytes + 1024) <= 228 * 1024, "resident CTAs per SM");
-  static_assert(kPageSets <= kStages, "a set never waits for a stage it holds itself");
-};
-constexpr int kStatusSmemMisaligned = 2;
-
-// Four bytes u -> fp16 pairs (0, 1), (2, 3) of u - bias (0x6400 | u is 1024 + u; bias_h = 1024 + bias).
-__device__ __forceinline__ void Bytes4(std::uint32_t u, __half2 bias_h, std::uint32_t& h01, std::uint32_t& h23) {
-  const std::uint32_t a = __byte_perm(u, 0x64646464U, 0x4140), b = __byte_perm(u, 0x64646464U, 0x4342);
-  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias_h), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias_h);
-  h01 = *reinterpret_cast<const std::uint32_t*>(&x), h23 = *reinterpret_cast<const std::uint32_t*>(&y);
-}
-__device__ __forceinline__ float HalfOf(const uint2& v, int i) {   // fp16 number i of four, i a constant after unrolling
-  const std::uint32_t w = i < 2 ? v.x : v.y;
-  const __half2 h = *reinterpret_cast<const __half2*>(&w);
-  return (i & 1) ? __high2float(h) : __low2float(h);
-}
-// D(16 x 8, f32) = A(16 x 16, f16) . B(16 x 8, f16), no accumulator input
-__device__ __forceinline__ void MmaF16Zero(float (&d)[4], std::uint32_t a0, std::uint32_t a1, std::uint32_t a2, std::uint32_t a3,
-                                           std::uint32_t b0, std::uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0F));
-}
-
-template <int kFmt>
-__global__ void __launch_bounds__(kWeightThreads, WeightSmem<kFmt>::kCtas)
-    AttnWeightsKernel(const __grid_constant__ CUtensorMap kmap, PoolView pool, int layer,
-                      const std::int32_t* __restrict__ tables, int table_stride, const DecodeUnit* __restrict__ units,
-                      const CombineItem* __restrict__ items, const __half* __restrict__ q, float scale_log2,
-                      const float* __restrict__ partial_ml, float* __restrict__ weights, long long weights_stride, int* status) {
-  using L = WeightSmem<kFmt>;
-  extern __shared__ __align__(1024) std::uint8_t smem[];
+__global__ void __launch_bounds__(kWeightThreads)
+    AttnWeightsKernel(const DecodeUnit* __restrict__ units, const CombineItem* __restrict__ items,
+                      const float* __restrict__ partial_ml, const float* __restrict__ scores, float* __restrict__ weights,
+                      long long weights_stride) {
+  __shared__ float norm_s[kGroup];   // M + log2 L per query head
   ChainedKernelEntry();
-  float* norm_s = reinterpret_cast<float*>(smem + L::kNormOff);   // M + log2 L per query head
-  std::uint64_t* full_bar = reinterpret_cast<std::uint64_t*>(smem + L::kBarOff);
-  int* done_cnt = reinterpret_cast<int*>(smem + L::kDoneOff);
-  int* fill_cnt = reinterpret_cast<int*>(smem + L::kFillOff);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOff);
-  if ((SmemAddr(smem) & 1023U) != 0) {   // never seen; a misaligned swizzle would corrupt results
-    if (threadIdx.x == 0) atomicExch(status, kStatusSmemMisaligned);
-    return;
-  }
   const DecodeUnit u = units[blockIdx.x];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int kw = warp & (kKeyGroups - 1), par = warp / kKeyGroups;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_pages = u.page_end - u.page_begin;
-  if (n_pages <= 0) return;
-  const std::int32_t* row = tables + static_cast<std::size_t>(u.seq) * table_stride + u.page_begin;
-
-  // Gather of one page's K into a ring stage; a whole converged warp calls it, one elected lane issues. Once a wait has
-  // given up nothing more is fetched.
-  auto issue = [&](int s, std::int32_t page) {
-    if (*abort_flag != 0) return;
-    page = min(max(page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
-    const std::size_t rec = (static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + u.kvh;
-    if (ElectOne()) {
-      fill_cnt[s] += 1;
-      MbarArriveExpectTx(&full_bar[s], L::kTx);
+  // the scores of the first turn are on their way while the norms are made
+  float s[kGroup];
+  auto load = [&](int i) {
+    const float* src = scores + (static_cast<std::size_t>(u.pad) + i) * (kGroup * kPageTokens) + threadIdx.x % kPageTokens;
 #pragma unroll
-      for (int b = 0; b < L::kBoxes; ++b)
-        TmaLoad2D(smem + (s * L::kBoxes + b) * kBoxBytes, &kmap, b * 128, static_cast<int>(rec * kPageTokens), &full_bar[s]);
-      if constexpr (L::kScaleBytes > 0)
-        BulkLoad(smem + L::kScaleOff + s * L::kScaleBytes, pool.kscales + rec * (kPageTokens * kBlocksPerRow), L::kScaleBytes, &full_bar[s]);
-    }
+    for (int h = 0; h < kGroup; ++h) s[h] = i < n_pages ? src[h * kPageTokens] : -INFINITY;
   };
-  if (warp == 0) {
-    if (lane == 0) {
-      PrefetchTensorMap(&kmap);
-      for (int s = 0; s < L::kStages; ++s) {
-        MbarInit(&full_bar[s], 1);
-        done_cnt[s] = 0;
-        fill_cnt[s] = 0;
-      }
-      *abort_flag = 0;
-      FenceBarrierInit();
-    }
-    __syncwarp();
-    for (int i = 0; i < L::kStages && i < n_pages; ++i) issue(i, __ldg(row + i));
-  }
-
-  // M + log2 L of the six heads from the partials of the decode call, warp h < 6 for head h
+  int i = threadIdx.x / kPageTokens;
+  load(i);
   if (warp < kGroup) {
     const CombineItem it = items[u.batch * kKvHeads + u.kvh];
     const float* ml = partial_ml + static_cast<std::size_t>(it.first_partial) * kPartialMlFloats + 2 * warp;
     float m = -INFINITY, l = 0.0F;
-    for (int i = lane; i < it.n_partials; i += 32) m = fmaxf(m, ml[static_cast<std::size_t>(i) * kPartialMlFloats]);
+    for (int k = lane; k < it.n_partials; k += 32) m = fmaxf(m, ml[static_cast<std::size_t>(k) * kPartialMlFloats]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFU, m, o));
-    for (int i = lane; i < it.n_partials; i += 32) {
-      const float mi = ml[static_cast<std::size_t>(i) * kPartialMlFloats];
-      l += mi == -INFINITY ? 0.0F : exp2f(mi - m) * ml[static_cast<std::size_t>(i) * kPartialMlFloats + 1];
+    for (int k = lane; k < it.n_partials; k += 32) {
+      const float mk = ml[static_cast<std::size_t>(k) * kPartialMlFloats];
+      l += mk == -INFINITY ? 0.0F : exp2f(mk - m) * ml[static_cast<std::size_t>(k) * kPartialMlFloats + 1];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFU, l, o);
     if (lane == 0) norm_s[warp] = m + log2f(l);
   }
-  // S[key][head] = K[key][dim] . Q^T[dim][head]: A = 16 keys as ldmatrix hands them over, B = the query, column g = head g.
-  // fp16: dims 16 s + 2t, + 1 and 16 s + 8 + 2t, + 1 of step s. Codes: a 16-byte piece is 16 codes (q8_0) or a block's 32
-  // nibbles (q4_0), lane t has its bytes 4t .. 4t + 3: elements 4t .. of a 32-element block and 16 + 4t ..
-  std::uint32_t qa[kFmt == kFmtF16 ? 32 : 1];
-  if constexpr (kFmt == kFmtF16) {
-    const __half* src = q + (static_cast<std::size_t>(u.batch) * kQHeads + u.kvh * kGroup + min(g, kGroup - 1)) * kHeadDim;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) qa[i] = g < kGroup ? __ldg(reinterpret_cast<const std::uint32_t*>(src + 8 * i + 2 * t)) : 0U;
-  } else {   // warp b lays out block b: lane (g, t) dims 32 b + 4t .. + 3 and 32 b + 16 + 4t .. + 3 of head g
-    const __half* src = q + (static_cast<std::size_t>(u.batch) * kQHeads + u.kvh * kGroup + min(g, kGroup - 1)) * kHeadDim + 32 * warp;
-    uint2 lo = __ldg(reinterpret_cast<const uint2*>(src + 4 * t)), hi = __ldg(reinterpret_cast<const uint2*>(src + 16 + 4 * t));
-    if (g >= kGroup) lo = hi = make_uint2(0, 0);
-    *reinterpret_cast<uint4*>(smem + L::kQOff + (warp * 32 + lane) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-    static_assert(kWeightWarps == kBlocksPerRow, "a warp per block");
-  }
-  __syncthreads();   // barriers initialised, norms visible
-  // this thread's results are heads 2t, 2t + 1 of keys g and g + 8; the padding heads weigh nothing
-  const float norm0 = t < 3 ? norm_s[2 * t] : INFINITY, norm1 = t < 3 ? norm_s[2 * t + 1] : INFINITY;
-  float* w_out = weights + (static_cast<std::size_t>(u.seq) * kKvHeads + u.kvh) * static_cast<std::size_t>(weights_stride);
-  const __half2 bias = __half2half2(__ushort_as_half(kFmt == kFmtQ8 ? 0x6480 : 0x6408));
-  // ldmatrix rows: matrices = (keys 0-7 | 8-15 of the group) x (16-byte pieces 2x | 2x + 1); piece p of row r sits at p ^ (r % 8)
-  const int lm_key = kw * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
-  const std::uint32_t lm0 = lm_key * 128 + (((lane >> 4) ^ (lm_key & 7)) << 4);
-
-  bool alive = true;
-  for (int i = par; i < n_pages; i += kPageSets) {
-    const int s = i % L::kStages, gen = i / L::kStages;
-    std::int32_t refill_page = 0;
-    if (lane == 0 && i + L::kStages < n_pages) refill_page = __ldg(row + i + L::kStages);
-    alive = RingWait(alive, fill_cnt + s, &full_bar[s], gen, abort_flag);
-    const std::uint32_t k_base = SmemAddr(smem + s * L::kBoxes * kBoxBytes);
-    float sc[4] = {0.0F, 0.0F, 0.0F, 0.0F};   // (key g, head 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1)
-    if constexpr (kFmt == kFmtF16) {
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        std::uint32_t w[4];
-        LdMatrixX4(k_base + (x >> 2) * kBoxBytes + (lm0 ^ (static_cast<std::uint32_t>(x & 3) << 5)), w);
-        MmaF16(sc, w[0], w[1], w[2], w[3], qa[2 * x], qa[2 * x + 1]);
-      }
-    } else {
-      const std::uint8_t* scales = smem + L::kScaleOff + s * L::kScaleBytes + (kw * 16 + g) * (kBlocksPerRow * 2);
-      const std::uint32_t q_base = SmemAddr(smem + L::kQOff) + lane * 16;
-#pragma unroll
-      for (int dh = 0; dh < 2; ++dh) {   // blocks 4 dh .. + 3; scales fetched per half to keep registers low
-        const uint2 d0 = *reinterpret_cast<const uint2*>(scales + dh * 8);
-        const uint2 d1 = *reinterpret_cast<const uint2*>(scales + 8 * (kBlocksPerRow * 2) + dh * 8);
-        // one block of 32 elements: two k-steps into a fresh accumulator, then the keys' scales
-        auto block = [&](int b, std::uint32_t lo0, std::uint32_t lo1, std::uint32_t hi0, std::uint32_t hi1) {
-          std::uint32_t qb[4], a0, a1, a2, a3;
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(qb[0]), "=r"(qb[1]), "=r"(qb[2]), "=r"(qb[3])
-                       : "r"(q_base + (4 * dh + b) * 512));
-          float acc[4];
-          Bytes4(lo0, bias, a0, a2);
-          Bytes4(lo1, bias, a1, a3);
-          MmaF16Zero(acc, a0, a1, a2, a3, qb[0], qb[1]);
-          Bytes4(hi0, bias, a0, a2);
-          Bytes4(hi1, bias, a1, a3);
-          MmaF16(acc, a0, a1, a2, a3, qb[2], qb[3]);
-          const float s0 = HalfOf(d0, b), s1 = HalfOf(d1, b);
-          sc[0] = fmaf(s0, acc[0], sc[0]), sc[1] = fmaf(s0, acc[1], sc[1]);
-          sc[2] = fmaf(s1, acc[2], sc[2]), sc[3] = fmaf(s1, acc[3], sc[3]);
-        };
-        if constexpr (kFmt == kFmtQ8) {
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {   // pieces 2b, 2b + 1 of box dh: one block
-            std::uint32_t w[4];
-            LdMatrixX4(k_base + dh * kBoxBytes + (lm0 ^ (static_cast<std::uint32_t>(b) << 5)), w);
-            block(b, w[0] ^ kQ8FlipWord, w[1] ^ kQ8FlipWord, w[2] ^ kQ8FlipWord, w[3] ^ kQ8FlipWord);
-          }
-        } else {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {   // a piece is a block
-            std::uint32_t w[4];
-            LdMatrixX4(k_base + (lm0 ^ (static_cast<std::uint32_t>(2 * dh + x) << 5)), w);
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              block(2 * x + k, w[2 * k] & 0x0F0F0F0FU, w[2 * k + 1] & 0x0F0F0F0FU, (w[2 * k] >> 4) & 0x0F0F0F0FU,
-                    (w[2 * k + 1] >> 4) & 0x0F0F0F0FU);
-          }
-        }
-      }
-    }
-    // the stage is in registers: the last of the page's four warps refills it
-    const bool last = RingRelease(&done_cnt[s], lane, kKeyGroups);
-    if (last && i + L::kStages < n_pages) issue(s, __shfl_sync(0xFFFFFFFFU, refill_page, 0));
-    float p0 = exp2f(fmaf(sc[0], scale_log2, -norm0)) + exp2f(fmaf(sc[1], scale_log2, -norm1));
-    float p1 = exp2f(fmaf(sc[2], scale_log2, -norm0)) + exp2f(fmaf(sc[3], scale_log2, -norm1));
-    p0 += __shfl_xor_sync(0xFFFFFFFFU, p0, 1), p1 += __shfl_xor_sync(0xFFFFFFFFU, p1, 1);
-    p0 += __shfl_xor_sync(0xFFFFFFFFU, p0, 2), p1 += __shfl_xor_sync(0xFFFFFFFFU, p1, 2);
-    // lanes t = 0 and 1 add keys g and g + 8: one addition per key and call, so the order of CTAs does not matter
-    const int key = (u.page_begin + i) * kPageTokens + kw * 16 + 8 * t + g;
-    if (t < 2 && key < u.n_keys) atomicAdd(w_out + key, t == 0 ? p0 : p1);
-  }
-  if (!alive && lane == 0) atomicExch(status, kStatusWaitTimeout);
   __syncthreads();
-  RingDrainAfterAbort(abort_flag, fill_cnt, full_bar, L::kStages);
+  float norm[kGroup];
+#pragma unroll
+  for (int h = 0; h < kGroup; ++h) norm[h] = norm_s[h];
+  float* w_out = weights + (static_cast<std::size_t>(u.seq) * kKvHeads + u.kvh) * static_cast<std::size_t>(weights_stride);
+  for (; i < n_pages; i += kWeightPages) {
+    float p = 0.0F;
+#pragma unroll
+    for (int h = 0; h < kGroup; ++h) p += exp2f(s[h] - norm[h]);
+    const int key = (u.page_begin + i) * kPageTokens + threadIdx.x % kPageTokens;
+    load(i + kWeightPages);
+    // one addition per key and call, so the order of CTAs does not matter; nothing waits for it
+    if (key < u.n_keys) atomicAdd(w_out + key, p);
+  }
 }
 
 // ----------------------------------------------------------------------------------------------------------------
@@ -263,7 +90,7 @@ constexpr int kSelectTile = kSelectThreads * kSelectPer;
 constexpr int kSelectCache = 36 * 1024;                        // keys whose words are kept in shared memory (144 KB)
 // Histograms: a lane counts into copy lane % 8, copies an odd number of words apart, so that equal weights (zeros above
 // all) meet four at a time and not 32 at a time. (One histogram with the lanes of equal bins joined by match.any first:
-// 33 us for 128 rows of 14,000 keys against TODO us.)
+// 33 us for 128 rows of 14,000 keys against 26.)
 constexpr int kHistCopies = 8, kHistBins = 2048, kHistStride = kHistBins + 1;
 
 // Order-preserving bits of a weight: larger weight, larger word; NaN below everything, -0 equal to +0.
@@ -480,28 +307,16 @@ __global__ void __launch_bounds__(256) CopyPageKernel(PoolView pool, int src, in
 
 int SelectSmem(int n_cache) { return 4 * (kHistCopies * kHistStride + n_cache); }
 
-template <int kFmt>
-cudaError_t LaunchWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream) {
-  return LaunchChained(AttnWeightsKernel<kFmt>, a.n_units, kWeightThreads, WeightSmem<kFmt>::kBytes, stream, *a.kmap, a.pool, a.layer,
-                       a.tables_dev, a.table_stride, a.units_dev, a.items_dev, static_cast<const __half*>(a.q_dev), a.scale_log2,
-                       a.partial_ml, weights, weights_stride, a.status_dev);
-}
-
 }  // namespace
 
 cudaError_t ConfigureEvictKernels() {
-  cudaError_t e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtF16>::kBytes);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtQ8>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtQ8>::kBytes);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(AttnWeightsKernel<kFmtQ4>, cudaFuncAttributeMaxDynamicSharedMemorySize, WeightSmem<kFmtQ4>::kBytes);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(EvictSelectKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SelectSmem(kSelectCache));
-  return e;
+  return cudaFuncSetAttribute(EvictSelectKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SelectSmem(kSelectCache));
 }
 
 cudaError_t LaunchAttnWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream) {
   if (a.n_units <= 0) return cudaSuccess;
-  if (a.pool.fmt == kFmtF16) return LaunchWeights<kFmtF16>(a, weights, weights_stride, stream);
-  return a.pool.fmt == kFmtQ8 ? LaunchWeights<kFmtQ8>(a, weights, weights_stride, stream)
-                              : LaunchWeights<kFmtQ4>(a, weights, weights_stride, stream);
+  return LaunchChained(AttnWeightsKernel, a.n_units, kWeightThreads, 0, stream, a.units_dev, a.items_dev, a.partial_ml, a.scores_dev,
+                       weights, weights_stride);
 }
 
 cudaError_t LaunchEvict(const EvictLaunch& a, cudaStream_t stream) {

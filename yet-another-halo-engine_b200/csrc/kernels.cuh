@@ -88,7 +88,7 @@ struct DecodeUnit {
   std::int32_t page_end;
   std::int32_t n_keys;      // visible keys of the sequence (its length)
   std::int32_t partial;     // row of the partial workspace this unit writes
-  std::int32_t pad;
+  std::int32_t pad;         // tile formats: the current open-tile buffer; others: slot of the unit's first page in the scores
 };
 // Where the partials of one (batch row, kv head) lie, for the combine pass.
 struct CombineItem {
@@ -237,6 +237,7 @@ struct DecodeLaunch {
   float* partial_ml;
   int* status_dev;          // sticky error word, 0 = ok
   bool beside;              // the part kernel may run beside the kernel launched just before it (fp16 query only)
+  float* scores_dev;        // not null: the part kernel keeps its scores here, [page slot][6][64] (fp16 query only)
 };
 cudaError_t LaunchDecodePart(const DecodeLaunch& a, cudaStream_t stream);
 // fp16 pages (decode_f16.cu)
@@ -319,9 +320,9 @@ struct EvictLaunch {
   std::int32_t* kept;
 };
 cudaError_t LaunchEvict(const EvictLaunch& a, cudaStream_t stream);
-// After LaunchDecodePart of the same plan (its partial_ml holds the rows' statistics); fp16 query.
+// After the part kernel of the same plan with scores_dev set: its scores and its partial_ml are read.
 cudaError_t LaunchAttnWeights(const DecodeLaunch& a, float* weights, long long weights_stride, cudaStream_t stream);
-cudaError_t ConfigureEvictKernels();   // weights and selection
+cudaError_t ConfigureEvictKernels();
 cudaError_t LaunchCopyPage(const PoolView& pool, int src, int dst, cudaStream_t stream);
 
 // Rotary positions on given rows (rope.cu).

@@ -357,6 +357,7 @@ class KvHost {
     auto_pages = std::min(std::max(auto_pages, 1), 24);
     std::vector<DecodeUnit> units;
     std::vector<CombineItem> items(static_cast<std::size_t>(n_seqs) * kKvHeads);
+    std::int32_t slot = 0;   // pages of the units so far
     for (int b = 0; b < n_seqs; ++b) {
       const int s = seq_ids[b];
       const std::int64_t n = len(s, layer);
@@ -371,6 +372,8 @@ class KvHost {
           u.page_begin = k == 0 ? 0 : bounds_[static_cast<std::size_t>(k) - 1], u.page_end = bounds_[static_cast<std::size_t>(k)];
           u.n_keys = static_cast<std::int32_t>(n);
           u.partial = static_cast<std::int32_t>(units.size());
+          u.pad = slot;
+          slot += u.page_end - u.page_begin;
           units.push_back(u);
         }
       }
@@ -382,6 +385,7 @@ class KvHost {
     std::stable_sort(units.begin(), units.end(), [](const DecodeUnit& a, const DecodeUnit& b) {
       return a.page_end - a.page_begin > b.page_end - b.page_begin;
     });
+    unit_pages_ = slot;
     units_ = std::move(units);
     items_ = std::move(items);
     plan_key_ = key_scratch_;
@@ -694,6 +698,7 @@ class KvHost {
     if (open_cur_.empty()) return;
     for (int l = 0; l < cfg_.n_layers; ++l) open_cur_[static_cast<std::size_t>(seq) * static_cast<std::size_t>(cfg_.n_layers) + static_cast<std::size_t>(l)] = 0;
   }
+  std::int64_t unit_pages() const { return unit_pages_; }   // pages of all units of the plan: slots of their scores
   const std::vector<DecodeUnit>& units() const { return units_; }
   const std::vector<CombineItem>& items() const { return items_; }
 
@@ -886,6 +891,7 @@ class KvHost {
   std::vector<std::pair<int, std::int64_t>> scratch_len_;
   std::vector<std::int64_t> key_scratch_, plan_key_;
   std::vector<DecodeUnit> units_;
+  std::int64_t unit_pages_ = 0;
   std::vector<CombineItem> items_;
   SharedPlan shared_;           // cached plan of attend_decode_shared
   std::vector<int> open_cur_;   // kv8a16: current open-tile buffer per (sequence, layer)

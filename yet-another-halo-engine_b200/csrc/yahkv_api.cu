@@ -161,6 +161,9 @@ struct yahkv_ctx {
     float *part_acc = nullptr, *part_ml = nullptr;
     CUtensorMap k16map{}, v16map{};   // fp16 pages as [rows][256] fp16
   } shared;
+  // scores of a weight-accumulating decode call, grown to the largest call seen
+  float* scores_dev = nullptr;
+  std::int64_t score_pages = 0;
   // eviction work lists, allocated by the first call
   char* evict_dev = nullptr;
   std::vector<EvictSeq> evict_scratch;
@@ -313,7 +316,7 @@ void FreeDevice(yahkv_ctx* ctx) {
                   ctx->merges_dev, ctx->part_acc_dev, ctx->part_ml_dev,
                   ctx->rope_tab_dev, ctx->rope_pos_dev, ctx->open_tiles_dev, ctx->kmean_dev, ctx->state_rows_dev,
                   ctx->vwork_dev,   ctx->rope_kv16_dev, ctx->shared.plan_dev, ctx->shared.part_acc,
-                  ctx->shared.part_ml, ctx->evict_dev};
+                  ctx->shared.part_ml, ctx->evict_dev, ctx->scores_dev};
   for (void* p : ptrs)
     if (p != nullptr) cudaFree(p);
   for (cudaStream_t st : {ctx->h2d_stream, ctx->d2h_stream})
@@ -797,6 +800,20 @@ int yahkv_attend_decode_qraw(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, cons
                       n_splits, nullptr, 0, stream);
 }
 
+// Room for the scores of `pages` pages of one kv head each (1.5 KB), grown by half at least so that contexts which grow page
+// by page rarely find it too small; growing waits for the device.
+static int EnsureScores(yahkv_ctx* ctx, std::int64_t pages) {
+  if (pages <= ctx->score_pages) return YAHKV_OK;
+  constexpr std::int64_t kFloats = kGroup * kPageTokens;
+  const std::int64_t want = std::max<std::int64_t>({pages, ctx->score_pages + ctx->score_pages / 2, 1024});
+  YAHKV_CUDA(ctx, cudaDeviceSynchronize());
+  if (ctx->scores_dev != nullptr) cudaFree(ctx->scores_dev), ctx->device_bytes -= ctx->score_pages * kFloats * 4;
+  ctx->scores_dev = nullptr, ctx->score_pages = 0;
+  YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->scores_dev, static_cast<std::size_t>(want * kFloats), false));
+  ctx->score_pages = want;
+  return YAHKV_OK;
+}
+
 static int AttendDecode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev, bool q_raw,
                         const float* q_weight_dev, float eps, const float* gate_dev, void* out_dev, int32_t out_dtype,
                         int32_t n_splits, float* weights_dev, int64_t weights_stride, void* stream) {
@@ -854,6 +871,10 @@ static int AttendDecode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int
   a.q_raw = q_raw, a.q_weight_dev = q_weight_dev, a.q_eps = eps, a.rope_tab_dev = ctx->rope_tab_dev, a.rope_rows = ctx->rope_rows;
   a.scale_log2 = ctx->scale_log2;
   a.partial_acc = ctx->partial_acc, a.partial_ml = ctx->partial_ml, a.status_dev = ctx->status_dev;
+  if (weights_dev != nullptr) {
+    if (int r = EnsureScores(ctx, ctx->host.unit_pages()); r != YAHKV_OK) return r;
+    a.scores_dev = ctx->scores_dev;
+  }
   // The merge runs as its own small launch: letting the last-arriving unit merge inside the part kernel was measured
   // 1% slower end to end (every CTA then pays a fence and an atomic on exit).
   TimedLaunch tp(ctx, YAHKV_KERNEL_DECODE_PART, st);
