@@ -72,6 +72,13 @@ __global__ void BatchAdvanceKernel(std::int32_t* __restrict__ lens, int n_seqs, 
   if (b < n_seqs) lens[b] += by;
 }
 
+__global__ void TableUploadKernel(const TableRange* __restrict__ ranges, const std::int32_t* __restrict__ data,
+                                  std::int32_t* __restrict__ tables) {
+  ChainedKernelEntry();
+  const TableRange r = ranges[blockIdx.x];
+  for (int i = threadIdx.x; i < r.count; i += blockDim.x) tables[r.dst + i] = data[r.src + i];
+}
+
 // A wait that cannot succeed: the barrier expects one arrival and nobody arrives. The kernel leaves by the same path
 // a real kernel takes when a copy never lands: it stops waiting at the limit, sets the sticky status word, returns.
 __global__ void WaitProbeKernel(int* status, std::uint64_t limit_ns) {
@@ -101,6 +108,11 @@ cudaError_t LaunchBatchPlan(const std::int32_t* lens_dev, const BatchSeq* seqs_d
   return LaunchChained(BatchPlanKernel, (threads + 127) / 128, 128, 0, stream, lens_dev, seqs_dev, n_seqs, tables_dev,
                        table_stride, unit_pages, num_pages, units_dev, items_dev, slots_dev, vwork_dev, state_rows_dev,
                        n_layers);
+}
+
+cudaError_t LaunchTableUpload(const TableRange* ranges, int n, const std::int32_t* data, std::int32_t* tables_dev, cudaStream_t stream) {
+  if (n <= 0) return cudaSuccess;
+  return LaunchChained(TableUploadKernel, n, 128, 0, stream, ranges, data, tables_dev);
 }
 
 cudaError_t LaunchBatchAdvance(std::int32_t* lens_dev, int n_seqs, int by, cudaStream_t stream) {

@@ -112,6 +112,14 @@ cudaError_t LaunchBatchPlan(const std::int32_t* lens_dev, const BatchSeq* seqs_d
                             const std::int32_t* tables_dev, int table_stride, int unit_pages, int num_pages,
                             DecodeUnit* units_dev, CombineItem* items_dev, std::int64_t* slots_dev,
                             VTileWork* vwork_dev, std::int32_t* state_rows_dev, int n_layers, cudaStream_t stream);
+// Changed runs of block-table rows: `count` entries from data[src] on go to tables[dst] on. ranges and data are page-locked
+// host memory that the device reads where it lies.
+struct TableRange {
+  std::int64_t dst;
+  std::int32_t src;
+  std::int32_t count;
+};
+cudaError_t LaunchTableUpload(const TableRange* ranges, int n, const std::int32_t* data, std::int32_t* tables_dev, cudaStream_t stream);
 cudaError_t LaunchBatchAdvance(std::int32_t* lens_dev, int n_seqs, int by, cudaStream_t stream);
 
 // Prefill attention reads a dequantized fp16 copy of the sequences' K and V (the reference's yah_kdeq / yah_vdeq

@@ -400,12 +400,33 @@ int FlushTables(yahkv_ctx* ctx, cudaStream_t stream) {
     for (const Range& r : ranges) ctx->host.MarkDirtyAgain(r.seq, r.lo, r.hi);
     return FailCuda(ctx, what, e);
   };
+  ranges.erase(std::remove_if(ranges.begin(), ranges.end(), [](const Range& r) { return r.hi <= r.lo; }), ranges.end());
+  if (ranges.empty()) return YAHKV_OK;
+  const std::size_t heads = ranges.size() * sizeof(TableRange);
   char* buf = nullptr;
-  if (cudaError_t e = ctx->staging.Acquire(total, &buf); e != cudaSuccess) return fail("table staging", e);
+  if (cudaError_t e = ctx->staging.Acquire(heads + total, &buf); e != cudaSuccess) return fail("table staging", e);
+  if (ranges.size() > 1) {
+    // several rows: one kernel reads them from the (page-locked, mapped) staging buffer; a copy each took 2 us of stream
+    // time per row
+    std::int32_t* data = reinterpret_cast<std::int32_t*>(buf + heads);
+    std::int32_t at = 0;
+    for (std::size_t i = 0; i < ranges.size(); ++i) {
+      const Range& r = ranges[i];
+      const TableRange t{static_cast<std::int64_t>(r.seq) * ctx->cfg.max_pages_per_seq + r.lo, at, r.hi - r.lo};
+      std::memcpy(buf + i * sizeof(TableRange), &t, sizeof(t));
+      std::memcpy(data + at, ctx->host.table_row(r.seq) + r.lo, static_cast<std::size_t>(r.hi - r.lo) * 4);
+      at += r.hi - r.lo;
+    }
+    if (cudaError_t e = LaunchTableUpload(reinterpret_cast<const TableRange*>(buf), static_cast<int>(ranges.size()), data, ctx->tables_dev, stream);
+        e != cudaSuccess)
+      return fail("table upload", e);
+    if (cudaError_t e = ctx->staging.Release(stream); e != cudaSuccess) return fail("table staging event", e);
+    ctx->launches += 1;
+    return YAHKV_OK;
+  }
   std::size_t off = 0;
   for (const Range& r : ranges) {
     const std::size_t bytes = static_cast<std::size_t>(r.hi - r.lo) * 4;
-    if (bytes == 0) continue;
     std::memcpy(buf + off, ctx->host.table_row(r.seq) + r.lo, bytes);
     if (cudaError_t e = cudaMemcpyAsync(ctx->tables_dev + static_cast<std::size_t>(r.seq) * ctx->cfg.max_pages_per_seq + r.lo,
                                         buf + off, bytes, cudaMemcpyHostToDevice, stream);
