@@ -158,6 +158,10 @@ __device__ __forceinline__ void BulkLoad(void* smem_dst, const void* gsrc, std::
                "l"(reinterpret_cast<std::uint64_t>(gsrc)), "r"(bytes), "r"(SmemAddr(bar))
                : "memory");
 }
+// Asks for `bytes` (a multiple of 16, from a 16-byte boundary on) to be brought into L2. Nothing waits for it.
+__device__ __forceinline__ void PrefetchL2(const void* p, std::uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<std::uint64_t>(p)), "r"(bytes) : "memory");
+}
 // 1-D bulk copy shared -> global, same alignment rules; the calling thread's earlier shared-memory writes must have been
 // fenced with FenceProxyAsync. BulkStoreWait waits until this thread's copies are complete.
 __device__ __forceinline__ void BulkStore(void* gdst, const void* smem_src, std::uint32_t bytes) {

@@ -16,15 +16,18 @@
 //
 // Operands. fp16 pages are the operands as they lie in the pool: a page of one kv head is 64 rows of 512 B, and each CTA
 // of the pair loads half of it (keys 32 rank .. + 31 of K, dims 128 rank .. + 127 of V) by TMA with 128-byte swizzle,
-// no multicast. q8_0 / q4_0 pages arrive as codes and block scales in a ring of raw stages (linear bulk copies; q8_0 V
-// as a TMA box) and four more warps turn each CTA's half into the same fp16 tiles: the code is an exact fp16 integer,
+// no multicast. q8_0 / q4_0 pages are loaded as codes and block scales by eight more warps (two groups taking alternate
+// tiles, a tile ahead in registers) which write each CTA's half as the same fp16 tiles: the code is an exact fp16 integer,
 // the product with the block's fp16 scale is rounded once to fp16, the values the prefill pass works on too. Rounding
 // K and V to 11 bits (the codes have 8 and the scales 11) costs about 2e-4 of an output's size each, as much as the fp16
 // rounding of the output itself; exact products would need a second MMA per operand.
 //
-// What bounds it: HBM as long as a group has few rows (a 64-key tile is 64 KB of fp16, 34 KB of q8_0, 18 KB of q4_0
-// pages per kv head, and takes the pair's tensor pipes 1,024 clocks whatever the number of rows), the tensor pipe from
-// about 42 rows per group on (a second pair re-reads the pages from L2).
+// What bounds it. fp16 pages: HBM as long as a group has at most 42 rows (a 64-key tile is 64 KB and takes the pair's
+// tensor pipes 1,024 clocks whatever the number of rows): 16 rows x 65536 in 47 us = 5.7 TB/s; with more rows a second
+// pair re-reads the pages from L2 and the tensor pipe bounds (96 rows x 32768: 0.75 us a tile at the 1.6 GHz the power
+// cap leaves, 70 % of the pipe over the whole kernel, 6 us of it prologue and epilogue). Quantized pages: a tile takes
+// 0.9 us for any number of rows, two thirds of it tensor time; with the conversion's stores left out it takes 0.79, with
+// its arithmetic left out no less, so what is left over fp16 is shared-memory traffic (32 KB written per tile and CTA).
 #include <cuda_fp16.h>
 
 #include <cmath>
@@ -52,32 +55,22 @@ constexpr int kTmemCols = 512, kColS = 0, kColO = 128, kColQ = 384;   // S 2 x 6
 constexpr float kLazyRescale = 8.0F;
 constexpr int kStatusAbort = 5;
 constexpr int kOutPitch = kHeadDim * 4 + 16;   // an output row in shared memory: four banks further per row
-constexpr int kMaxStages = 5, kMaxRaw = 4;
+constexpr int kMaxStages = 5;
 
 template <int kFmt>
 struct Shape {
   static constexpr bool kQuant = kFmt != kFmtF16;
   // fp16 half tiles of K and of V in flight, each with barriers of its own: S runs two tiles ahead of P V, so K is done
   // with long before V is, and the stage of K(j + 3) must not wait for P(j) V(j) (one ring for both: the conversion of a
-  // tile and its products took turns, 3,500 clocks per q4_0 tile against 1,700 with two)
+  // tile and its products took turns, 3,500 clocks per q4_0 tile against 2,400 with two)
   static constexpr int kKStages = kQuant ? 3 : 5;
   static constexpr int kVStages = kQuant ? 4 : 5;
-  static constexpr int kThreads = kQuant ? 32 * (kWarpDequant + kDequantWarps * kDequantGroups) : kSoftmaxThreads + 64;
-  // One raw stage of this CTA's half of a page: V codes (q8_0: a 64 x 128 B box of the half's dims; q4_0: the whole
-  // record, whose rows are 128 B), K codes of 32 keys, block scales of 32 K rows and of 64 V rows.
-  static constexpr int kRawStages = kQuant ? kMaxRaw : 0;
-  static constexpr int kRawV = 0, kRawVBytes = kTileN * 128;
-  static constexpr int kRawK = kRawVBytes, kRawKBytes = (kTileN / 2) * CodeBytes(kFmt);
-  static constexpr int kRawKs = kRawK + kRawKBytes, kRawKsBytes = (kTileN / 2) * kBlocksPerRow * 2;
-  static constexpr int kRawVs = kRawKs + kRawKsBytes, kRawVsBytes = kTileN * kBlocksPerRow * 2;
-  static constexpr int kRawTx = kRawVBytes + kRawKBytes + kRawKsBytes + kRawVsBytes;
-  static constexpr int kRawBytes = (kRawTx + 1023) / 1024 * 1024;
+  static constexpr int kThreads = kSoftmaxThreads + 64 + (kQuant ? 32 * kDequantWarps * kDequantGroups : 0);
   static constexpr int kSmemK = 0;
   static constexpr int kSmemV = kSmemK + kKStages * kKHalfBytes;
   static constexpr int kSmemP = kSmemV + kVStages * kVHalfBytes;
-  static constexpr int kSmemRaw = kSmemP + 2 * kPBytes;
-  static constexpr int kSmemBars = kSmemRaw + kRawStages * kRawBytes;
-  static_assert(kTileM * kOutPitch <= kSmemRaw, "the output rows take the place of the tiles");
+  static constexpr int kSmemBars = kSmemP + 2 * kPBytes;
+  static_assert(kTileM * kOutPitch <= kSmemBars, "the output rows take the place of the tiles");
   static constexpr int kBarBytes = 512;
   static constexpr int kBytes = kSmemBars + kBarBytes + 3 * kTileM * 4;   // barriers, then the max / sum exchange
   static_assert(kBytes <= 232448, "shared memory of one CTA");
@@ -91,8 +84,6 @@ struct SharedBars {
   std::uint64_t v_full[kMaxStages];
   std::uint64_t k_empty[kMaxStages];     // both: MMA -> the stage's writer: S(j) is complete
   std::uint64_t v_empty[kMaxStages];     // both: P(j) V(j) is complete
-  std::uint64_t raw_full[kMaxRaw];       // local: TMA -> dequantizing warps
-  std::uint64_t raw_empty[kMaxRaw];      // local: dequantizing warps -> TMA
   std::uint64_t s_full[2];               // both
   std::uint64_t s_free[2];               // leader
   std::uint64_t p_full[2];               // leader
@@ -101,6 +92,7 @@ struct SharedBars {
   std::uint64_t o_done;                  // both
   std::uint32_t tmem_base;
   int abort_flag;
+  int converted[2];                      // local: per group of dequantizing warps, tiles up to this one are converted
 };
 
 // Eight values of a row as fp16: exact integer codes times the block scale, one rounding.
@@ -145,6 +137,13 @@ __device__ __forceinline__ uint4 DequantChunk(uint2 codes, int c8, std::uint16_t
   return ScaleCodes(h, scale);
 }
 
+// 8 bytes that are read once: past L1.
+__device__ __forceinline__ uint2 LoadStream8(const std::uint8_t* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
 template <int kFmt>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThreads, 1)
     SharedPrefixKernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PoolView pool,
@@ -177,10 +176,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
       MbarInit(&bars->v_full[s], S::kQuant ? 2 * kDequantWarps : 1);
       MbarInit(&bars->v_empty[s], 1);
     }
-    for (int s = 0; s < S::kRawStages; ++s) {
-      MbarInit(&bars->raw_full[s], 1);
-      MbarInit(&bars->raw_empty[s], kDequantWarps);
-    }
     for (int g = 0; g < 2; ++g) {
       MbarInit(&bars->s_full[g], 1);
       MbarInit(&bars->s_free[g], 2 * kSoftmaxThreads / 64);
@@ -190,6 +185,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
     }
     MbarInit(&bars->o_done, 1);
     bars->abort_flag = 0;
+    bars->converted[0] = bars->converted[1] = 0;
     FenceBarrierInit();
   }
   if (warp == kWarpMma) {
@@ -208,26 +204,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
   const std::int32_t* table = tables + static_cast<std::size_t>(tile.seq) * table_stride + tile.page_begin;
 
   if (warp == kWarpTma) {
-    // ------------------------------ producer: this CTA's half of every page ------------------------------
-    const bool elected = ElectOne();
-    if (elected) {
-      PrefetchTensorMap(&kmap);
-      PrefetchTensorMap(&vmap);
-    }
-    bool ok = true;
-    constexpr int kRing = S::kQuant ? S::kRawStages : S::kKStages;
-    static_assert(S::kQuant || S::kKStages == S::kVStages, "one stage index for both");
-    int s = 0, issued = 0, issued_k = 0;
-    std::uint32_t ph = 1;
-    std::int32_t next_page = __ldg(table);
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      const std::int32_t page = min(max(next_page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
-      if (j + 1 < n_tiles) next_page = __ldg(table + j + 1);
-      const std::size_t rec = (static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + tile.kvh;
-      const int y = static_cast<int>(rec * kPageTokens);
-      if (j >= kRing) ok = WaitOrAbort(S::kQuant ? &bars->raw_empty[s] : &bars->k_empty[s], ph, abort_flag);
-      if (!ok) break;
-      if constexpr (!S::kQuant) {
+    // ------------------------------ producer of fp16 pages: this CTA's half of every page ------------------------------
+    if constexpr (!S::kQuant) {
+      const bool elected = ElectOne();
+      if (elected) {
+        PrefetchTensorMap(&kmap);
+        PrefetchTensorMap(&vmap);
+      }
+      static_assert(S::kKStages == S::kVStages, "one stage index for both");
+      constexpr int kRing = S::kKStages;
+      bool ok = true;
+      int s = 0, issued_k = 0, issued_v = 0;
+      std::uint32_t ph = 1;
+      std::int32_t next_page = __ldg(table);
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const std::int32_t page = min(max(next_page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
+        if (j + 1 < n_tiles) next_page = __ldg(table + j + 1);
+        const std::size_t rec = (static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + tile.kvh;
+        const int y = static_cast<int>(rec * kPageTokens);
+        if (j >= kRing) ok = WaitOrAbort(&bars->k_empty[s], ph, abort_flag);
+        if (!ok) break;
         if (elected) {
           const std::uint32_t full = MapToCta(SmemAddr(&bars->k_full[s]), 0);
           if (rank == 0) MbarArriveExpectTx(&bars->k_full[s], 2 * kKHalfBytes);
@@ -247,32 +243,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
             TmaLoad2DPair(smem + S::kSmemV + s * kVHalfBytes + kb * kVBlockBytes, &vmap, (static_cast<int>(rank) * 2 + kb) * 64,
                           y, full);
         }
-      } else {
-        if (elected) {
-          std::uint8_t* st = smem + S::kSmemRaw + s * S::kRawBytes;
-          const int k0 = static_cast<int>(rank) * (kTileN / 2);
-          MbarArriveExpectTx(&bars->raw_full[s], S::kRawTx);
-          BulkLoad(st + S::kRawK, pool.kcodes + rec * RecordCodeBytes(kFmt) + k0 * CodeBytes(kFmt), S::kRawKBytes, &bars->raw_full[s]);
-          if constexpr (kFmt == kFmtQ8)
-            TmaLoad2D(st + S::kRawV, &vmap, static_cast<int>(rank) * 128, y, &bars->raw_full[s]);
-          else
-            BulkLoad(st + S::kRawV, pool.vcodes + rec * RecordCodeBytes(kFmt), S::kRawVBytes, &bars->raw_full[s]);
-          BulkLoad(st + S::kRawKs, pool.kscales + (rec * kPageTokens + k0) * kBlocksPerRow, S::kRawKsBytes, &bars->raw_full[s]);
-          BulkLoad(st + S::kRawVs, pool.vscales + rec * (kPageTokens * kBlocksPerRow), S::kRawVsBytes, &bars->raw_full[s]);
+        issued_v = j + 1;
+        if (++s == kRing) s = 0, ph ^= 1U;
+      }
+      // After a wait that gave up, the copies still in flight get one more bounded wait each (the last fill of a stage
+      // says which phase is outstanding), so that none lands in shared memory after the CTA has left it. The bytes of
+      // both CTAs are counted on the leader's barriers, and both CTAs meet at the cluster barrier below.
+      if (*abort_flag != 0 && rank == 0) {
+        for (int x = 0; x < kRing; ++x) {
+          const int k_fills = issued_k / kRing + (x < issued_k % kRing ? 1 : 0), v_fills = issued_v / kRing + (x < issued_v % kRing ? 1 : 0);
+          if (k_fills > 0) MbarWait(&bars->k_full[x], static_cast<std::uint32_t>(k_fills - 1) & 1U, 20000000ULL);
+          if (v_fills > 0) MbarWait(&bars->v_full[x], static_cast<std::uint32_t>(v_fills - 1) & 1U, 20000000ULL);
         }
       }
-      ++issued;
-      if (++s == kRing) s = 0, ph ^= 1U;
-    }
-    // After a wait that gave up, the copies still in flight get one more bounded wait each (the last fill of a stage
-    // says which phase is outstanding), so that none lands in shared memory after the CTA has left it. fp16 pages: the
-    // bytes of both CTAs are counted on the leader's barriers, and both CTAs meet at the cluster barrier below.
-    if (*abort_flag != 0 && (S::kQuant || rank == 0)) {
-      for (int x = 0; x < kRing; ++x) {
-        const int fills = issued / kRing + (x < issued % kRing ? 1 : 0);
-        if (fills > 0) MbarWait(S::kQuant ? &bars->raw_full[x] : &bars->v_full[x], static_cast<std::uint32_t>(fills - 1) & 1U, 20000000ULL);
-        const int k_fills = issued_k / kRing + (x < issued_k % kRing ? 1 : 0);
-        if (!S::kQuant && k_fills > 0) MbarWait(&bars->k_full[x], static_cast<std::uint32_t>(k_fills - 1) & 1U, 20000000ULL);
+    } else {
+      // Quantized pages are loaded by the dequantizing warps, one tile of theirs ahead; this warp brings the pages after
+      // that into L2: the pair's two CTAs a half each, kAhead tiles before they are converted. It follows the counter of
+      // converted tiles and no mbarrier: nothing waits for this warp, so a barrier could be two phases ahead of it.
+      constexpr int kAhead = 6;
+      const bool elected = ElectOne();
+      volatile int* converted = bars->converted;
+      for (int j = 2; j < n_tiles; ++j) {
+        bool ok = true;
+        if (const int done = j - kAhead; done >= 0) {
+          const std::uint64_t t0 = GlobalTimerNs();
+          while (max(converted[0], converted[1]) <= done && ok) ok = *abort_flag == 0 && GlobalTimerNs() - t0 < kWaitLimitNs;
+        }
+        if (!__all_sync(0xFFFFFFFFU, ok)) break;
+        const std::int32_t page = min(max(__ldg(table + j), 0), pool.num_pages - 1);
+        const std::size_t row = ((static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + tile.kvh) * kPageTokens + rank * (kTileN / 2);
+        if (elected) {
+          PrefetchL2(pool.kcodes + row * CodeBytes(kFmt), (kTileN / 2) * CodeBytes(kFmt));
+          PrefetchL2(pool.vcodes + row * CodeBytes(kFmt), (kTileN / 2) * CodeBytes(kFmt));
+          PrefetchL2(pool.kscales + row * kBlocksPerRow, (kTileN / 2) * kBlocksPerRow * 2);
+          PrefetchL2(pool.vscales + row * kBlocksPerRow, (kTileN / 2) * kBlocksPerRow * 2);
+        }
       }
     }
   } else if (warp == kWarpMma) {
@@ -330,69 +335,83 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
       if (ok && elected) UmmaCommitPair(&bars->o_done);
     }
   } else if (S::kQuant && warp >= kWarpDequant) {
-    // ------------------------------ dequantizing warps: raw stage -> fp16 half tiles ------------------------------
+    // ------------------------------ dequantizing warps: pages -> fp16 half tiles ------------------------------
+    // A chunk = 8 dims of a row = 16 B of fp16; lanes run along the row. A group holds the codes of its next tile in
+    // registers: they are loaded (past L1) as soon as the tile before has been converted, two tile periods ahead. Staging
+    // them in shared memory by TMA first cost 32 KB more of shared-memory traffic per tile and CTA: 60 us against 58 for 16
+    // rows x 65536 of q8_0, 85 against 82 for 96 rows x 32768.
     if constexpr (S::kQuant) {
       const int group = (warp - kWarpDequant) / kDequantWarps;
       const int t = threadIdx.x - 32 * (kWarpDequant + group * kDequantWarps);   // 0 .. 127
+      const int k8 = t & 31, k_key0 = t >> 5;                                    // K: 32 keys x 32 chunks, key = k_key0 + 4 i
+      const int vl = t & 15, v8 = static_cast<int>(rank) * 16 + vl, v_key0 = t >> 4;   // V: 64 keys x 16 chunks, key = v_key0 + 8 i
+      uint2 kw[8], vw[8];
+      std::uint16_t ksc[8], vsc[8];
+      // offset of a chunk's codes in its row: q8_0 8 bytes per chunk; q4_0 elements 8 (c & 1) .. of the low or high
+      // nibbles of block c / 4's 16 bytes
+      auto code_at = [](int c) { return kFmt == kFmtQ8 ? c * 8 : (c >> 2) * 16 + (c & 1) * 8; };
+      auto row_of = [&](std::int32_t page) -> std::size_t {
+        page = min(max(page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
+        return ((static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + tile.kvh) * kPageTokens;
+      };
+      auto fetch_k = [&](std::size_t row) {
+        const std::size_t k_row = row + rank * (kTileN / 2) + k_key0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          kw[i] = LoadStream8(pool.kcodes + (k_row + 4 * i) * CodeBytes(kFmt) + code_at(k8));
+          ksc[i] = __ldg(pool.kscales + (k_row + 4 * i) * kBlocksPerRow + (k8 >> 2));
+        }
+      };
+      auto fetch_v = [&](std::size_t row) {
+        const std::size_t v_row = row + v_key0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          vw[i] = LoadStream8(pool.vcodes + (v_row + 8 * i) * CodeBytes(kFmt) + code_at(v8));
+          vsc[i] = __ldg(pool.vscales + (v_row + 8 * i) * kBlocksPerRow + (v8 >> 2));
+        }
+      };
+      if (group < n_tiles) {
+        const std::size_t row = row_of(__ldg(table + group));
+        fetch_k(row);
+        fetch_v(row);
+      }
+      std::int32_t next_page = group + kDequantGroups < n_tiles ? __ldg(table + group + kDequantGroups) : 0;
       for (int j = group; j < n_tiles; j += kDequantGroups) {
-        const int rs = j % S::kRawStages, ks = j % S::kKStages, vs = j % S::kVStages;
-        bool ok = WaitOrAbort(&bars->raw_full[rs], static_cast<std::uint32_t>(j / S::kRawStages) & 1U, abort_flag);
-        if (ok && j >= S::kKStages)
+        const int ks = j % S::kKStages, vs = j % S::kVStages;
+        bool ok = true;
+        if (j >= S::kKStages)
           ok = WaitOrAbort<true>(&bars->k_empty[ks], static_cast<std::uint32_t>(j / S::kKStages - 1) & 1U, abort_flag);
         ok = __all_sync(0xFFFFFFFFU, ok);
         if (!ok) break;
-        const std::uint8_t* st = smem + S::kSmemRaw + rs * S::kRawBytes;
         std::uint8_t* kd = smem + S::kSmemK + ks * kKHalfBytes;
         std::uint8_t* vd = smem + S::kSmemV + vs * kVHalfBytes;
-        const std::uint16_t* ksc = reinterpret_cast<const std::uint16_t*>(st + S::kRawKs);
-        const std::uint16_t* vsc = reinterpret_cast<const std::uint16_t*>(st + S::kRawVs);
-        // A chunk = 8 dims of a row = 16 B of fp16; lanes run along the row. All loads of a side come before its stores:
-        // the compiler cannot tell that the raw stage and the tiles do not overlap, and took turns (2,500 clocks a tile).
-        uint2 w[8];
-        std::uint16_t sc[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {   // K: 32 keys x 32 chunks
-          const int c = t + i * (32 * kDequantWarps), key = c >> 5, c8 = c & 31;
-          if constexpr (kFmt == kFmtQ8)
-            w[i] = *reinterpret_cast<const uint2*>(st + S::kRawK + key * 256 + c8 * 8);
-          else   // block c8 / 4 is 16 bytes; elements 8 (c8 & 1) .. of its low or high nibbles
-            w[i] = *reinterpret_cast<const uint2*>(st + S::kRawK + key * 128 + (c8 >> 2) * 16 + (c8 & 1) * 8);
-          sc[i] = ksc[key * kBlocksPerRow + (c8 >> 2)];
-        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int c = t + i * (32 * kDequantWarps), key = c >> 5, c8 = c & 31;
-          *reinterpret_cast<uint4*>(kd + (c8 >> 3) * kKBlockBytes + key * 128 + (((c8 & 7) ^ (key & 7)) << 4)) =
-              DequantChunk<kFmt, false>(w[i], c8, sc[i]);
-        }
-        const int cl = t & 15, vc8 = static_cast<int>(rank) * 16 + cl;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {   // V: 64 keys x 16 chunks of this CTA's 128 dims; loaded before K's fence
-          const int c = t + i * (32 * kDequantWarps), key = c >> 4;
-          if constexpr (kFmt == kFmtQ8)   // the TMA box is swizzled: 16-byte piece p of row key sits at p ^ (key % 8)
-            w[i] = *reinterpret_cast<const uint2*>(st + S::kRawV + key * 128 + (((cl >> 1) ^ (key & 7)) << 4) + (cl & 1) * 8);
-          else
-            w[i] = *reinterpret_cast<const uint2*>(st + S::kRawV + key * 128 + (vc8 >> 2) * 16 + (vc8 & 1) * 8);
-          sc[i] = vsc[key * kBlocksPerRow + (vc8 >> 2)];
+          const int key = k_key0 + 4 * i;
+          *reinterpret_cast<uint4*>(kd + (k8 >> 3) * kKBlockBytes + key * 128 + (((k8 & 7) ^ (key & 7)) << 4)) =
+              DequantChunk<kFmt, false>(kw[i], k8, ksc[i]);
         }
         FenceProxyAsync();   // the tensor core reads the tiles through the async proxy
         __syncwarp();
         if (lane == 0) MbarArriveCluster(MapToCta(SmemAddr(&bars->k_full[ks]), 0));
+        if (t == 0) *const_cast<volatile int*>(&bars->converted[group]) = j + 1;
+        const bool more = j + kDequantGroups < n_tiles;
+        const std::size_t next_row = row_of(next_page);
+        if (more) fetch_k(next_row);
         if (j >= S::kVStages) ok = WaitOrAbort<true>(&bars->v_empty[vs], static_cast<std::uint32_t>(j / S::kVStages - 1) & 1U, abort_flag);
         ok = __all_sync(0xFFFFFFFFU, ok);
         if (!ok) break;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int c = t + i * (32 * kDequantWarps), key = c >> 4;
-          *reinterpret_cast<uint4*>(vd + (cl >> 3) * kVBlockBytes + key * 128 + (((cl & 7) ^ (key & 7)) << 4)) =
-              DequantChunk<kFmt, true>(w[i], vc8, sc[i]);
+          const int key = v_key0 + 8 * i;
+          *reinterpret_cast<uint4*>(vd + (vl >> 3) * kVBlockBytes + key * 128 + (((vl & 7) ^ (key & 7)) << 4)) =
+              DequantChunk<kFmt, true>(vw[i], v8, vsc[i]);
         }
         FenceProxyAsync();
         __syncwarp();
-        if (lane == 0) {
-          MbarArrive(&bars->raw_empty[rs]);
-          MbarArriveCluster(MapToCta(SmemAddr(&bars->v_full[vs]), 0));
-        }
+        if (lane == 0) MbarArriveCluster(MapToCta(SmemAddr(&bars->v_full[vs]), 0));
+        if (more) fetch_v(next_row);
+        if (j + 2 * kDequantGroups < n_tiles) next_page = __ldg(table + j + 2 * kDequantGroups);
       }
     }
   } else if (warp < kWarpTma) {
