@@ -233,9 +233,10 @@ int yahkv_attend_prefill_qraw(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, con
 int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, void* stream);
 
 /* yahkv_attend_decode with every shared prefix computed once for all the rows that share it: same arguments, same result up
- * to rounding. Rows whose block tables start with the same pages form a group (found here, any order, several groups
- * and rows without one in a call); its prefix is what all of its rows have in common and filled. The prefix runs on the
- * tensor cores for the whole group: K and V enter as fp16 (quantized values rounded once, as in
+ * to rounding. Rows whose block tables start with the same pages are grouped (found here; any order, several groups,
+ * forks of forks and rows that share nothing in one call) so that the most page reads are saved; a prefix that saves
+ * fewer than 64 page reads is left to its rows. The prefix runs on the tensor
+ * cores for the whole group: K and V enter as fp16 (quantized values rounded once, as in
  * yahkv_attend_prefill) and the softmax weights too, so a result is about 1e-3 of the largest output's size from
  * yahkv_attend_decode's at worst and about 4e-4 of an output's size on average. n_splits: split-K units of what lies
  * behind the prefix, 0 = automatic. q_dev 16-byte aligned. The first call allocates a workspace (about 40 MB; 24 KB
@@ -417,6 +418,9 @@ int yahkv_launch_count(const yahkv_ctx* ctx, int64_t* launches);
  * path this way. */
 int yahkv_debug_wait_timeout(yahkv_ctx* ctx, int64_t limit_us, void* stream);
 int yahkv_debug_set_prefill_sms(yahkv_ctx* ctx, int32_t n_sm);
+/* Sets how many page reads computing a shared prefix once must save for it to be done (default 64), so that a small test
+ * reaches that path. Takes effect with the next plan. */
+int yahkv_debug_set_shared_min(yahkv_ctx* ctx, int32_t pages);
 
 /* Per-kernel device time for benchmarks: while enabled, every launch is bracketed by a CUDA event pair on its own
  * stream (the reference's counterpart is its per-dispatch timer, engine/run/hal_run.cc:124-135). Enabling or

@@ -43,12 +43,13 @@ static std::int32_t Grow(KvHost& host, std::int32_t s, std::int64_t len) {
 }
 
 // groups: (prefix tokens, rows); every row of a group is a fork at the prefix with a suffix of its own
-static void CheckShared(const std::vector<std::pair<int, int>>& groups, int singles, int n_splits, int n_pairs, unsigned seed) {
+static void CheckShared(const std::vector<std::pair<int, int>>& groups, int singles, int n_splits, int n_pairs, unsigned seed, int min_saved = 1) {
   std::mt19937 rng(seed);
   int n_rows = singles;
   for (auto& g : groups) n_rows += g.second;
   const int cap = n_rows + static_cast<int>(groups.size());
   KvHost host(Config(cap, 2048, cap * 2048));
+  host.SetSharedMinSaved(min_saved);
   std::vector<std::int32_t> ids;
   std::vector<int> group_of;
   for (std::size_t gi = 0; gi < groups.size(); ++gi) {
@@ -106,7 +107,8 @@ static void CheckShared(const std::vector<std::pair<int, int>>& groups, int sing
     const std::int64_t len = host.len(s, 0);
     const int pages = static_cast<int>((len + kPageTokens - 1) / kPageTokens);
     const int g = group_of[static_cast<std::size_t>(b)];
-    const int shared = g >= 0 && groups[static_cast<std::size_t>(g)].second >= 2 ? groups[static_cast<std::size_t>(g)].first / kPageTokens : 0;
+    int shared = g >= 0 ? groups[static_cast<std::size_t>(g)].first / kPageTokens : 0;
+    if (g >= 0 && (groups[static_cast<std::size_t>(g)].second - 1) * shared < min_saved) shared = 0;
     EXPECT(p.first_page[static_cast<std::size_t>(b)] == shared);
     EXPECT(static_cast<std::int64_t>(shared) * kPageTokens <= len);
     for (int h = 0; h < kKvHeads; ++h) {
@@ -139,6 +141,66 @@ static void CheckShared(const std::vector<std::pair<int, int>>& groups, int sing
   EXPECT(host.PlanDecodeShared(0, n, ids.data(), n_splits, 64, cap * kKvHeads * 64, n_pairs, max_rows, &changed).code == YAHKV_OK && !changed);
   EXPECT(host.SeqReserve(ids[0], host.len(ids[0], 0) + 200).code == YAHKV_OK);   // a changed table is a changed plan
   EXPECT(host.PlanDecodeShared(0, n, ids.data(), n_splits, 64, cap * kKvHeads * 64, n_pairs, max_rows, &changed).code == YAHKV_OK && changed);
+}
+
+// Forks of forks: the grouping that saves the most page reads.
+static void CheckNested() {
+  KvHost host(Config(40, 512, 4096));
+  host.SetSharedMinSaved(1);
+  std::int32_t src, dst;
+  auto fork = [&](std::int32_t from, std::int64_t n, std::int64_t len) {
+    std::int32_t s = -1;
+    EXPECT(host.SeqFork(from, n, &s, &src, &dst).code == YAHKV_OK);
+    return Grow(host, s, len);
+  };
+  const std::int32_t root = Grow(host, -1, 100 * 64);
+  std::vector<std::int32_t> ids;
+  for (int i = 0; i < 8; ++i) ids.push_back(fork(root, 100 * 64, 100 * 64 + 10));
+  ids.push_back(fork(root, 64, 70));   // a short row: one page in common with all
+  auto pages = [&] {
+    std::vector<std::int64_t> lens;
+    for (int s : ids) lens.push_back(host.len(s, 0));
+    std::vector<int> first(ids.size(), 0);
+    std::set<std::int32_t> seen;
+    for (const auto& g : host.FindPrefixes(static_cast<int>(ids.size()), ids.data(), lens.data()))
+      for (std::int32_t b : g.rows) {
+        EXPECT(seen.insert(b).second);
+        first[static_cast<std::size_t>(b)] = g.pages;
+      }
+    return first;
+  };
+  auto first = pages();
+  for (int i = 0; i < 8; ++i) EXPECT(first[static_cast<std::size_t>(i)] == 100);
+  EXPECT(first[8] == 0);
+  // two conversations behind one system prompt: 20 pages for all six rows save 100, 20 + 100 pages for 3 + 3 save 2 x 2 x 120
+  ids.clear();
+  const std::int32_t sys = Grow(host, -1, 20 * 64);
+  for (int c = 0; c < 2; ++c) {
+    const std::int32_t conv = fork(sys, 20 * 64, 120 * 64);
+    for (int i = 0; i < 3; ++i) ids.push_back(fork(conv, 120 * 64, 120 * 64 + 1 + i));
+  }
+  for (int p : pages()) EXPECT(p == 120);
+  // the same with conversations of two pages each: the system prompt saves more
+  ids.clear();
+  for (int c = 0; c < 2; ++c) {
+    const std::int32_t conv = fork(sys, 20 * 64, 22 * 64);
+    for (int i = 0; i < 3; ++i) ids.push_back(fork(conv, 22 * 64, 22 * 64 + 1 + i));
+  }
+  for (int p : pages()) EXPECT(p == 20);
+  // a chain of forks, each one page further
+  ids.clear();
+  std::int32_t last = Grow(host, -1, 64);
+  for (int i = 0; i < 12; ++i) ids.push_back(last = fork(last, (i + 1) * 64, (i + 2) * 64));
+  std::int64_t saved = 0;
+  std::map<int, int> sizes;
+  for (int p : pages()) ++sizes[p];
+  for (auto& e : sizes)
+    if (e.first > 0) saved += static_cast<std::int64_t>(e.first) * (e.second - 1);
+  // row k holds k + 2 pages and shares them with every later row: rows k .. 11 save (11 - k)(k + 2), 42 at most (k = 4, 5)
+  EXPECT(sizes.size() <= 2 && saved == 42);
+  // below the threshold nothing is grouped
+  host.SetSharedMinSaved(43);
+  for (int p : pages()) EXPECT(p == 0);
 }
 
 static void CheckEvict() {
@@ -199,6 +261,8 @@ int main() {
     for (unsigned g = 0; g < rng() % 40; ++g) groups.push_back({1 + static_cast<int>(rng() % 3000), 1 + static_cast<int>(rng() % 5)});
     CheckShared(groups, static_cast<int>(rng() % 5) + 1, static_cast<int>(rng() % 9), s % 2 ? 74 : 3, s);
   }
+  CheckShared({{640, 8}, {128, 2}, {64 * 64, 2}, {64 * 64 - 1, 2}}, 2, 0, 74, 77, 64);
+  CheckNested();
   CheckEvict();
   std::printf("shared_planner_test: ok\n");
   return 0;

@@ -10,7 +10,7 @@ import yahkv
 from gpu_util import dev
 from longctx_util import attend64, rows64, select
 from test_rope_rows_gpu import freqs, rotate64
-from test_shared_gpu import FMTS, check, grow, normal, shared
+from test_shared_gpu import FMTS, check, grow, normal, shared, small_cache
 
 pytestmark = pytest.mark.gpu
 EPS = 1e-6
@@ -18,7 +18,7 @@ EPS = 1e-6
 
 def forked_batch(fmt, rng, layers=2, extra=8, prefix=200, max_seqs=8):
     """Two groups of forks and a lone row: (cache, sequences)."""
-    cache = yahkv.KvCache(n_layers=layers, num_pages=80, fmt=fmt, max_seqs=max_seqs, max_pages_per_seq=30)
+    cache = small_cache(n_layers=layers, num_pages=80, fmt=fmt, max_seqs=max_seqs, max_pages_per_seq=30)
     seqs = []
     for n, rows in ((prefix, 3), (700, 2)):
         root = cache.seq_create()
@@ -179,7 +179,7 @@ def test_a_prompt_forked_decoded_cut_and_continued(fmt):
     watched; that branch is cut, its slots stop being positions, and it goes on at its true positions."""
     rng = np.random.default_rng(83)
     prompt, steps, keep = 450, 6, 150
-    cache = yahkv.KvCache(num_pages=60, fmt=fmt, max_seqs=5, max_pages_per_seq=12)
+    cache = small_cache(num_pages=60, fmt=fmt, max_seqs=5, max_pages_per_seq=12)
     rope = yahkv.Rope(cache, layout="interleaved", rotary_dim=128, theta=1e6, scaling="yarn", factor=8.0, original_len=4096.0,
                       max_positions=40000)
     f, m = freqs(128, 1e6, "yarn", 8.0, 4096.0, 32.0, 1.0, 0.0)

@@ -24,6 +24,13 @@ def normal(rng, *shape):
     return rng.standard_normal(shape, dtype=np.float32).astype(np.float16)
 
 
+def small_cache(**kw):
+    """A cache that computes every shared prefix once, however little it saves, so that small tests reach that path."""
+    cache = yahkv.KvCache(**kw)
+    cache.debug_set_shared_min(1)
+    return cache
+
+
 def extend(cache, layer, seq, k, v):
     n0 = cache.seq_len(seq, layer)
     cache.seq_reserve(seq, n0 + len(k))
@@ -63,7 +70,7 @@ def check(cache, layer, seqs, q, got, gate=None, heads=slice(0, 24)):
                                                 (43, 129, 100), (64, 1000, 5), (4, 5000, 200)])
 def test_one_group(fmt, rows, prefix, suffix):
     rng = np.random.default_rng(rows * 1000 + prefix)
-    cache = yahkv.KvCache(num_pages=(prefix + 63) // 64 + rows * ((suffix + 127) // 64 + 1), fmt=fmt, max_seqs=rows + 1,
+    cache = small_cache(num_pages=(prefix + 63) // 64 + rows * ((suffix + 127) // 64 + 1), fmt=fmt, max_seqs=rows + 1,
                           max_pages_per_seq=(prefix + suffix + 127) // 64)
     root = cache.seq_create()
     grow(cache, rng, root, prefix)
@@ -77,7 +84,7 @@ def test_one_group(fmt, rows, prefix, suffix):
 @pytest.mark.parametrize("fmt", FMTS)
 def test_groups_single_rows_and_repeats_in_any_order(fmt):
     rng = np.random.default_rng(7)
-    cache = yahkv.KvCache(n_layers=2, num_pages=150, fmt=fmt, max_seqs=24, max_pages_per_seq=40)
+    cache = small_cache(n_layers=2, num_pages=150, fmt=fmt, max_seqs=24, max_pages_per_seq=40)
     seqs = []
     for prefix, rows in ((300, 5), (64, 2), (1500, 3)):
         root = cache.seq_create()
@@ -108,7 +115,7 @@ def test_groups_single_rows_and_repeats_in_any_order(fmt):
 def test_steps_interleaved_with_plain_decode(fmt):
     """The two calls keep plans of their own; tables and lengths change between the steps."""
     rng = np.random.default_rng(11)
-    cache = yahkv.KvCache(num_pages=60, fmt=fmt, max_seqs=5, max_pages_per_seq=20)
+    cache = small_cache(num_pages=60, fmt=fmt, max_seqs=5, max_pages_per_seq=20)
     root = cache.seq_create()
     grow(cache, rng, root, 250)
     seqs = [cache.seq_fork(root, 250) for _ in range(4)]
@@ -133,7 +140,7 @@ def test_steps_interleaved_with_plain_decode(fmt):
 @pytest.mark.parametrize("fmt", FMTS)
 def test_a_fork_and_its_origin_grow_apart(fmt):
     rng = np.random.default_rng(5)
-    cache = yahkv.KvCache(n_layers=3, num_pages=12, fmt=fmt, max_seqs=3, max_pages_per_seq=6)
+    cache = small_cache(n_layers=3, num_pages=12, fmt=fmt, max_seqs=3, max_pages_per_seq=6)
     a = cache.seq_create()
     grow(cache, rng, a, 100, (0, 1, 2))
     before = [rows64(cache, l, a, 100) for l in range(3)]
@@ -150,10 +157,36 @@ def test_a_fork_and_its_origin_grow_apart(fmt):
     check(cache, 1, [b], q, shared(cache, 1, [b], q))
 
 
+def test_long_groups_short_rows_and_forks_of_forks_at_the_default_threshold():
+    """Groups that save too little, a short row among long ones, two conversations behind one prompt."""
+    rng = np.random.default_rng(17)
+    cache = yahkv.KvCache(num_pages=160, fmt=yahkv.FMT_Q8_0, max_seqs=24, max_pages_per_seq=40)
+    root = cache.seq_create()
+    grow(cache, rng, root, 1100)
+    seqs = [cache.seq_fork(root, 1100) for _ in range(6)] + [cache.seq_fork(root, 100)]       # 17 pages x 5, one row of 1
+    for _ in range(2):
+        conv = cache.seq_fork(root, 640)
+        grow(cache, rng, conv, 900)
+        seqs += [cache.seq_fork(conv, 1540) for _ in range(4)]                                  # 24 pages x 3 behind 10
+    lone = cache.seq_create()
+    grow(cache, rng, lone, 64)
+    seqs += [lone, cache.seq_fork(lone, 64)]                                                    # saves one page
+    for i, s in enumerate(seqs):
+        grow(cache, rng, s, 1 + 7 * i)
+    seqs = [seqs[i] for i in rng.permutation(len(seqs))]
+    q = normal(rng, len(seqs), 24, 256)
+    before = cache.launch_count()
+    got = shared(cache, 0, seqs, q)
+    assert cache.launch_count() - before >= 3      # a prefix pass ran
+    check(cache, 0, seqs, q, got)
+    few = [seqs.index(s) for s in seqs[:2]]
+    check(cache, 0, [seqs[i] for i in few], q[few], shared(cache, 0, [seqs[i] for i in few], q[few]))
+
+
 def test_a_head_sharded_context_writes_its_own_heads_only():
     rng = np.random.default_rng(3)
     for fmt in (yahkv.FMT_F16, yahkv.FMT_Q8_0):
-        cache = yahkv.KvCache(num_pages=30, fmt=fmt, max_seqs=4, max_pages_per_seq=10, kv_head_begin=1, kv_head_count=2)
+        cache = small_cache(num_pages=30, fmt=fmt, max_seqs=4, max_pages_per_seq=10, kv_head_begin=1, kv_head_count=2)
         root = cache.seq_create()
         grow(cache, rng, root, 320)
         seqs = [cache.seq_fork(root, 320) for _ in range(3)]
@@ -167,7 +200,7 @@ def test_a_head_sharded_context_writes_its_own_heads_only():
 
 def test_refusals():
     rng = np.random.default_rng(1)
-    cache = yahkv.KvCache(num_pages=8, max_seqs=3, max_pages_per_seq=4)
+    cache = small_cache(num_pages=8, max_seqs=3, max_pages_per_seq=4)
     a = cache.seq_create()
     grow(cache, rng, a, 128)
     b = cache.seq_fork(a, 128)
@@ -200,6 +233,7 @@ def test_refusals():
     cache.seq_free(a)
     cache.append(0, [b], [100], x, x)               # its own page now
     cache.sync()
-    tile = yahkv.KvCache(num_pages=2, fmt=yahkv.FMT_KV8A16, max_seqs=1, max_pages_per_seq=2)
+    assert code(cache.debug_set_shared_min, 0) == yahkv.ERR_INVALID
+    tile = small_cache(num_pages=2, fmt=yahkv.FMT_KV8A16, max_seqs=1, max_pages_per_seq=2)
     s = tile.seq_create()
     assert code(tile.attend_decode_shared, 0, [s], q, out) == yahkv.ERR_INVALID

@@ -190,7 +190,7 @@ struct PrefixItem {
   std::int32_t pad;
 };
 static_assert(sizeof(PrefixItem) == 16, "uploaded as an array");
-constexpr int kSharedMinPages = 1;         // shortest prefix read once for a group
+constexpr int kSharedMinSaved = 64;        // page reads that computing a prefix once must save (KvHost::FindPrefixes)
 
 // Partial workspace per unit: acc [6][256] f32 (unnormalised), then ml [6][2] f32 (max in log2 units, sum).
 constexpr int kPartialAccFloats = kGroup * kHeadDim;

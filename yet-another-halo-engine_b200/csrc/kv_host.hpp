@@ -176,9 +176,6 @@ class KvHost {
     return {};
   }
 
-  // A new sequence whose first n_tokens / 64 pages are seq's own (counted references, never written while shared) and
-  // whose length is n_tokens in every layer. A prefix that ends inside a page takes a page of its own for the rest:
-  // *copy_src / *copy_dst then name the page to copy (-1: nothing to copy). Nothing changes on error.
   HostError CheckFork(int seq, std::int64_t n_tokens) const {
     if (!live(seq)) return {YAHKV_ERR_INVALID, "seq_fork: not a live sequence: " + std::to_string(seq)};
     if (n_tokens < 0) return {YAHKV_ERR_INVALID, "seq_fork: negative token count"};
@@ -188,6 +185,9 @@ class KvHost {
                                      " tokens in layer " + std::to_string(l) + ", " + std::to_string(n_tokens) + " asked for"};
     return {};
   }
+  // A new sequence whose first n_tokens / 64 pages are seq's own (counted references, never written while shared) and
+  // whose length is n_tokens in every layer. A prefix that ends inside a page takes a page of its own for the rest:
+  // *copy_src / *copy_dst then name the page to copy (-1: nothing to copy). Nothing changes on error.
   HostError SeqFork(int seq, std::int64_t n_tokens, std::int32_t* out, std::int32_t* copy_src, std::int32_t* copy_dst) {
     if (HostError bad = CheckFork(seq, n_tokens); bad.code != YAHKV_OK) return bad;
     const int whole = static_cast<int>(n_tokens / kPageTokens);
@@ -486,36 +486,70 @@ class KvHost {
     int pages = 0;                    // the prefix they share
     int n_mt = 0;                     // CTA pairs of 256 (row, query head) pairs
   };
-  // Rows whose tables start with the same page, and the longest run of pages common to all of them that each has filled.
+  // Which rows compute a prefix together. The rows' full pages form a tree (forks of forks branch where their tables
+  // differ); a group is all the rows below one node, with the pages down to it, and saves (rows - 1) x pages page reads.
+  // From the root down, a node's rows are one group where that saves more than the best groups below it do, so that a
+  // short row does not cut the prefix of the long ones. Savings below shared_min_saved_ pages are left to the ordinary
+  // units: the pass costs two launches' time and its pairs work on half-empty tiles (measured, us per call with / without
+  // the pass: 2 rows x 4096 tokens fp16 12.6 / 11.1, q8_0 13.8 / 13.9; 4 x 4096 13.5 / 18.8 and 14.5 / 15.5; 8 x 256 9.4 /
+  // 11.8 and 10.0 / 10.5; 32 x 256 13.0 / 27.4 and 14.4 / 21.9; 32 x 16384 28 / 196 and 33 / 158).
   std::vector<PrefixGroup> FindPrefixes(int n_seqs, const std::int32_t* seq_ids, const std::int64_t* lens) const {
     std::vector<PrefixGroup> groups;
-    std::vector<std::pair<std::int32_t, std::int32_t>> by_page;   // (first page, row), rows in order
+    std::vector<std::int32_t> rows;
     for (int b = 0; b < n_seqs; ++b)
-      if (lens[b] >= kPageTokens) by_page.emplace_back(table_row(seq_ids[b])[0], b);
-    std::stable_sort(by_page.begin(), by_page.end(), [](const auto& x, const auto& y) { return x.first < y.first; });
-    for (std::size_t i = 0; i < by_page.size();) {
+      if (lens[b] >= kPageTokens) rows.push_back(b);
+    // rows with a common first page, in the order of their first row
+    std::stable_sort(rows.begin(), rows.end(), [&](std::int32_t x, std::int32_t y) { return table_row(seq_ids[x])[0] < table_row(seq_ids[y])[0]; });
+    for (std::size_t i = 0; i < rows.size();) {
       std::size_t j = i;
-      while (j < by_page.size() && by_page[j].first == by_page[i].first) ++j;
-      if (j - i >= 2) {
-        PrefixGroup g;
-        const std::int32_t* base = table_row(seq_ids[by_page[i].second]);
-        std::int64_t pages = lens[by_page[i].second] / kPageTokens;
-        for (std::size_t k = i; k < j; ++k) {
-          const int b = by_page[k].second;
-          const std::int32_t* row = table_row(seq_ids[b]);
-          pages = std::min(pages, lens[b] / kPageTokens);
-          std::int64_t same = 0;
-          while (same < pages && row[same] == base[same]) ++same;
-          pages = same;
-          g.rows.push_back(b);
-        }
-        g.pages = static_cast<int>(pages);
-        g.n_mt = (static_cast<int>(g.rows.size()) * kGroup + 2 * kPrefillTileRows - 1) / (2 * kPrefillTileRows);
-        if (g.pages >= kSharedMinPages) groups.push_back(std::move(g));
-      }
+      while (j < rows.size() && table_row(seq_ids[rows[j]])[0] == table_row(seq_ids[rows[i]])[0]) ++j;
+      std::vector<PrefixGroup> found;
+      BestPrefixes(std::vector<std::int32_t>(rows.begin() + static_cast<std::ptrdiff_t>(i), rows.begin() + static_cast<std::ptrdiff_t>(j)), 0, seq_ids, lens, &found);
+      for (PrefixGroup& g : found) groups.push_back(std::move(g));
       i = j;
     }
+    for (PrefixGroup& g : groups)
+      g.n_mt = (static_cast<int>(g.rows.size()) * kGroup + 2 * kPrefillTileRows - 1) / (2 * kPrefillTileRows);
     return groups;
+  }
+  // The best groups among rows that agree in their first `from` pages; returns the pages they save.
+  std::int64_t BestPrefixes(const std::vector<std::int32_t>& rows, int from, const std::int32_t* seq_ids, const std::int64_t* lens,
+                            std::vector<PrefixGroup>* out) const {
+    if (rows.size() < 2) return 0;
+    int common = static_cast<int>(lens[rows[0]] / kPageTokens);
+    for (std::size_t i = 1; i < rows.size(); ++i) {
+      const std::int32_t *x = table_row(seq_ids[rows[0]]), *y = table_row(seq_ids[rows[i]]);
+      common = std::min(common, static_cast<int>(lens[rows[i]] / kPageTokens));
+      int same = std::min(from, common);
+      while (same < common && x[same] == y[same]) ++same;
+      common = same;
+    }
+    const std::int64_t whole = static_cast<std::int64_t>(rows.size() - 1) * common;
+    // what the branches behind the common pages save by themselves; rows that end there are in none of them
+    std::vector<std::pair<std::int32_t, std::vector<std::int32_t>>> branches;
+    for (std::int32_t b : rows) {
+      if (lens[b] / kPageTokens <= common) continue;
+      const std::int32_t next = table_row(seq_ids[b])[common];
+      auto it = std::find_if(branches.begin(), branches.end(), [&](const auto& e) { return e.first == next; });
+      if (it == branches.end()) it = branches.insert(branches.end(), {next, {}});
+      it->second.push_back(b);
+    }
+    std::vector<PrefixGroup> below;
+    std::int64_t saved = 0;
+    for (const auto& e : branches)
+      if (e.second.size() < rows.size()) saved += BestPrefixes(e.second, common, seq_ids, lens, &below);
+    if (whole >= saved && whole >= shared_min_saved_) {
+      PrefixGroup g;
+      g.rows = rows, g.pages = common;
+      out->push_back(std::move(g));
+      return whole;
+    }
+    for (PrefixGroup& g : below) out->push_back(std::move(g));
+    return saved;
+  }
+  void SetSharedMinSaved(int pages) {
+    shared_min_saved_ = pages;
+    InvalidateSharedPlan();
   }
 
   // How a shared plan is cut: pages per prefix part and pages per suffix unit.
@@ -894,6 +928,7 @@ class KvHost {
   std::int64_t unit_pages_ = 0;
   std::vector<CombineItem> items_;
   SharedPlan shared_;           // cached plan of attend_decode_shared
+  int shared_min_saved_ = kSharedMinSaved;
   std::vector<int> open_cur_;   // kv8a16: current open-tile buffer per (sequence, layer)
   std::vector<int> bounds_;     // PlanDecode: page boundaries of one sequence's units
 };

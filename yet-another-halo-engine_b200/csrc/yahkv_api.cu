@@ -2035,6 +2035,13 @@ int yahkv_debug_set_prefill_sms(yahkv_ctx* ctx, int32_t n_sm) {
   return YAHKV_OK;
 }
 
+int yahkv_debug_set_shared_min(yahkv_ctx* ctx, int32_t pages) {
+  if (int r = RequireDevice(ctx, "debug_set_shared_min"); r != YAHKV_OK) return r;
+  if (pages < 1) return Fail(ctx, YAHKV_ERR_INVALID, "debug_set_shared_min: at least one page");
+  ctx->host.SetSharedMinSaved(pages);
+  return YAHKV_OK;
+}
+
 int yahkv_device_bytes(const yahkv_ctx* ctx, int64_t* bytes) {
   if (ctx == nullptr || bytes == nullptr) return YAHKV_ERR_INVALID;
   *bytes = ctx->device_bytes;

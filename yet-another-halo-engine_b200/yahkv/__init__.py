@@ -198,6 +198,7 @@ SIGNATURES = {
     "yahkv_noalloc_status": (_I32, [_PI32, _VP]),
     "yahkv_debug_wait_timeout": (_I32, [_VP, _I64, _VP]),
     "yahkv_debug_set_prefill_sms": (_I32, [_VP, _I32]),
+    "yahkv_debug_set_shared_min": (_I32, [_VP, _I32]),
     "yahkv_kernel_timing": (_I32, [_VP, _I32]),
     "yahkv_kernel_timing_read": (_I32, [_VP, _I32, _c.POINTER(_c.c_double), _PI64]),
 }
@@ -609,6 +610,10 @@ class KvCache:
 
     def debug_set_prefill_sms(self, n_sm):
         self._check(lib.yahkv_debug_set_prefill_sms(self._h, int(n_sm)))
+
+    def debug_set_shared_min(self, pages):
+        """Page reads that computing a shared prefix once must save (default 64)."""
+        self._check(lib.yahkv_debug_set_shared_min(self._h, int(pages)))
 
     def launch_count(self):
         n = ctypes.c_int64()
