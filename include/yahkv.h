@@ -229,7 +229,7 @@ int yahkv_attend_prefill_qraw(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, con
  * sequence may be freed or appended to afterwards; a page stays allocated while any sequence names it. A shared page is
  * never written: yahkv_append and the decode steps refuse, with YAHKV_ERR_INVALID, a position in a page that another
  * sequence holds too (a sequence rolled back below its fork with yahkv_seq_set_len). yahkv_append_slots and
- * yahkv_write_page write where they are told to. */
+ * yahkv_write_page write where they are told to. A fork that copies cannot be captured (YAHKV_ERR_ORDER). */
 int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, void* stream);
 
 /* yahkv_attend_decode with every shared prefix computed once for all the rows that share it: same arguments, same result up
@@ -240,7 +240,8 @@ int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, 
  * yahkv_attend_prefill) and the softmax weights too, so a result is about 1e-3 of the largest output's size from
  * yahkv_attend_decode's at worst and about 4e-4 of an output's size on average. n_splits: split-K units of what lies
  * behind the prefix, 0 = automatic. q_dev 16-byte aligned. The first call allocates a workspace (about 40 MB; 24 KB
- * per sequence of max_seqs where that is more). */
+ * per sequence of max_seqs where that is more). Its lists come from the host, so it refuses a stream under capture
+ * (YAHKV_ERR_ORDER): yahkv_batch_set_shared is the form for a graph. */
 int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
                                const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, void* stream);
 
@@ -253,7 +254,7 @@ int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, co
  * yahkv_attend_decode's to the bit; for the quantized formats the query enters in 20-bit steps of its largest element
  * where yahkv_attend_decode takes 16, so the two agree within that rounding (1e-4 of the largest output). q_dev 16-byte aligned. The scores
  * pass through a workspace (96 B per cached key of the call) that grows to the largest call seen: growing waits for
- * the device. */
+ * the device. Refuses a stream under capture (YAHKV_ERR_ORDER). */
 int yahkv_attend_decode_weights(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
                                 const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, float* weights_dev,
                                 int64_t weights_stride, void* stream);
@@ -271,7 +272,7 @@ int yahkv_attend_decode_weights(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, c
  * its position: the next yahkv_append continues at position n_keep with a K row that the caller rotated at the true
  * position (yahkv_rope_rows); yahkv_rope_append and the raw-projection calls refuse the sequence and its forks with
  * YAHKV_ERR_ORDER until yahkv_seq_set_len(seq, -1, 0). A sequence in a prepared yahkv_batch must not be evicted: create
- * the batch again. */
+ * the batch again. Cannot be captured (YAHKV_ERR_ORDER). */
 int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t n_keep, int64_t n_sink, int64_t n_recent,
                 float* weights_dev, int64_t weights_stride, int64_t weights_layer_stride, int32_t* kept_dev, void* stream);
 
@@ -301,7 +302,7 @@ typedef struct yahkv_rope_config {
   double beta_fast;      /* YARN only */
   double beta_slow;      /* YARN only */
   double magnitude;      /* 0 = the scaling's own */
-  int64_t max_positions; /* positions 0 .. max_positions - 1, at most 2^31 */
+  int64_t max_positions; /* positions 0 .. max_positions - 1, at most 2^26 */
 } yahkv_rope_config;
 typedef struct yahkv_rope yahkv_rope;
 /* Builds the angle tables (8 B x rotary_dim / 2 x (1024 + max_positions / 1024)). Destroy it before the context, with its
@@ -373,7 +374,8 @@ void yahkv_batch_destroy(yahkv_batch* batch);
 int yahkv_batch_set_splits(yahkv_batch* batch, int32_t n_splits);
 /* on != 0: from the next batch_prepare on, the steps compute every prefix that rows of the batch share (yahkv_seq_fork) once
  * for all of them, as yahkv_attend_decode_shared does; the groups are found at batch_prepare and hold for its horizon.
- * Allocates on first use, so call it before a capture. Refused for the tile formats. The number of prefix tiles is part
+ * Allocates on first use, so call it before a capture. The batches of a context share its workspaces: replay their graphs
+ * one after the other, not side by side. Refused for the tile formats. The number of prefix tiles is part
  * of the layout that *layout_changed reports. */
 int yahkv_batch_set_shared(yahkv_batch* batch, int32_t on);
 int yahkv_batch_prepare(yahkv_batch* batch, int32_t horizon_steps, int32_t* layout_changed, void* stream);

@@ -243,6 +243,17 @@ def test_refusals_and_positions_after_an_eviction(tmp_path):
     assert code(ev, [b], 50, w, kept) == yahkv.ERR_ORDER                # unequal layers
     assert cache.seq_len(a, 0) == 200 and cache.seq_len(b, 0) == 100    # nothing happened
     ev([], 50, w, torch.empty(2, 0, 4, 50, device="cuda", dtype=torch.int32))
+    # host tables change or host lists are read: not inside a capture
+    graph, spare = torch.cuda.CUDAGraph(), torch.zeros(1, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        spare += 1
+        sp = torch.cuda.current_stream().cuda_stream
+        assert code(ev, [a], 50, w, kept, stream=sp) == yahkv.ERR_ORDER
+        assert code(cache.seq_fork, a, 70, stream=sp) == yahkv.ERR_ORDER
+        assert code(aw, 0, [a], q, out, w[0], stream=sp) == yahkv.ERR_ORDER
+        assert code(cache.attend_decode_shared, 0, [a], q, out, stream=sp) == yahkv.ERR_ORDER
+    assert cache.seq_len(a, 0) == 200 and cache.pages_free() == 10
     ev([a], 50, w, kept)
     # slots are not positions any more: the calls that would take them for positions refuse, for forks as well
     f32 = [dev(rng.standard_normal((1, n, 256)).astype(np.float32)) for n in (24, 4, 4)]

@@ -257,6 +257,9 @@ class KvHost {
   void CommitEvict(std::int64_t n_keep, const std::vector<EvictSeq>& seqs, const std::vector<std::int32_t>& dst_pages) {
     const int np = static_cast<int>((n_keep + kPageTokens - 1) / kPageTokens);
     std::vector<std::int32_t> dropped;
+    std::size_t held = 0;
+    for (const EvictSeq& e : seqs) held += static_cast<std::size_t>(n_pages(e.seq));
+    dropped.reserve(held);   // before anything changes
     for (const EvictSeq& e : seqs) {
       if (e.n_keys <= n_keep) continue;
       std::int32_t* row = mutable_row(e.seq);

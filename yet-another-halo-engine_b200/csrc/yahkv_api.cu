@@ -181,6 +181,20 @@ int FailCuda(const yahkv_ctx* ctx, const char* what, cudaError_t e) {
   return Fail(ctx, YAHKV_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+// The body of an entry point that builds lists on the host: an allocation that fails is an error code like any other.
+template <class F>
+int NoThrow(const yahkv_ctx* ctx, const char* what, F&& body) {
+  try {
+    return body();
+  } catch (...) {
+    try {
+      return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": out of host memory");
+    } catch (...) {
+      return YAHKV_ERR_INVALID;
+    }
+  }
+}
+
 #define YAHKV_CUDA(ctx, call)                                     \
   do {                                                            \
     const cudaError_t e_ = (call);                                \
@@ -369,6 +383,14 @@ int RequireDevice(yahkv_ctx* ctx, const char* what) {
   if (!ctx->has_device)
     return Fail(ctx, YAHKV_ERR_NO_DEVICE, std::string(what) + ": host-only context (no GPU, no CPU fallback)");
   if (cudaSetDevice(ctx->cfg.device) != cudaSuccess) return Fail(ctx, YAHKV_ERR_CUDA, "cudaSetDevice failed");
+  return YAHKV_OK;
+}
+
+// What changes host state, allocates or waits cannot be part of a captured graph: it would happen once, at the capture.
+int RefuseCapture(yahkv_ctx* ctx, const char* what, cudaStream_t stream) {
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  YAHKV_CUDA(ctx, cudaStreamIsCapturing(stream, &cs));
+  if (cs != cudaStreamCaptureStatusNone) return Fail(ctx, YAHKV_ERR_ORDER, std::string(what) + " while the stream is being captured");
   return YAHKV_OK;
 }
 
@@ -778,7 +800,7 @@ int yahkv_attend_decode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int
 }
 
 // The accumulators hold one row of `stride` floats per (sequence id, kv head).
-static int CheckWeights(yahkv_ctx* ctx, const char* what, int32_t n_seqs, const int32_t* seq_ids, const float* weights_dev,
+static int CheckWeights(yahkv_ctx* ctx, const char* what, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const float* weights_dev,
                         int64_t stride) {
   if (IsTileFmt(ctx->cfg.fmt))
     return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (a key has no row of its own)");
@@ -791,7 +813,7 @@ static int CheckWeights(yahkv_ctx* ctx, const char* what, int32_t n_seqs, const 
     if (seen[static_cast<std::size_t>(seq_ids[i])]++)
       return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": sequence " + std::to_string(seq_ids[i]) + " is listed twice");
     for (int l = 0; l < ctx->cfg.n_layers; ++l)
-      if (ctx->host.len(seq_ids[i], l) > stride)
+      if ((layer < 0 || l == layer) && ctx->host.len(seq_ids[i], l) > stride)
         return Fail(ctx, YAHKV_ERR_CAPACITY, std::string(what) + ": sequence " + std::to_string(seq_ids[i]) + " holds more keys than a row of the weights");
   }
   return YAHKV_OK;
@@ -800,11 +822,14 @@ static int CheckWeights(yahkv_ctx* ctx, const char* what, int32_t n_seqs, const 
 int yahkv_attend_decode_weights(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
                                 const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, float* weights_dev,
                                 int64_t weights_stride, void* stream) {
-  if (int r = RequireDevice(ctx, "attend_decode_weights"); r != YAHKV_OK) return r;
-  if (int r = CheckWeights(ctx, "attend_decode_weights", n_seqs, seq_ids, weights_dev, weights_stride); r != YAHKV_OK) return r;
-  if ((reinterpret_cast<std::uintptr_t>(q_dev) & 15) != 0) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_weights: q must be 16-byte aligned");
-  return AttendDecode(ctx, layer, n_seqs, seq_ids, q_dev, false, nullptr, 0.0F, gate_dev, out_dev, out_dtype, n_splits,
-                      weights_dev, weights_stride, stream);
+  return NoThrow(ctx, "attend_decode_weights", [&]() -> int {
+    if (int r = RequireDevice(ctx, "attend_decode_weights"); r != YAHKV_OK) return r;
+    if (int r = CheckWeights(ctx, "attend_decode_weights", std::max(layer, 0), n_seqs, seq_ids, weights_dev, weights_stride); r != YAHKV_OK) return r;
+    if ((reinterpret_cast<std::uintptr_t>(q_dev) & 15) != 0) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_weights: q must be 16-byte aligned");
+    if (int r = RefuseCapture(ctx, "attend_decode_weights: lists from the host", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
+    return AttendDecode(ctx, layer, n_seqs, seq_ids, q_dev, false, nullptr, 0.0F, gate_dev, out_dev, out_dtype, n_splits,
+                        weights_dev, weights_stride, stream);
+  });
 }
 
 int yahkv_attend_decode_qraw(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const float* q_raw_dev,
@@ -922,25 +947,29 @@ static int AttendDecode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int
 
 // ---- shared prefixes -------------------------------------------------------------------------------------------
 int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, void* stream) {
-  if (ctx == nullptr) return YAHKV_ERR_INVALID;
-  if (out == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "seq_fork: null out pointer");
-  if (IsTileFmt(ctx->cfg.fmt))
-    return Fail(ctx, YAHKV_ERR_INVALID, "seq_fork: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (the newest tile is no page)");
-  if (HostError bad = ctx->host.CheckFork(seq, n_tokens); bad.code != YAHKV_OK) return FailHost(ctx, std::move(bad));
-  if (n_tokens % kPageTokens != 0)
-    if (int r = RequireDevice(ctx, "seq_fork"); r != YAHKV_OK) return r;   // the last page is copied
-  std::int32_t src = -1, dst = -1, made = -1;
-  HostError e = ctx->host.SeqFork(seq, n_tokens, &made, &src, &dst);
-  if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
-  if (src >= 0) {
-    if (cudaError_t le = LaunchCopyPage(ctx->pool, src, dst, StreamOf(ctx, stream)); le != cudaSuccess) {
-      ctx->host.SeqFree(made);
-      return FailCuda(ctx, "seq_fork: page copy", le);
+  return NoThrow(ctx, "seq_fork", [&]() -> int {
+    if (ctx == nullptr) return YAHKV_ERR_INVALID;
+    if (out == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "seq_fork: null out pointer");
+    if (IsTileFmt(ctx->cfg.fmt))
+      return Fail(ctx, YAHKV_ERR_INVALID, "seq_fork: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (the newest tile is no page)");
+    if (HostError bad = ctx->host.CheckFork(seq, n_tokens); bad.code != YAHKV_OK) return FailHost(ctx, std::move(bad));
+    if (n_tokens % kPageTokens != 0)
+      if (int r = RequireDevice(ctx, "seq_fork"); r != YAHKV_OK) return r;   // the last page is copied
+    if (n_tokens % kPageTokens != 0)
+      if (int r = RefuseCapture(ctx, "seq_fork: the copy of a page", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
+    std::int32_t src = -1, dst = -1, made = -1;
+    HostError e = ctx->host.SeqFork(seq, n_tokens, &made, &src, &dst);
+    if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
+    if (src >= 0) {
+      if (cudaError_t le = LaunchCopyPage(ctx->pool, src, dst, StreamOf(ctx, stream)); le != cudaSuccess) {
+        ctx->host.SeqFree(made);
+        return FailCuda(ctx, "seq_fork: page copy", le);
+      }
+      ctx->launches += 1;
     }
-    ctx->launches += 1;
-  }
-  *out = made;
-  return YAHKV_OK;
+    *out = made;
+    return YAHKV_OK;
+  });
 }
 
 // The lists of a shared plan in one buffer (one upload): tiles, units, prefix items, items, rows; the sizes of all but the
@@ -989,118 +1018,124 @@ static SharedLaunch SharedArgs(yahkv_ctx* ctx) {
 
 int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
                                const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, void* stream) {
-  if (int r = RequireDevice(ctx, "attend_decode_shared"); r != YAHKV_OK) return r;
-  if (IsTileFmt(ctx->cfg.fmt))
-    return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (their sequences share no pages)");
-  if (out_dtype != YAHKV_OUT_F16 && out_dtype != YAHKV_OUT_F32) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: bad out_dtype");
-  if (n_seqs > 0 && (q_dev == nullptr || out_dev == nullptr)) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: null q or out pointer");
-  if ((reinterpret_cast<std::uintptr_t>(q_dev) & 15) != 0) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: q must be 16-byte aligned");
-  if (int r = EnsureShared(ctx); r != YAHKV_OK) return r;   // before the plan: a failure here changes no state
-  auto& sh = ctx->shared;
-  bool changed = false;
-  HostError e = ctx->host.PlanDecodeShared(layer, n_seqs, seq_ids, n_splits, ctx->cfg.max_splits, ctx->max_units, sh.n_pairs,
-                                           sh.max_part_rows, &changed);
-  if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
-  if (n_seqs == 0) return YAHKV_OK;
-  struct PlanGuard {   // as in AttendDecode: a plan that never reached the device is dropped
-    KvHost* host;
-    bool keep = false;
-    ~PlanGuard() {
-      if (!keep) host->InvalidateSharedPlan();
+  return NoThrow(ctx, "attend_decode_shared", [&]() -> int {
+    if (int r = RequireDevice(ctx, "attend_decode_shared"); r != YAHKV_OK) return r;
+    if (IsTileFmt(ctx->cfg.fmt))
+      return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (their sequences share no pages)");
+    if (out_dtype != YAHKV_OUT_F16 && out_dtype != YAHKV_OUT_F32) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: bad out_dtype");
+    if (n_seqs > 0 && (q_dev == nullptr || out_dev == nullptr)) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: null q or out pointer");
+    if ((reinterpret_cast<std::uintptr_t>(q_dev) & 15) != 0) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: q must be 16-byte aligned");
+    if (int r = RefuseCapture(ctx, "attend_decode_shared: lists from the host", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
+    if (int r = EnsureShared(ctx); r != YAHKV_OK) return r;   // before the plan: a failure here changes no state
+    auto& sh = ctx->shared;
+    bool changed = false;
+    HostError e = ctx->host.PlanDecodeShared(layer, n_seqs, seq_ids, n_splits, ctx->cfg.max_splits, ctx->max_units, sh.n_pairs,
+                                             sh.max_part_rows, &changed);
+    if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
+    if (n_seqs == 0) return YAHKV_OK;
+    struct PlanGuard {   // as in AttendDecode: a plan that never reached the device is dropped
+      KvHost* host;
+      bool keep = false;
+      ~PlanGuard() {
+        if (!keep) host->InvalidateSharedPlan();
+      }
+    } guard{&ctx->host};
+    const KvHost::SharedPlan& plan = ctx->host.shared_plan();
+    if (static_cast<int>(plan.tiles.size()) > sh.max_tiles) return Fail(ctx, YAHKV_ERR_CAPACITY, "attend_decode_shared: too many prefix tiles");
+    cudaStream_t st = StreamOf(ctx, stream);
+    if (int r = FlushTables(ctx, st); r != YAHKV_OK) return r;
+    const std::pair<const void*, std::size_t> lists[] = {{plan.tiles.data(), plan.tiles.size() * sizeof(PrefixTile)},
+                                                         {plan.units.data(), plan.units.size() * sizeof(DecodeUnit)},
+                                                         {plan.prefix_items.data(), plan.prefix_items.size() * sizeof(PrefixItem)},
+                                                         {plan.items.data(), plan.items.size() * sizeof(CombineItem)},
+                                                         {plan.rows.data(), plan.rows.size() * sizeof(std::int32_t)}};
+    std::size_t at[6] = {0};
+    for (int i = 0; i < 5; ++i) at[i + 1] = at[i] + lists[i].second;
+    if (at[5] > sh.plan_bytes) return Fail(ctx, YAHKV_ERR_CAPACITY, "attend_decode_shared: plan larger than its buffer");
+    if (changed) {
+      char* buf = nullptr;
+      YAHKV_CUDA(ctx, ctx->staging.Acquire(at[5], &buf));
+      for (int i = 0; i < 5; ++i)
+        if (lists[i].second > 0) std::memcpy(buf + at[i], lists[i].first, lists[i].second);
+      YAHKV_CUDA(ctx, cudaMemcpyAsync(sh.plan_dev, buf, at[5], cudaMemcpyHostToDevice, st));
+      YAHKV_CUDA(ctx, ctx->staging.Release(st));
     }
-  } guard{&ctx->host};
-  const KvHost::SharedPlan& plan = ctx->host.shared_plan();
-  if (static_cast<int>(plan.tiles.size()) > sh.max_tiles) return Fail(ctx, YAHKV_ERR_CAPACITY, "attend_decode_shared: too many prefix tiles");
-  cudaStream_t st = StreamOf(ctx, stream);
-  if (int r = FlushTables(ctx, st); r != YAHKV_OK) return r;
-  const std::pair<const void*, std::size_t> lists[] = {{plan.tiles.data(), plan.tiles.size() * sizeof(PrefixTile)},
-                                                       {plan.units.data(), plan.units.size() * sizeof(DecodeUnit)},
-                                                       {plan.prefix_items.data(), plan.prefix_items.size() * sizeof(PrefixItem)},
-                                                       {plan.items.data(), plan.items.size() * sizeof(CombineItem)},
-                                                       {plan.rows.data(), plan.rows.size() * sizeof(std::int32_t)}};
-  std::size_t at[6] = {0};
-  for (int i = 0; i < 5; ++i) at[i + 1] = at[i] + lists[i].second;
-  if (at[5] > sh.plan_bytes) return Fail(ctx, YAHKV_ERR_CAPACITY, "attend_decode_shared: plan larger than its buffer");
-  if (changed) {
-    char* buf = nullptr;
-    YAHKV_CUDA(ctx, ctx->staging.Acquire(at[5], &buf));
-    for (int i = 0; i < 5; ++i)
-      if (lists[i].second > 0) std::memcpy(buf + at[i], lists[i].first, lists[i].second);
-    YAHKV_CUDA(ctx, cudaMemcpyAsync(sh.plan_dev, buf, at[5], cudaMemcpyHostToDevice, st));
-    YAHKV_CUDA(ctx, ctx->staging.Release(st));
-  }
-  DecodeLaunch a{};
-  a.kmap = &ctx->kmap, a.vmap = &ctx->vmap, a.pool = ctx->pool, a.layer = layer;
-  a.tables_dev = ctx->tables_dev, a.table_stride = ctx->cfg.max_pages_per_seq;
-  a.units_dev = reinterpret_cast<const DecodeUnit*>(sh.plan_dev + at[1]), a.n_units = static_cast<int>(plan.units.size());
-  a.items_dev = reinterpret_cast<const CombineItem*>(sh.plan_dev + at[3]), a.n_seqs = n_seqs;
-  a.q_dev = q_dev, a.gate_dev = gate_dev, a.out_dev = out_dev, a.out_f32 = out_dtype == YAHKV_OUT_F32;
-  a.scale_log2 = ctx->scale_log2;
-  a.partial_acc = ctx->partial_acc, a.partial_ml = ctx->partial_ml, a.status_dev = ctx->status_dev;
-  SharedLaunch p = SharedArgs(ctx);
-  p.tiles_dev = reinterpret_cast<const PrefixTile*>(sh.plan_dev), p.n_tiles = static_cast<int>(plan.tiles.size());
-  p.prefix_items_dev = reinterpret_cast<const PrefixItem*>(sh.plan_dev + at[2]);
-  p.rows_dev = reinterpret_cast<const std::int32_t*>(sh.plan_dev + at[4]);
-  a.beside = p.n_tiles > 0;   // the suffixes run beside the prefix pass
-  TimedLaunch ts(ctx, YAHKV_KERNEL_SHARED_PREFIX, st);
-  cudaError_t le = LaunchSharedPrefix(a, p, st);
-  if (p.n_tiles > 0) ts.End();
-  if (le == cudaSuccess) {
-    TimedLaunch tp(ctx, YAHKV_KERNEL_DECODE_PART, st);
-    le = ctx->cfg.fmt == YAHKV_FMT_F16 ? LaunchF16DecodePart(a, st) : LaunchDecodePart(a, st);
-    if (a.n_units > 0) tp.End();
-  }
-  if (le == cudaSuccess) {
-    TimedLaunch tc(ctx, YAHKV_KERNEL_DECODE_COMBINE, st);
-    le = LaunchSharedCombine(a, p, st);
-    tc.End();
-  }
-  if (le != cudaSuccess) return FailCuda(ctx, "shared-prefix decode attention launch", le);
-  guard.keep = true;
-  ctx->launches += 1 + (p.n_tiles > 0 ? 1 : 0) + (a.n_units > 0 ? 1 : 0);
-  return YAHKV_OK;
+    DecodeLaunch a{};
+    a.kmap = &ctx->kmap, a.vmap = &ctx->vmap, a.pool = ctx->pool, a.layer = layer;
+    a.tables_dev = ctx->tables_dev, a.table_stride = ctx->cfg.max_pages_per_seq;
+    a.units_dev = reinterpret_cast<const DecodeUnit*>(sh.plan_dev + at[1]), a.n_units = static_cast<int>(plan.units.size());
+    a.items_dev = reinterpret_cast<const CombineItem*>(sh.plan_dev + at[3]), a.n_seqs = n_seqs;
+    a.q_dev = q_dev, a.gate_dev = gate_dev, a.out_dev = out_dev, a.out_f32 = out_dtype == YAHKV_OUT_F32;
+    a.scale_log2 = ctx->scale_log2;
+    a.partial_acc = ctx->partial_acc, a.partial_ml = ctx->partial_ml, a.status_dev = ctx->status_dev;
+    SharedLaunch p = SharedArgs(ctx);
+    p.tiles_dev = reinterpret_cast<const PrefixTile*>(sh.plan_dev), p.n_tiles = static_cast<int>(plan.tiles.size());
+    p.prefix_items_dev = reinterpret_cast<const PrefixItem*>(sh.plan_dev + at[2]);
+    p.rows_dev = reinterpret_cast<const std::int32_t*>(sh.plan_dev + at[4]);
+    a.beside = p.n_tiles > 0;   // the suffixes run beside the prefix pass
+    TimedLaunch ts(ctx, YAHKV_KERNEL_SHARED_PREFIX, st);
+    cudaError_t le = LaunchSharedPrefix(a, p, st);
+    if (p.n_tiles > 0) ts.End();
+    if (le == cudaSuccess) {
+      TimedLaunch tp(ctx, YAHKV_KERNEL_DECODE_PART, st);
+      le = ctx->cfg.fmt == YAHKV_FMT_F16 ? LaunchF16DecodePart(a, st) : LaunchDecodePart(a, st);
+      if (a.n_units > 0) tp.End();
+    }
+    if (le == cudaSuccess) {
+      TimedLaunch tc(ctx, YAHKV_KERNEL_DECODE_COMBINE, st);
+      le = LaunchSharedCombine(a, p, st);
+      tc.End();
+    }
+    if (le != cudaSuccess) return FailCuda(ctx, "shared-prefix decode attention launch", le);
+    guard.keep = true;
+    ctx->launches += 1 + (p.n_tiles > 0 ? 1 : 0) + (a.n_units > 0 ? 1 : 0);
+    return YAHKV_OK;
+  });
 }
 
 // ---- eviction --------------------------------------------------------------------------------------------------
 int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t n_keep, int64_t n_sink, int64_t n_recent,
                 float* weights_dev, int64_t weights_stride, int64_t weights_layer_stride, int32_t* kept_dev, void* stream) {
-  if (int r = RequireDevice(ctx, "evict"); r != YAHKV_OK) return r;
-  if (int r = CheckWeights(ctx, "evict", n_seqs, seq_ids, weights_dev, weights_stride); r != YAHKV_OK) return r;
-  if (n_seqs > 0 && kept_dev == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "evict: null kept list");
-  if (n_keep < 1 || n_keep > static_cast<int64_t>(ctx->cfg.max_pages_per_seq) * kPageTokens || n_sink < 0 || n_recent < 0 ||
-      n_sink > n_keep || n_recent > n_keep - n_sink)
-    return Fail(ctx, YAHKV_ERR_INVALID, "evict: n_keep must be a slot count of at least 1, n_sink + n_recent at most n_keep");
-  if (ctx->cfg.n_layers > 1 && weights_layer_stride < static_cast<int64_t>(ctx->cfg.max_seqs) * kKvHeads * weights_stride)
-    return Fail(ctx, YAHKV_ERR_INVALID, "evict: the layers of the weights overlap (weights_layer_stride below max_seqs * 4 * weights_stride)");
-  bool any = false;
-  HostError e = ctx->host.PlanEvict(n_seqs, seq_ids, n_keep, &ctx->evict_scratch, &ctx->evict_page_scratch, &any);
-  if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
-  if (n_seqs == 0) return YAHKV_OK;
-  const yahkv_config& c = ctx->cfg;
-  if (ctx->evict_dev == nullptr)   // the sequences, then their pages
-    YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_dev, static_cast<std::size_t>(c.max_seqs) * (sizeof(EvictSeq) + 4 * static_cast<std::size_t>(c.max_pages_per_seq)), false));
-  cudaStream_t st = StreamOf(ctx, stream);
-  if (int r = FlushTables(ctx, st); r != YAHKV_OK) return r;   // the kernels read the tables as they are before the call
-  const std::size_t sb = ctx->evict_scratch.size() * sizeof(EvictSeq), pb = ctx->evict_page_scratch.size() * sizeof(std::int32_t);
-  char* buf = nullptr;
-  YAHKV_CUDA(ctx, ctx->staging.Acquire(sb + pb, &buf));
-  std::memcpy(buf, ctx->evict_scratch.data(), sb);
-  if (pb > 0) std::memcpy(buf + sb, ctx->evict_page_scratch.data(), pb);
-  YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->evict_dev, buf, sb + pb, cudaMemcpyHostToDevice, st));
-  YAHKV_CUDA(ctx, ctx->staging.Release(st));
-  EvictLaunch a{};
-  a.pool = ctx->pool, a.tables_dev = ctx->tables_dev, a.table_stride = c.max_pages_per_seq;
-  a.seqs_dev = reinterpret_cast<const EvictSeq*>(ctx->evict_dev), a.n_seqs = n_seqs;
-  a.dst_pages_dev = reinterpret_cast<const std::int32_t*>(ctx->evict_dev + sb);
-  a.n_keep = static_cast<int>(n_keep), a.n_sink = static_cast<int>(n_sink), a.n_recent = static_cast<int>(n_recent);
-  a.weights = weights_dev, a.weights_stride = weights_stride, a.layer_stride = weights_layer_stride, a.kept = kept_dev;
-  for (const EvictSeq& s : ctx->evict_scratch) a.max_keys = std::max(a.max_keys, s.n_keys);
-  TimedLaunch tl(ctx, YAHKV_KERNEL_EVICT, st);
-  YAHKV_CUDA(ctx, LaunchEvict(a, st));
-  tl.End();
-  ctx->launches += 2;
-  if (any) ctx->host.CommitEvict(n_keep, ctx->evict_scratch, ctx->evict_page_scratch);
-  return YAHKV_OK;
+  return NoThrow(ctx, "evict", [&]() -> int {
+    if (int r = RequireDevice(ctx, "evict"); r != YAHKV_OK) return r;
+    if (int r = CheckWeights(ctx, "evict", -1, n_seqs, seq_ids, weights_dev, weights_stride); r != YAHKV_OK) return r;
+    if (n_seqs > 0 && kept_dev == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "evict: null kept list");
+    if (n_keep < 1 || n_keep > static_cast<int64_t>(ctx->cfg.max_pages_per_seq) * kPageTokens || n_sink < 0 || n_recent < 0 ||
+        n_sink > n_keep || n_recent > n_keep - n_sink)
+      return Fail(ctx, YAHKV_ERR_INVALID, "evict: n_keep must be a slot count of at least 1, n_sink + n_recent at most n_keep");
+    if (ctx->cfg.n_layers > 1 && weights_layer_stride < static_cast<int64_t>(ctx->cfg.max_seqs) * kKvHeads * weights_stride)
+      return Fail(ctx, YAHKV_ERR_INVALID, "evict: the layers of the weights overlap (weights_layer_stride below max_seqs * 4 * weights_stride)");
+    if (int r = RefuseCapture(ctx, "evict: host tables change", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
+    bool any = false;
+    HostError e = ctx->host.PlanEvict(n_seqs, seq_ids, n_keep, &ctx->evict_scratch, &ctx->evict_page_scratch, &any);
+    if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
+    if (n_seqs == 0) return YAHKV_OK;
+    const yahkv_config& c = ctx->cfg;
+    if (ctx->evict_dev == nullptr)   // the sequences, then their pages
+      YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_dev, static_cast<std::size_t>(c.max_seqs) * (sizeof(EvictSeq) + 4 * static_cast<std::size_t>(c.max_pages_per_seq)), false));
+    cudaStream_t st = StreamOf(ctx, stream);
+    if (int r = FlushTables(ctx, st); r != YAHKV_OK) return r;   // the kernels read the tables as they are before the call
+    const std::size_t sb = ctx->evict_scratch.size() * sizeof(EvictSeq), pb = ctx->evict_page_scratch.size() * sizeof(std::int32_t);
+    char* buf = nullptr;
+    YAHKV_CUDA(ctx, ctx->staging.Acquire(sb + pb, &buf));
+    std::memcpy(buf, ctx->evict_scratch.data(), sb);
+    if (pb > 0) std::memcpy(buf + sb, ctx->evict_page_scratch.data(), pb);
+    YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->evict_dev, buf, sb + pb, cudaMemcpyHostToDevice, st));
+    YAHKV_CUDA(ctx, ctx->staging.Release(st));
+    EvictLaunch a{};
+    a.pool = ctx->pool, a.tables_dev = ctx->tables_dev, a.table_stride = c.max_pages_per_seq;
+    a.seqs_dev = reinterpret_cast<const EvictSeq*>(ctx->evict_dev), a.n_seqs = n_seqs;
+    a.dst_pages_dev = reinterpret_cast<const std::int32_t*>(ctx->evict_dev + sb);
+    a.n_keep = static_cast<int>(n_keep), a.n_sink = static_cast<int>(n_sink), a.n_recent = static_cast<int>(n_recent);
+    a.weights = weights_dev, a.weights_stride = weights_stride, a.layer_stride = weights_layer_stride, a.kept = kept_dev;
+    for (const EvictSeq& s : ctx->evict_scratch) a.max_keys = std::max(a.max_keys, s.n_keys);
+    TimedLaunch tl(ctx, YAHKV_KERNEL_EVICT, st);
+    YAHKV_CUDA(ctx, LaunchEvict(a, st));
+    tl.End();
+    ctx->launches += 2;
+    if (any) ctx->host.CommitEvict(n_keep, ctx->evict_scratch, ctx->evict_page_scratch);
+    return YAHKV_OK;
+  });
 }
 
 // ---- rotary positions on given rows ----------------------------------------------------------------------------
@@ -1111,69 +1146,65 @@ struct yahkv_rope {
 };
 
 int yahkv_rope_create(yahkv_ctx* ctx, const yahkv_rope_config* cfg, yahkv_rope** out) {
-  if (int r = RequireDevice(ctx, "rope_create"); r != YAHKV_OK) return r;
-  if (out == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: null out pointer");
-  *out = nullptr;
-  if (cfg == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: null config");
-  const yahkv_rope_config& c = *cfg;
-  if (c.layout != YAHKV_ROPE_HALF && c.layout != YAHKV_ROPE_INTERLEAVED) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: bad layout");
-  if (c.rotary_dim < 2 || c.rotary_dim > kHeadDim || c.rotary_dim % 2 != 0)
-    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: rotary_dim must be even, 2 .. 256");
-  if (!(c.theta > 1.0) || !std::isfinite(c.theta)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: theta must be a number above 1");
-  if (c.scaling < YAHKV_ROPE_SCALE_NONE || c.scaling > YAHKV_ROPE_SCALE_YARN) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: bad scaling");
-  if (c.scaling != YAHKV_ROPE_SCALE_NONE && (!(c.factor >= 1.0) || !std::isfinite(c.factor)))
-    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: factor must be a number of at least 1");
-  if (c.scaling == YAHKV_ROPE_SCALE_NTK && c.rotary_dim < 4)
-    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: NTK scaling needs a rotary_dim of at least 4");
-  if (c.scaling == YAHKV_ROPE_SCALE_YARN && (!(c.original_len > 0.0) || !(c.beta_slow >= 0.0) || !(c.beta_fast > c.beta_slow) ||
-                                             !std::isfinite(c.original_len) || !std::isfinite(c.beta_fast)))
-    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: YaRN scaling needs original_len > 0 and beta_fast > beta_slow >= 0");
-  if (!(c.magnitude >= 0.0) || !std::isfinite(c.magnitude)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: magnitude must not be negative");
-  if (c.max_positions < 1 || c.max_positions > (1LL << 31)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: max_positions must be 1 .. 2^31");
-  const int half = c.rotary_dim / 2;
-  const int low = 1 << kRopeLowBits;
-  const std::int64_t n_hi = (c.max_positions + low - 1) / low;
-  std::vector<double> freq(static_cast<std::size_t>(half));
-  double magnitude = c.magnitude > 0.0 ? c.magnitude : 1.0;
-  if (c.scaling == YAHKV_ROPE_SCALE_YARN && c.magnitude == 0.0) magnitude = 0.1 * std::log(c.factor) + 1.0;
-  const double theta = c.scaling == YAHKV_ROPE_SCALE_NTK ? c.theta * std::pow(c.factor, c.rotary_dim / (c.rotary_dim - 2.0)) : c.theta;
-  for (int p = 0; p < half; ++p) {
-    double f = std::pow(theta, -2.0 * p / c.rotary_dim);
-    if (c.scaling == YAHKV_ROPE_SCALE_LINEAR) f /= c.factor;
-    if (c.scaling == YAHKV_ROPE_SCALE_YARN) {   // by the turns a pair makes over the original length
-      const double turns = c.original_len * f / (2.0 * 3.14159265358979323846);
-      const double keep = std::min(std::max((turns - c.beta_slow) / (c.beta_fast - c.beta_slow), 0.0), 1.0);
-      f = (1.0 - keep) * f / c.factor + keep * f;
-    }
-    freq[static_cast<std::size_t>(p)] = f;
-  }
-  auto* r = new (std::nothrow) yahkv_rope();
-  if (r == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: out of host memory");
-  r->ctx = ctx, r->cfg = c;
-  std::vector<float2> tab;
-  try {
-    tab.resize(static_cast<std::size_t>(n_hi + low) * half);
-  } catch (const std::bad_alloc&) {
-    delete r;
-    return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: out of host memory");
-  }
-  for (std::int64_t i = 0; i < n_hi + low; ++i)
+  return NoThrow(ctx, "rope_create", [&]() -> int {
+    if (int r = RequireDevice(ctx, "rope_create"); r != YAHKV_OK) return r;
+    if (out == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: null out pointer");
+    *out = nullptr;
+    if (cfg == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: null config");
+    const yahkv_rope_config& c = *cfg;
+    if (c.layout != YAHKV_ROPE_HALF && c.layout != YAHKV_ROPE_INTERLEAVED) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: bad layout");
+    if (c.rotary_dim < 2 || c.rotary_dim > kHeadDim || c.rotary_dim % 2 != 0)
+      return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: rotary_dim must be even, 2 .. 256");
+    if (!(c.theta > 1.0) || !std::isfinite(c.theta)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: theta must be a number above 1");
+    if (c.scaling < YAHKV_ROPE_SCALE_NONE || c.scaling > YAHKV_ROPE_SCALE_YARN) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: bad scaling");
+    if (c.scaling != YAHKV_ROPE_SCALE_NONE && (!(c.factor >= 1.0) || !std::isfinite(c.factor)))
+      return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: factor must be a number of at least 1");
+    if (c.scaling == YAHKV_ROPE_SCALE_NTK && c.rotary_dim < 4)
+      return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: NTK scaling needs a rotary_dim of at least 4");
+    if (c.scaling == YAHKV_ROPE_SCALE_YARN && (!(c.original_len > 0.0) || !(c.beta_slow >= 0.0) || !(c.beta_fast > c.beta_slow) ||
+                                               !std::isfinite(c.original_len) || !std::isfinite(c.beta_fast)))
+      return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: YaRN scaling needs original_len > 0 and beta_fast > beta_slow >= 0");
+    if (!(c.magnitude >= 0.0) || !std::isfinite(c.magnitude)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: magnitude must not be negative");
+    if (c.max_positions < 1 || c.max_positions > (1LL << 26)) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: max_positions must be 1 .. 2^26");
+    const int half = c.rotary_dim / 2;
+    const int low = 1 << kRopeLowBits;
+    const std::int64_t n_hi = (c.max_positions + low - 1) / low;
+    std::vector<double> freq(static_cast<std::size_t>(half));
+    double magnitude = c.magnitude > 0.0 ? c.magnitude : 1.0;
+    if (c.scaling == YAHKV_ROPE_SCALE_YARN && c.magnitude == 0.0) magnitude = 0.1 * std::log(c.factor) + 1.0;
+    const double theta = c.scaling == YAHKV_ROPE_SCALE_NTK ? c.theta * std::pow(c.factor, c.rotary_dim / (c.rotary_dim - 2.0)) : c.theta;
     for (int p = 0; p < half; ++p) {
-      const double n = static_cast<double>(i < n_hi ? i * low : i - n_hi);
-      const double m = i < n_hi ? magnitude : 1.0;
-      const double a = n * freq[static_cast<std::size_t>(p)];
-      tab[static_cast<std::size_t>(i) * half + p] = make_float2(static_cast<float>(m * std::cos(a)), static_cast<float>(m * std::sin(a)));
+      double f = std::pow(theta, -2.0 * p / c.rotary_dim);
+      if (c.scaling == YAHKV_ROPE_SCALE_LINEAR) f /= c.factor;
+      if (c.scaling == YAHKV_ROPE_SCALE_YARN) {   // by the turns a pair makes over the original length
+        const double turns = c.original_len * f / (2.0 * 3.14159265358979323846);
+        const double keep = std::min(std::max((turns - c.beta_slow) / (c.beta_fast - c.beta_slow), 0.0), 1.0);
+        f = (1.0 - keep) * f / c.factor + keep * f;
+      }
+      freq[static_cast<std::size_t>(p)] = f;
     }
-  cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&r->hi), tab.size() * sizeof(float2));
-  if (e == cudaSuccess) e = cudaMemcpy(r->hi, tab.data(), tab.size() * sizeof(float2), cudaMemcpyHostToDevice);
-  if (e != cudaSuccess) {
-    if (r->hi != nullptr) cudaFree(r->hi);
-    delete r;
-    return FailCuda(ctx, "rope_create", e);
-  }
-  r->lo = r->hi + static_cast<std::size_t>(n_hi) * half;
-  *out = r;
-  return YAHKV_OK;
+    std::vector<float2> tab(static_cast<std::size_t>(n_hi + low) * half);
+    auto* r = new (std::nothrow) yahkv_rope();
+    if (r == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: out of host memory");
+    r->ctx = ctx, r->cfg = c;
+    for (std::int64_t i = 0; i < n_hi + low; ++i)
+      for (int p = 0; p < half; ++p) {
+        const double n = static_cast<double>(i < n_hi ? i * low : i - n_hi);
+        const double m = i < n_hi ? magnitude : 1.0;
+        const double a = n * freq[static_cast<std::size_t>(p)];
+        tab[static_cast<std::size_t>(i) * half + p] = make_float2(static_cast<float>(m * std::cos(a)), static_cast<float>(m * std::sin(a)));
+      }
+    cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&r->hi), tab.size() * sizeof(float2));
+    if (e == cudaSuccess) e = cudaMemcpy(r->hi, tab.data(), tab.size() * sizeof(float2), cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+      if (r->hi != nullptr) cudaFree(r->hi);
+      delete r;
+      return FailCuda(ctx, "rope_create", e);
+    }
+    r->lo = r->hi + static_cast<std::size_t>(n_hi) * half;
+    *out = r;
+    return YAHKV_OK;
+  });
 }
 
 void yahkv_rope_destroy(yahkv_rope* r) {
@@ -1601,8 +1632,13 @@ int yahkv_batch_set_shared(yahkv_batch* b, int32_t on) {
   return YAHKV_OK;
 }
 
+static int BatchPrepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_changed, void* stream);
 int yahkv_batch_prepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_changed, void* stream) {
   if (b == nullptr) return YAHKV_ERR_INVALID;
+  return NoThrow(b->ctx, "batch_prepare", [&] { return BatchPrepare(b, horizon_steps, layout_changed, stream); });
+}
+
+static int BatchPrepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_changed, void* stream) {
   yahkv_ctx* ctx = b->ctx;
   if (int r = RequireDevice(ctx, "batch_prepare"); r != YAHKV_OK) return r;
   if (horizon_steps < 1) return Fail(ctx, YAHKV_ERR_INVALID, "batch_prepare: horizon must be at least one step");
