@@ -235,6 +235,8 @@ static void CheckEvict() {
   std::int32_t d = -1;
   EXPECT(host.SeqFork(b, 64, &d, &src, &dst).code == YAHKV_OK && host.evicted(d));
   EXPECT(host.SeqSetLen(d, -1, 0).code == YAHKV_OK && !host.evicted(d));
+  std::int32_t none = -1;   // a fork that holds nothing has no such slots
+  EXPECT(host.SeqFork(b, 0, &none, &src, &dst).code == YAHKV_OK && !host.evicted(none) && host.SeqFree(none).code == YAHKV_OK);
   // appending into a page that is shared is refused, and nothing changes
   std::int64_t slot = -1;
   const std::int64_t pos = 0;

@@ -232,6 +232,9 @@ def test_refusals_and_positions_after_an_eviction(tmp_path):
     for n_keep, sink, recent in ((50, -1, 0), (50, 0, -1), (50, 51, 0), (50, 30, 21)):
         assert code(ev, [a], n_keep, w, kept, n_sink=sink, n_recent=recent) == yahkv.ERR_INVALID
     assert code(ev, [a], 0, w, kept[..., :0].contiguous()) == yahkv.ERR_INVALID
+    raw = yahkv.lib.yahkv_evict
+    assert raw(cache._h, 1, yahkv._ptr(yahkv._i32([a])), 50, 0, 0, w.data_ptr() + 2, 200, 2400, yahkv._ptr(kept), None) == yahkv.ERR_INVALID
+    assert raw(cache._h, 1, yahkv._ptr(yahkv._i32([a])), 50, 0, 0, yahkv._ptr(w), 200, 2400, kept.data_ptr() + 2, None) == yahkv.ERR_INVALID
     assert code(ev, [a, a], 50, w, two) == yahkv.ERR_INVALID
     assert code(ev, [2], 50, w, kept) == yahkv.ERR_INVALID
     assert yahkv.lib.yahkv_evict(cache._h, 1, yahkv._ptr(yahkv._i32([a])), 50, 0, 0, yahkv._ptr(w), 200, 100, yahkv._ptr(kept), None) == yahkv.ERR_INVALID

@@ -183,6 +183,31 @@ def test_long_groups_short_rows_and_forks_of_forks_at_the_default_threshold():
     check(cache, 0, [seqs[i] for i in few], q[few], shared(cache, 0, [seqs[i] for i in few], q[few]))
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+def test_values_at_the_end_of_fp16(fmt):
+    """Blocks whose largest value is fp16's largest: q8_0 stores it as 127 x 516 = 65532, which as fp16 would be infinite; the
+    pass takes 65504, off by less than half a step (28 of 65532 < 2^-11). A block whose scale is infinite stays that."""
+    rng = np.random.default_rng(23)
+    cache = small_cache(num_pages=8, fmt=fmt, max_seqs=3, max_pages_per_seq=3)
+    root = cache.seq_create()
+    k, v = normal(rng, 128, 4, 256), (normal(rng, 128, 4, 256) * np.float16(1000)).astype(np.float16)
+    v[..., ::32] = 65504
+    v[::2, :, 3::32] = -65504
+    extend(cache, 0, root, k, v)
+    seqs = [cache.seq_fork(root, 128) for _ in range(2)]
+    q = normal(rng, 2, 24, 256)
+    check(cache, 0, seqs, q, shared(cache, 0, seqs, q))
+    if fmt != yahkv.FMT_F16:
+        page = int(cache.seq_table(root)[0])
+        codes, scales = cache.read_page(0, yahkv.SIDE_V, page)
+        scales = scales.copy()
+        scales.view(np.float16)[0, 5, 1] = np.inf           # kv head 0, token 5, dims 32 .. 63
+        cache.write_page(0, yahkv.SIDE_V, page, codes, scales)
+        got = shared(cache, 0, seqs, q)
+        assert not np.isfinite(got[:, :6, 32:64]).any()
+        assert np.isfinite(got[:, 6:]).all() and np.isfinite(got[:, :6, :32]).all() and np.isfinite(got[:, :6, 64:]).all()
+
+
 def test_a_head_sharded_context_writes_its_own_heads_only():
     rng = np.random.default_rng(3)
     for fmt in (yahkv.FMT_F16, yahkv.FMT_Q8_0):

@@ -136,6 +136,8 @@ class KvHost {
     // Validate everything before changing anything.
     std::vector<std::int32_t> sorted(pages, pages + n);
     std::sort(sorted.begin(), sorted.end());
+    std::vector<char> mine(static_cast<std::size_t>(cfg_.num_pages), 0);
+    for (int i = 0; i < n_pages(seq); ++i) mine[static_cast<std::size_t>(table_row(seq)[i])] = 1;
     for (int i = 0; i < n; ++i) {
       const std::int32_t p = sorted[static_cast<std::size_t>(i)];
       if (p < 0 || p >= cfg_.num_pages)
@@ -143,8 +145,8 @@ class KvHost {
       if (i > 0 && sorted[static_cast<std::size_t>(i - 1)] == p)
         return {YAHKV_ERR_INVALID, "page table names page " + std::to_string(p) + " twice"};
       // free, or held by this sequence alone
-      if (const int holder = OtherHolder(p, seq); holder >= 0)
-        return {YAHKV_ERR_INVALID, "page " + std::to_string(p) + " belongs to sequence " + std::to_string(holder)};
+      if (refs_[static_cast<std::size_t>(p)] > mine[static_cast<std::size_t>(p)])
+        return {YAHKV_ERR_INVALID, "page " + std::to_string(p) + " belongs to sequence " + std::to_string(OtherHolder(p, seq))};
     }
     ReleasePages(seq);
     // Take the named pages out of the free list.
@@ -210,7 +212,7 @@ class KvHost {
       *copy_src = from[whole], *copy_dst = row[whole];
     }
     n_pages_[static_cast<std::size_t>(s)] = whole + (rest ? 1 : 0);
-    evicted_[static_cast<std::size_t>(s)] = evicted_[static_cast<std::size_t>(seq)];
+    evicted_[static_cast<std::size_t>(s)] = n_tokens > 0 ? evicted_[static_cast<std::size_t>(seq)] : 0;
     MarkDirty(s, 0, n_pages_[static_cast<std::size_t>(s)]);
     SetLenAll(s, n_tokens);
     *out = s;
@@ -891,11 +893,8 @@ class KvHost {
   void Unref(std::int32_t page) {
     if (--refs_[static_cast<std::size_t>(page)] == 0) free_pages_.push_back(page);
   }
-  // A live sequence that keeps `seq` from having page p to itself; -1: the page is free or only seq's.
+  // A live sequence other than `seq` whose table names page p; -1: there is none.
   int OtherHolder(std::int32_t p, int seq) const {
-    const int refs = refs_[static_cast<std::size_t>(p)];
-    if (refs == 0 || (refs == 1 && std::find(table_row(seq), table_row(seq) + n_pages(seq), p) != table_row(seq) + n_pages(seq)))
-      return -1;
     for (int s = 0; s < cfg_.max_seqs; ++s) {
       if (s == seq || !live(s)) continue;
       for (int i = 0; i < n_pages(s); ++i)

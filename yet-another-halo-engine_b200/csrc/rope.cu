@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(32 * kRopeRowWarps) RopeRowsKernel(const RopeR
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long task = static_cast<long long>(blockIdx.x) * kRopeRowWarps + warp;
   const int head_groups = (a.n_heads + kHeads - 1) / kHeads;
-  const int token = static_cast<int>(task / head_groups), h0 = static_cast<int>(task % head_groups) * kHeads;
+  const long long token = task / head_groups;
+  const int h0 = static_cast<int>(task % head_groups) * kHeads;
   if (token >= a.n_tokens) return;
   long long pos = __ldg(a.positions + token);
   const std::size_t x_at = static_cast<std::size_t>(token) * a.x_stride + static_cast<std::size_t>(h0) * kHeadDim + 8 * lane;

@@ -95,14 +95,17 @@ struct SharedBars {
   int converted[2];                      // local: per group of dequantizing warps, tiles up to this one are converted
 };
 
-// Eight values of a row as fp16: exact integer codes times the block scale, one rounding.
+// Eight values of a row as fp16: exact integer codes times the block scale, one rounding. A product that the rounded
+// scale takes beyond fp16 (127 x 516 for a block of 65,504) is the largest number, not infinity; with a scale that is no
+// number it is none either.
 __device__ __forceinline__ uint4 ScaleCodes(const std::uint32_t (&h)[4], std::uint16_t scale) {
   const __half2 d = __half2half2(__ushort_as_half(scale));
+  const __half2 most = __half2half2(__ushort_as_half((scale & 0x7FFFU) < 0x7C00U ? 0x7BFF : 0x7C00));
   uint4 o;
   std::uint32_t* w = &o.x;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), d);
+    const __half2 v = __hmax2_nan(__hmin2_nan(__hmul2(*reinterpret_cast<const __half2*>(&h[i]), d), most), __hneg2(most));
     w[i] = *reinterpret_cast<const std::uint32_t*>(&v);
   }
   return o;

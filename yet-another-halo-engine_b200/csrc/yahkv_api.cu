@@ -807,6 +807,7 @@ static int CheckWeights(yahkv_ctx* ctx, const char* what, int32_t layer, int32_t
   if (n_seqs < 0 || (n_seqs > 0 && seq_ids == nullptr)) return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": bad sequence list");
   if (n_seqs > ctx->cfg.max_seqs) return Fail(ctx, YAHKV_ERR_CAPACITY, std::string(what) + ": more rows than max_seqs");
   if (n_seqs > 0 && weights_dev == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": null weights");
+  if ((reinterpret_cast<std::uintptr_t>(weights_dev) & 3) != 0) return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": weights not 4-byte aligned");
   std::vector<char> seen(static_cast<std::size_t>(ctx->cfg.max_seqs), 0);
   for (int i = 0; i < n_seqs; ++i) {
     if (!ctx->host.live(seq_ids[i])) return Fail(ctx, YAHKV_ERR_INVALID, std::string(what) + ": not a live sequence: " + std::to_string(seq_ids[i]));
@@ -1099,7 +1100,8 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
   return NoThrow(ctx, "evict", [&]() -> int {
     if (int r = RequireDevice(ctx, "evict"); r != YAHKV_OK) return r;
     if (int r = CheckWeights(ctx, "evict", -1, n_seqs, seq_ids, weights_dev, weights_stride); r != YAHKV_OK) return r;
-    if (n_seqs > 0 && kept_dev == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "evict: null kept list");
+    if (n_seqs > 0 && (kept_dev == nullptr || (reinterpret_cast<std::uintptr_t>(kept_dev) & 3) != 0))
+      return Fail(ctx, YAHKV_ERR_INVALID, "evict: the kept list is null or not 4-byte aligned");
     if (n_keep < 1 || n_keep > static_cast<int64_t>(ctx->cfg.max_pages_per_seq) * kPageTokens || n_sink < 0 || n_recent < 0 ||
         n_sink > n_keep || n_recent > n_keep - n_sink)
       return Fail(ctx, YAHKV_ERR_INVALID, "evict: n_keep must be a slot count of at least 1, n_sink + n_recent at most n_keep");
