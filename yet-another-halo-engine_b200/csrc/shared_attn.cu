@@ -23,11 +23,16 @@
 // rounding of the output itself; exact products would need a second MMA per operand.
 //
 // What bounds it. fp16 pages: HBM as long as a group has at most 42 rows (a 64-key tile is 64 KB and takes the pair's
-// tensor pipes 1,024 clocks whatever the number of rows): 16 rows x 65536 in 47 us = 5.7 TB/s; with more rows a second
-// pair re-reads the pages from L2 and the tensor pipe bounds (96 rows x 32768: 0.75 us a tile at the 1.6 GHz the power
-// cap leaves, 70 % of the pipe over the whole kernel, 6 us of it prologue and epilogue). Quantized pages: a tile takes
-// 0.9 us for any number of rows, two thirds of it tensor time; with the conversion's stores left out it takes 0.79, with
-// its arithmetic left out no less, so what is left over fp16 is shared-memory traffic (32 KB written per tile and CTA).
+// tensor pipes 1,024 clocks whatever the number of rows): 16 rows x 65536 in 53 us with launch and drain = 5.1 TB/s; with
+// more rows a second pair re-reads the pages from L2 and the tensor pipe bounds (96 rows x 32768 in 75 us: 0.75 us a tile at
+// the 1.6 GHz the power cap leaves, 70 % of the pipe over the whole kernel, 6 us of it prologue and epilogue). Quantized
+// pages: a tile takes 0.9 us for any number of rows, two thirds of it tensor time (16 x 65536 of q4_0 57 us, 96 x 32768
+// 80); with the conversion's stores left out it takes 0.79, and eight more instructions per 16 bytes cost a tenth.
+//
+// Why pairs. Single CTAs of 128 rows double the bytes that an SM converts or fetches per tile, and the parts that the
+// combine joins. They are a little faster for groups of at most 21 rows, whose second CTA has no rows (21 x 262144 of
+// q8_0: 166 us against 204; 16 x 65536: 53 against 57, but the combine 14 against 10) and slower for all others (64 x
+// 32768 of q8_0: 75 us against 59, 42 x 65536 of fp16: 77 against 57).
 #include <cuda_fp16.h>
 
 #include <cmath>
