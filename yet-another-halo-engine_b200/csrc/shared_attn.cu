@@ -135,27 +135,52 @@ __device__ __forceinline__ void Nibs4ToHalf2(std::uint32_t n, std::uint32_t& h01
   const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
   h01 = *reinterpret_cast<const std::uint32_t*>(&x), h23 = *reinterpret_cast<const std::uint32_t*>(&y);
 }
-// 16-byte chunk c8 (dims 8 c8 .. + 7) of a token row. row: the row's codes; kFlipped: q8_0 bytes are code + 128 already.
-template <int kFmt, bool kFlipped, bool kLimit>
-__device__ __forceinline__ uint4 DequantChunk(uint2 codes, int c8, std::uint16_t scale) {
+// What a dequantizing thread takes of a row at a time, one load and one block scale: 16 dims = two chunks of 8, 16 bytes of
+// fp16 each. Item m of q8_0: 16 bytes of codes, chunks 2 m and 2 m + 1. Of q4_0: 8 bytes, whose low nibbles are chunk
+// 4 (m / 2) + m % 2 and whose high nibbles are two chunks further (elements 0-15 of a block are the low nibbles of its
+// 16 bytes). (A chunk at a time, with a load and a scale each: 67 us a call against 66 for 16 rows x 65536 of q4_0.)
+template <int kFmt>
+struct Item;
+template <>
+struct Item<kFmtQ8> {
+  using Codes = uint4;
+  static constexpr int kBytes = 16, kSecond = 1;   // of codes; chunks from the first to the second
+  static __device__ __forceinline__ int First(int m) { return 2 * m; }
+};
+template <>
+struct Item<kFmtQ4> {
+  using Codes = uint2;
+  static constexpr int kBytes = 8, kSecond = 2;
+  static __device__ __forceinline__ int First(int m) { return 4 * (m >> 1) + (m & 1); }
+};
+template <bool kFlipped, bool kLimit>   // kFlipped: the bytes are code + 128 already
+__device__ __forceinline__ void DequantItem(const uint4& codes, std::uint16_t scale, uint4 (&out)[2]) {
+  const std::uint32_t flip = kFlipped ? 0U : kQ8FlipWord;
   std::uint32_t h[4];
-  if constexpr (kFmt == kFmtQ8) {
-    const std::uint32_t flip = kFlipped ? 0U : kQ8FlipWord;
-    Bytes4ToHalf2(codes.x ^ flip, h[0], h[1]);
-    Bytes4ToHalf2(codes.y ^ flip, h[2], h[3]);
-  } else {   // elements 0-15 of a block are the low nibbles of its 16 bytes, 16-31 the high ones
-    const int sh = (c8 & 2) != 0 ? 4 : 0;
-    Nibs4ToHalf2((codes.x >> sh) & 0x0F0F0F0FU, h[0], h[1]);
-    Nibs4ToHalf2((codes.y >> sh) & 0x0F0F0F0FU, h[2], h[3]);
+  Bytes4ToHalf2(codes.x ^ flip, h[0], h[1]);
+  Bytes4ToHalf2(codes.y ^ flip, h[2], h[3]);
+  out[0] = ScaleCodes<kLimit>(h, scale);
+  Bytes4ToHalf2(codes.z ^ flip, h[0], h[1]);
+  Bytes4ToHalf2(codes.w ^ flip, h[2], h[3]);
+  out[1] = ScaleCodes<kLimit>(h, scale);
+}
+template <bool kFlipped, bool kLimit>
+__device__ __forceinline__ void DequantItem(const uint2& codes, std::uint16_t scale, uint4 (&out)[2]) {
+  std::uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    Nibs4ToHalf2((codes.x >> (4 * i)) & 0x0F0F0F0FU, h[0], h[1]);
+    Nibs4ToHalf2((codes.y >> (4 * i)) & 0x0F0F0F0FU, h[2], h[3]);
+    out[i] = ScaleCodes<kLimit>(h, scale);
   }
-  return ScaleCodes<kLimit>(h, scale);
 }
 
-// 8 bytes that are read once: past L1.
-__device__ __forceinline__ uint2 LoadStream8(const std::uint8_t* p) {
-  uint2 v;
+// Codes that are read once: past L1.
+__device__ __forceinline__ void LoadStream(const std::uint8_t* p, uint2& v) {
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+}
+__device__ __forceinline__ void LoadStream(const std::uint8_t* p, uint4& v) {
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
 }
 
 template <int kFmt>
@@ -350,20 +375,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
     }
   } else if (S::kQuant && warp >= kWarpDequant) {
     // ------------------------------ dequantizing warps: pages -> fp16 half tiles ------------------------------
-    // A chunk = 8 dims of a row = 16 B of fp16; lanes run along the row. A group holds the codes of its next tile in
-    // registers: they are loaded (past L1) as soon as the tile before has been converted, two tile periods ahead. Staging
-    // them in shared memory by TMA first cost 32 KB more of shared-memory traffic per tile and CTA: 60 us against 58 for 16
-    // rows x 65536 of q8_0, 85 against 82 for 96 rows x 32768.
+    // A group holds the codes of its next tile in registers: they are loaded (past L1) as soon as the tile before has been
+    // converted, two tile periods ahead. Staging them in shared memory by TMA first cost 32 KB more of shared-memory
+    // traffic per tile and CTA: 60 us against 58 for 16 rows x 65536 of q8_0, 85 against 82 for 96 rows x 32768.
     if constexpr (S::kQuant) {
-      const int group = (warp - kWarpDequant) / kDequantWarps;
-      const int t = threadIdx.x - 32 * (kWarpDequant + group * kDequantWarps);   // 0 .. 127
-      const int k8 = t & 31, k_key0 = t >> 5;                                    // K: 32 keys x 32 chunks, key = k_key0 + 4 i
-      const int vl = t & 15, v8 = static_cast<int>(rank) * 16 + vl, v_key0 = t >> 4;   // V: 64 keys x 16 chunks, key = v_key0 + 8 i
-      uint2 kw[8], vw[8];
-      std::uint16_t ksc[8], vsc[8];
-      // offset of a chunk's codes in its row: q8_0 8 bytes per chunk; q4_0 elements 8 (c & 1) .. of the low or high
-      // nibbles of block c / 4's 16 bytes
-      auto code_at = [](int c) { return kFmt == kFmtQ8 ? c * 8 : (c >> 2) * 16 + (c & 1) * 8; };
+      using It = Item<kFmt>;
+      const int group = (warp - kWarpDequant) / kDequantWarps, w = (warp - kWarpDequant) % kDequantWarps;
+      // Items of a thread: K 32 keys x 16 items, key k_key0 + 8 i; V 64 keys x 8 items (this CTA's half row), key
+      // v_key0 + 16 i. Eight lanes store four items of two keys at once: chunk c of a key lies at c ^ (key % 8), so the
+      // eight fall on different banks with neighbouring keys where an item's chunks are 0, 2, 4, 6 (q8_0), and with
+      // keys two apart where they are 0, 1, 4, 5 (q4_0).
+      const int kb = (lane >> 2) & 1;
+      const int k_key0 = kFmt == kFmtQ8 ? 2 * w + kb : 4 * (w >> 1) + (w & 1) + 2 * kb;   // 0 .. 7 over the group
+      const int v_key0 = k_key0 + 8 * (lane >> 4);
+      const int km = (lane & 3) | ((lane >> 3) << 2), vm = (lane & 3) | (((lane >> 3) & 1) << 2);
+      const int vm_row = static_cast<int>(rank) * 8 + vm;   // the item in its row
+      const int kc = It::First(km), vc = It::First(vm);
+      typename It::Codes kw[4], vw[4];
+      std::uint16_t ksc[4], vsc[4];
       auto row_of = [&](std::int32_t page) -> std::size_t {
         page = min(max(page, 0), pool.num_pages - 1);   // never trust a table entry read from memory
         return ((static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + tile.kvh) * kPageTokens;
@@ -371,23 +400,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
       auto fetch_k = [&](std::size_t row) {
         const std::size_t k_row = row + rank * (kTileN / 2) + k_key0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          kw[i] = LoadStream8(pool.kcodes + (k_row + 4 * i) * CodeBytes(kFmt) + code_at(k8));
-          ksc[i] = __ldg(pool.kscales + (k_row + 4 * i) * kBlocksPerRow + (k8 >> 2));
+        for (int i = 0; i < 4; ++i) {
+          LoadStream(pool.kcodes + (k_row + 8 * i) * CodeBytes(kFmt) + km * It::kBytes, kw[i]);
+          ksc[i] = __ldg(pool.kscales + (k_row + 8 * i) * kBlocksPerRow + (km >> 1));
         }
       };
       auto fetch_v = [&](std::size_t row) {
         const std::size_t v_row = row + v_key0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          vw[i] = LoadStream8(pool.vcodes + (v_row + 8 * i) * CodeBytes(kFmt) + code_at(v8));
-          vsc[i] = __ldg(pool.vscales + (v_row + 8 * i) * kBlocksPerRow + (v8 >> 2));
+        for (int i = 0; i < 4; ++i) {
+          LoadStream(pool.vcodes + (v_row + 16 * i) * CodeBytes(kFmt) + vm_row * It::kBytes, vw[i]);
+          vsc[i] = __ldg(pool.vscales + (v_row + 16 * i) * kBlocksPerRow + (vm_row >> 1));
         }
       };
-      auto large = [](const std::uint16_t (&sc)[8]) {   // the same answer in the whole warp
-        std::uint32_t bits = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) bits |= sc[i];
+      auto large = [](const std::uint16_t (&sc)[4]) {   // the same answer in the whole warp
+        const std::uint32_t bits = static_cast<std::uint32_t>(sc[0]) | sc[1] | sc[2] | sc[3];
         return __any_sync(0xFFFFFFFFU, (bits & kLimitBits<kFmt>) == kLimitBits<kFmt>);
       };
       if (group < n_tiles) {
@@ -407,10 +434,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
         std::uint8_t* vd = smem + S::kSmemV + vs * kVHalfBytes;
         auto convert_k = [&](auto limit) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = k_key0 + 4 * i;
-            *reinterpret_cast<uint4*>(kd + (k8 >> 3) * kKBlockBytes + key * 128 + (((k8 & 7) ^ (key & 7)) << 4)) =
-                DequantChunk<kFmt, false, limit.value>(kw[i], k8, ksc[i]);
+          for (int i = 0; i < 4; ++i) {
+            const int key = k_key0 + 8 * i;
+            uint4 o[2];
+            DequantItem<false, limit.value>(kw[i], ksc[i], o);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int c = kc + x * It::kSecond;
+              *reinterpret_cast<uint4*>(kd + (c >> 3) * kKBlockBytes + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = o[x];
+            }
           }
         };
         if (large(ksc)) convert_k(std::true_type());
@@ -418,7 +450,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
         FenceProxyAsync();   // the tensor core reads the tiles through the async proxy
         __syncwarp();
         if (lane == 0) MbarArriveCluster(MapToCta(SmemAddr(&bars->k_full[ks]), 0));
-        if (t == 0) *const_cast<volatile int*>(&bars->converted[group]) = j + 1;
+        if (w == 0 && lane == 0) *const_cast<volatile int*>(&bars->converted[group]) = j + 1;
         const bool more = j + kDequantGroups < n_tiles;
         const std::size_t next_row = row_of(next_page);
         if (more) fetch_k(next_row);
@@ -427,10 +459,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<kFmt>::kThread
         if (!ok) break;
         auto convert_v = [&](auto limit) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = v_key0 + 8 * i;
-            *reinterpret_cast<uint4*>(vd + (vl >> 3) * kVBlockBytes + key * 128 + (((vl & 7) ^ (key & 7)) << 4)) =
-                DequantChunk<kFmt, true, limit.value>(vw[i], v8, vsc[i]);
+          for (int i = 0; i < 4; ++i) {
+            const int key = v_key0 + 16 * i;
+            uint4 o[2];
+            DequantItem<true, limit.value>(vw[i], vsc[i], o);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int c = vc + x * It::kSecond;
+              *reinterpret_cast<uint4*>(vd + (c >> 3) * kVBlockBytes + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = o[x];
+            }
           }
         };
         if (large(vsc)) convert_v(std::true_type());
