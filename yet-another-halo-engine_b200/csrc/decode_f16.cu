@@ -23,27 +23,34 @@
 namespace yahkv {
 namespace {
 
-constexpr int kStages = 3;
 constexpr int kKeyGroups = 4;
-constexpr int kPageSets = 2;
-constexpr int kWarps = kKeyGroups * kPageSets;
-constexpr int kThreads = kWarps * 32;
 constexpr int kBoxBytes = 64 * 128;                       // 64 token rows x 64 dims of fp16
 constexpr int kBoxesPerSide = kHeadDim * 2 / 128;         // 4
 constexpr int kSideBytes = kBoxesPerSide * kBoxBytes;     // 32768
 static_assert(kSideBytes == RecordCodeBytes(kFmtF16), "record size");
 constexpr int kStageBytes = 2 * kSideBytes;
-constexpr int kRingBytes = kStages * kStageBytes;
 constexpr int kQLanes = 24;
 constexpr int kQSteps = kHeadDim / 16;                    // k-steps of the score product
-constexpr int kQfragOff = kRingBytes;                     // [16 steps][24 lanes][2] u32
-constexpr int kBarOff = kQfragOff + kQSteps * kQLanes * 8;
-constexpr int kDoneOff = kBarOff + 8 * kStages;
-constexpr int kFillOff = kDoneOff + 4 * kStages;
-constexpr int kAbortOff = kFillOff + 4 * kStages;
-constexpr int kSmemBytes = (kAbortOff + 4 + 127) / 128 * 128;
-static_assert(kSmemBytes + 1024 <= 228 * 1024, "one CTA per SM");
-static_assert(kWarps * kDecodeMergeWarpFloats * 4 <= kRingBytes, "the merge scratch aliases the ring");
+// kBeside: units behind shared prefixes are many and short, so it is their fixed cost that counts: three CTAs per SM, each
+// of four warps on one page at a time, overlap it; the loads in flight per SM are as many. (96 rows x 16421 with
+// suffixes of up to 512 tokens: 69 us a call against 76 with the other form; the units alone 31 against 44 at two per row.)
+template <bool kBeside>
+struct Shape {
+  static constexpr int kStages = kBeside ? 1 : 3;
+  static constexpr int kPageSets = kBeside ? 1 : 2;
+  static constexpr int kCtas = kBeside ? 3 : 1;            // per SM
+  static constexpr int kWarps = kKeyGroups * kPageSets;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kRingBytes = kStages * kStageBytes;
+  static constexpr int kQfragOff = kRingBytes;             // [16 steps][24 lanes][2] u32
+  static constexpr int kBarOff = kQfragOff + kQSteps * kQLanes * 8;
+  static constexpr int kDoneOff = kBarOff + 8 * kStages;
+  static constexpr int kFillOff = kDoneOff + 4 * kStages;
+  static constexpr int kAbortOff = kFillOff + 4 * kStages;
+  static constexpr int kSmemBytes = (kAbortOff + 4 + 127) / 128 * 128;
+  static_assert(kCtas * (kSmemBytes + 1024) <= 228 * 1024, "shared memory of an SM");
+  static_assert(kWarps * kDecodeMergeWarpFloats * 4 <= kRingBytes, "the merge scratch aliases the ring");
+};
 constexpr float kLazyRescale = 4.0F;
 constexpr int kStatusSmemMisaligned = 2;
 
@@ -51,22 +58,24 @@ constexpr int kStatusSmemMisaligned = 2;
 // kernel launched just before computes; see ChainedKernelEntryBeside.
 // kScores: the scores are kept for the pass that accumulates attention weights (evict.cu).
 template <bool kQRaw, bool kBeside, bool kScores>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<kBeside>::kThreads, Shape<kBeside>::kCtas)
     F16DecodePartKernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                         PoolView pool, int layer, const std::int32_t* __restrict__ tables, int table_stride,
                         const DecodeUnit* __restrict__ units, const __half* __restrict__ q, const QueryRaw qraw,
                         float scale_log2,
                         float* __restrict__ partial_acc, float* __restrict__ partial_ml, float* __restrict__ scores, int* status) {
+  using Sh = Shape<kBeside>;
+  constexpr int kStages = Sh::kStages, kPageSets = Sh::kPageSets, kWarps = Sh::kWarps;
   if constexpr (kBeside)
     ChainedKernelEntryBeside();
   else
     ChainedKernelEntry();
   extern __shared__ __align__(1024) std::uint8_t smem[];
-  std::uint32_t* qfrag = reinterpret_cast<std::uint32_t*>(smem + kQfragOff);
-  std::uint64_t* full_bar = reinterpret_cast<std::uint64_t*>(smem + kBarOff);
-  int* done_cnt = reinterpret_cast<int*>(smem + kDoneOff);
-  int* fill_cnt = reinterpret_cast<int*>(smem + kFillOff);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kAbortOff);
+  std::uint32_t* qfrag = reinterpret_cast<std::uint32_t*>(smem + Sh::kQfragOff);
+  std::uint64_t* full_bar = reinterpret_cast<std::uint64_t*>(smem + Sh::kBarOff);
+  int* done_cnt = reinterpret_cast<int*>(smem + Sh::kDoneOff);
+  int* fill_cnt = reinterpret_cast<int*>(smem + Sh::kFillOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Sh::kAbortOff);
   if ((SmemAddr(smem) & 1023U) != 0) {   // never seen; a misaligned swizzle would corrupt results
     if (threadIdx.x == 0) atomicExch(status, kStatusSmemMisaligned);
     if constexpr (kBeside) ChainedKernelExitBeside();
@@ -120,16 +129,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kStages && i < n_pages; ++i) issue(i, __ldg(row + i));
   }
 
-  // Query operands: warp h < 6 lays out head h. For k-step ks (dims 16 ks .. 16 ks + 15) the A registers of lane
+  // Query operands: a warp lays out head h. For k-step ks (dims 16 ks .. 16 ks + 15) the A registers of lane
   // (g = head, t) are a0 = dims 16 ks + 2t, + 1 and a2 = dims 16 ks + 8 + 2t, + 1 (rows 8-15 of the MMA stay zero).
   // Lane l of the warp holds dims 8 l .. 8 l + 7 = step l / 2, half l % 2: its four dword pairs go to t = 0 .. 3.
-  if (warp < kGroup) {
-    const uint4 raw = LoadQueryLane8<kQRaw>(q, qraw, static_cast<std::size_t>(u.batch) * kQHeads + u.kvh * kGroup + warp,
+  for (int h = warp; h < kGroup; h += kWarps) {
+    const uint4 raw = LoadQueryLane8<kQRaw>(q, qraw, static_cast<std::size_t>(u.batch) * kQHeads + u.kvh * kGroup + h,
                                             u.n_keys - 1, lane);
     const std::uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
     const int ks = lane >> 1, half = lane & 1;
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt) qfrag[((ks * kQLanes + warp * 4 + tt) << 1) + half] = w[tt];
+    for (int tt = 0; tt < 4; ++tt) qfrag[((ks * kQLanes + h * 4 + tt) << 1) + half] = w[tt];
   }
   __syncthreads();   // barriers initialised, query operands visible
   const int qlane = lane < kQLanes ? lane : lane - 8;   // the two padding rows of the MMA reuse heads 4, 5
@@ -249,28 +258,36 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 }  // namespace
 
+template <bool kQRaw, bool kBeside, bool kScores>
+static cudaError_t ConfigureOne() {
+  return cudaFuncSetAttribute(F16DecodePartKernel<kQRaw, kBeside, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Shape<kBeside>::kSmemBytes);
+}
 cudaError_t ConfigureF16Kernels() {
-  for (auto kernel : {F16DecodePartKernel<false, false, false>, F16DecodePartKernel<true, false, false>,
-                      F16DecodePartKernel<false, true, false>, F16DecodePartKernel<false, false, true>})
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes); e != cudaSuccess) return e;
+  for (auto configure : {ConfigureOne<false, false, false>, ConfigureOne<true, false, false>, ConfigureOne<false, true, false>,
+                         ConfigureOne<false, false, true>})
+    if (cudaError_t e = configure(); e != cudaSuccess) return e;
   return cudaSuccess;
 }
 
+template <bool kQRaw, bool kBeside, bool kScores>
+static cudaError_t LaunchOne(const DecodeLaunch& a, const __half* q, const QueryRaw& qr, cudaStream_t stream) {
+  return LaunchChained(F16DecodePartKernel<kQRaw, kBeside, kScores>, a.n_units, Shape<kBeside>::kThreads, Shape<kBeside>::kSmemBytes,
+                       stream, *a.kmap, *a.vmap, a.pool, a.layer, a.tables_dev, a.table_stride, a.units_dev, q, qr, a.scale_log2,
+                       a.partial_acc, a.partial_ml, a.scores_dev, a.status_dev);
+}
 cudaError_t LaunchF16DecodePart(const DecodeLaunch& a, cudaStream_t stream) {
   if (a.n_units <= 0 || a.n_seqs <= 0) return cudaSuccess;
+  if (a.beside && a.scores_dev != nullptr) return cudaErrorInvalidValue;
   if (a.q_raw) {
     if (a.beside || a.scores_dev != nullptr) return cudaErrorInvalidValue;
     const QueryRaw qr{static_cast<const float*>(a.q_dev), a.q_weight_dev, a.rope_tab_dev, a.q_eps, a.rope_rows};
-    return LaunchChained(F16DecodePartKernel<true, false, false>, a.n_units, kThreads, kSmemBytes, stream, *a.kmap, *a.vmap, a.pool,
-                         a.layer, a.tables_dev, a.table_stride, a.units_dev, static_cast<const __half*>(nullptr), qr,
-                         a.scale_log2, a.partial_acc, a.partial_ml, a.scores_dev, a.status_dev);
+    return LaunchOne<true, false, false>(a, nullptr, qr, stream);
   }
-  if (a.beside && a.scores_dev != nullptr) return cudaErrorInvalidValue;
-  const auto kernel = a.beside                  ? F16DecodePartKernel<false, true, false>
-                      : a.scores_dev != nullptr ? F16DecodePartKernel<false, false, true>
-                                                : F16DecodePartKernel<false, false, false>;
-  return LaunchChained(kernel, a.n_units, kThreads, kSmemBytes, stream, *a.kmap, *a.vmap, a.pool, a.layer, a.tables_dev, a.table_stride,
-                       a.units_dev, static_cast<const __half*>(a.q_dev), QueryRaw{}, a.scale_log2, a.partial_acc, a.partial_ml, a.scores_dev, a.status_dev);
+  const __half* q = static_cast<const __half*>(a.q_dev);
+  if (a.beside) return LaunchOne<false, true, false>(a, q, QueryRaw{}, stream);
+  if (a.scores_dev != nullptr) return LaunchOne<false, false, true>(a, q, QueryRaw{}, stream);
+  return LaunchOne<false, false, false>(a, q, QueryRaw{}, stream);
 }
 
 }  // namespace yahkv

@@ -563,9 +563,9 @@ class KvHost {
   // long as the largest part. The suffix units run beside the prefix pass on the SMs it leaves free, and on all of them
   // once it is done, so the wave need not be the whole device: for every wave size the suffixes' end is estimated from
   // the measured times of a pair (6 us and 0.75 us per fp16 page, 0.95 us where pages are dequantized) and of a unit
-  // (f16 one CTA per SM, 5 us and 0.9 us per page; q8_0 two, 4 and 0.9; q4_0 four, 4 and 1.6), and the cheapest pair of
+  // (f16 three CTAs per SM, 7 us and 2 us per page; q8_0 two, 4 and 0.9; q4_0 four, 4 and 1.6), and the cheapest pair of
   // sizes is taken. 96 rows x 16421 fp16, the same inputs again and again: 83 us with the whole device and units of two
-  // pages, 66 us as chosen here.
+  // pages, 66 us as chosen here, 60 with the units' present form.
   struct SharedShape {
     int part_pages = 1, unit_pages = 1;
   };
@@ -574,8 +574,8 @@ class KvHost {
     const int hc = kv_head_count();
     const bool f16 = cfg_.fmt == YAHKV_FMT_F16, q8 = cfg_.fmt == YAHKV_FMT_Q8_0;
     const double pair_fixed = 6.0, pair_page = f16 ? 0.75 : 0.95;
-    const double unit_fixed = f16 ? 5.0 : 4.0, unit_page = f16 || q8 ? 0.9 : 1.6;
-    const int ctas = f16 ? 1 : q8 ? 2 : 4;
+    const double unit_fixed = f16 ? 7.0 : 4.0, unit_page = f16 ? 2.0 : q8 ? 0.9 : 1.6;
+    const int ctas = f16 ? 3 : q8 ? 2 : 4;
     auto pairs_at = [&](int per) {
       long long n = 0;
       for (const PrefixGroup& g : groups) n += static_cast<long long>(g.n_mt) * hc * ((g.pages + per - 1) / per);
