@@ -228,6 +228,8 @@ def test_refusals_and_positions_after_an_eviction(tmp_path):
         aw(0, [a], q, out, w[0, :2])
     with pytest.raises(ValueError):
         aw(0, [a], q, out, w[0].double())
+    with pytest.raises(ValueError):
+        aw(0, [a], q, out, w[0].cpu())
     ev = cache.evict
     for n_keep, sink, recent in ((50, -1, 0), (50, 0, -1), (50, 51, 0), (50, 30, 21)):
         assert code(ev, [a], n_keep, w, kept, n_sink=sink, n_recent=recent) == yahkv.ERR_INVALID

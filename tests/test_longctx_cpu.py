@@ -117,3 +117,10 @@ def test_cpp_adapter_calls_on_a_host_only_context(tmp_path):
     assert r.returncode == 0, r.stderr[-3000:]
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "longctx_test: ok" in r.stdout, r.stdout + r.stderr
+
+
+def test_sequence_ids_of_any_kind():
+    for ids in ([3, 0, 7], (3, 0, 7), np.array([3, 0, 7]), np.array([3, 0, 7], np.int64), [3.0, 0.0, 7.0], np.array([[3], [0], [7]])):
+        keep, address, n = yahkv._ids(ids)
+        assert n == 3 and list(keep) == [3, 0, 7] and address == keep.buffer_info()[0]
+    assert yahkv._ids([])[1:] == (None, 0)

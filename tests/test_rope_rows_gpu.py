@@ -178,6 +178,16 @@ def test_refusals(cache):
     with pytest.raises(ValueError):
         rope.rows(x[:, :, :128], p, x)
     with pytest.raises(ValueError):
+        rope.rows(x, p.cpu(), x)
+    with pytest.raises(ValueError):
+        rope.rows(x.cpu(), p, x)
+    other = yahkv.KvCache(num_pages=1, max_seqs=1, max_pages_per_seq=1)
+    left = yahkv.Rope(other, max_positions=64)
+    other.close()                                   # out of order: nothing of the cache is touched any more
+    with pytest.raises(ValueError):
+        left.rows(x, p, x)
+    left.close()
+    with pytest.raises(ValueError):
         rope.rows(x, p.int(), x)
     with pytest.raises(ValueError):
         rope.rows(x, p, x.transpose(0, 1).contiguous().transpose(0, 1))

@@ -179,7 +179,7 @@ constexpr float kLazyRescale = 4.0F;
 // at the position of the sequence's newest key (qrope.cuh).
 // kBeside: the units lie behind prefixes that the kernel launched just before computes; see ChainedKernelEntryBeside.
 // kScores: the scores (log2 units, -inf behind the last key) are kept for the pass that accumulates attention weights
-// (evict.cu), [page slot][6 heads][64 keys], and the query has 20 bits in three planes (see kScorePlanes) where the other
+// (evict.cu), [page slot][6 heads][64 keys], and the query has 20 bits in three planes (see MmaQK3) where the other
 // variants have 16 in two: an accumulated weight is held in fp32, and 16 bits would leave it 2e-5 off.
 template <int kFmt, bool kQRaw, bool kBeside, bool kScores>
 __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)

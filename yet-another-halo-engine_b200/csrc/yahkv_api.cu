@@ -1143,6 +1143,7 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
 // ---- rotary positions on given rows ----------------------------------------------------------------------------
 struct yahkv_rope {
   yahkv_ctx* ctx = nullptr;
+  int device = 0;   // destroying it needs nothing else of the context
   yahkv_rope_config cfg{};
   float2 *hi = nullptr, *lo = nullptr;
 };
@@ -1188,7 +1189,7 @@ int yahkv_rope_create(yahkv_ctx* ctx, const yahkv_rope_config* cfg, yahkv_rope**
     std::vector<float2> tab(static_cast<std::size_t>(n_hi + low) * half);
     auto* r = new (std::nothrow) yahkv_rope();
     if (r == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "rope_create: out of host memory");
-    r->ctx = ctx, r->cfg = c;
+    r->ctx = ctx, r->device = ctx->cfg.device, r->cfg = c;
     for (std::int64_t i = 0; i < n_hi + low; ++i)
       for (int p = 0; p < half; ++p) {
         const double n = static_cast<double>(i < n_hi ? i * low : i - n_hi);
@@ -1211,7 +1212,7 @@ int yahkv_rope_create(yahkv_ctx* ctx, const yahkv_rope_config* cfg, yahkv_rope**
 
 void yahkv_rope_destroy(yahkv_rope* r) {
   if (r == nullptr) return;
-  cudaSetDevice(r->ctx->cfg.device);
+  cudaSetDevice(r->device);
   cudaFree(r->hi);
   delete r;
 }

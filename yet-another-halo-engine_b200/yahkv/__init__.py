@@ -241,7 +241,10 @@ def _i32(a):
 def _ids(seq_ids):
     """(int32 array to keep alive during the call, its address, its length): what a call costs on the host counts where
     the kernels take ten microseconds, and a numpy array's address alone costs four."""
-    a = array.array("i", seq_ids.tolist() if hasattr(seq_ids, "tolist") else seq_ids)
+    try:
+        a = array.array("i", seq_ids.tolist() if hasattr(seq_ids, "tolist") else seq_ids)
+    except (TypeError, OverflowError):   # anything else numpy makes int32 of
+        a = array.array("i", _i32(seq_ids).ravel().tolist())
     address, n = a.buffer_info()
     return a, address if n else None, n
 
@@ -363,7 +366,11 @@ class Rope:
     def rows(self, x, positions, out, weight=None, eps=0.0, stream=None):
         """x, out: CUDA tensors [tokens, heads, 256], fp16 or f32, heads and dims contiguous (tokens may be strided);
         positions: CUDA int64 [tokens]; weight: CUDA f32 [256] or None."""
+        if not self._h or not self.cache._h:
+            raise ValueError("rows: the rope or its cache is closed")
         n, heads, dim = x.shape
+        if not (x.is_cuda and out.is_cuda and positions.is_cuda and (weight is None or weight.is_cuda)):
+            raise ValueError("rows: tensors must be on the GPU")
         if out.shape != x.shape or dim != HEAD_DIM or positions.shape != (n,):
             raise ValueError("rows: x and out are [tokens, heads, 256], positions [tokens]")
         kinds, steps = [], []
@@ -494,11 +501,11 @@ class KvCache:
     def _weights(self, weights, dims):
         """Row pitch of the accumulators of attend_decode_weights / evict."""
         shape, stride = weights.shape, weights.stride()
-        if len(shape) != dims or weights.dtype.itemsize != 4 or not weights.dtype.is_floating_point or \
+        if len(shape) != dims or not weights.is_cuda or weights.dtype.itemsize != 4 or not weights.dtype.is_floating_point or \
                 shape[-3] != self.cfg.max_seqs or shape[-2] != KV_HEADS or \
                 stride[-1] != 1 or stride[-2] != shape[-1] or (shape[-3] > 1 and stride[-3] != KV_HEADS * shape[-1]) or \
                 (dims == 4 and shape[0] != self.cfg.n_layers):
-            raise ValueError("weights must be f32 [%smax_seqs, 4, keys], every layer contiguous" % ("n_layers, " if dims == 4 else ""))
+            raise ValueError("weights must be CUDA f32 [%smax_seqs, 4, keys], every layer contiguous" % ("n_layers, " if dims == 4 else ""))
         return shape[-1]
 
     def attend_decode_weights(self, layer, seq_ids, q, out, weights, gate=None, out_dtype=OUT_F16, n_splits=0, stream=None):
@@ -512,9 +519,9 @@ class KvCache:
         """Cuts every sequence to n_keep keys by weights (CUDA f32 [n_layers, max_seqs, 4, keys]); kept: CUDA int32
         [n_layers, n_seqs, 4, n_keep] receives the old slots."""
         keep, ids, n = _ids(seq_ids)
-        if kept.dtype.itemsize != 4 or kept.dtype.is_floating_point or not kept.is_contiguous() or \
+        if not kept.is_cuda or kept.dtype.itemsize != 4 or kept.dtype.is_floating_point or not kept.is_contiguous() or \
                 kept.shape != (self.cfg.n_layers, n, KV_HEADS, n_keep):
-            raise ValueError("kept must be contiguous int32 [n_layers, n_seqs, 4, n_keep]")
+            raise ValueError("kept must be contiguous CUDA int32 [n_layers, n_seqs, 4, n_keep]")
         stride = self._weights(weights, 4)
         self._check(lib.yahkv_evict(self._h, n, ids, n_keep, n_sink, n_recent, _adr(weights), stride, weights.stride(0), _adr(kept),
                                     _ptr(stream)))
