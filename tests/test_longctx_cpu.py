@@ -119,6 +119,29 @@ def test_cpp_adapter_calls_on_a_host_only_context(tmp_path):
     assert r.returncode == 0 and "longctx_test: ok" in r.stdout, r.stdout + r.stderr
 
 
+def test_tables_of_shared_pages_cannot_be_set_by_hand():
+    cache = yahkv.KvCache(device=-1, num_pages=8, max_seqs=3, max_pages_per_seq=8)
+    a = cache.seq_create()
+    cache.seq_reserve(a, 256)
+    cache.seq_set_len(a, 256)
+    table = cache.seq_table(a)
+    cache.seq_set_table(a, table[::-1].copy())                 # its own pages, in another order
+    cache.seq_set_table(a, table)
+    cache.seq_set_len(a, 256)
+    b = cache.seq_fork(a, 128)
+    for s, pages in ((a, table), (b, table[:2]), (b, table[2:3])):
+        with pytest.raises(yahkv.YahkvError) as e:
+            cache.seq_set_table(s, pages)
+        assert e.value.code == yahkv.ERR_INVALID
+    assert list(cache.seq_table(a)) == list(table) and list(cache.seq_table(b)) == list(table[:2])
+    cache.seq_set_table(a, table[2:])                          # what only it holds
+    assert cache.pages_free() == 4
+    cache.seq_set_table(b, table[:2])                          # alone in them now
+    cache.seq_free(b)
+    cache.seq_free(a)
+    assert cache.pages_free() == 8
+
+
 def test_sequence_ids_of_any_kind():
     for ids in ([3, 0, 7], (3, 0, 7), np.array([3, 0, 7]), np.array([3, 0, 7], np.int64), [3.0, 0.0, 7.0], np.array([[3], [0], [7]])):
         keep, address, n = yahkv._ids(ids)

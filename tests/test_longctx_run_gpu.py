@@ -10,7 +10,7 @@ import yahkv
 from gpu_util import dev
 from longctx_util import attend64, rows64, select
 from test_rope_rows_gpu import freqs, rotate64
-from test_shared_gpu import FMTS, check, grow, normal, shared, small_cache
+from test_shared_gpu import FMTS, check, extend, grow, normal, shared, small_cache
 
 pytestmark = pytest.mark.gpu
 EPS = 1e-6
@@ -245,3 +245,127 @@ def test_a_prompt_forked_decoded_cut_and_continued(fmt):
     assert cache.seq_len(watched, 0) == keep + 1
     q = rotate(rng.standard_normal((3, 24, 256)).astype(np.float32), [base + n] * 3).cpu().numpy()
     check(cache, 0, rows, q, shared(cache, 0, rows, q))
+
+
+def test_contexts_on_their_own_streams_at_once():
+    """Three contexts, a stream each, calls queued in turn without waiting: the bits of the same calls made one at a time."""
+    rng = np.random.default_rng(83)
+    jobs = []
+    for fmt in FMTS:
+        cache, seqs = forked_batch(fmt, rng, layers=1)
+        n = len(seqs)
+        q = [dev(normal(rng, n, 24, 256)) for _ in range(6)]
+        x = dev(rng.standard_normal((40, 24, 256)).astype(np.float32))
+        jobs.append((cache, seqs, q, x, yahkv.Rope(cache, rotary_dim=128, max_positions=4096), dev(rng.integers(0, 4096, 40))))
+
+    def call(job, i, outs, stream=None):
+        cache, seqs, q, x, rope, pos = job
+        shared_out, plain_out, w, turned = outs
+        cache.attend_decode_shared(0, seqs, q[i], shared_out[i], out_dtype=yahkv.OUT_F32, stream=stream)
+        cache.attend_decode_weights(0, seqs, q[i], plain_out[i], w, out_dtype=yahkv.OUT_F32, stream=stream)
+        rope.rows(x, pos, turned[i], stream=stream)
+
+    def buffers(job):
+        n = len(job[1])
+        return (torch.zeros(6, n, 24, 256, device="cuda"), torch.zeros(6, n, 24, 256, device="cuda"),
+                torch.zeros(job[0].cfg.max_seqs, 4, 900, device="cuda"), torch.zeros(6, 40, 24, 256, device="cuda"))
+    alone = [buffers(j) for j in jobs]
+    torch.cuda.synchronize()
+    for job, outs in zip(jobs, alone):
+        for i in range(6):
+            call(job, i, outs)
+            job[0].sync()
+    together = [buffers(j) for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for i in range(6):
+        for job, outs, st in zip(jobs, together, streams):
+            call(job, i, outs, st.cuda_stream)
+    torch.cuda.synchronize()
+    for job, a, b in zip(jobs, alone, together):
+        job[0].sync()
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_evict_and_fork_in_a_loop_reuse_pages():
+    """Cut, forked, appended and freed again and again with no page to spare: what a sequence holds stays its own."""
+    rng = np.random.default_rng(89)
+    cache = small_cache(num_pages=13, fmt=yahkv.FMT_Q8_0, max_seqs=3, max_pages_per_seq=6)
+    a = cache.seq_create()
+    grow(cache, rng, a, 150)
+    w = torch.rand(1, 3, 4, 400, device="cuda")
+    for turn in range(12):
+        n = cache.seq_len(a)
+        b = cache.seq_fork(a, n - turn % 3)
+        grow(cache, rng, b, 90)
+        w.uniform_()
+        w0 = w.double().cpu().numpy()
+        before = {s: rows64(cache, 0, s, cache.seq_len(s)) for s in (a, b)}
+        kept = torch.empty(1, 2, 4, 100, device="cuda", dtype=torch.int32)
+        torch.cuda.synchronize()
+        cache.evict([b, a], 100, w, kept, n_sink=2, n_recent=5)
+        cache.sync()
+        for r, s in enumerate((b, a)):
+            assert cache.seq_len(s) == 100
+            now = rows64(cache, 0, s, 100)
+            for h in range(4):
+                want = select(w0[0, s, h], len(before[s][0]), 100, 2, 5)
+                assert kept[0, r, h].tolist() == want
+                for side in (0, 1):
+                    assert np.array_equal(now[side][:, h], before[s][side][want, h])
+        q = normal(rng, 2, 24, 256)
+        check(cache, 0, [a, b], q, shared(cache, 0, [a, b], q))
+        cache.seq_free(a)
+        a = b
+        grow(cache, rng, a, 50)
+    cache.seq_free(a)
+    assert cache.pages_free() == 13
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("sharded", [True, False])
+def test_forks_of_a_cut_sequence(fmt, sharded):
+    """Forks of a sequence that was cut: eager calls of a context of kv heads 1 and 2 (which makes no batches), and a
+    batch with a fixed number of units per row."""
+    rng = np.random.default_rng(97)
+    heads = slice(6, 18) if sharded else slice(0, 24)
+    cache = small_cache(num_pages=40, fmt=fmt, max_seqs=4, max_pages_per_seq=12, **(dict(kv_head_begin=1, kv_head_count=2) if sharded else {}))
+    root = cache.seq_create()
+    grow(cache, rng, root, 500)
+    kept = torch.full((1, 1, 4, 330), -7, device="cuda", dtype=torch.int32)
+    w = torch.rand(1, 4, 4, 500, device="cuda")
+    torch.cuda.synchronize()
+    cache.evict([root], 330, w, kept)
+    cache.sync()
+    assert (kept[0, 0, [1, 2]] >= 0).all() and (kept[0, 0, [0, 3]] == -7).all().item() == sharded   # other heads are left alone
+    seqs = [cache.seq_fork(root, 330) for _ in range(3)]
+    batch = None
+    if not sharded:
+        batch = yahkv.DecodeBatch(cache, seqs)
+        batch.set_splits(3)
+        batch.set_shared()
+        batch.prepare(4)
+    for _ in range(3):
+        k, v, q = normal(rng, 3, 4, 256), normal(rng, 3, 4, 256), normal(rng, 3, 24, 256)
+        out = torch.full((3, 24, 256), float("nan"), device="cuda")
+        if sharded:
+            for i, s in enumerate(seqs):
+                extend(cache, 0, s, k[i:i + 1], v[i:i + 1])
+            got = shared(cache, 0, seqs, q, n_splits=3)
+            assert np.isnan(got[:, :6]).all() and np.isnan(got[:, 18:]).all()
+        else:
+            batch.plan()
+            torch.cuda.synchronize()
+            batch.decode_layer(0, dev(k), dev(v), dev(q), out, out_dtype=yahkv.OUT_F32)
+            batch.advance()
+            batch.commit(1)
+            cache.sync()
+            got = out.double().cpu().numpy()
+        check(cache, 0, seqs, q, got, heads=heads)
+    if batch is not None:
+        with pytest.raises(yahkv.YahkvError) as e:      # positions are not slots
+            x = [torch.zeros(3, h, 256, device="cuda") for h in (24, 4, 4)]
+            one = torch.ones(256, device="cuda")
+            batch.decode_layer_raw(0, *x, one, one, EPS, torch.zeros(3, 24, 256, device="cuda"))
+        assert e.value.code == yahkv.ERR_ORDER
+        batch.close()
