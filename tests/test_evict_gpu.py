@@ -272,7 +272,14 @@ def test_refusals_and_positions_after_an_eviction(tmp_path):
     batch.prepare(2)
     batch.plan()
     assert code(batch.decode_layer_raw, 0, *f32, ones, ones, 1e-6, out, out_dtype=yahkv.OUT_F32) == yahkv.ERR_ORDER
+    # a batch's lengths are on the device: its sequences are not cut under it
+    few = torch.empty(2, 1, 4, 20, device="cuda", dtype=torch.int32)
+    n = cache.seq_len(a, 0)
+    second = yahkv.DecodeBatch(cache, [a])
+    assert n > 20 and code(ev, [a], 20, w, few) == yahkv.ERR_ORDER
     batch.close()
+    assert code(ev, [a], 20, w, few) == yahkv.ERR_ORDER and cache.seq_len(a, 0) == n
+    second.close()
     # a snapshot keeps the mark
     cache.snapshot_save([b], tmp_path / "plain")
     cache.snapshot_save([a, b], tmp_path / "marked")

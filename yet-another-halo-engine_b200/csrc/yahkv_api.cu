@@ -165,6 +165,7 @@ struct yahkv_ctx {
   float* scores_dev = nullptr;
   std::int64_t score_pages = 0;
   // eviction work lists, allocated by the first call
+  std::vector<int> batch_uses;   // per sequence: live batches that hold it (their device-side lengths and tables)
   char* evict_dev = nullptr;
   std::vector<EvictSeq> evict_scratch;
   std::vector<std::int32_t> evict_page_scratch;
@@ -1107,6 +1108,9 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
       return Fail(ctx, YAHKV_ERR_INVALID, "evict: n_keep must be a slot count of at least 1, n_sink + n_recent at most n_keep");
     if (ctx->cfg.n_layers > 1 && weights_layer_stride < static_cast<int64_t>(ctx->cfg.max_seqs) * kKvHeads * weights_stride)
       return Fail(ctx, YAHKV_ERR_INVALID, "evict: the layers of the weights overlap (weights_layer_stride below max_seqs * 4 * weights_stride)");
+    for (int i = 0; i < n_seqs && !ctx->batch_uses.empty(); ++i)
+      if (ctx->batch_uses[static_cast<std::size_t>(seq_ids[i])] > 0)
+        return Fail(ctx, YAHKV_ERR_ORDER, "evict: sequence " + std::to_string(seq_ids[i]) + " is in a decode batch (destroy the batch first)");
     if (int r = RefuseCapture(ctx, "evict: host tables change", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
     bool any = false;
     HostError e = ctx->host.PlanEvict(n_seqs, seq_ids, n_keep, &ctx->evict_scratch, &ctx->evict_page_scratch, &any);
@@ -1543,6 +1547,7 @@ struct yahkv_batch {
   int units_cap = 0;
   int n_splits = 0;      // units per (sequence, kv head) asked for with yahkv_batch_set_splits; 0 = automatic
   int unit_pages = 0;    // pages per unit of the prepared horizon (a parameter of the plan kernel)
+  bool counted = false;  // in the context's batch_uses
   // shared prefixes (yahkv_batch_set_shared): the prepared horizon's prefix tiles, row list and prefix items, one buffer
   bool shared = false;
   char* prefix_dev = nullptr;
@@ -1554,6 +1559,8 @@ struct yahkv_batch {
 namespace {
 constexpr int kBatchUnitPages = 24;   // the automatic planner's unit size on large batches (kv_host.hpp)
 void BatchFree(yahkv_batch* b) {
+  if (b->counted)
+    for (std::int32_t s : b->seqs) b->ctx->batch_uses[static_cast<std::size_t>(s)] -= 1;
   for (void* p : {static_cast<void*>(b->lens_dev), static_cast<void*>(b->rows_dev), static_cast<void*>(b->units_dev),
                   static_cast<void*>(b->items_dev), static_cast<void*>(b->slots_dev), static_cast<void*>(b->vwork_dev),
                   static_cast<void*>(b->state_rows_dev), static_cast<void*>(b->prefix_dev), b->q16_dev})
@@ -1598,6 +1605,9 @@ int yahkv_batch_create(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, y
     BatchFree(b);
     return FailCuda(ctx, "batch_create", e);
   }
+  ctx->batch_uses.resize(static_cast<std::size_t>(ctx->cfg.max_seqs), 0);
+  for (std::int32_t s : b->seqs) ctx->batch_uses[static_cast<std::size_t>(s)] += 1;
+  b->counted = true;
   *out = b;
   return YAHKV_OK;
 }
