@@ -443,7 +443,13 @@ __global__ void __launch_bounds__(Shape<kFmt>::kThreads, Shape<kFmt>::kCtas)
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-          if (key_pos0 + kt * 8 + j >= u.n_keys) sc[kt][j] = -INFINITY;
+          if (key_pos0 + kt * 8 + j >= u.n_keys) {
+            sc[kt][j] = -INFINITY;
+            // A row behind the last key may hold anything (a page's former owner, a cut sequence, a fork's source), and
+            // a weight of zero times a scale that is inf or no number is no number: every thread clears the V scales of
+            // the keys that it reads them of. No later page takes this stage.
+            *reinterpret_cast<uint4*>(const_cast<std::uint8_t*>(st) + L::kVsOff + (my_key0 + kt * 8 + j) * 16) = make_uint4(0, 0, 0, 0);
+          }
     }
     if constexpr (kScores) {
       if (lane < kQLanes) {

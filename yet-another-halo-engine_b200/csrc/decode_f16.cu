@@ -189,6 +189,14 @@ __global__ void __launch_bounds__(Shape<kBeside>::kThreads, Shape<kBeside>::kCta
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           if (key_pos0 + kt * 8 + j >= u.n_keys) sc[kt][j] = -INFINITY;
+      // A row behind the last key may hold anything (a page's former owner, a cut sequence, a fork's source), and a
+      // weight of zero times inf or no number is no number: the warp clears such rows of V among its own sixteen, 16 bytes
+      // per lane. No later page takes this stage.
+      std::uint8_t* v_rows = smem + s * kStageBytes + kSideBytes + (lane >> 3) * kBoxBytes + (lane & 7) * 16;
+#pragma unroll 1
+      for (int r = min(max(u.n_keys - (u.page_begin + i) * kPageTokens, kw * 16), kw * 16 + 16); r < kw * 16 + 16; ++r)
+        *reinterpret_cast<uint4*>(v_rows + r * 128) = make_uint4(0, 0, 0, 0);
+      __syncwarp();
     }
 
     if constexpr (kScores) {
