@@ -76,6 +76,9 @@ __global__ void __launch_bounds__(kDequantThreads)
   const std::size_t rec = (static_cast<std::size_t>(layer) * pool.num_pages + page) * kKvHeads + kvh;
   const std::size_t out_row0 = static_cast<std::size_t>(ps.kv_row0) + static_cast<std::size_t>(kvh) * ps.kv_rows +
                                static_cast<std::size_t>(p) * kPageTokens;
+  // Rows of V behind the last key become zero: the page may hold anything there, and the product of a weight of zero with
+  // inf or no number is no number. (Scores of such keys are replaced, so K may stay.)
+  const int v_end = ps.kv_len - p * kPageTokens;
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const std::uint8_t* codes = (side == 0 ? pool.kcodes : pool.vcodes) + rec * RecordCodeBytes(kFmt);
@@ -84,7 +87,7 @@ __global__ void __launch_bounds__(kDequantThreads)
     if constexpr (kFmt == kFmtF16) {   // fp16 pages: a gather of the rows as they are
       for (int gidx = threadIdx.x; gidx < kPageTokens * (kHeadDim / 8); gidx += kDequantThreads)
         *reinterpret_cast<uint4*>(out + static_cast<std::size_t>(gidx >> 5) * kHeadDim + (gidx & 31) * 8) =
-            *reinterpret_cast<const uint4*>(codes + static_cast<std::size_t>(gidx) * 16);
+            side == 1 && gidx >> 5 >= v_end ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(codes + static_cast<std::size_t>(gidx) * 16);
       continue;
     }
     // thread -> 8 consecutive elements of a token row; 64 tokens x 32 groups = 2048 groups, 8 per thread
@@ -112,6 +115,7 @@ __global__ void __launch_bounds__(kDequantThreads)
       __half2* oh = reinterpret_cast<__half2*>(&o);
 #pragma unroll
       for (int i = 0; i < 4; ++i) oh[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      if (side == 1 && tok >= v_end) o = make_uint4(0, 0, 0, 0);
       *reinterpret_cast<uint4*>(out + static_cast<std::size_t>(tok) * kHeadDim + grp * 8) = o;
     }
   }
