@@ -563,7 +563,8 @@ __global__ void __launch_bounds__(kDequantThreads)
 #pragma unroll
       for (int k = 0; k < kTileKeys; ++k)
         *reinterpret_cast<__half2*>(out + static_cast<std::size_t>(tl * kTileKeys + k) * kHeadDim + ch) =
-            __floats2half2_rn(val[0][k], val[1][k]);
+            tile * kTileKeys + k < ps.kv_len ? __floats2half2_rn(val[0][k], val[1][k])
+                                             : __floats2half2_rn(0.0F, 0.0F);   // behind the last key: as in DequantPagesKernel
     }
   }
 }

@@ -114,9 +114,11 @@ __global__ void __launch_bounds__(kHeadDim) Kv8AppendVKernel(PoolView pool, int 
   }
 #pragma unroll
   for (int j = 0; j < kTileKeys; ++j)
-    if (j >= wk.n_old && j < wk.n_keys)
+    if (j >= wk.n_keys)
+      v[j] = __ushort_as_half(0);   // a tile before this one, or the row's former sequence: inf there times a weight of zero is no number
+    else if (j >= wk.n_old)
       v[j] = v_in[(static_cast<std::size_t>(wk.src[j]) * kKvHeads + h) * kHeadDim + ch];
-  if (wk.write_buf >= 0) {   // the sequence's newest tile: its keys stay available in fp16 (stale columns are masked)
+  if (wk.write_buf >= 0) {   // the sequence's newest tile: its keys stay available in fp16 (the columns behind them are zero)
     uint4* dst = reinterpret_cast<uint4*>(open_pair + static_cast<std::size_t>(wk.write_buf) * kOpenTileHalfs + ch_off);
     dst[0] = *reinterpret_cast<const uint4*>(v);
     dst[1] = *reinterpret_cast<const uint4*>(v + 8);
@@ -612,7 +614,8 @@ __global__ void __launch_bounds__(kKv8DequantThreads)
 #pragma unroll
       for (int k = 0; k < kTileKeys; ++k)
         *reinterpret_cast<__half2*>(out + static_cast<std::size_t>(tl * kTileKeys + k) * kHeadDim + ch) =
-            __floats2half2_rn(val[0][k], val[1][k]);
+            tile * kTileKeys + k < ps.kv_len ? __floats2half2_rn(val[0][k], val[1][k])
+                                             : __floats2half2_rn(0.0F, 0.0F);   // behind the last key: as in DequantPagesKernel
     }
   }
 }
