@@ -492,9 +492,11 @@ class KvHost {
     int n_mt = 0;                     // CTA pairs of 256 (row, query head) pairs
   };
   // Which rows compute a prefix together. The rows' full pages form a tree (forks of forks branch where their tables
-  // differ); a group is all the rows below one node, with the pages down to it, and saves (rows - 1) x pages page reads.
-  // From the root down, a node's rows are one group where that saves more than the best groups below it do, so that a
-  // short row does not cut the prefix of the long ones. Savings below shared_min_saved_ pages are left to the ordinary
+  // differ); a group is rows below one node, with the pages down to it, and saves (rows - 1) x pages page reads. Every
+  // row is in at most one group. A node's rows are one group, or groups further down with the rows that are in none of
+  // those as a group of their own, whichever saves most in all: a short row does not cut the prefix of the long ones, and
+  // a few long rows do not take the common prefix from the others.
+  // Savings below shared_min_saved_ pages are left to the ordinary
   // units: the pass costs two launches' time and its pairs work on half-empty tiles (measured, us per call with / without
   // the pass: 2 rows x 4096 tokens fp16 12.6 / 11.1, q8_0 13.8 / 13.9; 4 x 4096 13.5 / 18.8 and 14.5 / 15.5; 8 x 256 9.4 /
   // 11.8 and 10.0 / 10.5; 32 x 256 13.0 / 27.4 and 14.4 / 21.9; 32 x 16384 28 / 196 and 33 / 158).
@@ -503,54 +505,19 @@ class KvHost {
     std::vector<std::int32_t> rows;
     for (int b = 0; b < n_seqs; ++b)
       if (lens[b] >= kPageTokens) rows.push_back(b);
-    // rows with a common first page, in the order of their first row
-    std::stable_sort(rows.begin(), rows.end(), [&](std::int32_t x, std::int32_t y) { return table_row(seq_ids[x])[0] < table_row(seq_ids[y])[0]; });
-    for (std::size_t i = 0; i < rows.size();) {
-      std::size_t j = i;
-      while (j < rows.size() && table_row(seq_ids[rows[j]])[0] == table_row(seq_ids[rows[i]])[0]) ++j;
-      std::vector<PrefixGroup> found;
-      BestPrefixes(std::vector<std::int32_t>(rows.begin() + static_cast<std::ptrdiff_t>(i), rows.begin() + static_cast<std::ptrdiff_t>(j)), 0, seq_ids, lens, &found);
-      for (PrefixGroup& g : found) groups.push_back(std::move(g));
-      i = j;
-    }
+    std::vector<PrefixNode> tree;
+    ForEachBranch(rows, 0, seq_ids, [&](std::vector<std::int32_t>& together) {
+      if (together.size() < 2) return;
+      tree.clear();
+      BuildPrefixTree(together, 0, seq_ids, lens, &tree);
+      std::vector<int> above{0};
+      SolvePrefixes(&tree, 0, &above);
+      std::vector<std::int32_t> alone;
+      EmitPrefixes(tree, 0, 0, &alone, &groups);
+    });
     for (PrefixGroup& g : groups)
       g.n_mt = (static_cast<int>(g.rows.size()) * kGroup + 2 * kPrefillTileRows - 1) / (2 * kPrefillTileRows);
     return groups;
-  }
-  // The best groups among rows that agree in their first `from` pages; returns the pages they save.
-  std::int64_t BestPrefixes(const std::vector<std::int32_t>& rows, int from, const std::int32_t* seq_ids, const std::int64_t* lens,
-                            std::vector<PrefixGroup>* out) const {
-    if (rows.size() < 2) return 0;
-    int common = static_cast<int>(lens[rows[0]] / kPageTokens);
-    for (std::size_t i = 1; i < rows.size(); ++i) {
-      const std::int32_t *x = table_row(seq_ids[rows[0]]), *y = table_row(seq_ids[rows[i]]);
-      common = std::min(common, static_cast<int>(lens[rows[i]] / kPageTokens));
-      int same = std::min(from, common);
-      while (same < common && x[same] == y[same]) ++same;
-      common = same;
-    }
-    const std::int64_t whole = static_cast<std::int64_t>(rows.size() - 1) * common;
-    // what the branches behind the common pages save by themselves; rows that end there are in none of them
-    std::vector<std::pair<std::int32_t, std::vector<std::int32_t>>> branches;
-    for (std::int32_t b : rows) {
-      if (lens[b] / kPageTokens <= common) continue;
-      const std::int32_t next = table_row(seq_ids[b])[common];
-      auto it = std::find_if(branches.begin(), branches.end(), [&](const auto& e) { return e.first == next; });
-      if (it == branches.end()) it = branches.insert(branches.end(), {next, {}});
-      it->second.push_back(b);
-    }
-    std::vector<PrefixGroup> below;
-    std::int64_t saved = 0;
-    for (const auto& e : branches)
-      if (e.second.size() < rows.size()) saved += BestPrefixes(e.second, common, seq_ids, lens, &below);
-    if (whole >= saved && whole >= shared_min_saved_) {
-      PrefixGroup g;
-      g.rows = rows, g.pages = common;
-      out->push_back(std::move(g));
-      return whole;
-    }
-    for (PrefixGroup& g : below) out->push_back(std::move(g));
-    return saved;
   }
   void SetSharedMinSaved(int pages) {
     shared_min_saved_ = pages;
@@ -850,6 +817,112 @@ class KvHost {
   }
 
  private:
+  // ---- the tree of shared prefixes (FindPrefixes) ----
+  // Rows that agree in their first `pages` pages. What is best below a node depends on the nearest group above it, which
+  // its rows may join instead: with D pages in that group (0: there is none) a row that joins it counts D. Entry k of the
+  // three lists is for the k-th of the possible groups above, from none to the parent.
+  struct PrefixNode {
+    int pages = 0, count = 0;             // the agreed pages; rows at and below the node
+    std::vector<std::int32_t> rows;       // rows that end here or go on alone
+    std::vector<int> children;
+    enum Choice : char { kJoin, kWhole, kSplit };
+    std::vector<std::int64_t> value;      // page reads saved below, plus D for every row that joins the group above
+    std::vector<int> up;                  // rows that join it
+    std::vector<Choice> choice;           // no group here; all rows one group; a group of the rows that are in none below
+  };
+  // Calls fn with the rows that have the same page `at`, page by page.
+  template <class F>
+  void ForEachBranch(const std::vector<std::int32_t>& rows, int at, const std::int32_t* seq_ids, F&& fn) const {
+    std::vector<std::pair<std::int32_t, std::int32_t>> by_page;   // (page, row)
+    by_page.reserve(rows.size());
+    for (std::int32_t b : rows) by_page.emplace_back(table_row(seq_ids[b])[at], b);
+    std::sort(by_page.begin(), by_page.end());
+    std::vector<std::int32_t> branch;
+    for (std::size_t i = 0; i < by_page.size();) {
+      branch.clear();
+      const std::int32_t page = by_page[i].first;
+      for (; i < by_page.size() && by_page[i].first == page; ++i) branch.push_back(by_page[i].second);
+      fn(branch);
+    }
+  }
+  // The node of two rows or more that agree in their first `from` pages; its children behind it. Returns its index.
+  int BuildPrefixTree(const std::vector<std::int32_t>& rows, int from, const std::int32_t* seq_ids, const std::int64_t* lens,
+                      std::vector<PrefixNode>* tree) const {
+    const std::int32_t* first = table_row(seq_ids[rows[0]]);
+    int common = static_cast<int>(lens[rows[0]] / kPageTokens);
+    for (std::size_t i = 1; i < rows.size(); ++i) {
+      common = std::min(common, static_cast<int>(lens[rows[i]] / kPageTokens));
+      const int known = std::min(from, common);
+      common = static_cast<int>(std::mismatch(first + known, first + common, table_row(seq_ids[rows[i]]) + known).first - first);
+    }
+    const int at = static_cast<int>(tree->size());
+    tree->emplace_back();
+    (*tree)[static_cast<std::size_t>(at)].pages = common;
+    (*tree)[static_cast<std::size_t>(at)].count = static_cast<int>(rows.size());
+    std::vector<std::int32_t> longer;
+    for (std::int32_t b : rows)
+      if (lens[b] / kPageTokens <= common) (*tree)[static_cast<std::size_t>(at)].rows.push_back(b);
+      else longer.push_back(b);
+    ForEachBranch(longer, common, seq_ids, [&](const std::vector<std::int32_t>& branch) {
+      if (branch.size() == 1) {
+        (*tree)[static_cast<std::size_t>(at)].rows.push_back(branch[0]);
+      } else {
+        const int child = BuildPrefixTree(branch, common, seq_ids, lens, tree);
+        (*tree)[static_cast<std::size_t>(at)].children.push_back(child);
+      }
+    });
+    return at;
+  }
+  // Fills value, up and choice of a node and of what is below it; above: the pages of the groups that may lie above.
+  void SolvePrefixes(std::vector<PrefixNode>* tree, int at, std::vector<int>* above) const {
+    PrefixNode& v = (*tree)[static_cast<std::size_t>(at)];
+    above->push_back(v.pages);
+    for (int c : v.children) SolvePrefixes(tree, c, above);
+    above->pop_back();
+    const std::size_t self = above->size();
+    const std::int64_t own = static_cast<std::int64_t>(v.rows.size());
+    std::int64_t split = v.pages * (own - 1);
+    int left = static_cast<int>(own);
+    for (int c : v.children) split += (*tree)[static_cast<std::size_t>(c)].value[self], left += (*tree)[static_cast<std::size_t>(c)].up[self];
+    const std::int64_t whole = static_cast<std::int64_t>(v.pages) * (v.count - 1);
+    const bool may_whole = whole >= shared_min_saved_;
+    // beside groups below, a group must be worth its own tiles
+    const std::int64_t rest = static_cast<std::int64_t>(v.pages) * (left - 1);
+    const bool may_split = left >= 2 && left < v.count && rest >= std::max(shared_min_saved_, kSharedMinSaved);
+    v.value.resize(self), v.up.resize(self), v.choice.resize(self);
+    for (std::size_t k = 0; k < self; ++k) {
+      v.value[k] = (*above)[k] * own, v.up[k] = static_cast<int>(own), v.choice[k] = PrefixNode::kJoin;
+      for (int c : v.children) v.value[k] += (*tree)[static_cast<std::size_t>(c)].value[k], v.up[k] += (*tree)[static_cast<std::size_t>(c)].up[k];
+      if (may_whole && (whole > v.value[k] || (k == 0 && whole == v.value[k]))) v.value[k] = whole, v.up[k] = 0, v.choice[k] = PrefixNode::kWhole;
+      if (may_split && split > v.value[k]) v.value[k] = split, v.up[k] = 0, v.choice[k] = PrefixNode::kSplit;
+    }
+  }
+  void RowsBelow(const std::vector<PrefixNode>& tree, int at, std::vector<std::int32_t>* rows) const {
+    const PrefixNode& v = tree[static_cast<std::size_t>(at)];
+    rows->insert(rows->end(), v.rows.begin(), v.rows.end());
+    for (int c : v.children) RowsBelow(tree, c, rows);
+  }
+  // The groups that were chosen at and below a node, given the k-th possible group above; `up` receives the rows that join it.
+  void EmitPrefixes(const std::vector<PrefixNode>& tree, int at, std::size_t k, std::vector<std::int32_t>* up,
+                    std::vector<PrefixGroup>* groups, std::size_t depth = 1) const {
+    const PrefixNode& v = tree[static_cast<std::size_t>(at)];
+    if (v.choice[k] == PrefixNode::kJoin) {
+      up->insert(up->end(), v.rows.begin(), v.rows.end());
+      for (int c : v.children) EmitPrefixes(tree, c, k, up, groups, depth + 1);
+      return;
+    }
+    PrefixGroup g;
+    g.pages = v.pages;
+    if (v.choice[k] == PrefixNode::kWhole) {
+      RowsBelow(tree, at, &g.rows);
+    } else {
+      g.rows = v.rows;
+      for (int c : v.children) EmitPrefixes(tree, c, depth, &g.rows, groups, depth + 1);
+    }
+    std::sort(g.rows.begin(), g.rows.end());
+    groups->push_back(std::move(g));
+  }
+
   // Page boundaries of one sequence's split-K units over `pages` pages, into bounds_.
   void CutUnits(int pages, int n_splits, int max_splits, int auto_pages) {
     int per = n_splits > 0 ? (pages + n_splits - 1) / n_splits : auto_pages;
