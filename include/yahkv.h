@@ -368,6 +368,9 @@ int yahkv_sync(yahkv_ctx* ctx);
  *                       graph), so sequence lengths and later non-batch calls see them. At most the prepared horizon. */
 typedef struct yahkv_batch yahkv_batch;
 int yahkv_batch_create(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, yahkv_batch** out);
+/* Destroy a batch before its context or after it: once the context is gone every other call on the batch returns
+ * YAHKV_ERR_INVALID. batch_prepare and batch_commit refuse (YAHKV_ERR_ORDER) when a sequence of the batch was freed, also if
+ * its id has been given out again. */
 void yahkv_batch_destroy(yahkv_batch* batch);
 /* Split-K units per (sequence, kv head) for the batch's longest sequence, as n_splits of yahkv_attend_decode (0 =
  * automatic, the default); shorter sequences get units of the same page count. Takes effect at the next batch_prepare. */

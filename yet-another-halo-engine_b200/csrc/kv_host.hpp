@@ -35,6 +35,7 @@ class KvHost {
     dirty_hi_.assign(ns, 0);
     refs_.assign(static_cast<std::size_t>(cfg.num_pages), 0);
     evicted_.assign(ns, 0);
+    generation_.assign(ns, 0);
     // LIFO free list: page 0 is handed out first.
     free_pages_.reserve(static_cast<std::size_t>(cfg.num_pages));
     for (int p = cfg.num_pages - 1; p >= 0; --p) free_pages_.push_back(p);
@@ -77,6 +78,8 @@ class KvHost {
   int kv_head_count() const { return cfg_.kv_head_count == 0 ? kKvHeads : cfg_.kv_head_count; }
   int pages_free() const { return static_cast<int>(free_pages_.size()); }
   bool live(int seq) const { return seq >= 0 && seq < cfg_.max_seqs && live_[static_cast<std::size_t>(seq)] != 0; }
+  // Tells a sequence from the ones that had its id before.
+  std::uint32_t generation(int seq) const { return generation_[static_cast<std::size_t>(seq)]; }
   int n_pages(int seq) const { return n_pages_[static_cast<std::size_t>(seq)]; }
   const std::int32_t* table_row(int seq) const {
     return table_.data() + static_cast<std::size_t>(seq) * static_cast<std::size_t>(cfg_.max_pages_per_seq);
@@ -90,6 +93,7 @@ class KvHost {
     const int s = free_seqs_.back();
     free_seqs_.pop_back();
     live_[static_cast<std::size_t>(s)] = 1;
+    generation_[static_cast<std::size_t>(s)] += 1;
     n_pages_[static_cast<std::size_t>(s)] = 0;
     evicted_[static_cast<std::size_t>(s)] = 0;
     SetLenAll(s, 0);
@@ -994,6 +998,7 @@ class KvHost {
   std::vector<std::int64_t> len_;
   std::vector<int> dirty_lo_, dirty_hi_, dirty_list_;
   std::vector<int> refs_;       // sequences whose table names the page
+  std::vector<std::uint32_t> generation_;   // sequences created under the id so far
   std::vector<char> evicted_;   // per sequence: keys were evicted, slots are not positions
   std::int64_t table_epoch_ = 0;   // counts table changes: what a cached prefix grouping depends on
   std::vector<std::int32_t> free_pages_;

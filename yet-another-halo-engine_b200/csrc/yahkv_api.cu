@@ -164,8 +164,8 @@ struct yahkv_ctx {
   // scores of a weight-accumulating decode call, grown to the largest call seen
   float* scores_dev = nullptr;
   std::int64_t score_pages = 0;
+  std::vector<yahkv_batch*> batches;   // not destroyed yet
   // eviction work lists, allocated by the first call
-  std::vector<int> batch_uses;   // per sequence: live batches that hold it (their device-side lengths and tables)
   char* evict_dev = nullptr;
   std::vector<EvictSeq> evict_scratch;
   std::vector<std::int32_t> evict_page_scratch;
@@ -562,8 +562,10 @@ int yahkv_create(const yahkv_config* cfg, yahkv_ctx** out) {
   return YAHKV_OK;
 }
 
+static void OrphanBatches(yahkv_ctx* ctx);
 void yahkv_destroy(yahkv_ctx* ctx) {
   if (ctx == nullptr) return;
+  OrphanBatches(ctx);
   FreeDevice(ctx);
   delete ctx;
 }
@@ -1095,6 +1097,8 @@ int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, co
   });
 }
 
+static bool InBatch(const yahkv_ctx* ctx, int seq);
+
 // ---- eviction --------------------------------------------------------------------------------------------------
 int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t n_keep, int64_t n_sink, int64_t n_recent,
                 float* weights_dev, int64_t weights_stride, int64_t weights_layer_stride, int32_t* kept_dev, void* stream) {
@@ -1108,8 +1112,8 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
       return Fail(ctx, YAHKV_ERR_INVALID, "evict: n_keep must be a slot count of at least 1, n_sink + n_recent at most n_keep");
     if (ctx->cfg.n_layers > 1 && weights_layer_stride < static_cast<int64_t>(ctx->cfg.max_seqs) * kKvHeads * weights_stride)
       return Fail(ctx, YAHKV_ERR_INVALID, "evict: the layers of the weights overlap (weights_layer_stride below max_seqs * 4 * weights_stride)");
-    for (int i = 0; i < n_seqs && !ctx->batch_uses.empty(); ++i)
-      if (ctx->batch_uses[static_cast<std::size_t>(seq_ids[i])] > 0)
+    for (int i = 0; i < n_seqs; ++i)
+      if (InBatch(ctx, seq_ids[i]))
         return Fail(ctx, YAHKV_ERR_ORDER, "evict: sequence " + std::to_string(seq_ids[i]) + " is in a decode batch (destroy the batch first)");
     if (int r = RefuseCapture(ctx, "evict: host tables change", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
     bool any = false;
@@ -1531,8 +1535,10 @@ int yahkv_kernel_timing_read(yahkv_ctx* ctx, int32_t kernel, double* total_ms, i
 
 // ---- device-resident decode batches ------------------------------------------------------------------------
 struct yahkv_batch {
-  yahkv_ctx* ctx = nullptr;
+  yahkv_ctx* ctx = nullptr;             // null once the context is gone: nothing but destroying the batch is left
+  int device = 0;
   std::vector<std::int32_t> seqs;
+  std::vector<std::uint32_t> generations;   // of the sequences: an id may have been freed and given out again since
   std::vector<std::int32_t> lens;       // host mirror of lens_dev (committed steps only)
   std::vector<BatchSeq> rows;
   int total_units = 0;
@@ -1547,7 +1553,6 @@ struct yahkv_batch {
   int units_cap = 0;
   int n_splits = 0;      // units per (sequence, kv head) asked for with yahkv_batch_set_splits; 0 = automatic
   int unit_pages = 0;    // pages per unit of the prepared horizon (a parameter of the plan kernel)
-  bool counted = false;  // in the context's batch_uses
   // shared prefixes (yahkv_batch_set_shared): the prepared horizon's prefix tiles, row list and prefix items, one buffer
   bool shared = false;
   char* prefix_dev = nullptr;
@@ -1559,15 +1564,31 @@ struct yahkv_batch {
 namespace {
 constexpr int kBatchUnitPages = 24;   // the automatic planner's unit size on large batches (kv_host.hpp)
 void BatchFree(yahkv_batch* b) {
-  if (b->counted)
-    for (std::int32_t s : b->seqs) b->ctx->batch_uses[static_cast<std::size_t>(s)] -= 1;
+  if (b->ctx != nullptr) {
+    auto& all = b->ctx->batches;
+    all.erase(std::remove(all.begin(), all.end(), b), all.end());
+  }
   for (void* p : {static_cast<void*>(b->lens_dev), static_cast<void*>(b->rows_dev), static_cast<void*>(b->units_dev),
                   static_cast<void*>(b->items_dev), static_cast<void*>(b->slots_dev), static_cast<void*>(b->vwork_dev),
                   static_cast<void*>(b->state_rows_dev), static_cast<void*>(b->prefix_dev), b->q16_dev})
     if (p != nullptr) cudaFree(p);
   delete b;
 }
+// Row i of the batch is still the sequence that the batch was made with.
+bool SameSequence(const yahkv_batch* b, std::size_t i) {
+  return b->ctx->host.live(b->seqs[i]) && b->ctx->host.generation(b->seqs[i]) == b->generations[i];
+}
 }  // namespace
+static void OrphanBatches(yahkv_ctx* ctx) {
+  for (yahkv_batch* b : ctx->batches) b->ctx = nullptr;
+}
+// A batch that was not destroyed yet holds the sequence (its length and table rows on the device).
+static bool InBatch(const yahkv_ctx* ctx, int seq) {
+  for (const yahkv_batch* b : ctx->batches)
+    for (std::size_t i = 0; i < b->seqs.size(); ++i)
+      if (b->seqs[i] == seq && SameSequence(b, i)) return true;
+  return false;
+}
 
 int yahkv_batch_create(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, yahkv_batch** out) {
   if (int r = RequireDevice(ctx, "batch_create"); r != YAHKV_OK) return r;
@@ -1577,7 +1598,7 @@ int yahkv_batch_create(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, y
   if (ctx->host.kv_head_count() != kKvHeads) return Fail(ctx, YAHKV_ERR_INVALID, "batch_create: decode batches need a context that holds all four kv heads");
   auto* b = new (std::nothrow) yahkv_batch();
   if (b == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "batch_create: out of host memory");
-  b->ctx = ctx;
+  b->ctx = ctx, b->device = ctx->cfg.device;
   for (int i = 0; i < n_seqs; ++i) {
     const int s = seq_ids[i];
     if (!ctx->host.live(s)) {
@@ -1591,6 +1612,7 @@ int yahkv_batch_create(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, y
         return Fail(ctx, YAHKV_ERR_ORDER, "batch_create: sequence " + std::to_string(s) + " has different lengths in its layers");
       }
     b->seqs.push_back(s);
+    b->generations.push_back(ctx->host.generation(s));
     b->lens.push_back(static_cast<std::int32_t>(n));
   }
   b->units_cap = ctx->max_units;
@@ -1605,22 +1627,20 @@ int yahkv_batch_create(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, y
     BatchFree(b);
     return FailCuda(ctx, "batch_create", e);
   }
-  ctx->batch_uses.resize(static_cast<std::size_t>(ctx->cfg.max_seqs), 0);
-  for (std::int32_t s : b->seqs) ctx->batch_uses[static_cast<std::size_t>(s)] += 1;
-  b->counted = true;
+  ctx->batches.push_back(b);
   *out = b;
   return YAHKV_OK;
 }
 
 void yahkv_batch_destroy(yahkv_batch* b) {
   if (b == nullptr) return;
-  cudaSetDevice(b->ctx->cfg.device);
+  cudaSetDevice(b->device);
   cudaDeviceSynchronize();
   BatchFree(b);
 }
 
 int yahkv_batch_set_splits(yahkv_batch* b, int32_t n_splits) {
-  if (b == nullptr) return YAHKV_ERR_INVALID;
+  if (b == nullptr || b->ctx == nullptr) return YAHKV_ERR_INVALID;
   yahkv_ctx* ctx = b->ctx;
   if (n_splits < 0) return Fail(ctx, YAHKV_ERR_INVALID, "batch_set_splits: negative n_splits");
   if (n_splits > ctx->cfg.max_splits) return Fail(ctx, YAHKV_ERR_CAPACITY, "batch_set_splits: n_splits above max_splits");
@@ -1629,7 +1649,7 @@ int yahkv_batch_set_splits(yahkv_batch* b, int32_t n_splits) {
 }
 
 int yahkv_batch_set_shared(yahkv_batch* b, int32_t on) {
-  if (b == nullptr) return YAHKV_ERR_INVALID;
+  if (b == nullptr || b->ctx == nullptr) return YAHKV_ERR_INVALID;
   yahkv_ctx* ctx = b->ctx;
   if (int r = RequireDevice(ctx, "batch_set_shared"); r != YAHKV_OK) return r;
   if (on != 0 && IsTileFmt(ctx->cfg.fmt))
@@ -1647,7 +1667,7 @@ int yahkv_batch_set_shared(yahkv_batch* b, int32_t on) {
 
 static int BatchPrepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_changed, void* stream);
 int yahkv_batch_prepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_changed, void* stream) {
-  if (b == nullptr) return YAHKV_ERR_INVALID;
+  if (b == nullptr || b->ctx == nullptr) return YAHKV_ERR_INVALID;
   return NoThrow(b->ctx, "batch_prepare", [&] { return BatchPrepare(b, horizon_steps, layout_changed, stream); });
 }
 
@@ -1660,7 +1680,7 @@ static int BatchPrepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_c
   // are checked for the whole batch first, so a refusal changes nothing
   std::int64_t new_pages = 0;
   for (int i = 0; i < n; ++i) {
-    if (!ctx->host.live(b->seqs[i]) || ctx->host.len(b->seqs[i], 0) != b->lens[i])
+    if (!SameSequence(b, static_cast<std::size_t>(i)) || ctx->host.len(b->seqs[i], 0) != b->lens[i])
       return Fail(ctx, YAHKV_ERR_ORDER, "batch_prepare: a sequence of the batch was freed or changed outside the batch");
     if (const std::int32_t p = ctx->host.SharedPageIn(b->seqs[i], b->lens[i], static_cast<std::int64_t>(b->lens[i]) + horizon_steps); p >= 0)
       return Fail(ctx, YAHKV_ERR_INVALID, "batch_prepare: sequence " + std::to_string(b->seqs[i]) + " would append to page " +
@@ -1769,7 +1789,7 @@ static int BatchPrepare(yahkv_batch* b, int32_t horizon_steps, int32_t* layout_c
 }
 
 int yahkv_batch_plan(yahkv_batch* b, void* stream) {
-  if (b == nullptr) return YAHKV_ERR_INVALID;
+  if (b == nullptr || b->ctx == nullptr) return YAHKV_ERR_INVALID;
   yahkv_ctx* ctx = b->ctx;
   if (int r = RequireDevice(ctx, "batch_plan"); r != YAHKV_OK) return r;
   if (b->total_units == 0) return Fail(ctx, YAHKV_ERR_ORDER, "batch_plan: call batch_prepare first");
@@ -1798,7 +1818,7 @@ static int BatchAttendShared(yahkv_batch* b, DecodeLaunch& a, int launches_befor
 
 int yahkv_batch_decode_layer(yahkv_batch* b, int32_t layer, const void* k_dev, const void* v_dev, const void* q_dev,
                              const float* gate_dev, void* out_dev, int32_t out_dtype, void* stream) {
-  if (b == nullptr) return YAHKV_ERR_INVALID;
+  if (b == nullptr || b->ctx == nullptr) return YAHKV_ERR_INVALID;
   yahkv_ctx* ctx = b->ctx;
   if (int r = RequireDevice(ctx, "batch_decode_layer"); r != YAHKV_OK) return r;
   if (layer < 0 || layer >= ctx->cfg.n_layers) return Fail(ctx, YAHKV_ERR_INVALID, "batch_decode_layer: layer out of range");
@@ -1839,7 +1859,7 @@ int yahkv_batch_decode_layer(yahkv_batch* b, int32_t layer, const void* k_dev, c
 int yahkv_batch_decode_layer_raw(yahkv_batch* b, int32_t layer, const float* q_dev, const float* k_dev, const float* v_dev,
                                  const float* q_weight_dev, const float* k_weight_dev, float eps, const float* gate_dev,
                                  void* out_dev, int32_t out_dtype, void* stream) {
-  if (b == nullptr) return YAHKV_ERR_INVALID;
+  if (b == nullptr || b->ctx == nullptr) return YAHKV_ERR_INVALID;
   yahkv_ctx* ctx = b->ctx;
   if (int r = RequireDevice(ctx, "batch_decode_layer_raw"); r != YAHKV_OK) return r;
   if (layer < 0 || layer >= ctx->cfg.n_layers) return Fail(ctx, YAHKV_ERR_INVALID, "batch_decode_layer_raw: layer out of range");
@@ -1897,7 +1917,7 @@ int yahkv_batch_decode_layer_raw(yahkv_batch* b, int32_t layer, const float* q_d
 }
 
 int yahkv_batch_advance(yahkv_batch* b, void* stream) {
-  if (b == nullptr) return YAHKV_ERR_INVALID;
+  if (b == nullptr || b->ctx == nullptr) return YAHKV_ERR_INVALID;
   yahkv_ctx* ctx = b->ctx;
   if (int r = RequireDevice(ctx, "batch_advance"); r != YAHKV_OK) return r;
   YAHKV_CUDA(ctx, LaunchBatchAdvance(b->lens_dev, static_cast<int>(b->seqs.size()), 1, StreamOf(ctx, stream)));
@@ -1906,9 +1926,11 @@ int yahkv_batch_advance(yahkv_batch* b, void* stream) {
 }
 
 int yahkv_batch_commit(yahkv_batch* b, int32_t steps) {
-  if (b == nullptr) return YAHKV_ERR_INVALID;
+  if (b == nullptr || b->ctx == nullptr) return YAHKV_ERR_INVALID;
   yahkv_ctx* ctx = b->ctx;
   if (steps < 0 || steps > b->horizon) return Fail(ctx, YAHKV_ERR_ORDER, "batch_commit: more steps than the prepared horizon");
+  for (std::size_t i = 0; i < b->seqs.size(); ++i)   // before any length changes
+    if (!SameSequence(b, i)) return Fail(ctx, YAHKV_ERR_ORDER, "batch_commit: a sequence of the batch was freed");
   for (std::size_t i = 0; i < b->seqs.size(); ++i) {
     HostError e = ctx->host.SeqSetLen(b->seqs[i], -1, static_cast<std::int64_t>(b->lens[i]) + steps);
     if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
