@@ -293,15 +293,26 @@ class DecodeBatch:
 
     def __init__(self, cache, seq_ids):
         self.cache = cache
-        seq_ids = _i32(seq_ids)
-        self.n = len(seq_ids)
         self._h = ctypes.c_void_p()
+        seq_ids = _i32(seq_ids)
+        self.n, self._ids = len(seq_ids), set(seq_ids.ravel().tolist())
         cache._check(lib.yahkv_batch_create(cache._h, self.n, _ptr(seq_ids), ctypes.byref(self._h)))
 
     def close(self):
         if self._h:
             lib.yahkv_batch_destroy(self._h)
             self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        # Dropped without close(): a captured graph may still use its device memory, so that stays until a sequence of the
+        # batch is cut or the cache is closed.
+        try:
+            if self._h and self.cache._h:
+                self.cache._dropped.append((self._h, self._ids))
+            else:
+                self.close()
+        except Exception:
+            pass
 
     def prepare(self, horizon_steps, stream=None):
         """Returns True when the unit layout changed (a captured graph must then be captured again)."""
@@ -400,13 +411,22 @@ class KvCache:
                           max_pages_per_seq, max_splits, max_batch_tokens, softmax_scale, kv_head_begin, kv_head_count,
                           max_prefill_keys)
         self.fmt = fmt
+        self._dropped = []      # decode batches that were dropped without being closed: (handle, sequence ids)
         self._h = ctypes.c_void_p()
         rc = lib.yahkv_create(ctypes.byref(self.cfg), ctypes.byref(self._h))
         if rc != OK:
             raise YahkvError(rc, lib.yahkv_last_error(None).decode())
 
+    def _close_dropped(self, seq_ids=None):
+        """Closes the dropped batches that hold one of seq_ids (None: all)."""
+        held = [d for d in self._dropped if seq_ids is None or not d[1].isdisjoint(seq_ids)]
+        self._dropped = [d for d in self._dropped if d not in held]
+        for handle, _ in held:
+            lib.yahkv_batch_destroy(handle)
+
     def close(self):
         if self._h:
+            self._close_dropped()
             lib.yahkv_destroy(self._h)
             self._h = ctypes.c_void_p()
 
@@ -523,6 +543,8 @@ class KvCache:
                 kept.shape != (self.cfg.n_layers, n, KV_HEADS, n_keep):
             raise ValueError("kept must be contiguous CUDA int32 [n_layers, n_seqs, 4, n_keep]")
         stride = self._weights(weights, 4)
+        if self._dropped:
+            self._close_dropped(keep)
         self._check(lib.yahkv_evict(self._h, n, ids, n_keep, n_sink, n_recent, _adr(weights), stride, weights.stride(0), _adr(kept),
                                     _ptr(stream)))
 
