@@ -226,9 +226,10 @@ class KvHost {
   // Eviction of every listed sequence longer than n_keep (all layers equally long) down to n_keep slots: the pages it
   // will have. A page it holds alone is kept and overwritten; a page that another sequence holds too at the time of the
   // call is replaced by a free one, also when that other sequence is evicted by the same call and lets go of it.
-  // Changes nothing; CommitEvict with the same lists then moves the tables over.
+  // Changes no sequence; CommitEvict with the same lists then moves the tables over. The keys have been moved on the device
+  // by then, so it may not fail: what it needs room for is reserved here.
   HostError PlanEvict(int n_seqs, const std::int32_t* seq_ids, std::int64_t n_keep, std::vector<EvictSeq>* seqs,
-                      std::vector<std::int32_t>* dst_pages, bool* any) const {
+                      std::vector<std::int32_t>* dst_pages, bool* any) {
     seqs->clear();
     dst_pages->clear();
     *any = false;
@@ -258,21 +259,22 @@ class KvHost {
         dst_pages->push_back(page);
       }
     }
+    std::size_t held = 0;
+    for (const EvictSeq& e : *seqs) held += static_cast<std::size_t>(n_pages(e.seq));
+    evict_dropped_.clear();
+    evict_dropped_.reserve(held);
+    dirty_list_.reserve(dirty_list_.size() + seqs->size());
     return {};
   }
-  void CommitEvict(std::int64_t n_keep, const std::vector<EvictSeq>& seqs, const std::vector<std::int32_t>& dst_pages) {
+  void CommitEvict(std::int64_t n_keep, const std::vector<EvictSeq>& seqs, const std::vector<std::int32_t>& dst_pages) noexcept {
     const int np = static_cast<int>((n_keep + kPageTokens - 1) / kPageTokens);
-    std::vector<std::int32_t> dropped;
-    std::size_t held = 0;
-    for (const EvictSeq& e : seqs) held += static_cast<std::size_t>(n_pages(e.seq));
-    dropped.reserve(held);   // before anything changes
     for (const EvictSeq& e : seqs) {
       if (e.n_keys <= n_keep) continue;
       std::int32_t* row = mutable_row(e.seq);
       for (int i = 0; i < n_pages(e.seq); ++i) {
         const std::int32_t to = i < np ? dst_pages[static_cast<std::size_t>(e.first_dst + i)] : -1;
         if (to == row[i]) continue;
-        dropped.push_back(row[i]);
+        evict_dropped_.push_back(row[i]);
         if (to < 0) continue;
         free_pages_.pop_back();   // in PlanEvict's order
         refs_[static_cast<std::size_t>(to)] = 1;
@@ -283,7 +285,8 @@ class KvHost {
       SetEvicted(e.seq);
       MarkDirty(e.seq, 0, np);
     }
-    for (std::int32_t p : dropped) Unref(p);   // only now: a page let go of here was nobody's fresh page
+    for (std::int32_t p : evict_dropped_) Unref(p);   // only now: a page let go of here was nobody's fresh page
+    evict_dropped_.clear();
   }
   int page_refs(std::int32_t page) const { return refs_[static_cast<std::size_t>(page)]; }
   // Keys of the sequence have been evicted: its slots no longer count positions.
@@ -1001,7 +1004,8 @@ class KvHost {
   std::vector<std::uint32_t> generation_;   // sequences created under the id so far
   std::vector<char> evicted_;   // per sequence: keys were evicted, slots are not positions
   std::int64_t table_epoch_ = 0;   // counts table changes: what a cached prefix grouping depends on
-  std::vector<std::int32_t> free_pages_;
+  std::vector<std::int32_t> free_pages_;     // room for every page from the start: giving one back does not fail
+  std::vector<std::int32_t> evict_dropped_;
   std::vector<int> free_seqs_;
   std::vector<std::pair<int, std::int64_t>> scratch_len_;
   std::vector<std::int64_t> key_scratch_, plan_key_;
