@@ -51,7 +51,7 @@ int main() {
   int held = 0;
   for (std::int32_t s : ids) {
     EXPECT(host.len(s, 0) == 130 && host.len(s, 1) == 130 && host.n_pages(s) == 3);
-    for (int i = 0; i < 3; ++i) EXPECT(host.page_refs(host.table_row(s)[i]) == 1), ++held;
+    for (int i = 0; i < 3; ++i, ++held) EXPECT(host.page_refs(host.table_row(s)[i]) == 1);
   }
   EXPECT(held == 9 && host.pages_free() == 64 - held && host.pages_free() > free_before);
   int dirty = 0;
