@@ -271,7 +271,8 @@ int yahkv_attend_decode_weights(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, c
  * there is none, and nothing changes). Attention does not depend on the order of keys, but a key's slot is no longer
  * its position: the next yahkv_append continues at position n_keep with a K row that the caller rotated at the true
  * position (yahkv_rope_rows); yahkv_rope_append and the raw-projection calls refuse the sequence and its forks with
- * YAHKV_ERR_ORDER until yahkv_seq_set_len(seq, -1, 0). A sequence in a yahkv_batch is refused (YAHKV_ERR_ORDER: destroy
+ * YAHKV_ERR_ORDER until yahkv_seq_set_len(seq, -1, 0). A sequence whose table yahkv_seq_set_table made shorter than its length
+ * is refused (YAHKV_ERR_ORDER), here and in yahkv_seq_fork. A sequence in a yahkv_batch is refused (YAHKV_ERR_ORDER: destroy
  * the batch first and create it again). Cannot be captured (YAHKV_ERR_ORDER). After YAHKV_ERR_CUDA the listed sequences'
  * weights are undefined; the sequences are as they were. */
 int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t n_keep, int64_t n_sink, int64_t n_recent,

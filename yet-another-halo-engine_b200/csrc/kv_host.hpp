@@ -81,6 +81,7 @@ class KvHost {
   // Tells a sequence from the ones that had its id before.
   std::uint32_t generation(int seq) const { return generation_[static_cast<std::size_t>(seq)]; }
   int n_pages(int seq) const { return n_pages_[static_cast<std::size_t>(seq)]; }
+  std::int64_t PagesHold(int seq) const { return static_cast<std::int64_t>(n_pages(seq)) * kPageTokens; }   // tokens
   const std::int32_t* table_row(int seq) const {
     return table_.data() + static_cast<std::size_t>(seq) * static_cast<std::size_t>(cfg_.max_pages_per_seq);
   }
@@ -189,6 +190,8 @@ class KvHost {
       if (len(seq, l) < n_tokens)
         return {YAHKV_ERR_ORDER, "seq_fork: sequence " + std::to_string(seq) + " holds " + std::to_string(len(seq, l)) +
                                      " tokens in layer " + std::to_string(l) + ", " + std::to_string(n_tokens) + " asked for"};
+    if (n_tokens > PagesHold(seq))   // its table was set by hand and the length not yet
+      return {YAHKV_ERR_ORDER, "seq_fork: the table of sequence " + std::to_string(seq) + " has fewer pages than " + std::to_string(n_tokens) + " tokens need"};
     return {};
   }
   // A new sequence whose first n_tokens / 64 pages are seq's own (counted references, never written while shared) and
@@ -244,6 +247,8 @@ class KvHost {
       for (int l = 1; l < cfg_.n_layers; ++l)
         if (len(s, l) != n)
           return {YAHKV_ERR_ORDER, "evict: sequence " + std::to_string(s) + " has different lengths in its layers"};
+      if (n > PagesHold(s))
+        return {YAHKV_ERR_ORDER, "evict: the table of sequence " + std::to_string(s) + " has fewer pages than its length needs"};
       EvictSeq e{};
       e.seq = s, e.n_keys = static_cast<std::int32_t>(n), e.first_dst = static_cast<std::int32_t>(dst_pages->size());
       seqs->push_back(e);
