@@ -234,9 +234,9 @@ int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, 
 
 /* yahkv_attend_decode with every shared prefix computed once for all the rows that share it: same arguments, same result up
  * to rounding. Rows whose block tables start with the same pages are grouped (found here; any order, several groups,
- * forks of forks and rows that share nothing in one call) so that the most page reads are saved; a prefix that saves
- * fewer than 64 page reads is left to its rows. The prefix runs on the tensor
- * cores for the whole group: K and V enter as fp16 (quantized values rounded once, as in
+ * forks of forks and rows that share nothing in one call) so that the most page reads are saved; a prefix too
+ * short for its number of rows to pay (by measured times, from 20 to 54 saved page reads on) is left to its rows. The prefix
+ * runs on the tensor cores for the whole group: K and V enter as fp16 (quantized values rounded once, as in
  * yahkv_attend_prefill) and the softmax weights too, so a result is about 1e-3 of the largest output's size from
  * yahkv_attend_decode's at worst and about 4e-4 of an output's size on average. n_splits: split-K units of what lies
  * behind the prefix, 0 = automatic. q_dev 16-byte aligned. The first call allocates a workspace (about 40 MB; 24 KB
@@ -425,7 +425,7 @@ int yahkv_launch_count(const yahkv_ctx* ctx, int64_t* launches);
  * path this way. */
 int yahkv_debug_wait_timeout(yahkv_ctx* ctx, int64_t limit_us, void* stream);
 int yahkv_debug_set_prefill_sms(yahkv_ctx* ctx, int32_t n_sm);
-/* Sets how many page reads computing a shared prefix once must save for it to be done (default 64), so that a small test
+/* Sets how many page reads computing a shared prefix once must save for it to be done (without it, measured times decide), so that a small test
  * reaches that path. Takes effect with the next plan. */
 int yahkv_debug_set_shared_min(yahkv_ctx* ctx, int32_t pages);
 

@@ -190,7 +190,6 @@ struct PrefixItem {
   std::int32_t pad;
 };
 static_assert(sizeof(PrefixItem) == 16, "uploaded as an array");
-constexpr int kSharedMinSaved = 64;        // page reads that computing a prefix once must save (KvHost::FindPrefixes)
 
 // Partial workspace per unit: acc [6][256] f32 (unnormalised), then ml [6][2] f32 (max in log2 units, sum).
 constexpr int kPartialAccFloats = kGroup * kHeadDim;

@@ -508,10 +508,7 @@ class KvHost {
   // row is in at most one group. A node's rows are one group, or groups further down with the rows that are in none of
   // those as a group of their own, whichever saves most in all: a short row does not cut the prefix of the long ones, and
   // a few long rows do not take the common prefix from the others.
-  // Savings below shared_min_saved_ pages are left to the ordinary
-  // units: the pass costs two launches' time and its pairs work on half-empty tiles (measured, us per call with / without
-  // the pass: 2 rows x 4096 tokens fp16 12.6 / 11.1, q8_0 13.8 / 13.9; 4 x 4096 13.5 / 18.8 and 14.5 / 15.5; 8 x 256 9.4 /
-  // 11.8 and 10.0 / 10.5; 32 x 256 13.0 / 27.4 and 14.4 / 21.9; 32 x 16384 28 / 196 and 33 / 158).
+  // A prefix that does not pay (PrefixPays) is left to its rows.
   std::vector<PrefixGroup> FindPrefixes(int n_seqs, const std::int32_t* seq_ids, const std::int64_t* lens) const {
     std::vector<PrefixGroup> groups;
     std::vector<std::int32_t> rows;
@@ -531,6 +528,30 @@ class KvHost {
       g.n_mt = (static_cast<int>(g.rows.size()) * kGroup + 2 * kPrefillTileRows - 1) / (2 * kPrefillTileRows);
     return groups;
   }
+  // Whether computing `pages` pages once for `rows` rows is faster than leaving them to the rows' own units: it costs two
+  // launches' time and CTA pairs that work on half-empty tiles. It pays from a number of saved page reads on, and from a
+  // number of pages on that falls once the rows' units alone (four per row at least) no longer fit the device at once (f16
+  // one CTA per SM, q8_0 two). Measured in 483 cases of 2 .. 96 rows and 1 .. 256 pages with suffixes of up to 64 tokens, us
+  // per call with / without the pass:
+  //   f16   2 x 64 13.6 / 13.3   2 x 128 16.2 / 23.7    8 x 4 10.3 / 9.2    8 x 8 10.8 / 13.1   32 x 4 13.5 / 12.1   32 x 6 13.2 / 17.7
+  //         43 x 1 14.5 / 14.1   43 x 2 14.7 / 16.7    64 x 1 14.7 / 15.8
+  //   q8_0  2 x 16 12.8 / 11.7   2 x 32 13.4 / 13.5     8 x 1 10.7 / 10.7   8 x 4 11.0 / 11.3   24 x 2 13.5 / 13.0   24 x 4 13.7 / 15.4
+  //         48 x 4 17.8 / 15.9   48 x 6 16.5 / 18.2    96 x 3 23.5 / 22.6   96 x 4 21.7 / 24.8
+  //   q4_0  2 x 16 12.2 / 11.2   2 x 32 13.0 / 14.1     8 x 2 10.7 / 10.3   8 x 4 10.9 / 11.1   32 x 1 13.2 / 12.8   32 x 2 13.3 / 15.1
+  // The rule takes the faster side, or one at most 12 % slower; by mean 0.2, 0.4 and 0.1 % are lost.
+  bool PrefixPaysMeasured(int rows, int pages) const {
+    const std::int64_t saved = static_cast<std::int64_t>(rows - 1) * pages * kv_head_count() / kKvHeads;   // measured with all heads
+    switch (cfg_.fmt) {
+      case YAHKV_FMT_F16: return saved >= 54 && pages >= (rows < 40 ? 6 : rows < 60 ? 2 : 1);
+      case YAHKV_FMT_Q8_0: return saved >= 20 && pages >= (rows < 16 ? 1 : rows < 32 ? 4 : rows < 72 ? 6 : 4);
+      default: return saved >= 27 && pages >= (rows < 20 ? 3 : 2);
+    }
+  }
+  bool PrefixPays(int rows, int pages) const {
+    if (shared_min_saved_ > 0) return static_cast<std::int64_t>(rows - 1) * pages >= shared_min_saved_;
+    return PrefixPaysMeasured(rows, pages);
+  }
+  // The page reads a prefix must save instead of the measured rule.
   void SetSharedMinSaved(int pages) {
     shared_min_saved_ = pages;
     InvalidateSharedPlan();
@@ -897,10 +918,9 @@ class KvHost {
     int left = static_cast<int>(own);
     for (int c : v.children) split += (*tree)[static_cast<std::size_t>(c)].value[self], left += (*tree)[static_cast<std::size_t>(c)].up[self];
     const std::int64_t whole = static_cast<std::int64_t>(v.pages) * (v.count - 1);
-    const bool may_whole = whole >= shared_min_saved_;
+    const bool may_whole = PrefixPays(v.count, v.pages);
     // beside groups below, a group must be worth its own tiles
-    const std::int64_t rest = static_cast<std::int64_t>(v.pages) * (left - 1);
-    const bool may_split = left >= 2 && left < v.count && rest >= std::max(shared_min_saved_, kSharedMinSaved);
+    const bool may_split = left >= 2 && left < v.count && PrefixPays(left, v.pages) && PrefixPaysMeasured(left, v.pages);
     v.value.resize(self), v.up.resize(self), v.choice.resize(self);
     for (std::size_t k = 0; k < self; ++k) {
       v.value[k] = (*above)[k] * own, v.up[k] = static_cast<int>(own), v.choice[k] = PrefixNode::kJoin;
@@ -1018,7 +1038,7 @@ class KvHost {
   std::int64_t unit_pages_ = 0;
   std::vector<CombineItem> items_;
   SharedPlan shared_;           // cached plan of attend_decode_shared
-  int shared_min_saved_ = kSharedMinSaved;
+  int shared_min_saved_ = 0;    // 0: PrefixPaysMeasured decides
   std::vector<int> open_cur_;   // kv8a16: current open-tile buffer per (sequence, layer)
   std::vector<int> bounds_;     // PlanDecode: page boundaries of one sequence's units
 };

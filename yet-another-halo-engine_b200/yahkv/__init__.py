@@ -641,7 +641,7 @@ class KvCache:
         self._check(lib.yahkv_debug_set_prefill_sms(self._h, int(n_sm)))
 
     def debug_set_shared_min(self, pages):
-        """Page reads that computing a shared prefix once must save (default 64)."""
+        """Page reads that computing a shared prefix once must save, in place of the rule by measured times."""
         self._check(lib.yahkv_debug_set_shared_min(self._h, int(pages)))
 
     def launch_count(self):
