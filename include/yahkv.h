@@ -239,9 +239,9 @@ int yahkv_seq_fork(yahkv_ctx* ctx, int32_t seq, int64_t n_tokens, int32_t* out, 
  * runs on the tensor cores for the whole group: K and V enter as fp16 (quantized values rounded once, as in
  * yahkv_attend_prefill) and the softmax weights too, so a result is about 1e-3 of the largest output's size from
  * yahkv_attend_decode's at worst and about 4e-4 of an output's size on average. n_splits: split-K units of what lies
- * behind the prefix, 0 = automatic. q_dev 16-byte aligned. The first call allocates a workspace (about 40 MB; 24 KB
- * per sequence of max_seqs where that is more). Its lists come from the host, so it refuses a stream under capture
- * (YAHKV_ERR_ORDER): yahkv_batch_set_shared is the form for a graph. */
+ * behind the prefix, 0 = automatic. q_dev 16-byte aligned. Its workspace (at most 40 MB; 24 KB
+ * per sequence of max_seqs where that is more) is the context's from its creation on. Its lists come from the host, so it
+ * refuses a stream under capture (YAHKV_ERR_ORDER): yahkv_batch_set_shared is the form for a graph. */
 int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
                                const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, void* stream);
 
@@ -253,8 +253,9 @@ int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, co
  * (YAHKV_ERR_CAPACITY). A sequence may be listed once. The gate does not enter the weights. For fp16 pages the attention is
  * yahkv_attend_decode's to the bit; for the quantized formats the query enters in 20-bit steps of its largest element
  * where yahkv_attend_decode takes 16, so the two agree within that rounding (1e-4 of the largest output). q_dev 16-byte aligned. The scores
- * pass through a workspace (96 B per cached key of the call) that grows to the largest call seen: growing waits for
- * the device. Refuses a stream under capture (YAHKV_ERR_ORDER). */
+ * pass through a workspace (96 B per cached key of the call). A context has it from its creation on for the keys that its
+ * block tables can hold, or for 1.4 million where they can hold more; a call of still more keys lets it grow, which waits
+ * for the device. Refuses a stream under capture (YAHKV_ERR_ORDER). */
 int yahkv_attend_decode_weights(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int32_t* seq_ids, const void* q_dev,
                                 const float* gate_dev, void* out_dev, int32_t out_dtype, int32_t n_splits, float* weights_dev,
                                 int64_t weights_stride, void* stream);
@@ -379,7 +380,7 @@ void yahkv_batch_destroy(yahkv_batch* batch);
 int yahkv_batch_set_splits(yahkv_batch* batch, int32_t n_splits);
 /* on != 0: from the next batch_prepare on, the steps compute every prefix that rows of the batch share (yahkv_seq_fork) once
  * for all of them, as yahkv_attend_decode_shared does; the groups are found at batch_prepare and hold for its horizon.
- * Allocates on first use, so call it before a capture. The batches of a context share its workspaces: replay their graphs
+ * Allocates the batch's lists when first switched on, so call it before a capture. The batches of a context share its workspaces: replay their graphs
  * one after the other, not side by side. Refused for the tile formats. The number of prefix tiles is part
  * of the layout that *layout_changed reports. */
 int yahkv_batch_set_shared(yahkv_batch* batch, int32_t on);

@@ -110,6 +110,8 @@ cudaError_t LaunchBatchPlan(const std::int32_t* lens_dev, const BatchSeq* seqs_d
                        n_layers);
 }
 
+cudaError_t LoadTableUpload() { return LoadKernels(TableUploadKernel); }
+
 cudaError_t LaunchTableUpload(const TableRange* ranges, int n, const std::int32_t* data, std::int32_t* tables_dev, cudaStream_t stream) {
   if (n <= 0) return cudaSuccess;
   return LaunchChained(TableUploadKernel, n, 128, 0, stream, ranges, data, tables_dev);

@@ -641,7 +641,8 @@ static cudaError_t ConfigurePart() {
                               DecodeSmemBytes<kFmt, true>());
 }
 cudaError_t ConfigureDecodeKernels() {
-  const cudaError_t e = ConfigurePart<kFmtQ8>();
+  cudaError_t e = LoadKernels(DecodeCombineKernel);
+  if (e == cudaSuccess) e = ConfigurePart<kFmtQ8>();
   return e != cudaSuccess ? e : ConfigurePart<kFmtQ4>();
 }
 

@@ -310,6 +310,8 @@ int SelectSmem(int n_cache) { return 4 * (kHistCopies * kHistStride + n_cache); 
 }  // namespace
 
 cudaError_t ConfigureEvictKernels() {
+  const auto e = LoadKernels(AttnWeightsKernel, CopyPageKernel, EvictMoveKernel<kFmtF16>, EvictMoveKernel<kFmtQ8>, EvictMoveKernel<kFmtQ4>);
+  if (e != cudaSuccess) return e;
   return cudaFuncSetAttribute(EvictSelectKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SelectSmem(kSelectCache));
 }
 

@@ -119,6 +119,7 @@ struct TableRange {
   std::int32_t src;
   std::int32_t count;
 };
+cudaError_t LoadTableUpload();
 cudaError_t LaunchTableUpload(const TableRange* ranges, int n, const std::int32_t* data, std::int32_t* tables_dev, cudaStream_t stream);
 cudaError_t LaunchBatchAdvance(std::int32_t* lens_dev, int n_seqs, int by, cudaStream_t stream);
 
@@ -197,6 +198,15 @@ constexpr int kPartialMlFloats = kGroup * 2;
 // Split-K units one (batch row, kv head) may have: the combine kernel keeps one weight per unit in shared memory.
 // Every planner stays below it (yahkv_config.max_splits is refused above it).
 constexpr int kCombineMaxUnits = 1024;
+
+// Has the driver load kernels now and not at their first launch (up to a millisecond in a process that loads lazily).
+template <class... Kernels>
+cudaError_t LoadKernels(Kernels... kernels) {
+  cudaFuncAttributes attr{};
+  cudaError_t e = cudaSuccess;
+  ((e = e == cudaSuccess ? cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(kernels)) : e), ...);
+  return e;
+}
 
 // Launch with programmatic stream serialization allowed: see ChainedKernelEntry in ptx.cuh.
 template <class... Params, class... Args>
@@ -348,6 +358,7 @@ struct RopeRowsLaunch {
   bool interleaved, x_f32, out_f32;
 };
 cudaError_t LaunchRopeRows(const RopeRowsLaunch& a, cudaStream_t stream);
+cudaError_t LoadRopeRows(bool interleaved, int rotary_dim);   // the kernels that a rotation may launch
 
 struct PrefillLaunch {
   PoolView pool;

@@ -193,14 +193,17 @@ __global__ void __launch_bounds__(32 * kRopeRowWarps) RopeRowsKernel(const RopeR
 }
 
 template <bool kInF32, bool kOutF32, int kHeads>
+auto KernelOf(bool interleaved, int rotary_dim) {
+  return interleaved && rotary_dim % 8 == 0      ? RopeRowsKernel<kInF32, kOutF32, kHeads, kInterleavedPairs>
+         : !interleaved && rotary_dim % 16 == 0 ? RopeRowsKernel<kInF32, kOutF32, kHeads, kHalfPairs>
+                                                : RopeRowsKernel<kInF32, kOutF32, kHeads, kAnyPairs>;
+}
+template <bool kInF32, bool kOutF32, int kHeads>
 cudaError_t Launch(const RopeRowsLaunch& a, cudaStream_t stream) {
   const long long tasks = static_cast<long long>(a.n_tokens) * ((a.n_heads + kHeads - 1) / kHeads);
   const long long grid = (tasks + kRopeRowWarps - 1) / kRopeRowWarps;
   if (grid > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
-  const auto kernel = a.interleaved && a.rotary_dim % 8 == 0      ? RopeRowsKernel<kInF32, kOutF32, kHeads, kInterleavedPairs>
-                      : !a.interleaved && a.rotary_dim % 16 == 0 ? RopeRowsKernel<kInF32, kOutF32, kHeads, kHalfPairs>
-                                                                 : RopeRowsKernel<kInF32, kOutF32, kHeads, kAnyPairs>;
-  return LaunchChained(kernel, static_cast<unsigned>(grid), 32 * kRopeRowWarps, 0, stream, a);
+  return LaunchChained(KernelOf<kInF32, kOutF32, kHeads>(a.interleaved, a.rotary_dim), static_cast<unsigned>(grid), 32 * kRopeRowWarps, 0, stream, a);
 }
 template <bool kInF32, bool kOutF32>
 cudaError_t LaunchHeads(const RopeRowsLaunch& a, cudaStream_t stream) {
@@ -210,6 +213,14 @@ cudaError_t LaunchHeads(const RopeRowsLaunch& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+cudaError_t LoadRopeRows(bool interleaved, int rotary_dim) {
+  cudaError_t e = LoadKernels(KernelOf<true, true, 1>(interleaved, rotary_dim), KernelOf<true, true, 4>(interleaved, rotary_dim));
+  if (e == cudaSuccess) e = LoadKernels(KernelOf<true, false, 1>(interleaved, rotary_dim), KernelOf<true, false, 4>(interleaved, rotary_dim));
+  if (e == cudaSuccess) e = LoadKernels(KernelOf<false, true, 1>(interleaved, rotary_dim), KernelOf<false, true, 4>(interleaved, rotary_dim));
+  if (e == cudaSuccess) e = LoadKernels(KernelOf<false, false, 1>(interleaved, rotary_dim), KernelOf<false, false, 4>(interleaved, rotary_dim));
+  return e;
+}
 
 cudaError_t LaunchRopeRows(const RopeRowsLaunch& a, cudaStream_t stream) {
   if (a.n_tokens <= 0 || a.n_heads <= 0) return cudaSuccess;

@@ -734,6 +734,7 @@ cudaError_t Launch(const DecodeLaunch& a, const SharedLaunch& p, cudaStream_t st
 }  // namespace
 
 cudaError_t ConfigureSharedKernels(int fmt, int* max_active_pairs) {
+  if (cudaError_t e = LoadKernels(SharedCombineKernel); e != cudaSuccess) return e;
   return fmt == kFmtF16  ? Configure<kFmtF16>(max_active_pairs)
          : fmt == kFmtQ8 ? Configure<kFmtQ8>(max_active_pairs)
                          : Configure<kFmtQ4>(max_active_pairs);

@@ -37,27 +37,22 @@ class Staging {
       if (s.ev != nullptr) cudaEventDestroy(s.ev);
     }
   }
+  // Buffers of `bytes` each, so that the first calls need not make them.
+  cudaError_t Reserve(std::size_t bytes) {
+    for (Slot& s : slots_)
+      if (cudaError_t e = Grow(s, bytes); e != cudaSuccess) return e;
+    return cudaSuccess;
+  }
   cudaError_t Acquire(std::size_t bytes, char** out) {
     Slot& s = slots_[next_];
     cur_ = next_;
     next_ = (next_ + 1) % kSlots;
-    if (s.ev == nullptr) {
-      cudaError_t e = cudaEventCreateWithFlags(&s.ev, cudaEventDisableTiming);
-      if (e != cudaSuccess) return e;
-    }
     if (s.in_flight) {
       cudaError_t e = cudaEventSynchronize(s.ev);
       if (e != cudaSuccess) return e;
       s.in_flight = false;
     }
-    if (s.cap < bytes) {
-      if (s.host != nullptr) cudaFreeHost(s.host);
-      s.host = nullptr, s.cap = 0;
-      const std::size_t cap = std::max<std::size_t>(bytes, 1 << 16);
-      cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&s.host), cap, cudaHostAllocDefault);
-      if (e != cudaSuccess) return e;
-      s.cap = cap;
-    }
+    if (cudaError_t e = Grow(s, bytes); e != cudaSuccess) return e;
     *out = s.host;
     return cudaSuccess;
   }
@@ -75,6 +70,17 @@ class Staging {
     cudaEvent_t ev = nullptr;
     bool in_flight = false;
   };
+  static cudaError_t Grow(Slot& s, std::size_t bytes) {
+    if (s.ev == nullptr)
+      if (cudaError_t e = cudaEventCreateWithFlags(&s.ev, cudaEventDisableTiming); e != cudaSuccess) return e;
+    if (s.cap >= bytes && s.cap > 0) return cudaSuccess;
+    if (s.host != nullptr) cudaFreeHost(s.host);
+    s.host = nullptr, s.cap = 0;
+    const std::size_t cap = std::max<std::size_t>(bytes, 1 << 16);
+    if (cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&s.host), cap, cudaHostAllocDefault); e != cudaSuccess) return e;
+    s.cap = cap;
+    return cudaSuccess;
+  }
   Slot slots_[kSlots];
   int next_ = 0, cur_ = 0;
 };
@@ -150,9 +156,8 @@ struct yahkv_ctx {
   std::vector<VTileWork> vwork_scratch;
   std::vector<std::int32_t> state_row_scratch;
   std::vector<DecodeUnit> unit_scratch;
-  // shared-prefix decode attention, allocated by the first call
+  // shared-prefix decode attention (formats with rows of their own)
   struct Shared {
-    bool ready = false;
     int n_pairs = 0;            // CTA pairs of the prefix kernel the device runs at once
     int max_tiles = 0;
     std::int64_t max_part_rows = 0;
@@ -161,12 +166,11 @@ struct yahkv_ctx {
     float *part_acc = nullptr, *part_ml = nullptr;
     CUtensorMap k16map{}, v16map{};   // fp16 pages as [rows][256] fp16
   } shared;
-  // scores of a weight-accumulating decode call, grown to the largest call seen
+  // scores of a weight-accumulating decode call
   float* scores_dev = nullptr;
   std::int64_t score_pages = 0;
   std::vector<yahkv_batch*> batches;   // not destroyed yet
-  // eviction work lists, allocated by the first call
-  char* evict_dev = nullptr;
+  char* evict_dev = nullptr;   // eviction work lists: the sequences, then their pages
   std::vector<EvictSeq> evict_scratch;
   std::vector<std::int32_t> evict_page_scratch;
 };
@@ -310,7 +314,6 @@ int InitDevice(yahkv_ctx* ctx) {
     if (int r = ResizePrefillScratch(ctx, static_cast<std::int64_t>(c.max_prefill_keys) * kKvHeads); r != YAHKV_OK) return r;
   YAHKV_CUDA(ctx, ConfigureDecodeKernels());
   if (c.fmt == YAHKV_FMT_F16) YAHKV_CUDA(ctx, ConfigureF16Kernels());
-  if (!IsTileFmt(c.fmt)) YAHKV_CUDA(ctx, ConfigureEvictKernels());
   {
     int pairs = 0;   // CTA pairs of the prefill kernel that run at the same time: the planner's wave
     YAHKV_CUDA(ctx, ConfigurePrefillKernels(&pairs));
@@ -530,6 +533,8 @@ const char* yahkv_last_error(const yahkv_ctx* ctx) {
   return copy.c_str();
 }
 
+static int MakeWorkspaces(yahkv_ctx* ctx);
+
 int yahkv_create(const yahkv_config* cfg, yahkv_ctx** out) {
   auto fail = [&](int code, const std::string& msg) {
     std::lock_guard<std::mutex> lock(g_create_mu);
@@ -551,7 +556,9 @@ int yahkv_create(const yahkv_config* cfg, yahkv_ctx** out) {
   ctx->scale_log2 = c.softmax_scale * 1.4426950408889634F;
   ctx->slot_scratch.resize(static_cast<std::size_t>(c.max_batch_tokens));
   if (c.device >= 0) {
-    if (int r = InitDevice(ctx); r != YAHKV_OK) {
+    int r = InitDevice(ctx);
+    if (r == YAHKV_OK) r = MakeWorkspaces(ctx);
+    if (r != YAHKV_OK) {
       const std::string msg = ctx->err;
       FreeDevice(ctx);
       delete ctx;
@@ -850,16 +857,18 @@ int yahkv_attend_decode_qraw(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, cons
                       n_splits, nullptr, 0, stream);
 }
 
-// Room for the scores of `pages` pages of one kv head each (1.5 KB), grown by half at least so that contexts which grow page
-// by page rarely find it too small; growing waits for the device.
+// Room for the scores of `pages` pages of one kv head each (1.5 KB). A context has it for every call its block tables allow, or
+// for 128 MB (1.4 million cached keys in one call); beyond that it grows by half at least, which waits for the device.
+constexpr std::int64_t kScoreBytes = kGroup * kPageTokens * 4;
 static int EnsureScores(yahkv_ctx* ctx, std::int64_t pages) {
   if (pages <= ctx->score_pages) return YAHKV_OK;
-  constexpr std::int64_t kFloats = kGroup * kPageTokens;
-  const std::int64_t want = std::max<std::int64_t>({pages, ctx->score_pages + ctx->score_pages / 2, 1024});
-  YAHKV_CUDA(ctx, cudaDeviceSynchronize());
-  if (ctx->scores_dev != nullptr) cudaFree(ctx->scores_dev), ctx->device_bytes -= ctx->score_pages * kFloats * 4;
+  const std::int64_t want = std::max(pages, ctx->score_pages + ctx->score_pages / 2);
+  if (ctx->scores_dev != nullptr) {
+    YAHKV_CUDA(ctx, cudaDeviceSynchronize());
+    cudaFree(ctx->scores_dev), ctx->device_bytes -= ctx->score_pages * kScoreBytes;
+  }
   ctx->scores_dev = nullptr, ctx->score_pages = 0;
-  YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->scores_dev, static_cast<std::size_t>(want * kFloats), false));
+  YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->scores_dev, static_cast<std::size_t>(want * kScoreBytes / 4), false));
   ctx->score_pages = want;
   return YAHKV_OK;
 }
@@ -983,32 +992,47 @@ static std::size_t SharedPlanBytes(std::size_t tiles, std::size_t units, std::si
          rows * sizeof(std::int32_t);
 }
 
-// What shared-prefix attention needs beyond the context's own buffers; built by the first call that uses it.
-static int EnsureShared(yahkv_ctx* ctx) {
+// What shared-prefix attention needs beyond the context's own buffers.
+static int MakeShared(yahkv_ctx* ctx) {
   auto& sh = ctx->shared;
-  if (sh.ready) return YAHKV_OK;
   const yahkv_config& c = ctx->cfg;
-  if (sh.n_pairs == 0) {
-    int pairs = 0;
-    YAHKV_CUDA(ctx, ConfigureSharedKernels(c.fmt, &pairs));
-    sh.n_pairs = std::max(std::min(pairs, ctx->n_sm_device / 2), 1);
-    // up to four waves of pairs, or one pair per (group of at least two rows, kv head, 256 rows)
-    const int combos = kKvHeads * (c.max_seqs / 2 + c.max_seqs * kGroup / (2 * kPrefillTileRows) + 1);
-    sh.max_tiles = 2 * std::max(4 * sh.n_pairs, combos);
-    sh.max_part_rows = std::max<std::int64_t>(static_cast<std::int64_t>(c.max_seqs) * kQHeads, 4LL * kPrefillTileRows * sh.n_pairs);
-  }
-  auto alloc = [&](auto** p, std::size_t count) { return *p != nullptr ? cudaSuccess : DevAlloc(ctx, p, count, false); };
+  int pairs = 0;
+  YAHKV_CUDA(ctx, ConfigureSharedKernels(c.fmt, &pairs));
+  sh.n_pairs = std::max(std::min(pairs, ctx->n_sm_device / 2), 1);
+  // up to four waves of pairs, or one pair per (group of at least two rows, kv head, 256 rows)
+  const int combos = kKvHeads * (c.max_seqs / 2 + c.max_seqs * kGroup / (2 * kPrefillTileRows) + 1);
+  sh.max_tiles = 2 * std::max(4 * sh.n_pairs, combos);
+  // no more rows than every query head of every sequence and page
+  const std::int64_t heads = static_cast<std::int64_t>(c.max_seqs) * kQHeads;
+  sh.max_part_rows = std::min(heads * c.max_pages_per_seq, std::max<std::int64_t>(heads, 4LL * kPrefillTileRows * sh.n_pairs));
   sh.plan_bytes = SharedPlanBytes(static_cast<std::size_t>(sh.max_tiles), static_cast<std::size_t>(ctx->max_units), static_cast<std::size_t>(c.max_seqs));
-  YAHKV_CUDA(ctx, alloc(&sh.plan_dev, sh.plan_bytes));
-  YAHKV_CUDA(ctx, alloc(&sh.part_acc, static_cast<std::size_t>(sh.max_part_rows) * kHeadDim));
-  YAHKV_CUDA(ctx, alloc(&sh.part_ml, static_cast<std::size_t>(sh.max_part_rows) * 2));
+  YAHKV_CUDA(ctx, DevAlloc(ctx, &sh.plan_dev, sh.plan_bytes, false));
+  YAHKV_CUDA(ctx, DevAlloc(ctx, &sh.part_acc, static_cast<std::size_t>(sh.max_part_rows) * kHeadDim, false));
+  YAHKV_CUDA(ctx, DevAlloc(ctx, &sh.part_ml, static_cast<std::size_t>(sh.max_part_rows) * 2, false));
   if (c.fmt == YAHKV_FMT_F16) {
     const std::uint64_t rows = static_cast<std::uint64_t>(c.n_layers) * c.num_pages * kKvHeads * kPageTokens;
     if (!EncodeTensorMap2D(&sh.k16map, 2, ctx->pool.kcodes, kHeadDim, rows, 64, 32) ||
         !EncodeTensorMap2D(&sh.v16map, 2, ctx->pool.vcodes, kHeadDim, rows, 64, 64))
       return Fail(ctx, YAHKV_ERR_CUDA, "tensor map encode failed for the fp16 pools");
   }
-  sh.ready = true;
+  return YAHKV_OK;
+}
+
+// Everything that the calls of a context need and that its configuration bounds exists before the first of them: an
+// allocation or a page lock takes longer than a call does.
+static int MakeWorkspaces(yahkv_ctx* ctx) {
+  const yahkv_config& c = ctx->cfg;
+  std::size_t lists = static_cast<std::size_t>(ctx->max_units) * sizeof(DecodeUnit) + static_cast<std::size_t>(c.max_seqs) * kKvHeads * sizeof(CombineItem);
+  if (!IsTileFmt(c.fmt)) {
+    if (int r = MakeShared(ctx); r != YAHKV_OK) return r;
+    const std::int64_t pages = static_cast<std::int64_t>(c.max_seqs) * c.max_pages_per_seq * ctx->host.kv_head_count();
+    if (int r = EnsureScores(ctx, std::min<std::int64_t>(pages, (128LL << 20) / kScoreBytes)); r != YAHKV_OK) return r;
+    YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_dev, static_cast<std::size_t>(c.max_seqs) * (sizeof(EvictSeq) + 4 * static_cast<std::size_t>(c.max_pages_per_seq)), false));
+    YAHKV_CUDA(ctx, ConfigureEvictKernels());
+    lists = std::max(lists, ctx->shared.plan_bytes);
+  }
+  YAHKV_CUDA(ctx, LoadTableUpload());
+  YAHKV_CUDA(ctx, ctx->staging.Reserve(std::min<std::size_t>(lists, 256 << 10)));   // the longest lists there are do not come up
   return YAHKV_OK;
 }
 
@@ -1030,7 +1054,6 @@ int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, co
     if (n_seqs > 0 && (q_dev == nullptr || out_dev == nullptr)) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: null q or out pointer");
     if ((reinterpret_cast<std::uintptr_t>(q_dev) & 15) != 0) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: q must be 16-byte aligned");
     if (int r = RefuseCapture(ctx, "attend_decode_shared: lists from the host", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
-    if (int r = EnsureShared(ctx); r != YAHKV_OK) return r;   // before the plan: a failure here changes no state
     auto& sh = ctx->shared;
     bool changed = false;
     HostError e = ctx->host.PlanDecodeShared(layer, n_seqs, seq_ids, n_splits, ctx->cfg.max_splits, ctx->max_units, sh.n_pairs,
@@ -1120,9 +1143,6 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
     HostError e = ctx->host.PlanEvict(n_seqs, seq_ids, n_keep, &ctx->evict_scratch, &ctx->evict_page_scratch, &any);
     if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
     if (n_seqs == 0) return YAHKV_OK;
-    const yahkv_config& c = ctx->cfg;
-    if (ctx->evict_dev == nullptr)   // the sequences, then their pages
-      YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_dev, static_cast<std::size_t>(c.max_seqs) * (sizeof(EvictSeq) + 4 * static_cast<std::size_t>(c.max_pages_per_seq)), false));
     cudaStream_t st = StreamOf(ctx, stream);
     if (int r = FlushTables(ctx, st); r != YAHKV_OK) return r;   // the kernels read the tables as they are before the call
     const std::size_t sb = ctx->evict_scratch.size() * sizeof(EvictSeq), pb = ctx->evict_page_scratch.size() * sizeof(std::int32_t);
@@ -1133,7 +1153,7 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
     YAHKV_CUDA(ctx, cudaMemcpyAsync(ctx->evict_dev, buf, sb + pb, cudaMemcpyHostToDevice, st));
     YAHKV_CUDA(ctx, ctx->staging.Release(st));
     EvictLaunch a{};
-    a.pool = ctx->pool, a.tables_dev = ctx->tables_dev, a.table_stride = c.max_pages_per_seq;
+    a.pool = ctx->pool, a.tables_dev = ctx->tables_dev, a.table_stride = ctx->cfg.max_pages_per_seq;
     a.seqs_dev = reinterpret_cast<const EvictSeq*>(ctx->evict_dev), a.n_seqs = n_seqs;
     a.dst_pages_dev = reinterpret_cast<const std::int32_t*>(ctx->evict_dev + sb);
     a.n_keep = static_cast<int>(n_keep), a.n_sink = static_cast<int>(n_sink), a.n_recent = static_cast<int>(n_recent);
@@ -1205,7 +1225,8 @@ int yahkv_rope_create(yahkv_ctx* ctx, const yahkv_rope_config* cfg, yahkv_rope**
         const double a = n * freq[static_cast<std::size_t>(p)];
         tab[static_cast<std::size_t>(i) * half + p] = make_float2(static_cast<float>(m * std::cos(a)), static_cast<float>(m * std::sin(a)));
       }
-    cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&r->hi), tab.size() * sizeof(float2));
+    cudaError_t e = LoadRopeRows(c.layout == YAHKV_ROPE_INTERLEAVED, c.rotary_dim);
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&r->hi), tab.size() * sizeof(float2));
     if (e == cudaSuccess) e = cudaMemcpy(r->hi, tab.data(), tab.size() * sizeof(float2), cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
       if (r->hi != nullptr) cudaFree(r->hi);
@@ -1655,7 +1676,6 @@ int yahkv_batch_set_shared(yahkv_batch* b, int32_t on) {
   if (on != 0 && IsTileFmt(ctx->cfg.fmt))
     return Fail(ctx, YAHKV_ERR_INVALID, "batch_set_shared: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (their sequences share no pages)");
   if (on != 0) {   // everything a step needs exists before a capture
-    if (int r = EnsureShared(ctx); r != YAHKV_OK) return r;
     const std::size_t n = b->seqs.size();
     b->prefix_cap = SharedPlanBytes(static_cast<std::size_t>(ctx->shared.max_tiles), 0, n);
     if (b->prefix_dev == nullptr) YAHKV_CUDA(ctx, cudaMalloc(reinterpret_cast<void**>(&b->prefix_dev), b->prefix_cap));
