@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <cstring>
 #include <string>
 #include <utility>
 #include <vector>
@@ -21,6 +22,18 @@ namespace yahkv {
 struct HostError {
   int code = YAHKV_OK;
   std::string message;
+};
+
+// The layers that a plan has served since it was made. The layers of a decode step have equal lengths and share one plan; a
+// layer that comes again is another step and plans again, also where no length has changed since. (A yahkv_batch is the form
+// that keeps its work lists from step to step.)
+struct StepLayers {
+  std::vector<char> served;
+  bool Comes(int layer) const { return layer >= 0 && static_cast<std::size_t>(layer) < served.size() && served[static_cast<std::size_t>(layer)] != 0; }
+  void Serve(int layer, int n_layers, bool new_plan) {
+    if (new_plan || served.empty()) served.assign(static_cast<std::size_t>(n_layers), 0);
+    served[static_cast<std::size_t>(layer)] = 1;
+  }
 };
 
 class KvHost {
@@ -372,8 +385,11 @@ class KvHost {
     const int hb = kv_head_begin(), hc = kv_head_count();
     int auto_pages = static_cast<int>((total_pages * hc + 1479) / 1480);
     auto_pages = std::min(std::max(auto_pages, 1), 24);
-    std::vector<DecodeUnit> units;
-    std::vector<CombineItem> items(static_cast<std::size_t>(n_seqs) * kKvHeads);
+    // Built beside the present plan, in memory that is kept: fresh pages for the lists cost more than the planning.
+    std::vector<DecodeUnit>& units = next_units_;
+    std::vector<CombineItem>& items = next_items_;
+    units.clear();
+    items.assign(static_cast<std::size_t>(n_seqs) * kKvHeads, CombineItem{});
     std::int32_t slot = 0;   // pages of the units so far
     for (int b = 0; b < n_seqs; ++b) {
       const int s = seq_ids[b];
@@ -383,28 +399,16 @@ class KvHost {
       const int nu = static_cast<int>(bounds_.size());
       for (int h = hb; h < hb + hc; ++h) {   // heads outside the context's range keep n_partials = 0
         items[static_cast<std::size_t>(b) * kKvHeads + h] = {static_cast<std::int32_t>(units.size()), nu};
-        for (int k = 0; k < nu; ++k) {
-          DecodeUnit u{};
-          u.batch = b, u.seq = s, u.kvh = h;
-          u.page_begin = k == 0 ? 0 : bounds_[static_cast<std::size_t>(k) - 1], u.page_end = bounds_[static_cast<std::size_t>(k)];
-          u.n_keys = static_cast<std::int32_t>(n);
-          u.partial = static_cast<std::int32_t>(units.size());
-          u.pad = slot;
-          slot += u.page_end - u.page_begin;
-          units.push_back(u);
-        }
+        AddUnits(b, s, h, n, 0, &slot, &units);
       }
     }
     if (static_cast<long long>(units.size()) > max_units)
       return {YAHKV_ERR_CAPACITY, "attend_decode: split-K plan needs " + std::to_string(units.size()) +
                                       " units, workspace holds " + std::to_string(max_units)};
-    // Longest units first: CTAs are handed out in index order, so the short tail units fill the last wave.
-    std::stable_sort(units.begin(), units.end(), [](const DecodeUnit& a, const DecodeUnit& b) {
-      return a.page_end - a.page_begin > b.page_end - b.page_begin;
-    });
+    LongestFirst(&units);
     unit_pages_ = slot;
-    units_ = std::move(units);
-    items_ = std::move(items);
+    units_.swap(units);
+    items_.swap(items);
     plan_key_ = key_scratch_;
     *changed = true;
     return {};
@@ -440,8 +444,9 @@ class KvHost {
       *changed = false;
       return {};
     }
-    SharedPlan plan;
+    SharedPlan& plan = next_shared_;   // beside the present one, in memory that is kept
     plan.key = key_scratch_;
+    plan.tiles.clear(), plan.rows.clear(), plan.units.clear();
     std::vector<std::int64_t> lens(static_cast<std::size_t>(n_seqs));
     for (int b = 0; b < n_seqs; ++b) lens[static_cast<std::size_t>(b)] = len(seq_ids[b], layer);
     const std::vector<PrefixGroup> groups = FindPrefixes(n_seqs, seq_ids, lens.data());
@@ -455,7 +460,8 @@ class KvHost {
     const SharedShape shape = ChooseSharedShape(groups, suffix, n_pairs, n_splits, max_part_rows);
     BuildPrefixTiles(n_seqs, seq_ids, groups, shape.part_pages, &plan);
     const int hb = kv_head_begin(), hc = kv_head_count(), auto_pages = shape.unit_pages;
-    plan.items.resize(static_cast<std::size_t>(n_seqs) * kKvHeads);
+    std::int32_t slot = 0;
+    plan.items.assign(static_cast<std::size_t>(n_seqs) * kKvHeads, CombineItem{});
     for (int b = 0; b < n_seqs; ++b) {
       const int first = plan.first_page[static_cast<std::size_t>(b)];
       const std::int64_t n = lens[static_cast<std::size_t>(b)];
@@ -465,24 +471,14 @@ class KvHost {
       const int nu = static_cast<int>(bounds_.size());
       for (int h = hb; h < hb + hc; ++h) {
         plan.items[static_cast<std::size_t>(b) * kKvHeads + h] = {static_cast<std::int32_t>(plan.units.size()), nu};
-        for (int k = 0; k < nu; ++k) {
-          DecodeUnit u{};
-          u.batch = b, u.seq = seq_ids[b], u.kvh = h;
-          u.page_begin = first + (k == 0 ? 0 : bounds_[static_cast<std::size_t>(k) - 1]);
-          u.page_end = first + bounds_[static_cast<std::size_t>(k)];
-          u.n_keys = static_cast<std::int32_t>(n);
-          u.partial = static_cast<std::int32_t>(plan.units.size());
-          plan.units.push_back(u);
-        }
+        AddUnits(b, seq_ids[b], h, n, first, &slot, &plan.units);
       }
     }
     if (static_cast<long long>(plan.units.size()) > max_units)
       return {YAHKV_ERR_CAPACITY, "attend_decode_shared: split-K plan needs " + std::to_string(plan.units.size()) +
                                       " units, workspace holds " + std::to_string(max_units)};
-    std::stable_sort(plan.units.begin(), plan.units.end(), [](const DecodeUnit& a, const DecodeUnit& b) {
-      return a.page_end - a.page_begin > b.page_end - b.page_begin;
-    });
-    shared_ = std::move(plan);
+    LongestFirst(&plan.units);
+    std::swap(shared_, next_shared_);
     *changed = true;
     return {};
   }
@@ -886,7 +882,9 @@ class KvHost {
     for (std::size_t i = 1; i < rows.size(); ++i) {
       common = std::min(common, static_cast<int>(lens[rows[i]] / kPageTokens));
       const int known = std::min(from, common);
-      common = static_cast<int>(std::mismatch(first + known, first + common, table_row(seq_ids[rows[i]]) + known).first - first);
+      const std::int32_t* row = table_row(seq_ids[rows[i]]);
+      if (std::memcmp(first + known, row + known, static_cast<std::size_t>(common - known) * sizeof(*row)) != 0)
+        common = static_cast<int>(std::mismatch(first + known, first + common, row + known).first - first);
     }
     const int at = static_cast<int>(tree->size());
     tree->emplace_back();
@@ -955,6 +953,35 @@ class KvHost {
     groups->push_back(std::move(g));
   }
 
+  // The units that CutUnits has cut (bounds_), for one batch row and kv head, behind the row's first `first` pages. *slot counts
+  // the pages of all units.
+  void AddUnits(int b, int seq, int h, std::int64_t n_keys, int first, std::int32_t* slot, std::vector<DecodeUnit>* units) const {
+    const std::size_t at = units->size(), n = bounds_.size();
+    units->resize(at + n);
+    DecodeUnit* u = units->data() + at;
+    int page = 0;
+    for (std::size_t k = 0; k < n; ++k, ++u) {
+      u->batch = b, u->seq = seq, u->kvh = h;
+      u->page_begin = first + page, u->page_end = first + bounds_[k];
+      u->n_keys = static_cast<std::int32_t>(n_keys);
+      u->partial = static_cast<std::int32_t>(at + k);
+      u->pad = *slot;
+      *slot += bounds_[k] - page;
+      page = bounds_[k];
+    }
+  }
+  // Longest units first, equal ones in their order: CTAs are handed out in index order, so the short tail units fill the
+  // last wave. Counted by length: every call with changed lengths does this (1280 units: 5 us, a comparison sort 30).
+  void LongestFirst(std::vector<DecodeUnit>* units) {
+    int longest = 0;
+    for (const DecodeUnit& u : *units) longest = std::max(longest, u.page_end - u.page_begin);
+    sort_at_.assign(static_cast<std::size_t>(longest) + 2, 0);
+    for (const DecodeUnit& u : *units) ++sort_at_[static_cast<std::size_t>(longest - (u.page_end - u.page_begin)) + 1];
+    for (std::size_t i = 1; i < sort_at_.size(); ++i) sort_at_[i] += sort_at_[i - 1];
+    sort_scratch_.resize(units->size());
+    for (const DecodeUnit& u : *units) sort_scratch_[static_cast<std::size_t>(sort_at_[static_cast<std::size_t>(longest - (u.page_end - u.page_begin))]++)] = u;
+    units->swap(sort_scratch_);
+  }
   // Page boundaries of one sequence's split-K units over `pages` pages, into bounds_.
   void CutUnits(int pages, int n_splits, int max_splits, int auto_pages) {
     int per = n_splits > 0 ? (pages + n_splits - 1) / n_splits : auto_pages;
@@ -1034,10 +1061,14 @@ class KvHost {
   std::vector<int> free_seqs_;
   std::vector<std::pair<int, std::int64_t>> scratch_len_;
   std::vector<std::int64_t> key_scratch_, plan_key_;
+  std::vector<int> sort_at_;
+  std::vector<DecodeUnit> sort_scratch_;
   std::vector<DecodeUnit> units_;
   std::int64_t unit_pages_ = 0;
   std::vector<CombineItem> items_;
-  SharedPlan shared_;           // cached plan of attend_decode_shared
+  std::vector<DecodeUnit> next_units_;
+  std::vector<CombineItem> next_items_;
+  SharedPlan shared_, next_shared_;   // the plan of attend_decode_shared, and the memory of the one before
   int shared_min_saved_ = 0;    // 0: PrefixPaysMeasured decides
   std::vector<int> open_cur_;   // kv8a16: current open-tile buffer per (sequence, layer)
   std::vector<int> bounds_;     // PlanDecode: page boundaries of one sequence's units

@@ -165,10 +165,12 @@ struct yahkv_ctx {
     std::size_t plan_bytes = 0;
     float *part_acc = nullptr, *part_ml = nullptr;
     CUtensorMap k16map{}, v16map{};   // fp16 pages as [rows][256] fp16
+    StepLayers layers;
   } shared;
   // scores of a weight-accumulating decode call
   float* scores_dev = nullptr;
   std::int64_t score_pages = 0;
+  StepLayers weight_layers;
   std::vector<yahkv_batch*> batches;   // not destroyed yet
   char* evict_dev = nullptr;   // eviction work lists: the sequences, then their pages
   std::vector<EvictSeq> evict_scratch;
@@ -882,6 +884,7 @@ static int AttendDecode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int
   if (out_dtype != YAHKV_OUT_F16 && out_dtype != YAHKV_OUT_F32) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode: bad out_dtype");
   if (n_seqs > 0 && (q_dev == nullptr || out_dev == nullptr)) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode: null q or out pointer");
   bool changed = false;
+  if (weights_dev != nullptr && ctx->weight_layers.Comes(layer)) ctx->host.InvalidateDecodePlan();
   HostError e = ctx->host.PlanDecode(layer, n_seqs, seq_ids, n_splits, ctx->cfg.max_splits, ctx->max_units, &changed);
   if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
   if (n_seqs == 0) return YAHKV_OK;
@@ -954,6 +957,8 @@ static int AttendDecode(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, const int
   }
   if (le != cudaSuccess) return FailCuda(ctx, "decode attention launch", le);
   guard.keep = true;
+  if (changed) ctx->weight_layers.served.clear();
+  if (weights_dev != nullptr) ctx->weight_layers.Serve(layer, ctx->cfg.n_layers, false);
   ctx->launches += weights_dev != nullptr ? 3 : 2;
   return YAHKV_OK;
 }
@@ -1056,6 +1061,7 @@ int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, co
     if (int r = RefuseCapture(ctx, "attend_decode_shared: lists from the host", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
     auto& sh = ctx->shared;
     bool changed = false;
+    if (sh.layers.Comes(layer)) ctx->host.InvalidateSharedPlan();
     HostError e = ctx->host.PlanDecodeShared(layer, n_seqs, seq_ids, n_splits, ctx->cfg.max_splits, ctx->max_units, sh.n_pairs,
                                              sh.max_part_rows, &changed);
     if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
@@ -1115,6 +1121,7 @@ int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, co
     }
     if (le != cudaSuccess) return FailCuda(ctx, "shared-prefix decode attention launch", le);
     guard.keep = true;
+    sh.layers.Serve(layer, ctx->cfg.n_layers, changed);
     ctx->launches += 1 + (p.n_tiles > 0 ? 1 : 0) + (a.n_units > 0 ? 1 : 0);
     return YAHKV_OK;
   });
