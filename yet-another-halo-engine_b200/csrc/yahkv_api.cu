@@ -33,14 +33,18 @@ class Staging {
   static constexpr int kSlots = 8;
   ~Staging() {
     for (auto& s : slots_) {
-      if (s.host != nullptr) cudaFreeHost(s.host);
+      if (s.own) cudaFreeHost(s.host);
       if (s.ev != nullptr) cudaEventDestroy(s.ev);
     }
+    if (block_ != nullptr) cudaFreeHost(block_);
   }
-  // Buffers of `bytes` each, so that the first calls need not make them.
+  // Buffers of at least `bytes` each in one piece, so that the first calls need not make them.
   cudaError_t Reserve(std::size_t bytes) {
+    bytes = (std::max<std::size_t>(bytes, 1 << 16) + 255) / 256 * 256;
+    if (cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&block_), kSlots * bytes, cudaHostAllocDefault); e != cudaSuccess) return e;
+    for (int i = 0; i < kSlots; ++i) slots_[i].host = block_ + static_cast<std::size_t>(i) * bytes, slots_[i].cap = bytes;
     for (Slot& s : slots_)
-      if (cudaError_t e = Grow(s, bytes); e != cudaSuccess) return e;
+      if (cudaError_t e = cudaEventCreateWithFlags(&s.ev, cudaEventDisableTiming); e != cudaSuccess) return e;
     return cudaSuccess;
   }
   cudaError_t Acquire(std::size_t bytes, char** out) {
@@ -52,7 +56,12 @@ class Staging {
       if (e != cudaSuccess) return e;
       s.in_flight = false;
     }
-    if (cudaError_t e = Grow(s, bytes); e != cudaSuccess) return e;
+    if (s.cap < bytes) {
+      char* host = nullptr;
+      if (cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&host), bytes, cudaHostAllocDefault); e != cudaSuccess) return e;
+      if (s.own) cudaFreeHost(s.host);
+      s.host = host, s.cap = bytes, s.own = true;
+    }
     *out = s.host;
     return cudaSuccess;
   }
@@ -68,20 +77,10 @@ class Staging {
     char* host = nullptr;
     std::size_t cap = 0;
     cudaEvent_t ev = nullptr;
-    bool in_flight = false;
+    bool in_flight = false, own = false;   // own: outgrew the common block
   };
-  static cudaError_t Grow(Slot& s, std::size_t bytes) {
-    if (s.ev == nullptr)
-      if (cudaError_t e = cudaEventCreateWithFlags(&s.ev, cudaEventDisableTiming); e != cudaSuccess) return e;
-    if (s.cap >= bytes && s.cap > 0) return cudaSuccess;
-    if (s.host != nullptr) cudaFreeHost(s.host);
-    s.host = nullptr, s.cap = 0;
-    const std::size_t cap = std::max<std::size_t>(bytes, 1 << 16);
-    if (cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&s.host), cap, cudaHostAllocDefault); e != cudaSuccess) return e;
-    s.cap = cap;
-    return cudaSuccess;
-  }
   Slot slots_[kSlots];
+  char* block_ = nullptr;
   int next_ = 0, cur_ = 0;
 };
 
