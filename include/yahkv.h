@@ -314,7 +314,7 @@ int yahkv_rope_create(yahkv_ctx* ctx, const yahkv_rope_config* cfg, yahkv_rope**
 void yahkv_rope_destroy(yahkv_rope* rope);
 /* Rotates n_heads consecutive rows of 256 of each of n_tokens tokens at positions_dev[token] (device, int64): x_dev fp16
  * or f32 (x_dtype a YAHKV_OUT_* constant), tokens x_stride elements apart, so that x may be a slice of a wider projection output;
- * out_dev likewise, and may be x_dev itself with equal type and stride. weight_dev [256] f32 not NULL: each row is first
+ * out_dev likewise, and may be x_dev itself with equal type and stride (refused otherwise). weight_dev [256] f32 not NULL: each row is first
  * normed (x / sqrt(mean x^2 + eps) * weight, as yahkv_rope_append does). Arithmetic in f32, rounded once. Strides are
  * multiples of 8 elements, x, out and weight 16-byte aligned. Capturable. A position outside [0, max_positions) sets the
  * status word: the next yahkv_sync fails with YAHKV_ERR_CUDA, that token's rows are invalid (turned by the nearest

@@ -1270,6 +1270,8 @@ int yahkv_rope_rows(yahkv_rope* r, int32_t n_tokens, int32_t n_heads, const int6
   if (((reinterpret_cast<std::uintptr_t>(x_dev) | reinterpret_cast<std::uintptr_t>(out_dev) | reinterpret_cast<std::uintptr_t>(weight_dev)) & 15) != 0 ||
       (reinterpret_cast<std::uintptr_t>(positions_dev) & 7) != 0)
     return Fail(ctx, YAHKV_ERR_INVALID, "rope_rows: x, out and the norm weights must be 16-byte aligned, the positions 8-byte aligned");
+  if (x_dev == out_dev && (x_dtype != out_dtype || (n_tokens > 1 && x_stride != out_stride)))   // a row would be written before another is read
+    return Fail(ctx, YAHKV_ERR_INVALID, "rope_rows: in place needs equal types and strides");
   RopeRowsLaunch a{};
   a.x = x_dev, a.out = out_dev, a.positions = positions_dev, a.weight = weight_dev, a.tab_hi = r->hi, a.tab_lo = r->lo;
   a.status = ctx->status_dev, a.max_positions = r->cfg.max_positions, a.x_stride = x_stride, a.out_stride = out_stride;
