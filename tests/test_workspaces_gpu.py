@@ -55,3 +55,38 @@ def test_scores_of_forks_beyond_the_workspace():
     # the same cut for every row: the same bits in every row, and the weights of two calls are twice those of one
     assert torch.equal(out, out[:1].expand_as(out)) and torch.equal(out[:2], few)
     assert torch.equal(w[seqs[5]], 2 * wf[seqs[0]]) and torch.equal(w[seqs[-1]], w[seqs[0]])
+
+
+def test_a_context_on_a_full_device_does_without_them():
+    rng = np.random.default_rng(95)
+    kw = dict(num_pages=64, fmt=yahkv.FMT_Q8_0, max_seqs=24, max_pages_per_seq=60)
+    torch.cuda.empty_cache()
+    torch.cuda.synchronize()
+    free0 = torch.cuda.mem_get_info()[0]
+    cache = yahkv.KvCache(**kw)
+    whole = free0 - torch.cuda.mem_get_info()[0]               # 38 MB of it shared prefixes, 8.8 the scores
+    cache.close()
+    filler = torch.empty(torch.cuda.mem_get_info()[0] - whole + (24 << 20), dtype=torch.uint8, device="cuda")
+    try:
+        cache = yahkv.KvCache(**kw)                            # without them it fits
+        seq = cache.seq_create()
+        k, v = normal(rng, 200, 4, 256), normal(rng, 200, 4, 256)
+        cache.seq_reserve(seq, 200)
+        tensors = [torch.from_numpy(x).pin_memory() for x in (k, v, normal(rng, 1, 24, 256))]
+        out = torch.zeros(1, 24, 256).pin_memory()             # page-locked: the device has no room for tensors either
+        cache.append(0, [seq] * 200, np.arange(200), tensors[0], tensors[1])
+        cache.attend_decode(0, [seq], tensors[2], out, out_dtype=yahkv.OUT_F32)
+        cache.sync()
+        want = out.clone()
+        assert torch.isfinite(want).all() and want.abs().max() > 0
+        with pytest.raises(yahkv.YahkvError) as e:
+            cache.attend_decode_shared(0, [seq], tensors[2], out, out_dtype=yahkv.OUT_F32)
+        assert e.value.code == yahkv.ERR_CUDA and "memory" in e.value.message
+    finally:
+        del filler
+        torch.cuda.empty_cache()
+    out.zero_()
+    cache.attend_decode_shared(0, [seq], tensors[2], out, out_dtype=yahkv.OUT_F32)
+    cache.sync()
+    # the same scores and products, cut into units and joined in another order: a few roundings of f32 apart
+    assert (out - want).abs().max() <= 1e-5 * want.abs().max()

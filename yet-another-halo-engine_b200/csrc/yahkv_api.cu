@@ -95,6 +95,7 @@ struct yahkv_ctx {
   yahkv_config cfg;
   KvHost host;
   mutable std::string err;
+  mutable cudaError_t cuda_err = cudaSuccess;   // behind the last YAHKV_ERR_CUDA
   bool has_device = false;
   PoolView pool{};
   CUtensorMap kmap{}, vmap{};
@@ -157,6 +158,7 @@ struct yahkv_ctx {
   std::vector<DecodeUnit> unit_scratch;
   // shared-prefix decode attention (formats with rows of their own)
   struct Shared {
+    bool ready = false;
     int n_pairs = 0;            // CTA pairs of the prefix kernel the device runs at once
     int max_tiles = 0;
     std::int64_t max_part_rows = 0;
@@ -184,6 +186,8 @@ int Fail(const yahkv_ctx* ctx, int code, std::string msg) {
 }
 int FailHost(const yahkv_ctx* ctx, HostError e) { return Fail(ctx, e.code, std::move(e.message)); }
 int FailCuda(const yahkv_ctx* ctx, const char* what, cudaError_t e) {
+  ctx->cuda_err = e;
+  cudaGetLastError();   // reported here: a later launch check must not find it again
   return Fail(ctx, YAHKV_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
@@ -997,8 +1001,9 @@ static std::size_t SharedPlanBytes(std::size_t tiles, std::size_t units, std::si
 }
 
 // What shared-prefix attention needs beyond the context's own buffers.
-static int MakeShared(yahkv_ctx* ctx) {
+static int EnsureShared(yahkv_ctx* ctx) {
   auto& sh = ctx->shared;
+  if (sh.ready) return YAHKV_OK;
   const yahkv_config& c = ctx->cfg;
   int pairs = 0;
   YAHKV_CUDA(ctx, ConfigureSharedKernels(c.fmt, &pairs));
@@ -1010,28 +1015,39 @@ static int MakeShared(yahkv_ctx* ctx) {
   const std::int64_t heads = static_cast<std::int64_t>(c.max_seqs) * kQHeads;
   sh.max_part_rows = std::min(heads * c.max_pages_per_seq, std::max<std::int64_t>(heads, 4LL * kPrefillTileRows * sh.n_pairs));
   sh.plan_bytes = SharedPlanBytes(static_cast<std::size_t>(sh.max_tiles), static_cast<std::size_t>(ctx->max_units), static_cast<std::size_t>(c.max_seqs));
-  YAHKV_CUDA(ctx, DevAlloc(ctx, &sh.plan_dev, sh.plan_bytes, false));
-  YAHKV_CUDA(ctx, DevAlloc(ctx, &sh.part_acc, static_cast<std::size_t>(sh.max_part_rows) * kHeadDim, false));
-  YAHKV_CUDA(ctx, DevAlloc(ctx, &sh.part_ml, static_cast<std::size_t>(sh.max_part_rows) * 2, false));
+  auto alloc = [&](auto** p, std::size_t count) { return *p != nullptr ? cudaSuccess : DevAlloc(ctx, p, count, false); };
+  YAHKV_CUDA(ctx, alloc(&sh.plan_dev, sh.plan_bytes));
+  YAHKV_CUDA(ctx, alloc(&sh.part_acc, static_cast<std::size_t>(sh.max_part_rows) * kHeadDim));
+  YAHKV_CUDA(ctx, alloc(&sh.part_ml, static_cast<std::size_t>(sh.max_part_rows) * 2));
   if (c.fmt == YAHKV_FMT_F16) {
     const std::uint64_t rows = static_cast<std::uint64_t>(c.n_layers) * c.num_pages * kKvHeads * kPageTokens;
     if (!EncodeTensorMap2D(&sh.k16map, 2, ctx->pool.kcodes, kHeadDim, rows, 64, 32) ||
         !EncodeTensorMap2D(&sh.v16map, 2, ctx->pool.vcodes, kHeadDim, rows, 64, 64))
       return Fail(ctx, YAHKV_ERR_CUDA, "tensor map encode failed for the fp16 pools");
   }
+  sh.ready = true;
+  return YAHKV_OK;
+}
+
+static int EnsureEvictLists(yahkv_ctx* ctx) {
+  if (ctx->evict_dev != nullptr) return YAHKV_OK;
+  const yahkv_config& c = ctx->cfg;
+  YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_dev, static_cast<std::size_t>(c.max_seqs) * (sizeof(EvictSeq) + 4 * static_cast<std::size_t>(c.max_pages_per_seq)), false));
   return YAHKV_OK;
 }
 
 // Everything that the calls of a context need and that its configuration bounds exists before the first of them: an
-// allocation or a page lock takes longer than a call does.
+// allocation or a page lock takes longer than a call does. Where the device has no memory left for what only the long-context
+// calls need, the context is made without it; such a call then tries again, and reports it.
 static int MakeWorkspaces(yahkv_ctx* ctx) {
   const yahkv_config& c = ctx->cfg;
   std::size_t lists = static_cast<std::size_t>(ctx->max_units) * sizeof(DecodeUnit) + static_cast<std::size_t>(c.max_seqs) * kKvHeads * sizeof(CombineItem);
   if (!IsTileFmt(c.fmt)) {
-    if (int r = MakeShared(ctx); r != YAHKV_OK) return r;
+    auto failed = [&](int r) { return r != YAHKV_OK && !(r == YAHKV_ERR_CUDA && ctx->cuda_err == cudaErrorMemoryAllocation); };
+    if (int r = EnsureShared(ctx); failed(r)) return r;
     const std::int64_t pages = static_cast<std::int64_t>(c.max_seqs) * c.max_pages_per_seq * ctx->host.kv_head_count();
-    if (int r = EnsureScores(ctx, std::min<std::int64_t>(pages, (128LL << 20) / kScoreBytes)); r != YAHKV_OK) return r;
-    YAHKV_CUDA(ctx, DevAlloc(ctx, &ctx->evict_dev, static_cast<std::size_t>(c.max_seqs) * (sizeof(EvictSeq) + 4 * static_cast<std::size_t>(c.max_pages_per_seq)), false));
+    if (int r = EnsureScores(ctx, std::min<std::int64_t>(pages, (128LL << 20) / kScoreBytes)); failed(r)) return r;
+    if (int r = EnsureEvictLists(ctx); failed(r)) return r;
     YAHKV_CUDA(ctx, ConfigureEvictKernels());
     lists = std::max(lists, ctx->shared.plan_bytes);
   }
@@ -1058,6 +1074,7 @@ int yahkv_attend_decode_shared(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, co
     if (n_seqs > 0 && (q_dev == nullptr || out_dev == nullptr)) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: null q or out pointer");
     if ((reinterpret_cast<std::uintptr_t>(q_dev) & 15) != 0) return Fail(ctx, YAHKV_ERR_INVALID, "attend_decode_shared: q must be 16-byte aligned");
     if (int r = RefuseCapture(ctx, "attend_decode_shared: lists from the host", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
+    if (int r = EnsureShared(ctx); r != YAHKV_OK) return r;   // before the plan: a failure here changes no state
     auto& sh = ctx->shared;
     bool changed = false;
     if (sh.layers.Comes(layer)) ctx->host.InvalidateSharedPlan();
@@ -1145,6 +1162,7 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
       if (InBatch(ctx, seq_ids[i]))
         return Fail(ctx, YAHKV_ERR_ORDER, "evict: sequence " + std::to_string(seq_ids[i]) + " is in a decode batch (destroy the batch first)");
     if (int r = RefuseCapture(ctx, "evict: host tables change", StreamOf(ctx, stream)); r != YAHKV_OK) return r;
+    if (int r = EnsureEvictLists(ctx); r != YAHKV_OK) return r;
     bool any = false;
     HostError e = ctx->host.PlanEvict(n_seqs, seq_ids, n_keep, &ctx->evict_scratch, &ctx->evict_page_scratch, &any);
     if (e.code != YAHKV_OK) return FailHost(ctx, std::move(e));
@@ -1684,6 +1702,7 @@ int yahkv_batch_set_shared(yahkv_batch* b, int32_t on) {
   if (on != 0 && IsTileFmt(ctx->cfg.fmt))
     return Fail(ctx, YAHKV_ERR_INVALID, "batch_set_shared: not for YAHKV_FMT_KV8A16 / YAHKV_FMT_KV4A16 (their sequences share no pages)");
   if (on != 0) {   // everything a step needs exists before a capture
+    if (int r = EnsureShared(ctx); r != YAHKV_OK) return r;
     const std::size_t n = b->seqs.size();
     b->prefix_cap = SharedPlanBytes(static_cast<std::size_t>(ctx->shared.max_tiles), 0, n);
     if (b->prefix_dev == nullptr) YAHKV_CUDA(ctx, cudaMalloc(reinterpret_cast<void**>(&b->prefix_dev), b->prefix_cap));
