@@ -1,5 +1,5 @@
 // Host-only check that the second half of an eviction, which follows the kernels, cannot fail: with every allocation refused
-// after PlanEvict, CommitEvict still moves the tables over.
+// after PlanEvict, CommitEvict still moves the tables over. And that decode plans made before it are dropped.
 #include <cstdio>
 #include <cstdlib>
 #include <new>
@@ -57,6 +57,18 @@ int main() {
   int dirty = 0;
   host.ForEachDirty([&](int, int lo, int hi) { dirty += hi - lo; });
   EXPECT(dirty == 9);
+  // the lists of a decode call are made anew, also where id and length come again
+  bool changed = false;
+  EXPECT(host.PlanDecode(0, 1, &ids[1], 0, 64, 256, &changed).code == YAHKV_OK && changed);
+  EXPECT(host.PlanDecode(0, 1, &ids[1], 0, 64, 256, &changed).code == YAHKV_OK && !changed);
+  EXPECT(host.PlanDecodeShared(0, 1, &ids[1], 0, 64, 256, 74, 40000, &changed).code == YAHKV_OK && changed);
+  const std::int32_t id = ids[1];
+  EXPECT(host.SeqFree(ids[1]).code == YAHKV_OK && host.SeqCreate(&ids[1]).code == YAHKV_OK && ids[1] == id);
+  EXPECT(host.SeqReserve(id, 900).code == YAHKV_OK && host.SeqSetLen(id, -1, 900).code == YAHKV_OK);
+  EXPECT(host.PlanEvict(1, &id, 130, &seqs, &pages, &any).code == YAHKV_OK && any);
+  host.CommitEvict(130, seqs, pages);
+  EXPECT(host.PlanDecode(0, 1, &id, 0, 64, 256, &changed).code == YAHKV_OK && changed);
+  EXPECT(host.PlanDecodeShared(0, 1, &id, 0, 64, 256, 74, 40000, &changed).code == YAHKV_OK && changed);
   std::printf("evict_commit_test: ok\n");
   return 0;
 }

@@ -305,6 +305,7 @@ class KvHost {
     }
     for (std::int32_t p : evict_dropped_) Unref(p);   // only now: a page let go of here was nobody's fresh page
     evict_dropped_.clear();
+    InvalidateDecodePlan(), InvalidateSharedPlan();   // made for other sequences, even where a length comes again
   }
   int page_refs(std::int32_t page) const { return refs_[static_cast<std::size_t>(page)]; }
   // Keys of the sequence have been evicted: its slots no longer count positions.
