@@ -154,7 +154,8 @@ int yahkv_seq_set_kmean(yahkv_ctx* ctx, int32_t seq, int32_t layer, const float*
  * that holds the newest position is column j, columns past the sequence's length are stale. Blocks. */
 int yahkv_read_open_tile(yahkv_ctx* ctx, int32_t seq, int32_t layer, void* tile_host);
 
-/* ---- hot path (asynchronous on `stream`, a cudaStream_t; NULL = the context's own stream) -------------------- */
+/* ---- hot path (asynchronous on `stream`, a cudaStream_t; NULL = the context's own stream) --------------------
+ * The calls of a context share its pages, work lists and workspaces: on several streams, order them with events. */
 
 /* Replaces dattn_kvappend / dattn_kappend_q + dattn_vappend_q (engine/model/loom_decoder.hpp:254-264) and the chunk
  * writers yah_kq8 / yah_vq8 (engine/model/loom_prefill.hpp:3346-3366): quantizes n_tokens fp16 K and V rows
@@ -263,7 +264,7 @@ int yahkv_attend_decode_weights(yahkv_ctx* ctx, int32_t layer, int32_t n_seqs, c
 /* Cuts every listed sequence that is longer than n_keep down to n_keep keys, in all layers (which must be equally long:
  * YAHKV_ERR_ORDER), each kv head of each layer by its own weights: the first n_sink and the last n_recent keys are kept
  * and of the others the n_keep - n_sink - n_recent of largest weight; of equal weights the lowest slots, NaN counts as
- * less than any number. Kept keys move to slots 0 .. n_keep - 1 in their old order, their weights with them (weights
+ * less than any number. (Prefill and decode batches collect no weight: a prompt ranks by what watched steps saw of it.) Kept keys move to slots 0 .. n_keep - 1 in their old order, their weights with them (weights
  * of slots from n_keep to the old length become 0). weights_dev as above, layer l at weights_dev + l *
  * weights_layer_stride. kept_dev [n_layers][n_seqs][4][n_keep] i32 receives the old slots; a sequence of at most n_keep keys stays
  * as it is and its rows hold 0 .. len - 1, then -1. A head-sharded context cuts and writes its own kv heads only.
@@ -286,7 +287,11 @@ int yahkv_evict(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, int64_t 
  *   LINEAR  f_p / factor (position interpolation)
  *   NTK     theta * factor^(rotary_dim / (rotary_dim - 2)) in place of theta
  *   YARN    by parts: with r = original_len f_p / 2 pi turns over the original length and k = (r - beta_slow) / (beta_fast -
- *           beta_slow) clamped to [0, 1], f_p' = (1 - k) f_p / factor + k f_p; magnitude 0 stands for 0.1 ln(factor) + 1
+ *           beta_slow) clamped to [0, 1], f_p' = (1 - k) f_p / factor + k f_p; magnitude 0 stands for 0.1 ln(factor) + 1.
+ *           The ramp is linear in the turns r, as the method was published. Some implementations let it run linearly over the
+ *           pair index instead, between the pairs of beta_fast and beta_slow turns: their middle pairs have other angles (with
+ *           32 and 1, at r = 5.7, k is 0.5 there and 0.15 here), so weights tuned with that ramp must not be served with this
+ *           one. beta_slow 1, beta_fast 4 and magnitude 1 interpolate between the wavelengths original_len and original_len / 4
  * magnitude 0 = 1 otherwise. Angles are evaluated in double precision. max_positions bounds the positions. */
 #define YAHKV_ROPE_HALF 0
 #define YAHKV_ROPE_INTERLEAVED 1
@@ -381,7 +386,7 @@ int yahkv_batch_set_splits(yahkv_batch* batch, int32_t n_splits);
 /* on != 0: from the next batch_prepare on, the steps compute every prefix that rows of the batch share (yahkv_seq_fork) once
  * for all of them, as yahkv_attend_decode_shared does; the groups are found at batch_prepare and hold for its horizon.
  * Allocates the batch's lists when first switched on, so call it before a capture. The batches of a context share its workspaces: replay their graphs
- * one after the other, not side by side. Refused for the tile formats. The number of prefix tiles is part
+ * one after the other, not side by side nor beside the context's other attention calls. Refused for the tile formats. The number of prefix tiles is part
  * of the layout that *layout_changed reports. */
 int yahkv_batch_set_shared(yahkv_batch* batch, int32_t on);
 int yahkv_batch_prepare(yahkv_batch* batch, int32_t horizon_steps, int32_t* layout_changed, void* stream);

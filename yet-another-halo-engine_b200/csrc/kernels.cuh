@@ -302,8 +302,8 @@ cudaError_t ConfigureDecodeKernels();
 
 // The shared-prefix pass and the combine over prefix and suffix partials (shared_attn.cu).
 struct SharedLaunch {
-  const CUtensorMap* kmap;  // fp16 pages: K pool as [rows][256] fp16 in boxes of 64 dims x 32 keys
-  const CUtensorMap* vmap;  // fp16 pages: V pool, 64 dims x 64 keys; q8_0: V codes, 128 B x 64 keys
+  const CUtensorMap* kmap;  // fp16 pages: K pool as [rows][256] fp16 in boxes of 64 dims x 32 keys; else not read
+  const CUtensorMap* vmap;  // fp16 pages: V pool, 64 dims x 64 keys; else not read
   const PrefixTile* tiles_dev;
   int n_tiles;              // CTAs, a multiple of two
   const std::int32_t* rows_dev;

@@ -561,8 +561,8 @@ class KvHost {
   // once it is done, so the wave need not be the whole device: for every wave size the suffixes' end is estimated from
   // the measured times of a pair (6 us and 0.75 us per fp16 page, 0.95 us where pages are dequantized) and of a unit
   // (f16 three CTAs per SM, 7 us and 2 us per page; q8_0 two, 4 and 0.9; q4_0 four, 4 and 1.6), and the cheapest pair of
-  // sizes is taken. 96 rows x 16421 fp16, the same inputs again and again: 83 us with the whole device and units of two
-  // pages, 66 us as chosen here, 60 with the units' present form.
+  // sizes is taken. 96 rows x 16421 fp16: 83 us with the whole device and units of two pages, 76 as chosen here, 69 with the
+  // units' present form of three CTAs per SM.
   struct SharedShape {
     int part_pages = 1, unit_pages = 1;
   };

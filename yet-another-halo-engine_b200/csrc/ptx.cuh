@@ -76,6 +76,9 @@ __device__ __forceinline__ void ChainedKernelEntry() {
 //   resident and what came before A has completed;
 //   B begins with ChainedKernelEntryBeside, which does not wait, and its last CTA leaves through ChainedKernelExitBeside,
 //   which waits for A: B is complete only when A is, so whatever follows B may read what A wrote.
+// PTX promises the writes of earlier kernels to a grid that executes griddepcontrol.wait, and all but B's last CTA read them
+// (pages, tables, lists) without one. That rests on the order of events: the wait that saw their completion was A's, B starts
+// only behind it, and the fence at B's entry keeps B from reading lines that its SM held from before.
 __device__ __forceinline__ void ChainedKernelEntryBefore() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
