@@ -1637,31 +1637,33 @@ static bool InBatch(const yahkv_ctx* ctx, int seq) {
   return false;
 }
 
+static int BatchCreate(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, yahkv_batch** out);
 int yahkv_batch_create(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, yahkv_batch** out) {
+  return NoThrow(ctx, "batch_create", [&] { return BatchCreate(ctx, n_seqs, seq_ids, out); });
+}
+
+static int BatchCreate(yahkv_ctx* ctx, int32_t n_seqs, const int32_t* seq_ids, yahkv_batch** out) {
   if (int r = RequireDevice(ctx, "batch_create"); r != YAHKV_OK) return r;
   if (out == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "batch_create: null out pointer");
   *out = nullptr;
   if (n_seqs <= 0 || n_seqs > ctx->cfg.max_seqs || seq_ids == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "batch_create: bad sequence list");
   if (ctx->host.kv_head_count() != kKvHeads) return Fail(ctx, YAHKV_ERR_INVALID, "batch_create: decode batches need a context that holds all four kv heads");
-  auto* b = new (std::nothrow) yahkv_batch();
-  if (b == nullptr) return Fail(ctx, YAHKV_ERR_INVALID, "batch_create: out of host memory");
+  auto owned = std::make_unique<yahkv_batch>();
+  yahkv_batch* b = owned.get();
   b->ctx = ctx, b->device = ctx->cfg.device;
   for (int i = 0; i < n_seqs; ++i) {
     const int s = seq_ids[i];
-    if (!ctx->host.live(s)) {
-      delete b;
-      return Fail(ctx, YAHKV_ERR_INVALID, "batch_create: not a live sequence: " + std::to_string(s));
-    }
+    if (!ctx->host.live(s)) return Fail(ctx, YAHKV_ERR_INVALID, "batch_create: not a live sequence: " + std::to_string(s));
     const std::int64_t n = ctx->host.len(s, 0);
     for (int l = 1; l < ctx->cfg.n_layers; ++l)
-      if (ctx->host.len(s, l) != n) {
-        delete b;
+      if (ctx->host.len(s, l) != n)
         return Fail(ctx, YAHKV_ERR_ORDER, "batch_create: sequence " + std::to_string(s) + " has different lengths in its layers");
-      }
     b->seqs.push_back(s);
     b->generations.push_back(ctx->host.generation(s));
     b->lens.push_back(static_cast<std::int32_t>(n));
   }
+  ctx->batches.reserve(ctx->batches.size() + 1);   // nothing throws from here on
+  owned.release();
   b->units_cap = ctx->max_units;
   cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&b->lens_dev), sizeof(std::int32_t) * n_seqs);
   if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&b->rows_dev), sizeof(BatchSeq) * n_seqs);
